@@ -552,6 +552,94 @@ int spx_op_argmax_partial(spx_graph* g, const float* x, int64_t ldx, int32_t row
 int spx_op_argmax_merge(spx_graph* g, const float* packed, int32_t parts, int32_t rows,
                         int32_t* ids);
 
+/* ---- 8-bit key / value cache ------------------------------------------------
+ * A cache that holds a full block of `block` tokens as int8 with one scale per
+ * kv head for K and one for V, and the block that is still open in fp32.  A
+ * block is quantised once, when its last token arrives, so the contents depend
+ * on the tokens alone and not on how calls cut them:
+ *
+ *   scale = max|x| / 127 (over block x head_dim; 0 where that maximum is below
+ *   127 * 2^-126), q = x / scale rounded half to even, value = q * scale.
+ *   A block with a NaN or an infinity has that as its scale and reads as NaN.
+ *
+ * Slots 0 .. lens[b] - 1 of sequence b hold its tokens in order; every call
+ * that takes new tokens reads lens as it was before them, and sequence b
+ * brings new_lens[b] of the q_len rows that it has in q and qkv (NULL: all of
+ * them; rows behind are not read, and what belongs to them is left as it was).
+ * Tokens behind slot max_seq - 1 are dropped.  lens and new_lens live on the
+ * device, so a step can be captured once and replayed; values outside
+ * [0, max_seq] and [0, q_len] are taken as the nearest one inside.
+ * The buffers must be 16-byte aligned; max_seq a multiple of block; block 16,
+ * 32, 64 or 128; head_dim 64 or 128 (SPX_ERR_UNSUPPORTED otherwise). */
+typedef struct spx_kv8_cache {
+  int8_t* k;      /* [batch][kv_heads][max_seq][head_dim] */
+  int8_t* v;
+  float* k_scale; /* [batch][kv_heads][max_seq / block] */
+  float* v_scale;
+  float* k_tail;  /* [batch][kv_heads][block][head_dim]: slot j at row j % block */
+  float* v_tail;
+  int32_t* lens;  /* [batch] */
+  int32_t batch, kv_heads, max_seq, head_dim, block;
+} spx_kv8_cache;
+/* 1 if the operators below take a cache of these buffers and this shape, 0 if
+ * not, the reason in spx_last_error.  Host only. */
+int spx_kv8_supported(const spx_kv8_cache* cache);
+/* RoPE as in spx_op_rope_kv_append on q and k of the new tokens, token t of
+ * sequence b at position pos[b] + t (which an eviction leaves larger than its
+ * slot); q written to q_out, k and v taken into the cache.  The tables have
+ * table_rows rows; a position outside them gives NaN.  lens and pos are not
+ * changed (spx_op_kv8_advance). */
+int spx_op_rope_kv8_append(spx_graph* g, const float* qkv, int64_t ld_qkv, const float* cos_table,
+                           const float* sin_table, int32_t table_rows, const int32_t* pos,
+                           const int32_t* new_lens, int32_t q_len, int32_t q_heads, float* q_out,
+                           const spx_kv8_cache* cache);
+/* Causal grouped-query attention of the new tokens over the cache, after their
+ * append: the token in slot i sees the slots up to i, out = softmax(scale q
+ * k^T) v in fp32 accuracy.  q and out are [batch * q_len][q_heads][head_dim],
+ * 16-byte aligned.  lse (may be NULL): [batch * q_len][q_heads], the log of
+ * each softmax sum.  weights (may be NULL; needs lse): [batch][kv_heads]
+ * [max_seq], to which each slot's attention weight, summed over the new tokens
+ * and the heads of the group, is added; the new tokens' slots start from 0. */
+int spx_op_attention_kv8(spx_graph* g, const float* q, const spx_kv8_cache* cache,
+                         const int32_t* new_lens, int32_t q_len, int32_t q_heads, float scale,
+                         float* out, float* lse, float* weights);
+/* fp32 values of the slots starts[b] .. starts[b] + count - 1 (NULL: from 0) of
+ * every sequence into [batch][kv_heads][count][head_dim], 16-byte aligned;
+ * zeros outside the sequence's lens[b] + new tokens. */
+int spx_op_kv8_read(spx_graph* g, const spx_kv8_cache* cache, const int32_t* new_lens,
+                    int32_t q_len, const int32_t* starts, int32_t count, float* k_out,
+                    float* v_out);
+/* Eviction by accumulated weight.  Each sequence and kv head that holds more
+ * than `keep` tokens keeps the first `sink`, the last `recent` and, of those
+ * between, the ones with the largest weights (ties: the lower slot; NaN counts
+ * as lowest), moved to the front in order with their weights; idx [batch]
+ * [kv_heads][keep] gets the slots they had (-1 behind the last one).  The
+ * result goes to dst, which may be src itself (dst_weights then being weights)
+ * or share no memory with it, of the same heads and block, keep <= its
+ * max_seq.  In a new full block the scale is the largest of its members' and
+ * values are rounded to it again; members that had that scale keep their bits.
+ * lens is not changed: it becomes min(lens, keep), by spx_op_kv8_advance with
+ * limit = keep, once every cache that shares it has been cut. */
+int spx_op_kv8_evict(spx_graph* g, const spx_kv8_cache* src, const float* weights, int32_t keep,
+                     int32_t recent, int32_t sink, int32_t* idx, const spx_kv8_cache* dst,
+                     float* dst_weights);
+/* lens[b] = min(lens[b] + n, limit) and pos[b] += n, n the new tokens of
+ * sequence b as above; lens or pos may be NULL. */
+int spx_op_kv8_advance(spx_graph* g, int32_t* lens, int32_t* pos, const int32_t* new_lens,
+                       int32_t batch, int32_t q_len, int32_t limit);
+/* Of each row of logits (row stride ld): logprobs[r] = the log probability of
+ * token ids[r], entropy[r] in nats, rank[r] = 1 + the number of larger logits,
+ * and the top_k (0..64) largest logits' columns and log probabilities in
+ * falling order (ties: the lower column; NaN last).  logprobs, entropy and
+ * rank may be NULL; ids may be when neither logprobs nor rank is asked for.
+ * An id below 0 marks a row without a token (logprob 0, rank 0); one past the
+ * columns gives NaN and rank 0.  -inf logits have probability 0; a row of
+ * nothing else has log probabilities -inf and entropy 0; a NaN or +inf in the
+ * row makes its log probabilities and entropy NaN. */
+int spx_op_token_logprobs(spx_graph* g, const float* logits, int64_t ld, int32_t rows,
+                          int32_t cols, const int32_t* ids, float* logprobs, float* entropy,
+                          int32_t* rank, int32_t top_k, int32_t* top_ids, float* top_logprobs);
+
 /* ---- one-shot all-reduce over peer memory (tensor-parallel decode) ------
  * No counterpart in the reference (its TP plan names an NCCL all-reduce,
  * which this replaces for small messages).  Each rank creates a

@@ -78,6 +78,12 @@ class KvParams(Structure):
                                        "max_seq")]
 
 
+class Kv8CacheStruct(Structure):
+    _fields_ = ([(n, c_void_p) for n in ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail",
+                                         "lens")]
+                + [(n, c_int32) for n in ("batch", "kv_heads", "max_seq", "head_dim", "block")])
+
+
 class PoolParams(Structure):
     _fields_ = [(n, c_int32) for n in (
         "n", "ih", "iw", "c", "oh", "ow", "kh", "kw", "stride_h", "stride_w", "pad_top",
@@ -173,6 +179,20 @@ _SIGS = {
     "spx_op_argmax_partial": ([c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32,
                                c_void_p], c_int),
     "spx_op_argmax_merge": ([c_void_p, c_void_p, c_int32, c_int32, c_void_p], c_int),
+    "spx_kv8_supported": ([POINTER(Kv8CacheStruct)], c_int),
+    "spx_op_rope_kv8_append": ([c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int32,
+                                c_void_p, c_void_p, c_int32, c_int32, c_void_p,
+                                POINTER(Kv8CacheStruct)], c_int),
+    "spx_op_attention_kv8": ([c_void_p, c_void_p, POINTER(Kv8CacheStruct), c_void_p, c_int32,
+                              c_int32, c_float, c_void_p, c_void_p, c_void_p], c_int),
+    "spx_op_kv8_read": ([c_void_p, POINTER(Kv8CacheStruct), c_void_p, c_int32, c_void_p, c_int32,
+                         c_void_p, c_void_p], c_int),
+    "spx_op_kv8_evict": ([c_void_p, POINTER(Kv8CacheStruct), c_void_p, c_int32, c_int32, c_int32,
+                          c_void_p, POINTER(Kv8CacheStruct), c_void_p], c_int),
+    "spx_op_kv8_advance": ([c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32],
+                           c_int),
+    "spx_op_token_logprobs": ([c_void_p, c_void_p, c_int64, c_int32, c_int32, c_void_p, c_void_p,
+                               c_void_p, c_void_p, c_int32, c_void_p, c_void_p], c_int),
     "spx_ar_create": ([c_int32, c_int32, c_int32, ctypes.c_size_t, POINTER(c_void_p)], c_int),
     "spx_ar_handle_size": ([], ctypes.c_size_t),
     "spx_ar_handle": ([c_void_p, c_void_p, ctypes.c_size_t], c_int),

@@ -1059,6 +1059,64 @@ int spx_op_argmax_merge(spx_graph* g, const float* packed, int32_t parts, int32_
   return launch_argmax_merge(g->stream, &g->launches, packed, parts, rows, ids);
 }
 
+int spx_kv8_supported(const spx_kv8_cache* cache) {
+  return kv8_check(cache, "kv8_supported") == SPX_OK ? 1 : 0;
+}
+
+int spx_op_rope_kv8_append(spx_graph* g, const float* qkv, int64_t ld_qkv, const float* cos_table,
+                           const float* sin_table, int32_t table_rows, const int32_t* pos,
+                           const int32_t* new_lens, int32_t q_len, int32_t q_heads, float* q_out,
+                           const spx_kv8_cache* cache) {
+  SPX_G(g);
+  if (!qkv || !cos_table || !sin_table || !pos || !q_out || !cache)
+    return fail(SPX_ERR_INVALID_ARGUMENT, "rope_kv8_append: null");
+  return launch_rope_kv8_append(g->stream, &g->launches, qkv, ld_qkv, cos_table, sin_table,
+                                table_rows, pos, new_lens, q_len, q_heads, q_out, cache);
+}
+
+int spx_op_attention_kv8(spx_graph* g, const float* q, const spx_kv8_cache* cache,
+                         const int32_t* new_lens, int32_t q_len, int32_t q_heads, float scale,
+                         float* out, float* lse, float* weights) {
+  SPX_G(g);
+  if (!q || !cache || !out) return fail(SPX_ERR_INVALID_ARGUMENT, "attention_kv8: null");
+  return launch_attention_kv8(g->stream, &g->launches, q, cache, new_lens, q_len, q_heads, scale,
+                              out, lse, weights);
+}
+
+int spx_op_kv8_read(spx_graph* g, const spx_kv8_cache* cache, const int32_t* new_lens,
+                    int32_t q_len, const int32_t* starts, int32_t count, float* k_out,
+                    float* v_out) {
+  SPX_G(g);
+  if (!cache || !k_out || !v_out) return fail(SPX_ERR_INVALID_ARGUMENT, "kv8_read: null");
+  return launch_kv8_read(g->stream, &g->launches, cache, new_lens, q_len, starts, count, k_out,
+                         v_out);
+}
+
+int spx_op_kv8_evict(spx_graph* g, const spx_kv8_cache* src, const float* weights, int32_t keep,
+                     int32_t recent, int32_t sink, int32_t* idx, const spx_kv8_cache* dst,
+                     float* dst_weights) {
+  SPX_G(g);
+  if (!src || !weights || !idx || !dst || !dst_weights)
+    return fail(SPX_ERR_INVALID_ARGUMENT, "kv8_evict: null");
+  return launch_kv8_evict(g->stream, &g->launches, src, weights, keep, recent, sink, idx, dst,
+                          dst_weights);
+}
+
+int spx_op_kv8_advance(spx_graph* g, int32_t* lens, int32_t* pos, const int32_t* new_lens,
+                       int32_t batch, int32_t q_len, int32_t limit) {
+  SPX_G(g);
+  return launch_kv8_advance(g->stream, &g->launches, lens, pos, new_lens, batch, q_len, limit);
+}
+
+int spx_op_token_logprobs(spx_graph* g, const float* logits, int64_t ld, int32_t rows,
+                          int32_t cols, const int32_t* ids, float* logprobs, float* entropy,
+                          int32_t* rank, int32_t top_k, int32_t* top_ids, float* top_logprobs) {
+  SPX_G(g);
+  if (!logits) return fail(SPX_ERR_INVALID_ARGUMENT, "token_logprobs: null");
+  return launch_token_logprobs(g->stream, &g->launches, logits, ld, rows, cols, ids, logprobs,
+                               entropy, rank, top_k, top_ids, top_logprobs);
+}
+
 int spx_op_expand_dw_nhwc(spx_graph* g, const float* x, const float* w_expand,
                           const float* b_expand, const float* w_dw, const float* b_dw, float* y,
                           const spx_expand_dw_params* p) {

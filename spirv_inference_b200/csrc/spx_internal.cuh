@@ -224,6 +224,26 @@ int launch_argmax_merge(cudaStream_t s, int64_t* cnt, const float* packed, int p
                         int32_t* ids);
 int launch_swiglu_rows(cudaStream_t s, int64_t* cnt, const float* gu, int64_t ld, float* y,
                        int64_t ldy, int rows, int f);
+// 8-bit key / value cache (k_kv8.cu, k_attn_kv8.cu).
+int kv8_check(const spx_kv8_cache* c, const char* what);
+int launch_rope_kv8_append(cudaStream_t s, int64_t* cnt, const float* qkv, int64_t ld_qkv,
+                           const float* cos_t, const float* sin_t, int table_rows,
+                           const int32_t* pos, const int32_t* new_lens, int T, int Hq,
+                           float* q_out, const spx_kv8_cache* c);
+int launch_attention_kv8(cudaStream_t s, int64_t* cnt, const float* q, const spx_kv8_cache* c,
+                         const int32_t* new_lens, int T, int Hq, float scale, float* out,
+                         float* lse, float* weights);
+int launch_kv8_read(cudaStream_t s, int64_t* cnt, const spx_kv8_cache* c, const int32_t* new_lens,
+                    int q_len, const int32_t* starts, int count, float* k_out, float* v_out);
+int launch_kv8_evict(cudaStream_t s, int64_t* cnt, const spx_kv8_cache* src, const float* weights,
+                     int keep, int recent, int sink, int32_t* idx, const spx_kv8_cache* dst,
+                     float* dst_weights);
+int launch_kv8_advance(cudaStream_t s, int64_t* cnt, int32_t* lens, int32_t* pos,
+                       const int32_t* new_lens, int batch, int q_len, int limit);
+// Token log probabilities (k_logprobs.cu).
+int launch_token_logprobs(cudaStream_t s, int64_t* cnt, const float* x, int64_t ld, int rows,
+                          int cols, const int32_t* ids, float* logprobs, float* entropy,
+                          int32_t* rank, int top_k, int32_t* top_ids, float* top_logprobs);
 int launch_pad4(cudaStream_t s, int64_t* cnt, const float* x, float* y, float pad_value,
                 const int32_t* push);
 int launch_transpose4(cudaStream_t s, int64_t* cnt, const float* x, float* y,

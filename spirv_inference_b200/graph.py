@@ -45,6 +45,37 @@ class DeviceTensor:
                             tuple(shape), self.dtype, self.graph)
 
 
+class Kv8Cache:
+    """The buffers of an 8-bit key / value cache (see ``Graph.kv8_cache``).
+
+    k, v           int8 [batch][kv_heads][max_seq][head_dim]
+    k_scale, ...   fp32 [batch][kv_heads][max_seq / block]
+    k_tail, ...    fp32 [batch][kv_heads][block][head_dim], the open block
+    lens           int32 [batch]; caches of several layers may share it
+    """
+
+    def __init__(self, k, v, k_scale, v_scale, k_tail, v_tail, lens, *, block: int):
+        self.batch, self.kv_heads, self.max_seq, self.head_dim = k.shape
+        self.block = block
+        b, h, s, d = k.shape
+        if block <= 0 or s % block:
+            raise ValueError(f"max_seq {s} is not a whole number of blocks of {block}")
+        want = {"k": k.shape, "v": k.shape, "k_scale": (b, h, s // block),
+                "v_scale": (b, h, s // block), "k_tail": (b, h, block, d),
+                "v_tail": (b, h, block, d), "lens": (b,)}
+        types = {"k": np.int8, "v": np.int8, "lens": np.int32}
+        self._tensors = dict(k=k, v=v, k_scale=k_scale, v_scale=v_scale, k_tail=k_tail,
+                             v_tail=v_tail, lens=lens)
+        for name, x in self._tensors.items():
+            if tuple(x.shape) != tuple(want[name]) or x.dtype != types.get(name, np.float32):
+                raise ValueError(f"{name} has shape {x.shape} and type {x.dtype}; expected "
+                                 f"{want[name]} and {np.dtype(types.get(name, np.float32))}")
+            setattr(self, name, x)
+        self._struct = _lib.Kv8CacheStruct(
+            *(x.ptr for x in self._tensors.values()), b, h, s, d, block)
+        self.ref = ctypes.byref(self._struct)
+
+
 class Graph:
     """One device, one stream, owned device buffers, recorded ops."""
 
@@ -354,6 +385,75 @@ class Graph:
         p = _lib.KvParams(batch, q_len, q_heads, kv_heads, head_dim, max_seq)
         check(self._l.spx_op_attention_kv(self.h, self._p(q), self._p(k_cache), self._p(v_cache),
                                           self._p(out), self._p(state), ctypes.byref(p), scale))
+
+    # -- 8-bit key / value cache ---------------------------------------------
+    def kv8_cache(self, batch, kv_heads, max_seq, head_dim, *, block=32, lens=None) -> Kv8Cache:
+        """An empty 8-bit cache: full blocks of `block` tokens in int8 with one
+        scale per block and head, the open block in fp32.  `lens` (int32
+        [batch]): shared with other layers' caches, or allocated here as 0."""
+        shape = (batch, kv_heads, max_seq, head_dim)
+        if lens is None:
+            lens = self.alloc((batch,), np.int32)
+            self.zero(lens)
+        blocks = (batch, kv_heads, max_seq // block if block > 0 else 0)
+        tail = (batch, kv_heads, block, head_dim)
+        return Kv8Cache(self.alloc(shape, np.int8), self.alloc(shape, np.int8),
+                        self.alloc(blocks), self.alloc(blocks), self.alloc(tail),
+                        self.alloc(tail), lens, block=block)
+
+    def rope_kv8_append(self, qkv, ld_qkv, cos_t, sin_t, pos, q_out, cache, *, q_len, q_heads,
+                        new_lens=None):
+        """RoPE on q and k of the new tokens (token t of sequence b at position
+        pos[b] + t); q to q_out, k and v into the cache behind lens[b]."""
+        check(self._l.spx_op_rope_kv8_append(
+            self.h, qkv.ptr, ld_qkv, cos_t.ptr, sin_t.ptr, cos_t.shape[0], pos.ptr,
+            None if new_lens is None else new_lens.ptr, q_len, q_heads, q_out.ptr, cache.ref))
+
+    def attention_kv8(self, q, cache, out, *, q_len, q_heads, scale, new_lens=None, lse=None,
+                      weights=None):
+        """Causal attention of the appended tokens over the cache; `weights`
+        [batch][kv_heads][max_seq] gathers what each slot receives (needs
+        `lse`)."""
+        check(self._l.spx_op_attention_kv8(
+            self.h, q.ptr, cache.ref, None if new_lens is None else new_lens.ptr, q_len, q_heads,
+            scale, out.ptr, None if lse is None else lse.ptr,
+            None if weights is None else weights.ptr))
+
+    def kv8_read(self, cache, k_out, v_out, *, count, starts=None, q_len=0, new_lens=None):
+        """fp32 values of `count` slots per sequence from starts[b] (default 0)
+        on; zeros behind lens[b] (+ the new tokens, before an advance)."""
+        check(self._l.spx_op_kv8_read(
+            self.h, cache.ref, None if new_lens is None else new_lens.ptr, q_len,
+            None if starts is None else starts.ptr, count, k_out.ptr, v_out.ptr))
+
+    def kv8_evict(self, cache, weights, keep, *, idx, recent=0, sink=0, into=None,
+                  into_weights=None):
+        """Cuts every sequence and head to its first `sink`, last `recent` and
+        heaviest other slots, `keep` in all; in place, or into another cache.
+        idx [batch][kv_heads][keep] gets the slots that stay."""
+        if (into is None) != (into_weights is None):
+            raise ValueError("kv8_evict: into and into_weights go together")
+        check(self._l.spx_op_kv8_evict(
+            self.h, cache.ref, weights.ptr, keep, recent, sink, idx.ptr,
+            (cache if into is None else into).ref,
+            (weights if into is None else into_weights).ptr))
+
+    def kv8_advance(self, cache, pos=None, *, q_len=0, new_lens=None, limit=None):
+        """lens += the new tokens, at most `limit` (default max_seq); pos too,
+        without a limit."""
+        check(self._l.spx_op_kv8_advance(
+            self.h, cache.lens.ptr, None if pos is None else pos.ptr,
+            None if new_lens is None else new_lens.ptr, cache.batch, q_len,
+            cache.max_seq if limit is None else limit))
+
+    def token_logprobs(self, logits, ld, rows, cols, ids, logprobs, *, entropy=None, rank=None,
+                       top_k=0, top_ids=None, top_logprobs=None):
+        """Log probability, rank, entropy and the top_k alternatives of `rows`
+        rows of logits (row stride ld) for the tokens ids[rows]."""
+        opt = [None if x is None else x.ptr for x in (ids, logprobs, entropy, rank, top_ids,
+                                                      top_logprobs)]
+        check(self._l.spx_op_token_logprobs(self.h, logits.ptr, ld, rows, cols, *opt[:4], top_k,
+                                            *opt[4:]))
 
     def swiglu_linear(self, a, lda, w, ldw, m, f, k, c, ldc, rms_eps=-1.0):
         check(self._l.spx_op_swiglu_linear(self.h, self._p(a), lda, self._p(w), ldw, m, f, k,

@@ -25,6 +25,17 @@ by vocabulary and the greedy token is a (value, index) argmax merged over
 ranks.  With more ranks than kv heads, kv heads are replicated (rank r uses
 kv head r * kv_heads // world).
 
+Cache (`kv_cache`): "fp32" holds max_seq positions; "int8" holds them as int8
+blocks of `kv_block` tokens with a scale per block and head, and the open
+block in fp32.  With `kv_keep` the int8 cache is bounded: attention gathers
+the weight that each slot receives, and when the next step would not fit,
+every layer and head drops to its first `kv_sink`, last `kv_recent` and
+heaviest other slots, kv_keep in all; generation then goes on past max_seq.
+
+Answers: generate() gives tokens; with `logprobs` = k the decoder also keeps
+each token's log probability, rank, entropy and k alternatives
+(token_logprobs()), and score() gives the same for the tokens of a prompt.
+
 Weights (seeded, N(0, 0.02); norm gains 1 + N(0, 0.02)) are generated in the
 reference's shapes and argument order (export_llama.py:305-316, 360-361) and
 packed at load time: projection matrices transposed to [out][in], Q|K|V and
@@ -190,11 +201,32 @@ class LlamaDecoder:
     def __init__(self, cfg: LlamaConfig, weights: dict, batch: int, prompt_len: int,
                  n_new: int, *, device: int = 0, stream: int | None = None,
                  rank: int = 0, world: int = 1, group=None, capture: bool = True,
-                 peer_allreduce: bool = False):
+                 peer_allreduce: bool = False, kv_cache: str = "fp32", kv_block: int = 32,
+                 kv_keep: int | None = None, kv_recent: int | None = None, kv_sink: int = 4,
+                 logprobs: int | None = None):
         self.cfg, self.B, self.P, self.n_new = cfg, batch, prompt_len, n_new
-        if prompt_len + n_new - 1 > cfg.max_seq:
+        if kv_cache not in ("fp32", "int8"):
+            raise ValueError(f"kv_cache {kv_cache!r}: fp32 or int8")
+        self.kv8 = kv_cache == "int8"
+        # Slots of the int8 cache: whole blocks.
+        self.kv_slots = -(-cfg.max_seq // kv_block) * kv_block if self.kv8 else cfg.max_seq
+        self.kv_keep, self.kv_sink = kv_keep, kv_sink
+        if kv_keep is not None:
+            if not self.kv8:
+                raise ValueError("kv_keep needs kv_cache='int8'")
+            self.kv_recent = kv_keep // 2 if kv_recent is None else kv_recent
+            if not 0 < kv_keep < self.kv_slots or min(self.kv_recent, kv_sink) < 0 \
+                    or self.kv_recent + kv_sink > kv_keep:
+                raise ValueError(f"kv_keep {kv_keep} with kv_recent {self.kv_recent} and kv_sink "
+                                 f"{kv_sink} does not fit {self.kv_slots} slots")
+            if prompt_len > self.kv_slots:
+                raise ValueError(f"prompt {prompt_len} exceeds max_seq {cfg.max_seq}")
+        elif prompt_len + n_new - 1 > cfg.max_seq:
             raise ValueError(f"prompt {prompt_len} + {n_new} new tokens exceed max_seq "
                              f"{cfg.max_seq}")
+        if logprobs is not None and (world > 1 or not 0 <= logprobs <= min(64, cfg.vocab)):
+            raise ValueError("logprobs: 0..64 alternatives, on one rank")
+        self.n_top = logprobs
         self.rank, self.world, self.group = rank, world, group
         self.sh = tp_shard(cfg, rank, world)
         self.g = Graph(device, stream=stream)
@@ -214,7 +246,7 @@ class LlamaDecoder:
         self._split = {}
         for t in [self.lm_head] + [w for L in self.layers for w in L.values()]:
             self._split[t.ptr] = g.weights_split(t)
-        cos, sin = rope_tables(cfg, cfg.max_seq)
+        cos, sin = rope_tables(cfg, max(cfg.max_seq, prompt_len + n_new))
         self.cos, self.sin = g.tensor(cos), g.tensor(sin)
         # Activations (sized for the prefill block).
         M = batch * prompt_len
@@ -225,14 +257,28 @@ class LlamaDecoder:
         self.gu = g.alloc((M, 2 * sh.nf))
         self.mlp = g.alloc((M, sh.nf))
         self.logits = g.alloc((batch, sh.nv))
-        self.kc = [g.alloc((batch, sh.nkv, cfg.max_seq, D)) for _ in range(cfg.layers)]
-        self.vc = [g.alloc((batch, sh.nkv, cfg.max_seq, D)) for _ in range(cfg.layers)]
+        if self.kv8:
+            self.lens = g.alloc((batch,), np.int32)
+            self.pos = g.alloc((batch,), np.int32)
+            self.kv = [g.kv8_cache(batch, sh.nkv, self.kv_slots, D, block=kv_block,
+                                   lens=self.lens) for _ in range(cfg.layers)]
+            if kv_keep is not None:
+                self.lse = g.alloc((M, sh.nq))
+                self.kv_weights = [g.alloc((batch, sh.nkv, self.kv_slots))
+                                   for _ in range(cfg.layers)]
+                self.kept = [g.alloc((batch, sh.nkv, kv_keep), np.int32)
+                             for _ in range(cfg.layers)]
+        else:
+            self.kc = [g.alloc((batch, sh.nkv, cfg.max_seq, D)) for _ in range(cfg.layers)]
+            self.vc = [g.alloc((batch, sh.nkv, cfg.max_seq, D)) for _ in range(cfg.layers)]
         self.keys = g.alloc((batch,), np.uint64)
         g.zero(self.keys)
         self.prompt_ids = g.alloc((M,), np.int32)
         self.ids = g.alloc((batch,), np.int32)
         self.hist = g.alloc((n_new, batch), np.int32)
         self.state = g.alloc((2,), np.int32)
+        if logprobs is not None:
+            self.lp = self._logprob_buffers(n_new * batch, logprobs)
         self._torch_bufs = []
         if world > 1:
             import torch
@@ -257,7 +303,9 @@ class LlamaDecoder:
         self.capture = capture
         self._captured = False
         self._mark = None      # optional callback(label, bytes, flops) after each op
-        self._host_pos = 0
+        self._host_pos = 0     # slots in use, the same for every sequence
+        self._step = 0
+        self._score = {}       # buffers of score(), made when it is first called
 
     # -- helpers -----------------------------------------------------------
     def _torch_buf(self, t) -> DeviceTensor:
@@ -272,6 +320,31 @@ class LlamaDecoder:
     def _all_reduce(self, t: DeviceTensor, rows: int) -> None:
         import torch.distributed as dist
         dist.all_reduce(self._torch_view(t, rows, self.cfg.hidden), group=self.group)
+
+    def _logprob_buffers(self, rows: int, k: int) -> dict:
+        g = self.g
+        lp = {n: g.alloc((rows,), np.int32 if n == "rank" else np.float32)
+              for n in ("logprobs", "entropy", "rank")}
+        if k:
+            lp["top_ids"], lp["top_logprobs"] = g.alloc((rows, k), np.int32), g.alloc((rows, k))
+        return lp
+
+    def _logprobs_of(self, logits: DeviceTensor, rows: int, ids: DeviceTensor, lp: dict,
+                     first: int, k: int) -> None:
+        """Rows `first` .. of the buffers lp, from `rows` rows of logits."""
+        at = {n: t.view((rows,) + t.shape[1:], offset_elems=first * (k if t.shape[1:] else 1))
+              for n, t in lp.items()}
+        self.g.token_logprobs(logits, self.cfg.vocab, rows, self.cfg.vocab, ids, top_k=k, **at)
+
+    def _make_room(self, T: int) -> None:
+        """Cuts a bounded cache to kv_keep slots when T more would not fit."""
+        if self.kv_keep is None or self._host_pos + T <= self.kv_slots:
+            return
+        for cache, w, idx in zip(self.kv, self.kv_weights, self.kept):
+            self.g.kv8_evict(cache, w, self.kv_keep, recent=self.kv_recent, sink=self.kv_sink,
+                             idx=idx)
+        self.g.kv8_advance(self.kv[0], limit=self.kv_keep)
+        self._host_pos = self.kv_keep
 
     def _note(self, label: str, nbytes: float, flops: float = 0.0) -> None:
         if self._mark is not None:
@@ -333,12 +406,24 @@ class LlamaDecoder:
                 g.rmsnorm(self.x_a, None, self.h, M, H, eps)
                 self._note("small", 8.0 * M * H)
                 self._linear(self.h, H, L["wqkv"], M, self.qkv)
-            g.rope_kv_append(self.qkv, self.nqkv, self.cos, self.sin, self.state, self.q,
-                             self.kc[li], self.vc[li], **kv)
-            self._note("small", 8.0 * M * self.nqkv)
-            g.attention_kv(self.q, self.kc[li], self.vc[li], self.att, self.state,
-                           scale=float(1.0 / np.sqrt(np.float32(D))), **kv)
-            self._note("attention", 4.0 * (2 * B * sh.nkv * n_keys * D + 2 * M * sh.nq * D),
+            scale = float(1.0 / np.sqrt(np.float32(D)))
+            if self.kv8:
+                g.rope_kv8_append(self.qkv, self.nqkv, self.cos, self.sin, self.pos, self.q,
+                                  self.kv[li], q_len=T, q_heads=sh.nq)
+                self._note("small", 8.0 * M * self.nqkv)
+                gather = {} if self.kv_keep is None else dict(lse=self.lse,
+                                                              weights=self.kv_weights[li])
+                g.attention_kv8(self.q, self.kv[li], self.att, q_len=T, q_heads=sh.nq,
+                                scale=scale, **gather)
+                kv_bytes = 2.0 * B * sh.nkv * n_keys * D
+            else:
+                g.rope_kv_append(self.qkv, self.nqkv, self.cos, self.sin, self.state, self.q,
+                                 self.kc[li], self.vc[li], **kv)
+                self._note("small", 8.0 * M * self.nqkv)
+                g.attention_kv(self.q, self.kc[li], self.vc[li], self.att, self.state,
+                               scale=scale, **kv)
+                kv_bytes = 8.0 * B * sh.nkv * n_keys * D
+            self._note("attention", kv_bytes + 8.0 * M * sh.nq * D,
                        4.0 * B * sh.nq * T * n_keys * D)
             self._row_parallel(self.att, sh.nq * D, L["wo"], M, self.x_a, self.x_b)
             if few:
@@ -376,6 +461,8 @@ class LlamaDecoder:
                                         group=self.group)
             g.argmax_merge(self.packed_all, self.world, B, self.ids)
         g.token_commit(self.ids, self.hist, self.state, B, T, self.n_new, argmax_keys=keys)
+        if self.kv8:
+            g.kv8_advance(self.kv[0], self.pos, q_len=T)
         self._note("small", 4.0 * B * sh.nv)
         self._host_pos += T
 
@@ -387,13 +474,19 @@ class LlamaDecoder:
     def prefill(self) -> None:
         """Resets the position state and runs the prompt block."""
         self.g.zero(self.state)
+        if self.kv8:
+            self.g.zero(self.lens)
+            self.g.zero(self.pos)
         self._host_pos = 0
+        self._step = 0
         self._forward(self.prompt_ids, self.P)
+        self._after_step()
 
     def decode_step(self) -> None:
         """One cached decode step.  With `capture` the step (kernels and, at
         world > 1, its NCCL collectives) is recorded once as a CUDA graph and
         replayed; if recording fails the step runs eagerly from then on."""
+        self._make_room(1)
         if self.capture and not self._captured:
             try:
                 self.g.capture_begin()
@@ -410,6 +503,13 @@ class LlamaDecoder:
             self._host_pos += 1
         else:
             self._forward(self.ids, 1)
+        self._after_step()
+
+    def _after_step(self) -> None:
+        if self.n_top is not None and self._step < self.n_new:
+            self._logprobs_of(self.logits, self.B, self.ids, self.lp, self._step * self.B,
+                              self.n_top)
+        self._step += 1
 
     def run(self) -> None:
         """Prefill + n_new - 1 decode steps, all enqueued on the stream."""
@@ -425,6 +525,47 @@ class LlamaDecoder:
         self.run()
         self.g.sync()
         return self.tokens()
+
+    def token_logprobs(self) -> dict:
+        """Of the generated tokens (decoder made with `logprobs`): logprobs,
+        entropy and rank [B, n_new], top_ids and top_logprobs [B, n_new, k]."""
+        if self.n_top is None:
+            raise ValueError("the decoder was made without logprobs")
+        out = {}
+        for n, t in self.lp.items():
+            a = t.download()
+            out[n] = np.moveaxis(a.reshape((self.n_new, self.B) + a.shape[1:]), 0, 1).copy()
+        return out
+
+    def score(self, prompt: np.ndarray, top_k: int = 0) -> dict:
+        """Of the tokens 1 .. P - 1 of a prompt [B, P], given those before
+        them: logprobs, entropy and rank [B, P - 1], and with top_k top_ids and
+        top_logprobs [B, P - 1, top_k].  Leaves the cache as a prefill does."""
+        if self.world > 1:
+            raise ValueError("score() runs on one rank")
+        if not 0 <= top_k <= min(64, self.cfg.vocab):
+            raise ValueError("top_k: 0..64 alternatives")
+        g, B, P, H, V = self.g, self.B, self.P, self.cfg.hidden, self.cfg.vocab
+        self.upload_prompt(prompt)
+        self.prefill()
+        M = B * P
+        rows = min(M, 256)     # logits of so many positions at a time
+        buf = self._score
+        if not buf:
+            buf.update(logits=g.alloc((rows, V)), ids=g.alloc((M,), np.int32))
+        if top_k not in buf:
+            buf[top_k] = self._logprob_buffers(M, top_k)
+        logits, ids, lp = buf["logits"], buf["ids"], buf[top_k]
+        nxt = np.full((B, P), -1, np.int32)
+        nxt[:, :-1] = prompt[:, 1:]
+        g.upload(ids, nxt.reshape(-1))
+        g.rmsnorm(self.x_a, None, self.h, M, H, self.cfg.eps)
+        for r in range(0, M, rows):
+            n = min(rows, M - r)
+            self._linear(self.h.view((n, H), offset_elems=r * H), H, self.lm_head, n, logits)
+            self._logprobs_of(logits, n, ids.view((n,), offset_elems=r), lp, r, top_k)
+        return {n: t.download().reshape((B, P) + t.shape[1:])[:, :-1].copy()
+                for n, t in lp.items()}
 
     def last_logits(self) -> np.ndarray:
         """Logits of the last step for this rank's vocabulary slice, [B, nv]."""
