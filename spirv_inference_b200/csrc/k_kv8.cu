@@ -13,10 +13,14 @@
 // max|x| below 127 * 2^-126 (s would be subnormal) is held as zero.  A block
 // with a NaN or an infinity gets that as its scale, so all of it reads back
 // as NaN: the fault stays visible.
+#include <cooperative_groups.h>
+
 #include "spx_internal.cuh"
 
 namespace spx {
 namespace {
+
+namespace cg = cooperative_groups;
 
 constexpr float kTinyAmax = 127.0f * 1.17549435e-38f;
 
@@ -62,10 +66,13 @@ __device__ __forceinline__ KvView view_of(const spx_kv8_cache& c, int b, int h, 
 }
 
 // ---------------------------------------------------------------------------
-// Append.  Grid: the first `q_ctas` CTAs rotate the queries (elementwise);
-// each other CTA takes one block of one (sequence, head, K or V): its values
-// into shared memory (rotated where they are keys), the largest magnitude,
-// then the int8 block, or the tail while the block stays open.
+// Append.  Grid: one CTA per new token rotates that token's queries; each
+// other CTA takes one block of one (sequence, head, K or V).  A thread works on
+// four values of a row's lower half and the four of the upper half that RoPE
+// turns with them, and keeps its part of a block in registers between the
+// block's largest magnitude and its rounding.  Bound by the bytes of qkv and q
+// (two 16-byte loads and stores a thread and head); a row that does not start
+// on 16 bytes is read value by value.
 constexpr int kAppendThreads = 256;
 
 struct AppendArgs {
@@ -79,64 +86,108 @@ struct AppendArgs {
   int T, Hq;
   float* q_out;
   spx_kv8_cache c;
-  int blocks;   // blocks that one sequence's new tokens may touch
-  int64_t q_ctas;
+  int blocks;     // blocks that one sequence's new tokens may touch
+  int q_ctas;     // batch * T
+  int vec;        // qkv rows and tables on 16 bytes
 };
 
+// Values i .. i + 3 and half + i .. half + i + 3 of a row.
+struct Pair {
+  float lo[4], hi[4];
+};
+__device__ __forceinline__ Pair load_pair(const float* p, int i, int half, bool vec) {
+  Pair v;
+  if (vec) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p + i));
+    const float4 b = __ldg(reinterpret_cast<const float4*>(p + half + i));
+    v = {{a.x, a.y, a.z, a.w}, {b.x, b.y, b.z, b.w}};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v.lo[e] = __ldg(p + i + e);
+      v.hi[e] = __ldg(p + half + i + e);
+    }
+  }
+  return v;
+}
 // x * cos + rotate_half(x) * sin, each product and the sum rounded once; a
 // position outside the tables gives NaN.
-__device__ __forceinline__ float rotated(const AppendArgs& a, const float* src, int d, int p) {
-  const int D = a.c.head_dim, half = D >> 1;
-  if (p < 0 || p >= a.table_rows) return __int_as_float(0x7fc00000);
-  const float x = src[d];
-  const float o = d < half ? -src[d + half] : src[d - half];
-  return __fadd_rn(__fmul_rn(x, a.cos_t[(int64_t)p * D + d]),
-                   __fmul_rn(o, a.sin_t[(int64_t)p * D + d]));
+struct Turn {
+  Pair c, s;
+};
+__device__ __forceinline__ Turn load_turn(const AppendArgs& a, int p, int i, int half) {
+  Turn t;
+  if (p >= 0 && p < a.table_rows) {
+    t.c = load_pair(a.cos_t + (int64_t)p * 2 * half, i, half, a.vec);
+    t.s = load_pair(a.sin_t + (int64_t)p * 2 * half, i, half, a.vec);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      t.c.lo[e] = t.c.hi[e] = t.s.lo[e] = t.s.hi[e] = __int_as_float(0x7fc00000);
+  }
+  return t;
+}
+__device__ __forceinline__ Pair turned(const Pair& x, const Turn& t) {
+  Pair y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    y.lo[e] = __fadd_rn(__fmul_rn(x.lo[e], t.c.lo[e]), __fmul_rn(-x.hi[e], t.s.lo[e]));
+    y.hi[e] = __fadd_rn(__fmul_rn(x.hi[e], t.c.hi[e]), __fmul_rn(x.lo[e], t.s.hi[e]));
+  }
+  return y;
+}
+__device__ __forceinline__ void store_pair(float* p, int i, int half, const Pair& v) {
+  *reinterpret_cast<float4*>(p + i) = make_float4(v.lo[0], v.lo[1], v.lo[2], v.lo[3]);
+  *reinterpret_cast<float4*>(p + half + i) = make_float4(v.hi[0], v.hi[1], v.hi[2], v.hi[3]);
+}
+__device__ __forceinline__ char4 round4(const float (&x)[4], float s, float inv) {
+  return make_char4((signed char)round_div(x[0], s, inv), (signed char)round_div(x[1], s, inv),
+                    (signed char)round_div(x[2], s, inv), (signed char)round_div(x[3], s, inv));
 }
 
+// IPT: the items (eighths of a row of 64, sixteenths of 128) of a block that a
+// thread holds.
+template <int IPT>
 __global__ void __launch_bounds__(kAppendThreads) rope_kv8_append_kernel(const AppendArgs a) {
-  extern __shared__ float vals[];   // [block][D]
   __shared__ uint32_t warp_max[kAppendThreads / 32];
-  const int D = a.c.head_dim, Hkv = a.c.kv_heads, blk = a.c.block, T = a.T;
-  if ((int64_t)blockIdx.x < a.q_ctas) {
-    const int64_t total = (int64_t)a.c.batch * T * a.Hq * D;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-         i += a.q_ctas * blockDim.x) {
-      const int d = (int)(i % D);
-      const int64_t rh = i / D;
-      const int h = (int)(rh % a.Hq);
-      const int64_t r = rh / a.Hq;
-      const int t = (int)(r % T), b = (int)(r / T);
-      if (a.new_lens && t >= a.new_lens[b]) continue;
-      a.q_out[i] = rotated(a, a.qkv + r * a.ld + (int64_t)h * D, d, a.pos[b] + t);
-    }
+  const int D = a.c.head_dim, half = D >> 1, Hkv = a.c.kv_heads, blk = a.c.block, T = a.T;
+  const int per_row = D >> 3, log_items = 31 - __clz(per_row);
+  if ((int)blockIdx.x < a.q_ctas) {
+    const int b = blockIdx.x / T, tk = blockIdx.x - b * T;
+    if (a.new_lens && tk >= a.new_lens[b]) return;
+    const int i = (threadIdx.x & (per_row - 1)) * 4;   // the same for each of its heads
+    const Turn turn = load_turn(a, a.pos[b] + tk, i, half);
+    const float* src = a.qkv + (int64_t)blockIdx.x * a.ld;
+    float* dst = a.q_out + (int64_t)blockIdx.x * a.Hq * D;
+    for (int h = threadIdx.x >> log_items; h < a.Hq; h += kAppendThreads >> log_items)
+      store_pair(dst + (int64_t)h * D, i, half,
+                 turned(load_pair(src + (int64_t)h * D, i, half, a.vec), turn));
     return;
   }
-  int64_t w = (int64_t)blockIdx.x - a.q_ctas;
-  const int wb = (int)(w % a.blocks);
+  int w = (int)blockIdx.x - a.q_ctas;
+  const int wb = w % a.blocks;
   w /= a.blocks;
   const bool is_v = w & 1;
   w >>= 1;
-  const int h = (int)(w % Hkv), b = (int)(w / Hkv);
+  const int h = w % Hkv, b = w / Hkv;
   const int n = a.new_lens ? clamp_len(a.new_lens[b], T) : T;
   const int len = clamp_len(a.c.lens[b], a.c.max_seq);
   const int total = min(len + n, a.c.max_seq);
-  const int first = len / blk;                 // the block that is open before the call
-  const int blk_i = first + wb;
+  const int blk_i = len / blk + wb;            // from the block that is open before the call
   const int lo = blk_i * blk;
   if (n == 0 || lo >= total) return;
   const KvView kv = view_of(a.c, b, h, is_v);
-  const int64_t col = (int64_t)(a.Hq + (is_v ? Hkv : 0) + h) * D;
+  const float* src = a.qkv + (int64_t)b * T * a.ld + (int64_t)(a.Hq + (is_v ? Hkv : 0) + h) * D;
   const int pos = a.pos[b];
-  auto fresh = [&](int slot, int d) {
-    const int t = slot - len;
-    const float* src = a.qkv + ((int64_t)b * T + t) * a.ld + col;
-    return is_v ? src[d] : rotated(a, src, d, pos + t);
+  auto fresh = [&](int slot, int i) {
+    const int tk = slot - len;
+    const Pair x = load_pair(src + tk * a.ld, i, half, a.vec);
+    return is_v ? x : turned(x, load_turn(a, pos + tk, i, half));
   };
   auto to_tail = [&](int from, int to) {       // new tokens of an open block
-    for (int e = threadIdx.x; e < (to - from) * D; e += blockDim.x) {
-      const int slot = from + e / D, d = e % D;
-      kv.tail[(slot % blk) * D + d] = fresh(slot, d);
+    for (int e = threadIdx.x; e < (to - from) * per_row; e += kAppendThreads) {
+      const int slot = from + (e >> log_items), i = (e & (per_row - 1)) * 4;
+      store_pair(kv.tail + (slot & (blk - 1)) * D, i, half, fresh(slot, i));
     }
   };
   if (lo + blk > total) {
@@ -145,12 +196,24 @@ __global__ void __launch_bounds__(kAppendThreads) rope_kv8_append_kernel(const A
     if (wb == 0) to_tail(max(lo, len), total);
     return;
   }
+  Pair x[IPT];
   uint32_t mx = 0;
-  for (int e = threadIdx.x; e < blk * D; e += blockDim.x) {
-    const int slot = lo + e / D, d = e % D;
-    const float x = slot < len ? kv.tail[e] : fresh(slot, d);
-    vals[e] = x;
-    mx = max(mx, abs_bits(x));
+  const int items = blk * per_row;
+#pragma unroll
+  for (int k = 0; k < IPT; ++k) {
+    const int e = threadIdx.x + k * kAppendThreads;
+    if (e < items) {
+      const int r = e >> log_items, i = (e & (per_row - 1)) * 4, slot = lo + r;
+      if (slot < len) {   // not __ldg: this CTA writes the tail further down
+        const float4 p = *reinterpret_cast<const float4*>(kv.tail + r * D + i);
+        const float4 q = *reinterpret_cast<const float4*>(kv.tail + r * D + half + i);
+        x[k] = {{p.x, p.y, p.z, p.w}, {q.x, q.y, q.z, q.w}};
+      } else {
+        x[k] = fresh(slot, i);
+      }
+#pragma unroll
+      for (int f = 0; f < 4; ++f) mx = max(mx, max(abs_bits(x[k].lo[f]), abs_bits(x[k].hi[f])));
+    }
   }
   mx = __reduce_max_sync(0xffffffffu, mx);
   if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = mx;
@@ -161,14 +224,16 @@ __global__ void __launch_bounds__(kAppendThreads) rope_kv8_append_kernel(const A
   const bool ok = usable(s);
   const float inv = ok ? 1.0f / s : 0.0f;
   if (threadIdx.x == 0) kv.scale[blk_i] = s;
-  char4* out = reinterpret_cast<char4*>(kv.q8 + (int64_t)lo * D);
-  for (int e = threadIdx.x; e < blk * D / 4; e += blockDim.x) {
-    const float4 x = reinterpret_cast<const float4*>(vals)[e];
-    char4 q = make_char4(0, 0, 0, 0);
-    if (ok)
-      q = make_char4((signed char)round_div(x.x, s, inv), (signed char)round_div(x.y, s, inv),
-                     (signed char)round_div(x.z, s, inv), (signed char)round_div(x.w, s, inv));
-    out[e] = q;
+#pragma unroll
+  for (int k = 0; k < IPT; ++k) {
+    const int e = threadIdx.x + k * kAppendThreads;
+    if (e < items) {
+      const int i = (e & (per_row - 1)) * 4;
+      int8_t* out = kv.q8 + (int64_t)(lo + (e >> log_items)) * D;
+      const char4 zero = make_char4(0, 0, 0, 0);
+      *reinterpret_cast<char4*>(out + i) = ok ? round4(x[k].lo, s, inv) : zero;
+      *reinterpret_cast<char4*>(out + half + i) = ok ? round4(x[k].hi, s, inv) : zero;
+    }
   }
   if (wb == 0) {
     const int open = total / blk * blk;
@@ -177,37 +242,42 @@ __global__ void __launch_bounds__(kAppendThreads) rope_kv8_append_kernel(const A
 }
 
 // ---------------------------------------------------------------------------
-// Read-back of `count` slots from starts[b] on, as fp32; 0 behind the end.
-__global__ void kv8_read_kernel(const spx_kv8_cache c, const int32_t* __restrict__ new_lens,
-                                int q_len, const int32_t* __restrict__ starts, int count,
-                                float* __restrict__ k_out, float* __restrict__ v_out) {
-  const int D = c.head_dim, blk = c.block;
-  const int64_t per = (int64_t)c.batch * c.kv_heads * count * (D / 4);
-  const int64_t total = per * 2;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const bool is_v = i >= per;
-    const int64_t e = is_v ? i - per : i;
-    const int d = (int)(e % (D / 4)) * 4;
-    int64_t r = e / (D / 4);
-    const int at = (int)(r % count);
-    r /= count;
-    const int h = (int)(r % c.kv_heads), b = (int)(r / c.kv_heads);
-    const int n = new_lens ? clamp_len(new_lens[b], q_len) : q_len;
-    const int len = min(clamp_len(c.lens[b], c.max_seq) + n, c.max_seq);
-    const int64_t slot = (starts ? (int64_t)starts[b] : 0) + at;
+// Read-back of `count` slots from starts[b] on, as fp32; 0 behind the end.  A
+// CTA per 4096 values of one (sequence, head, K or V).
+constexpr int kReadValues = 4096;
+
+__global__ void __launch_bounds__(256)
+    kv8_read_kernel(const spx_kv8_cache c, const int32_t* __restrict__ new_lens, int q_len,
+                    const int32_t* __restrict__ starts, int count, int chunks,
+                    float* __restrict__ k_out, float* __restrict__ v_out) {
+  const int D = c.head_dim, blk = c.block, shift = 31 - __clz(D);
+  int u = blockIdx.x / chunks;
+  const int chunk = blockIdx.x - u * chunks;
+  const bool is_v = u & 1;
+  u >>= 1;
+  const int b = u / c.kv_heads, h = u - b * c.kv_heads;
+  const int n = new_lens ? clamp_len(new_lens[b], q_len) : q_len;
+  const int len = min(clamp_len(c.lens[b], c.max_seq) + n, c.max_seq);
+  const int closed = len / blk * blk;
+  const int64_t start = starts ? starts[b] : 0;
+  const KvView kv = view_of(c, b, h, is_v);
+  float* out = (is_v ? v_out : k_out) + (int64_t)u * count * D;
+  const int64_t all = (int64_t)count * D;
+#pragma unroll
+  for (int k = 0; k < kReadValues / 1024; ++k) {
+    const int64_t e = (int64_t)chunk * kReadValues + k * 1024 + threadIdx.x * 4;
+    if (e >= all) continue;
+    const int64_t slot = start + (e >> shift);
+    const int d = (int)(e & (D - 1));
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (slot >= 0 && slot < len) {
-      const KvView kv = view_of(c, b, h, is_v);
-      if (slot < len / blk * blk) {
-        const char4 q = *reinterpret_cast<const char4*>(kv.q8 + slot * D + d);
-        const float s = kv.scale[slot / blk];
-        x = make_float4(q.x * s, q.y * s, q.z * s, q.w * s);
-      } else {
-        x = *reinterpret_cast<const float4*>(kv.tail + (slot % blk) * D + d);
-      }
+    if (slot >= 0 && slot < closed) {
+      const char4 q = __ldg(reinterpret_cast<const char4*>(kv.q8 + slot * D + d));
+      const float s = __ldg(kv.scale + slot / blk);
+      x = make_float4(q.x * s, q.y * s, q.z * s, q.w * s);
+    } else if (slot >= 0 && slot < len) {
+      x = __ldg(reinterpret_cast<const float4*>(kv.tail + (slot & (blk - 1)) * D + d));
     }
-    reinterpret_cast<float4*>(is_v ? v_out : k_out)[e] = x;
+    __stcs(reinterpret_cast<float4*>(out + e), x);
   }
 }
 
@@ -323,76 +393,163 @@ __global__ void __launch_bounds__(kSelThreads)
 // Part 2: the kept rows to the front, in order.  A full block of the result
 // takes the largest scale of its members' (a row of the tail has the scale it
 // would have alone) and rounds each value to it once; members with that scale
-// keep their 8 bits.  Slot i of the result comes from a slot >= i, so walking
-// the blocks upwards and reading a block's rows before writing it also works
-// in place.  One CTA per (sequence, head, K or V).
-constexpr int kGatherThreads = 256;
+// keep their 8 bits.  A cluster of CTAs moves one (sequence, head, K or V), in
+// chunks of 256 rows a CTA: all of a chunk into registers, a cluster barrier,
+// then out.  Slot i of the result comes from a slot >= i, so in that order it
+// also works in place, without a second buffer.  Bound by the rows' bytes in
+// and out (64-byte pieces in no order).
+constexpr int kGatherRows = 256;
 
-__global__ void __launch_bounds__(kGatherThreads)
+// The int8 value nearest to q s / ns, halves to even, for |q s| <= 127 ns.
+// ratio + rest = s / ns to 2^-48; a quotient that is no half is at least
+// 2^-32 away from one.
+__device__ __forceinline__ int requant(int q, float ratio, float rest) {
+  const float fq = (float)q, p = fq * ratio;
+  float k = rintf(p);
+  const float e = fmaf(fq, rest, fmaf(fq, ratio, -p));
+  const float dir = p - k + e >= 0.0f ? 1.0f : -1.0f;
+  const float over = dir * ((p - k) - 0.5f * dir) + dir * e;   // past the half, if positive
+  if (over > 0x1p-36f || (over >= -0x1p-36f && ((int)k & 1))) k += dir;
+  return (int)k;
+}
+
+// Four values at once.  The product with the rounded ratio is within 2^-16 of
+// the quotient: away from the halves it rounds as the quotient does.
+__device__ __forceinline__ uint32_t requant4(uint32_t w, float ratio, float rest) {
+  uint32_t r[4];
+  float worst = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    // bytes to fp32: 0x4b000000 | (q + 128) is 2^23 + 128 + q
+    const float q = __uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4b000000u, 0x7550 | i)) -
+                    8388736.0f;
+    const float p = q * ratio, k = p + 12582912.0f;            // 1.5 2^23: rounds to a whole
+    r[i] = __float_as_uint(k);
+    worst = fmaxf(worst, fabsf(p - (k - 12582912.0f)));
+  }
+  if (worst > 0.4999f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = (uint32_t)requant((int8_t)(w >> (8 * i)), ratio, rest);
+  }
+  return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kGatherRows)
     kv8_gather_kernel(const spx_kv8_cache src, const spx_kv8_cache dst, const float* w_src,
-                      float* w_dst, const int32_t* __restrict__ idx, int keep, int in_place) {
-  extern __shared__ float vals[];   // [block][D] values
-  __shared__ float row_scale[128];
-  __shared__ int row_src[128];
-  const int D = src.head_dim, blk = src.block;
-  const int bh = blockIdx.x >> 1, b = bh / src.kv_heads, h = bh % src.kv_heads;
-  const bool is_v = blockIdx.x & 1;
+                      float* w_dst, const int32_t* __restrict__ idx, int keep, int in_place,
+                      int cluster) {
+  constexpr int P = D / 16;                    // 16-byte pieces of a row
+  extern __shared__ __align__(16) float open_rows[];   // [block][D], the open block
+  __shared__ float row_scale[kGatherRows];
+  __shared__ int row_src[kGatherRows];
+  __shared__ uint32_t blk_scale[kGatherRows / 16];
+  const int blk = src.block, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = blockIdx.x % cluster, unit = blockIdx.x / cluster;
+  const int bh = unit >> 1, b = bh / src.kv_heads, h = bh % src.kv_heads;
+  const bool is_v = unit & 1;
   const int n = clamp_len(src.lens[b], src.max_seq);
-  const int kept = min(n, keep);
-  if (in_place && n <= keep) return;
+  const int kept = min(n, keep), full = kept / blk * blk;
+  if (in_place && n <= keep) return;           // the whole cluster
   const KvView s = view_of(src, b, h, is_v), d = view_of(dst, b, h, is_v);
   const int closed = n / blk * blk;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  for (int lo = 0; lo < kept; lo += blk) {
-    const int rows = min(blk, kept - lo);
+  const int32_t* from = idx + (int64_t)bh * keep;
+  for (int base = 0; base < kept; base += cluster * kGatherRows) {
+    const int lo = base + rank * kGatherRows;  // this CTA's rows, whole blocks
+    const int rows = max(0, min(full - lo, kGatherRows));
     float wv = 0.0f;
-    for (int r = warp; r < rows; r += kGatherThreads / 32) {
-      const int j = idx[(int64_t)bh * keep + lo + r];
-      float sc;
-      if (j < closed) {
-        sc = s.scale[j / blk];
-        for (int e = lane; e < D; e += 32) vals[r * D + e] = s.q8[(int64_t)j * D + e] * sc;
-      } else {
-        uint32_t mx = 0;
-        for (int e = lane; e < D; e += 32) {
-          const float x = s.tail[(j % blk) * D + e];
-          vals[r * D + e] = x;
-          mx = max(mx, abs_bits(x));
-        }
-        sc = scale_of(__reduce_max_sync(0xffffffffu, mx));
+    const bool has_w = !is_v && lo + tid < kept;
+    if (tid < kGatherRows / 16) blk_scale[tid] = 0;
+    __syncthreads();
+    int j = 0;
+    bool in_tail = false;
+    if (lo + tid < kept) j = from[lo + tid];
+    if (has_w) wv = w_src[(int64_t)bh * src.max_seq + j];
+    if (tid < rows) {
+      row_src[tid] = j;
+      in_tail = j >= closed;
+      if (!in_tail) {
+        const float sc = s.scale[j / blk];
+        row_scale[tid] = sc;
+        atomicMax(&blk_scale[tid / blk], abs_bits(sc));
       }
+    }
+    for (uint32_t todo = __ballot_sync(0xffffffffu, in_tail); todo; todo &= todo - 1) {
+      const int r = warp * 32 + __ffs(todo) - 1;
+      const int jr = __shfl_sync(0xffffffffu, j, r & 31);
+      uint32_t mx = 0;
+#pragma unroll
+      for (int e = 0; e < D; e += 32)
+        mx = max(mx, abs_bits(s.tail[(jr & (blk - 1)) * D + e + lane]));
+      const float sc = scale_of(__reduce_max_sync(0xffffffffu, mx));
       if (lane == 0) {
         row_scale[r] = sc;
-        row_src[r] = j;
+        atomicMax(&blk_scale[r / blk], abs_bits(sc));
       }
     }
     __syncthreads();
-    if (tid < rows && !is_v) wv = w_src[(int64_t)bh * src.max_seq + row_src[tid]];
-    uint32_t mx = 0;
-    for (int r = 0; r < rows; ++r) mx = max(mx, __float_as_uint(row_scale[r]) & 0x7fffffffu);
-    const float ns = __uint_as_float(mx);
-    __syncthreads();
-    if (tid < rows && !is_v) w_dst[(int64_t)bh * dst.max_seq + lo + tid] = wv;
-    if (rows < blk) {
-      for (int e = tid; e < rows * D; e += blockDim.x) d.tail[e] = vals[e];
-    } else {
-      const bool ok = usable(ns);
-      if (tid == 0) d.scale[lo / blk] = ns;
-      for (int e = tid; e < rows * D; e += blockDim.x) {
-        int q = 0;
-        if (ok) {
-          const int j = row_src[e / D];
-          // exact value of an int8 row: q * scale needs more bits than fp32 has
-          const double x = j < closed ? (double)rint(vals[e] / row_scale[e / D]) * row_scale[e / D]
-                                      : (double)vals[e];
-          const double v = row_scale[e / D] > 0.0f || j >= closed ? x / ns : 0.0;
-          q = (int)rint(fmin(fmax(v, -127.0), 127.0));
+    uint4 out[P];
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      const int e = tid + k * kGatherRows, r = e / P, at = (e % P) * 16;
+      out[k] = make_uint4(0, 0, 0, 0);
+      if (r < rows && row_src[r] < closed)
+        out[k] = *reinterpret_cast<const uint4*>(s.q8 + (int64_t)row_src[r] * D + at);
+    }
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      const int e = tid + k * kGatherRows, r = e / P, at = (e % P) * 16;
+      if (r >= rows) continue;
+      const float ns = __uint_as_float(blk_scale[r / blk]), sc = row_scale[r];
+      uint32_t* o = reinterpret_cast<uint32_t*>(&out[k]);
+      if (!usable(ns)) {
+        out[k] = make_uint4(0, 0, 0, 0);
+      } else if (row_src[r] >= closed) {
+        const float* x = s.tail + (row_src[r] & (blk - 1)) * D + at;
+        const float inv = 1.0f / ns;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 v = *reinterpret_cast<const float4*>(x + 4 * i);
+          const char4 q = make_char4(
+              (signed char)round_div(v.x, ns, inv), (signed char)round_div(v.y, ns, inv),
+              (signed char)round_div(v.z, ns, inv), (signed char)round_div(v.w, ns, inv));
+          o[i] = *reinterpret_cast<const uint32_t*>(&q);
         }
-        d.q8[(int64_t)lo * D + e] = (int8_t)q;
+      } else if (sc != ns) {
+        // (far from subnormal remainders)
+        const float up = ns < 0x1p-60f ? 0x1p64f : 1.0f, sn = sc * up, nn = ns * up;
+        const float ratio = sn / nn, rest = fmaf(-ratio, nn, sn) / nn;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = requant4(o[i], ratio, rest);
       }
+    }
+    if (in_place) {
+      if (cluster > 1)
+        cg::this_cluster().sync();
+      else
+        __syncthreads();
+    }
+    if (has_w) w_dst[(int64_t)bh * dst.max_seq + lo + tid] = wv;
+    if (tid < rows && tid % blk == 0)
+      d.scale[(lo + tid) / blk] = __uint_as_float(blk_scale[tid / blk]);
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      const int e = tid + k * kGatherRows;
+      if (e / P < rows)
+        *reinterpret_cast<uint4*>(d.q8 + (int64_t)lo * D + (int64_t)e * 16) = out[k];
     }
     __syncthreads();
   }
+  // The open block, by one CTA: every row that others take from the tail has
+  // been read by now.
+  if (rank != 0 || full == kept) return;
+  for (int e = tid; e < (kept - full) * D; e += kGatherRows) {
+    const int j = from[full + e / D], x = e % D;
+    open_rows[e] = j < closed ? s.q8[(int64_t)j * D + x] * s.scale[j / blk]
+                              : s.tail[(j & (blk - 1)) * D + x];
+  }
+  __syncthreads();
+  for (int e = tid; e < (kept - full) * D; e += kGatherRows) d.tail[e] = open_rows[e];
 }
 
 __global__ void kv8_advance_kernel(int32_t* lens, int32_t* pos, const int32_t* new_lens, int batch,
@@ -436,6 +593,8 @@ int launch_rope_kv8_append(cudaStream_t s, int64_t* cnt, const float* qkv, int64
   if (T <= 0 || Hq <= 0 || table_rows <= 0 ||
       ld_qkv < (int64_t)(Hq + 2 * c->kv_heads) * c->head_dim)
     return fail(SPX_ERR_INVALID_ARGUMENT, "rope_kv8_append: bad shape");
+  if (!al16(q_out))
+    return fail(SPX_ERR_INVALID_ARGUMENT, "rope_kv8_append: q_out must be 16-byte aligned");
   AppendArgs a;
   a.qkv = qkv;
   a.ld = ld_qkv;
@@ -449,17 +608,20 @@ int launch_rope_kv8_append(cudaStream_t s, int64_t* cnt, const float* qkv, int64
   a.q_out = q_out;
   a.c = *c;
   a.blocks = (T + 2 * c->block - 2) / c->block;   // the open block and what follows
-  a.q_ctas = grid_for((int64_t)c->batch * T * Hq * c->head_dim, kAppendThreads);
-  const int64_t grid = a.q_ctas + (int64_t)c->batch * c->kv_heads * 2 * a.blocks;
+  const int64_t q_ctas = (int64_t)c->batch * T;
+  const int64_t grid = q_ctas + (int64_t)c->batch * c->kv_heads * 2 * a.blocks;
   if (grid > INT32_MAX) return fail(SPX_ERR_UNSUPPORTED, "rope_kv8_append: grid too large");
-  const size_t smem = (size_t)c->block * c->head_dim * sizeof(float);
-  if (smem > 48 * 1024) {
-    rc = check_cuda(cudaFuncSetAttribute(rope_kv8_append_kernel,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
-                    "rope_kv8_append: smem attribute");
-    if (rc) return rc;
-  }
-  rope_kv8_append_kernel<<<(int)grid, kAppendThreads, smem, s>>>(a);
+  a.q_ctas = (int)q_ctas;
+  a.vec = al16(qkv) && ld_qkv % 4 == 0 && al16(cos_t) && al16(sin_t);
+  const int items = c->block * c->head_dim / 8;
+  if (items <= kAppendThreads)
+    rope_kv8_append_kernel<1><<<(int)grid, kAppendThreads, 0, s>>>(a);
+  else if (items == 2 * kAppendThreads)
+    rope_kv8_append_kernel<2><<<(int)grid, kAppendThreads, 0, s>>>(a);
+  else if (items == 4 * kAppendThreads)
+    rope_kv8_append_kernel<4><<<(int)grid, kAppendThreads, 0, s>>>(a);
+  else
+    rope_kv8_append_kernel<8><<<(int)grid, kAppendThreads, 0, s>>>(a);
   return after_launch(cnt, "rope_kv8_append");
 }
 
@@ -470,9 +632,11 @@ int launch_kv8_read(cudaStream_t s, int64_t* cnt, const spx_kv8_cache* c, const 
   if (q_len < 0 || count <= 0) return fail(SPX_ERR_INVALID_ARGUMENT, "kv8_read: bad shape");
   if (!al16(k_out) || !al16(v_out))
     return fail(SPX_ERR_INVALID_ARGUMENT, "kv8_read: outputs must be 16-byte aligned");
-  const int64_t work = (int64_t)c->batch * c->kv_heads * count * (c->head_dim / 4) * 2;
-  kv8_read_kernel<<<grid_for(work, 256, 16), 256, 0, s>>>(*c, new_lens, q_len, starts, count, k_out,
-                                                          v_out);
+  const int64_t chunks = ceil_div((int64_t)count * c->head_dim, kReadValues);
+  const int64_t grid = (int64_t)c->batch * c->kv_heads * 2 * chunks;
+  if (grid > INT32_MAX) return fail(SPX_ERR_UNSUPPORTED, "kv8_read: grid too large");
+  kv8_read_kernel<<<(int)grid, 256, 0, s>>>(*c, new_lens, q_len, starts, count, (int)chunks, k_out,
+                                            v_out);
   return after_launch(cnt, "kv8_read");
 }
 
@@ -516,16 +680,34 @@ int launch_kv8_evict(cudaStream_t s, int64_t* cnt, const spx_kv8_cache* src, con
   kv8_select_kernel<<<(int)bh, kSelThreads, 0, s>>>(weights, src->lens, src->kv_heads,
                                                     src->max_seq, keep, recent, sink, idx);
   if ((rc = after_launch(cnt, "kv8_evict: select"))) return rc;
+  // CTAs enough to take all kept rows at once, a portable cluster at most.
+  int cluster = 1;
+  while (cluster < 8 && cluster * kGatherRows < keep) cluster *= 2;
+  if (2 * bh * cluster > INT32_MAX) return fail(SPX_ERR_UNSUPPORTED, "kv8_evict: grid too large");
   const size_t smem = (size_t)src->block * src->head_dim * sizeof(float);
+  auto kern = src->head_dim == 64 ? kv8_gather_kernel<64> : kv8_gather_kernel<128>;
   if (smem > 40 * 1024) {
-    rc = check_cuda(cudaFuncSetAttribute(kv8_gather_kernel,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+    rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)smem),
                     "kv8_evict: smem attribute");
     if (rc) return rc;
   }
-  kv8_gather_kernel<<<(int)(2 * bh), kGatherThreads, smem, s>>>(*src, *dst, weights, dst_weights,
-                                                                idx, keep, same ? 1 : 0);
-  return after_launch(cnt, "kv8_evict: gather");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * bh * cluster));
+  cfg.blockDim = dim3(kGatherRows);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  rc = check_cuda(cudaLaunchKernelEx(&cfg, kern, *src, *dst, weights, dst_weights, (const int32_t*)idx,
+                                     keep, same ? 1 : 0, cluster),
+                  "kv8_evict: gather");
+  return rc ? rc : after_launch(cnt, "kv8_evict: gather");
 }
 
 int launch_kv8_advance(cudaStream_t s, int64_t* cnt, int32_t* lens, int32_t* pos,
