@@ -5,16 +5,23 @@
 //   entropy = log l - sum e^(x - m) (x - m) / l
 //   rank = 1 + #{x_j > x_id},  ties among the top k go to the lowest index
 //
-// One pass over the logits.  A cluster of CTAs shares a row (one CTA when
-// there are rows enough); a CTA walks its part in tiles of 4096 values, 16 a
-// thread, in registers.  Maximum, sum and sum e^(x-m) (x-m) run per thread and
-// are joined at the end.  For the top k a CTA keeps a list of candidates in
-// shared memory: of its first tile each warp takes the k-th largest of its
-// lanes' maxima (so k values are at least that), the largest of these over
-// the warps is the threshold, and only values that reach it enter the list,
-// about a dozen of 4096; the list is cut to its k best when it grows.  A tile
-// that would overflow it (rising logits, ties) takes its k best one by one.
-// Bound by the logits' bytes.
+// One pass over the logits.  With rows enough for every SM a warp takes a row;
+// else the eight warps of a CTA, and with few rows a cluster of CTAs, share
+// one.  A warp walks tiles of 512 values, 16 a lane, which each lane copies to
+// shared memory for itself two tiles ahead (32 KB a CTA in flight, four CTAs an
+// SM, no barrier).  Maximum, sum and sum e^(x-m) (x-m) run per lane.
+//
+// For the top k a warp keeps a list of candidates in shared memory: the k-th
+// largest of its lanes' maxima in its first tile is a threshold that k values
+// reach, and only values that reach it enter the list; when the list grows it
+// is cut to its k best, and values then have to exceed the last of them.  A
+// tile that would overflow it (rising logits, ties) gives its k best one by
+// one.  Warps' and CTAs' lists are merged by binary searches.
+//
+// Bound by the logits' bytes; instructions come next (a maximum, a difference,
+// a product, ex2 and two sums a value), so pairs of values go through the
+// packed fp32 operations, and the rank is counted only in lanes whose maximum
+// exceeds the token's logit.
 #include <cooperative_groups.h>
 
 #include "spx_internal.cuh"
@@ -24,12 +31,16 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kLpThreads = 256;
-constexpr int kLpWarps = kLpThreads / 32;
-constexpr int kLpQuads = 4;                              // float4 a thread and tile
-constexpr int kLpTile = kLpThreads * kLpQuads * 4;
-constexpr int kLpCap = 512;                              // candidates
+constexpr int kLpWarps = 8;
+constexpr int kLpPerSm = 4;                    // CTAs an SM
+constexpr int kLpQuads = 4;                    // float4 a lane and tile
+constexpr int kLpTile = 32 * kLpQuads * 4;
+constexpr int kLpSlots = 2;                    // tiles of a warp in flight
+constexpr int kLpCap = 120;                    // candidates of a warp
+constexpr size_t kLpRing = sizeof(float) * kLpWarps * kLpSlots * kLpTile;
 constexpr int kLpMaxTop = 64;
+constexpr int kLpMaxCluster = 8;               // (merge_lists takes eight lists)
+static_assert(kLpWarps == 8 && kLpMaxCluster == 8 && kLpQuads == 4, "lists and maxima a lane");
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Order-preserving bits; NaN below everything, -0 equal to +0.
@@ -48,10 +59,17 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 struct LpArgs {
   const float* x;
   int64_t ld;
-  int cols;
+  int rows, cols;
   const int32_t* ids;
   float* logprobs;
   float* entropy;
@@ -74,226 +92,406 @@ struct Stats {          // of some values: maximum, sum e^(x-m), sum e^(x-m) (x-
     l *= f;
     m = to;
   }
-  __device__ __forceinline__ void join(Stats o) {
-    const float to = fmaxf(m, o.m);
-    rebase(to);
-    o.rebase(to);
-    l += o.l;
-    t += o.t;
-    above += o.above;
+  // Of the warp's lanes together, to all of them.
+  __device__ __forceinline__ void join_lanes() {
+    const uint32_t u = __float_as_uint(m);
+    const uint32_t key = __reduce_max_sync(0xffffffffu, u & 0x80000000u ? ~u : u | 0x80000000u);
+    rebase(__uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key));
+    above = __reduce_add_sync(0xffffffffu, above);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      l += __shfl_xor_sync(0xffffffffu, l, o);
+      t += __shfl_xor_sync(0xffffffffu, t, o);
+    }
   }
 };
 
-// The k best of n <= kLpCap distinct keys, in falling order, to the front.
-__device__ __forceinline__ void keep_best(unsigned long long* list, int n, int k) {
-  unsigned long long key[kLpCap / kLpThreads];
-  int at[kLpCap / kLpThreads];
-#pragma unroll
-  for (int i = 0; i < kLpCap / kLpThreads; ++i) {
-    const int e = threadIdx.x + i * kLpThreads;
-    at[i] = k;
-    if (e < n) {
-      key[i] = list[e];
-      int larger = 0;
-      for (int j = 0; j < n; ++j) larger += list[j] > key[i];
-      at[i] = larger;
-    }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kLpCap / kLpThreads; ++i)
-    if (at[i] < k) list[at[i]] = key[i];
-  __syncthreads();
+// Two fp32 operations in one instruction, each rounded as the single one is.
+__device__ __forceinline__ unsigned long long f2_bits(float2 v) {
+  return *reinterpret_cast<unsigned long long*>(&v);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(f2_bits(a)), "l"(f2_bits(b)), "l"(f2_bits(c)));
+  return *reinterpret_cast<float2*>(&d);
 }
 
-__global__ void __launch_bounds__(kLpThreads, 4)
-    token_logprobs_kernel(const LpArgs a, int cluster, int seg) {
-  __shared__ unsigned long long list[kLpCap];
-  __shared__ unsigned long long warp_best[kLpWarps];
-  __shared__ uint32_t warp_thr[kLpWarps];
-  __shared__ Stats warp_stats[kLpWarps];
-  __shared__ Stats cta_stats;
-  __shared__ int count[3], cta_count;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int r = blockIdx.x / cluster, rank = blockIdx.x - r * cluster;
-  const float* x = a.x + (int64_t)r * a.ld;
-  // Positions count from the 16-byte boundary at or before the row's start.
-  const int shift = (int)(((uintptr_t)x >> 2) & 3);
-  const int v0 = rank * seg, v1 = min(v0 + seg, a.cols + shift);
-  const int id = a.ids ? a.ids[r] : -1;
-  const bool has = id >= 0 && id < a.cols;
-  const float one = has ? __ldg(x + id) : 0.0f;
-  const int k = a.top_k;
-  if (tid == 0) count[0] = 0;
-  Stats st = {-INFINITY, 0.0f, 0.0f, 0};
-  uint32_t thr = 0;                  // the key that a candidate has to reach
-  int held = 0, slot = 0;            // candidates before this tile; its counter
-  for (int base = v0; base < v1; base += kLpTile) {
-    float v[kLpQuads * 4];
-    uint32_t in = 0;                 // which of them are values of the row
+// The k best of a warp's n <= kLpCap distinct keys, in falling order, to the
+// front of the list.
+__device__ __forceinline__ void keep_best(unsigned long long* list, int n, int k, int lane) {
+  unsigned long long key[4];
+  int at[4];
 #pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int e = lane + 32 * i;
+    key[i] = e < n ? list[e] : 0ull;
+    at[i] = e < n ? 0 : k;
+    if (32 * i < n) {
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) at[i] += list[j] > key[i];
+    }
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (at[i] < k) list[at[i]] = key[i];
+  __syncwarp();
+}
+
+// The k best of eight lists in falling order (counts[i] <= k keys, at lists +
+// i * stride), to `out`; of the CTA.  A key's place is its own plus the number
+// of larger keys in the seven others, by seven binary searches side by side.
+__device__ __forceinline__ void merge_lists(const unsigned long long* lists, int stride,
+                                            const int* counts, int k, unsigned long long* out,
+                                            int warp, int lane) {
+  const int first_step = 1 << (31 - __clz(k));
+  for (int i = lane; i < counts[warp]; i += 32) {
+    const unsigned long long key = lists[warp * stride + i];
+    int pos[kLpWarps] = {};
+#pragma unroll 1
+    for (int s = first_step; s > 0; s >>= 1) {
+#pragma unroll
+      for (int w = 0; w < kLpWarps; ++w)
+        if (pos[w] + s <= counts[w] && lists[w * stride + pos[w] + s - 1] > key) pos[w] += s;
+    }
+    int at = 0;
+#pragma unroll
+    for (int w = 0; w < kLpWarps; ++w) at += w == warp ? i : pos[w];
+    if (at < k) out[at] = key;
+  }
+}
+
+// The largest value that k >= 1 of 32 lanes' keys reach.
+__device__ __forceinline__ uint32_t kth_largest(uint32_t x, int k, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1)       // bitonic, falling
+#pragma unroll
+    for (int d = size >> 1; d > 0; d >>= 1) {
+      const uint32_t y = __shfl_xor_sync(0xffffffffu, x, d);
+      const bool low = !(lane & d), falls = !(lane & size) || size == 32;
+      x = low == falls ? max(x, y) : min(x, y);
+    }
+  return __shfl_sync(0xffffffffu, x, k - 1);
+}
+
+__device__ __forceinline__ unsigned long long packed(float v, uint32_t j) {
+  return ((unsigned long long)order_key(v) << 32) | (0xffffffffu - j);
+}
+
+__device__ __forceinline__ void copy_async(void* to, const float* from, bool quad) {
+  const uint32_t s = (uint32_t)__cvta_generic_to_shared(to);
+  if (quad)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(from) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s), "l"(from) : "memory");
+}
+
+// Starts the copies of a tile (positions base ..) into the lane's places of a
+// slot.  Positions outside [shift, v1) are not read.
+__device__ __forceinline__ void start_tile(float4* slot, const float* x, int base, int shift,
+                                           int v1, int lane) {
+  if (base >= shift && base + kLpTile <= v1) {
+    const float* from = x + (base - shift) + lane * 4;
+#pragma unroll
+    for (int q = 0; q < kLpQuads; ++q) copy_async(slot + q * 32 + lane, from + q * 128, true);
+  } else if (base < v1) {
     for (int q = 0; q < kLpQuads; ++q) {
-      const int p = base + (q * kLpThreads + tid) * 4;
+      const int p = base + (q * 32 + lane) * 4;
+      float* to = reinterpret_cast<float*>(slot + q * 32 + lane);
       if (p >= shift && p + 4 <= v1) {
-        const float4 f = __ldg(reinterpret_cast<const float4*>(x + (p - shift)));
-        v[4 * q] = f.x;
-        v[4 * q + 1] = f.y;
-        v[4 * q + 2] = f.z;
-        v[4 * q + 3] = f.w;
-        in |= 15u << (4 * q);
+        copy_async(to, x + (p - shift), true);
       } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool ok = p + e >= shift && p + e < v1;
-          v[4 * q + e] = ok ? __ldg(x + (p + e - shift)) : -INFINITY;
-          in |= (ok ? 1u : 0u) << (4 * q + e);
-        }
+        for (int e = 0; e < 4; ++e)
+          if (p + e >= shift && p + e < v1) copy_async(to + e, x + (p + e - shift), false);
       }
     }
-    // What lies outside is -inf and adds nothing to the sums or the rank.
-    float mt = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < kLpQuads * 4; ++i) mt = fmaxf(mt, v[i]);
-    const float to = fmaxf(st.m, mt);
-    st.rebase(to);
-    const float zero = to == -INFINITY ? 0.0f : to;
-#pragma unroll
-    for (int i = 0; i < kLpQuads * 4; ++i) {
-      const float d = v[i] - zero, e = ex2(d * kLog2e);
-      st.l += e;
-      st.t = fmaf(e, fmaxf(d, -3.4e38f), st.t);
-      st.above += v[i] > one;
-    }
-    if (k == 0) continue;
-    uint32_t best = in ? order_key(mt) : 0u;
-    if (st.l != st.l) {              // a NaN may be all that a thread has
-      best = 0u;
-#pragma unroll
-      for (int i = 0; i < kLpQuads * 4; ++i)
-        if (in >> i & 1u) best = max(best, order_key(v[i]));
-    }
-    if (base == v0) {
-      // k2 lanes of each of one warp, or of two, reach the threshold.
-      const int k2 = k > 32 ? (k + 1) / 2 : k;
-      uint32_t left = best, kth = 0;
-      for (int i = 0; i < k2; ++i) {
-        kth = __reduce_max_sync(0xffffffffu, left);
-        const uint32_t who = __ballot_sync(0xffffffffu, left == kth);
-        if (lane == __ffs(who) - 1) left = 0;
-      }
-      if (lane == 0) warp_thr[warp] = kth;
-      __syncthreads();
-      if (k > 32) {
-        for (int w = 0; w < kLpWarps; w += 2) thr = max(thr, min(warp_thr[w], warp_thr[w + 1]));
-      } else {
-        for (int w = 0; w < kLpWarps; ++w) thr = max(thr, warp_thr[w]);
-      }
-    }
-    if (in && best >= thr) {
-#pragma unroll
-      for (int i = 0; i < kLpQuads * 4; ++i) {
-        const uint32_t key = order_key(v[i]);
-        if (key >= thr && (in >> i & 1u)) {
-          const int at = held + atomicAdd(&count[slot], 1);
-          const uint32_t j = base + ((i >> 2) * kLpThreads + tid) * 4 + (i & 3) - shift;
-          if (at < kLpCap) list[at] = ((unsigned long long)key << 32) | (0xffffffffu - j);
-        }
-      }
-    }
-    // Three counters in turn: this tile's, the next one's, which nobody reads
-    // any more, and the last one's, which slower threads may still read.
-    if (tid == 0) count[slot == 2 ? 0 : slot + 1] = 0;
-    __syncthreads();
-    int n = held + count[slot];
-    slot = slot == 2 ? 0 : slot + 1;
-    if (n > kLpCap) {
-      // Too many: the tile's k best, each the largest below the one before.
-      unsigned long long below = ~0ull;
-      for (int i = 0; i < k; ++i) {
-        unsigned long long b = 0;
-#pragma unroll
-        for (int e = 0; e < kLpQuads * 4; ++e) {
-          const uint32_t j = base + ((e >> 2) * kLpThreads + tid) * 4 + (e & 3) - shift;
-          const unsigned long long key =
-              ((unsigned long long)order_key(v[e]) << 32) | (0xffffffffu - j);
-          if ((in >> e & 1u) && key < below && key > b) b = key;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          const unsigned long long other = __shfl_xor_sync(0xffffffffu, b, o);
-          b = other > b ? other : b;
-        }
-        if (lane == 0) warp_best[warp] = b;
-        __syncthreads();
-        for (int w = 0; w < kLpWarps; ++w) b = warp_best[w] > b ? warp_best[w] : b;
-        below = b;
-        if (tid == 0) list[held + i] = b;   // 0 where the tile has no more
-        __syncthreads();
-      }
-      n = held + k;
-    }
-    if (n > kLpCap / 2) {
-      keep_best(list, n, k);
-      n = k;
-      thr = max(thr, (uint32_t)(list[k - 1] >> 32));
-    }
-    held = n;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stats s;
-    s.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-    s.l = __shfl_xor_sync(0xffffffffu, st.l, o);
-    s.t = __shfl_xor_sync(0xffffffffu, st.t, o);
-    s.above = __shfl_xor_sync(0xffffffffu, st.above, o);
-    st.join(s);
-  }
-  if (lane == 0) warp_stats[warp] = st;
-  __syncthreads();
-  if (cluster > 1) {
-    if (k && held > k) {
-      keep_best(list, held, k);
-      held = k;
-    }
-    if (tid == 0) {
-      for (int w = 1; w < kLpWarps; ++w) st.join(warp_stats[w]);
-      cta_stats = st;
-      cta_count = held;
-    }
-    cg::cluster_group cl = cg::this_cluster();
-    cl.sync();
-    if (rank == 0) {
-      for (int c = 1; c < cluster; ++c) {
-        const int n = *cl.map_shared_rank(&cta_count, c);
-        const unsigned long long* theirs = cl.map_shared_rank(&list[0], c);
-        for (int i = tid; i < n; i += kLpThreads) list[held + i] = theirs[i];
-        held += n;
-        if (tid == 0) st.join(*cl.map_shared_rank(&cta_stats, c));
-      }
-      __syncthreads();
-    }
-    cl.sync();
-    if (rank != 0) return;
-  } else if (tid == 0) {
-    for (int w = 1; w < kLpWarps; ++w) st.join(warp_stats[w]);
-  }
-  if (tid == 0) cta_stats = st;
-  __syncthreads();
-  if (k) keep_best(list, held, k);
-  st = cta_stats;
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
+// A row's results, by `threads` threads of which this is number `me`.
+__device__ __forceinline__ void emit(const LpArgs& a, int r, const Stats& st,
+                                     const unsigned long long* top, int me, int threads, float one,
+                                     int id, bool has) {
   const bool empty = st.m == -INFINITY && st.l == 0.0f;   // every token is masked
   const float log_l = empty ? 0.0f : logf(st.l);
   auto logp = [&](float v) { return empty ? -INFINITY : (v - st.m) - log_l; };
-  if (tid == 0) {
+  if (me == 0) {
     if (a.logprobs)
       a.logprobs[r] = has ? logp(one) : id < 0 ? 0.0f : __int_as_float(0x7fc00000);
     if (a.entropy) a.entropy[r] = empty ? 0.0f : log_l - st.t / st.l;
     if (a.rank) a.rank[r] = has ? st.above + 1 : 0;
   }
-  if (tid < k) {
-    const unsigned long long b = list[tid];
-    a.top_ids[(int64_t)r * k + tid] = (int32_t)(0xffffffffu - (uint32_t)b);
-    a.top_logprobs[(int64_t)r * k + tid] = logp(key_value((uint32_t)(b >> 32)));
+  for (int i = me; i < a.top_k; i += threads) {
+    const unsigned long long b = top[i];
+    a.top_ids[(int64_t)r * a.top_k + i] = (int32_t)(0xffffffffu - (uint32_t)b);
+    a.top_logprobs[(int64_t)r * a.top_k + i] = logp(key_value((uint32_t)(b >> 32)));
+  }
+}
+
+template <bool ROW_PER_WARP>
+__global__ void __launch_bounds__(kLpWarps * 32, kLpPerSm)
+    token_logprobs_kernel(const LpArgs a, int cluster, int seg) {
+  __shared__ unsigned long long lists[kLpWarps][kLpCap];
+  __shared__ unsigned long long joined[ROW_PER_WARP ? 1 : kLpMaxTop];
+  __shared__ unsigned long long theirs[ROW_PER_WARP ? 1 : kLpMaxCluster][kLpMaxTop];
+  __shared__ Stats parts[kLpWarps], cta_parts[kLpMaxCluster];
+  __shared__ int counts[kLpWarps], cta_counts[kLpMaxCluster];
+  extern __shared__ float4 ring_all[];         // [warp][slot][quad][lane]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  float4* ring = ring_all + warp * (kLpSlots * kLpQuads * 32);
+  const int warps = blockDim.x >> 5;           // kLpWarps unless a warp has a row
+  int r = ROW_PER_WARP ? warp * gridDim.x + blockIdx.x : blockIdx.x / cluster;
+  const int rank = ROW_PER_WARP ? 0 : blockIdx.x - r * cluster;
+  if (ROW_PER_WARP && r >= a.rows) return;
+  cg::cluster_group cl = cg::this_cluster();
+  if (!ROW_PER_WARP && cluster > 1) cluster_arrive();
+  constexpr int kStep = ROW_PER_WARP ? kLpTile : kLpWarps * kLpTile;
+  const int k = a.top_k;
+  unsigned long long* list = lists[warp];
+  // The row: positions count from the 16-byte boundary at or before its start.
+  const float* x;
+  int shift, v1, base, id;
+  float one;
+  bool has;
+  auto take_row = [&]() {
+    x = a.x + (int64_t)r * a.ld;
+    shift = (int)(((uintptr_t)x >> 2) & 3);
+    v1 = min(rank * seg + seg, a.cols + shift);
+    base = rank * seg + (ROW_PER_WARP ? 0 : warp * kLpTile);
+    for (int s = 0; s < kLpSlots; ++s)
+      start_tile(ring + s * (kLpQuads * 32), x, base + s * kStep, shift, v1, lane);
+    id = a.ids ? a.ids[r] : -1;
+    has = id >= 0 && id < a.cols;
+    one = has ? __ldg(x + id) : 0.0f;
+  };
+  take_row();
+  for (;;) {                         // one row, or a warp's rows
+    Stats st = {-INFINITY, 0.0f, 0.0f, 0};
+    float thr = -INFINITY;             // what a candidate has to reach
+    int held = 0;
+    bool first = true;
+    float2 l2 = make_float2(0.f, 0.f), t2 = make_float2(0.f, 0.f);
+    int slot = 0;
+    for (; base < v1; base += kStep) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kLpSlots - 1) : "memory");
+      float4* here = ring + slot * (kLpQuads * 32);
+      slot = slot == kLpSlots - 1 ? 0 : slot + 1;
+      float v[kLpQuads * 4];
+#pragma unroll
+      for (int q = 0; q < kLpQuads; ++q) {
+        const float4 f = here[q * 32 + lane];   // the lane's own copies
+        v[4 * q] = f.x;
+        v[4 * q + 1] = f.y;
+        v[4 * q + 2] = f.z;
+        v[4 * q + 3] = f.w;
+      }
+      // Bit i: v[i] is a value of the row.  What lies outside is -inf and adds
+      // nothing to the sums or the rank.
+      uint32_t in = 0xffffffffu >> (32 - kLpQuads * 4);
+      if (base < shift || base + kLpTile > v1) {
+#pragma unroll
+        for (int i = 0; i < kLpQuads * 4; ++i) {
+          const int p = base + ((i >> 2) * 32 + lane) * 4 + (i & 3);
+          if (p < shift || p >= v1) {
+            v[i] = -INFINITY;
+            in &= ~(1u << i);
+          }
+        }
+      }
+      float top[kLpQuads];
+#pragma unroll
+      for (int q = 0; q < kLpQuads; ++q)
+        top[q] = fmaxf(fmaxf(v[4 * q], v[4 * q + 1]), fmaxf(v[4 * q + 2], v[4 * q + 3]));
+      float mt = top[0];
+#pragma unroll
+      for (int q = 1; q < kLpQuads; ++q) mt = fmaxf(mt, top[q]);
+      if (mt > st.m) {
+        if (st.m != -INFINITY) {
+          const float d = st.m - mt, f = ex2(d * kLog2e);
+          const float2 f2 = make_float2(f, f);
+          t2 = f == 0.0f ? make_float2(0.f, 0.f) : mul2(fma2(l2, make_float2(d, d), t2), f2);
+          l2 = mul2(l2, f2);
+        }
+        st.m = mt;
+      }
+      const float zero = st.m == -INFINITY ? 0.0f : -st.m;
+#pragma unroll
+      for (int i = 0; i < kLpQuads * 2; ++i) {
+        float2 d = add2(make_float2(v[2 * i], v[2 * i + 1]), make_float2(zero, zero));
+        const float2 p = mul2(d, make_float2(kLog2e, kLog2e));
+        const float2 e = make_float2(ex2(p.x), ex2(p.y));
+        l2 = add2(l2, e);
+        d = make_float2(fmaxf(d.x, -3.4e38f), fmaxf(d.y, -3.4e38f));   // 0 * -inf
+        t2 = fma2(e, d, t2);
+      }
+      if (mt > one) {
+#pragma unroll
+        for (int i = 0; i < kLpQuads * 4; ++i) st.above += v[i] > one;
+      }
+      const bool nan = l2.x != l2.x || l2.y != l2.y;   // a NaN may be all that a lane has
+      if (k) {
+        if (first) {
+          // Two maxima of eight values a lane; k values reach the k-th of 32
+          // lanes' larger ones, or half of k of each kind the lower half-k-th.
+          uint32_t best[2];
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            best[q] = in >> (8 * q) & 255u ? order_key(fmaxf(top[2 * q], top[2 * q + 1])) : 0u;
+            if (nan) {               // a NaN may be all that there is
+              best[q] = 0u;
+#pragma unroll
+              for (int i = 8 * q; i < 8 * q + 8; ++i)
+                if (in >> i & 1u) best[q] = max(best[q], order_key(v[i]));
+            }
+          }
+          uint32_t kth;
+          if (k <= 32)
+            kth = kth_largest(max(best[0], best[1]), k, lane);
+          else
+            kth = min(kth_largest(best[0], (k + 1) / 2, lane),
+                      kth_largest(best[1], (k + 1) / 2, lane));
+          // (below -inf there is NaN only)
+          thr = kth > 0x007fffffu ? key_value(kth) : -INFINITY;
+          first = false;
+        }
+        // (a NaN is not below the threshold, and is sorted out by its key)
+        int n = held;
+        if (__any_sync(0xffffffffu, !(mt < thr) || nan)) {
+#pragma unroll
+          for (int q = 0; q < kLpQuads; ++q)
+            if (__any_sync(0xffffffffu, !(top[q] < thr) || nan)) {
+#pragma unroll
+              for (int i = 4 * q; i < 4 * q + 4; ++i) {
+                const bool hit = !(v[i] < thr) && (in >> i & 1u);
+                const uint32_t who = __ballot_sync(0xffffffffu, hit);
+                const int at = n + __popc(who & ((1u << lane) - 1u));
+                if (hit && at < kLpCap)
+                  list[at] = packed(v[i], base + (q * 32 + lane) * 4 + (i & 3) - shift);
+                n += __popc(who);
+              }
+            }
+          __syncwarp();
+        }
+        if (n > kLpCap || (n >= 32 && n >= 2 * k)) {
+          if (n > kLpCap) {
+            // The tile's k best, each the largest below the one before.
+            unsigned long long below = ~0ull;
+            n = held;
+#pragma unroll 1
+            for (int i = 0; i < k; ++i) {
+              unsigned long long b = 0;
+#pragma unroll 1
+              for (int q = 0; q < kLpQuads; ++q) {
+                const float4 f = here[q * 32 + lane];
+                const float u[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const unsigned long long key =
+                      packed(u[e], base + (q * 32 + lane) * 4 + e - shift);
+                  if ((in >> (4 * q + e) & 1u) && key < below && key > b) b = key;
+                }
+              }
+#pragma unroll 1
+              for (int o = 16; o > 0; o >>= 1) {
+                const unsigned long long other = __shfl_xor_sync(0xffffffffu, b, o);
+                b = other > b ? other : b;
+              }
+              if (b == 0) break;
+              below = b;
+              if (n == kLpCap) {
+                __syncwarp();
+                keep_best(list, n, k, lane);
+                n = k;
+              }
+              if (lane == 0) list[n] = b;
+              ++n;
+            }
+            __syncwarp();
+          }
+          if (n > k) {
+            keep_best(list, n, k, lane);
+            n = k;
+          }
+          // Full and in order: what comes later loses a tie, so it has to be
+          // larger than the last.
+          const uint32_t kth = (uint32_t)(list[k - 1] >> 32);
+          if (n == k && kth) thr = fmaxf(thr, key_value(kth + 1));
+        }
+        held = n;
+      }
+      start_tile(here, x, base + kLpSlots * kStep, shift, v1, lane);
+    }
+    st.l = l2.x + l2.y;
+    st.t = t2.x + t2.y;
+    st.join_lanes();
+    if (k) keep_best(list, held, k, lane);
+    if constexpr (ROW_PER_WARP) {
+      const int done = r, done_id = id;
+      const float done_one = one;
+      const bool done_has = has;
+      r += warps * gridDim.x;
+      const bool more = r < a.rows;
+      if (more) take_row();            // its copies start before this row's results
+      emit(a, done, st, list, lane, 32, done_one, done_id, done_has);
+      __syncwarp();
+      if (!more) return;
+      continue;
+    }
+    if (lane == 0) {
+      parts[warp] = st;
+      counts[warp] = min(held, k);
+    }
+    __syncthreads();
+    auto join_parts = [&](const Stats* p, int n) {   // by every warp
+      st = {-INFINITY, 0.0f, 0.0f, 0};
+      if (lane < n) st = p[lane];
+      st.join_lanes();
+    };
+    join_parts(parts, kLpWarps);
+    if (cluster > 1) {
+      // Into the first CTA's shared memory.
+      if (k) {
+        merge_lists(lists[0], kLpCap, counts, k, joined, warp, lane);
+        __syncthreads();
+      }
+      int n = 0;
+      for (int w = 0; w < kLpWarps; ++w) n += counts[w];
+      n = min(n, k);
+      cluster_wait();                  // every CTA of the cluster has started
+      unsigned long long* to = cl.map_shared_rank(&theirs[0][0], 0) + rank * kLpMaxTop;
+      if (tid < n) to[tid] = joined[tid];
+      if (tid == 0) {
+        *cl.map_shared_rank(&cta_parts[rank], 0) = st;
+        *cl.map_shared_rank(&cta_counts[rank], 0) = n;
+      }
+      cl.sync();
+      if (rank != 0) return;
+      join_parts(cta_parts, cluster);
+      if (tid >= cluster && tid < kLpMaxCluster) cta_counts[tid] = 0;
+      __syncthreads();
+    }
+    if (k) {
+      if (cluster > 1)
+        merge_lists(theirs[0], kLpMaxTop, cta_counts, k, joined, warp, lane);
+      else
+        merge_lists(lists[0], kLpCap, counts, k, joined, warp, lane);
+      __syncthreads();
+    }
+    emit(a, r, st, joined, tid, kLpWarps * 32, one, id, has);
+    return;
   }
 }
 
@@ -310,20 +508,25 @@ int launch_token_logprobs(cudaStream_t s, int64_t* cnt, const float* x, int64_t 
     return fail(SPX_ERR_INVALID_ARGUMENT, "token_logprobs: top_k must be 0..64 and at most cols");
   if (top_k && (!top_ids || !top_logprobs))
     return fail(SPX_ERR_INVALID_ARGUMENT, "token_logprobs: top_k needs both outputs");
-  if (cols > INT32_MAX - 2 * kLpTile)
+  if (cols > INT32_MAX - 16 * kLpWarps * kLpTile)
     return fail(SPX_ERR_UNSUPPORTED, "token_logprobs: too many columns");
-  // Rows over several CTAs while there are fewer than two CTAs an SM and a
-  // part stays half a tile.
+  // A warp a row when that gives two CTAs an SM of at least half their warps:
+  // as few warps as take the same number of rounds, so that they end together.
+  // Else a CTA a row, or several while there are fewer than two CTAs an SM and
+  // half of a CTA's warps still have a tile.
+  const bool row_per_warp = rows >= kLpPerSm * kNumSms * kLpWarps / 2;
+  const int rounds = (int)ceil_div(rows, kLpPerSm * kNumSms * kLpWarps);
+  const int warps = row_per_warp ? (int)ceil_div(rows, kLpPerSm * kNumSms * rounds) : kLpWarps;
   int cluster = 1;
-  while (cluster < 8 && (int64_t)rows * cluster < 2 * kNumSms && cols / cluster > kLpTile / 2)
+  while (cluster < kLpMaxCluster && (int64_t)rows * cluster < 2 * kNumSms &&
+         cols / cluster > kLpWarps * kLpTile / 2)
     cluster *= 2;
   const int seg = (int)ceil_div(ceil_div(cols + 3, cluster), 4) * 4;
-  if ((int64_t)rows * cluster > INT32_MAX)
-    return fail(SPX_ERR_UNSUPPORTED, "token_logprobs: grid too large");
-  const LpArgs a{x, ld, cols, ids, logprobs, entropy, rank, top_k, top_ids, top_logprobs};
+  const LpArgs a{x, ld, rows, cols, ids, logprobs, entropy, rank, top_k, top_ids, top_logprobs};
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(rows * cluster));
-  cfg.blockDim = dim3(kLpThreads);
+  cfg.gridDim = dim3((unsigned)(row_per_warp ? kLpPerSm * kNumSms : rows * cluster));
+  cfg.blockDim = dim3((unsigned)warps * 32);
+  cfg.dynamicSmemBytes = kLpRing;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -332,8 +535,12 @@ int launch_token_logprobs(cudaStream_t s, int64_t* cnt, const float* x, int64_t 
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const int rc = check_cuda(cudaLaunchKernelEx(&cfg, token_logprobs_kernel, a, cluster, seg),
-                            "token_logprobs");
+  auto kern = row_per_warp ? token_logprobs_kernel<true> : token_logprobs_kernel<false>;
+  int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           (int)kLpRing),
+                      "token_logprobs: smem attribute");
+  if (rc) return rc;
+  rc = check_cuda(cudaLaunchKernelEx(&cfg, kern, a, cluster, seg), "token_logprobs");
   return rc ? rc : after_launch(cnt, "token_logprobs");
 }
 

@@ -57,7 +57,8 @@ def _check(got, want, x, k):
 @pytest.mark.parametrize("rows,cols,k,ld", [
     (1, 1, 1, None), (1, 2, 2, None), (3, 31, 5, 40), (2, 1000, 0, None), (5, 1001, 20, 1003),
     (1, 32000, 5, None), (64, 32000, 20, None), (7, 4097, 64, 4100), (300, 513, 3, None),
-    (2, 50257, 1, None), (1, 200003, 20, None), (3, 128256, 64, 128260), (700, 9000, 5, None)])
+    (2, 50257, 1, None), (1, 200003, 20, None), (3, 128256, 64, 128260), (700, 9000, 5, None), (2500, 1003, 7, 1003),
+    (2400, 700, 64, None)])
 def test_random_rows(g, rows, cols, k, ld):
     rng = np.random.default_rng(rows + cols)
     x = (rng.standard_normal((rows, cols)) * 3).astype(np.float32)
@@ -78,6 +79,28 @@ def test_orders_that_fill_the_candidates(g, cols, kind):
     x = np.stack([x, -x])
     ids = np.array([cols - 1, cols // 2], np.int32)
     _check(_run(g, x, ids, k), _ref(x, ids, k), x, k)
+
+
+@pytest.mark.parametrize("kind", ["equal", "rising", "falling", "masked"])
+def test_orders_many_rows(g, kind):
+    """The same with rows enough for each warp to have its own."""
+    cols, rows, k = 1500, 2400, 40
+    j = np.arange(cols)
+    x = {"equal": np.zeros(cols), "rising": j / cols, "falling": -j / cols,
+         "masked": np.where(j % 300 == 7, 1.0 + j, -np.inf)}[kind].astype(np.float32)
+    x = np.tile(x, (rows, 1))
+    ids = np.full(rows, 7, np.int32)
+    got, want = _run(g, x, ids, k), _ref(x[:1], ids[:1], k)
+    if kind == "masked":
+        assert np.array_equal(got[3][:, :5], np.tile(want[3][:, :5], (rows, 1)))
+        rest = [i for i in range(k) if i % 300 != 7][:k - 5]
+        assert np.array_equal(got[3][:, 5:], np.tile(rest, (rows, 1)))
+        assert np.all(np.isneginf(got[4][:, 5:]))
+    else:
+        assert np.array_equal(got[3], np.tile(want[3], (rows, 1)))
+    assert np.all(got[2] == want[2][0])
+    for i in (0, 1):
+        assert np.abs(got[i] - want[i][0]).max() <= 2.0 ** -19 * (1 + abs(want[i][0]))
 
 
 @pytest.mark.parametrize("cols", [40, 5000, 40000])
