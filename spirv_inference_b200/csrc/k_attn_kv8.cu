@@ -5,16 +5,21 @@
 //   weights[j] += sum over the new tokens and the heads of the group of
 //                 exp(s_j - lse)     (slots of the new tokens start from 0)
 //
-// Tensor cores in fp32 accuracy.  An int8 value is exact in fp16, so only the
-// other operand of each product is split: q (scaled by a power of two to
-// magnitude 1..2 a row) and p (at most 1) into fp16 hi + lo, 22 bits in all,
-// each product twice.  The scale of a 16-key tile (a block has at least 16
-// keys) multiplies its scores, and its share of p: p v_scale / v_ref, v_ref
-// the largest scale of the tiles in hand, keeps p within fp16's range.  The
-// tail (fp32 rows) is split the same way on both sides: three products.
-// Scores, sums and outputs are fp32; the products of a few tiles are summed
-// by the tensor core, whose additions round towards zero, and then added to
-// the running output in fp32.
+// Tensor cores in fp32 accuracy, with the int8 operand as it is.
+//
+// Scores: a row of q, scaled to whole numbers of 23 bits, is three digits of 8
+// bits, and the products of each digit with the int8 keys are exact in int32
+// (mma m16n8k32); the scale of the keys' block multiplies their sum.
+//
+// Outputs: an int8 value is exact in fp16, p as fp16 hi + lo has 22 bits, and
+// each product is taken twice with fp32 sums.  p is multiplied by its block's
+// share v_scale / v_ref (v_ref the largest scale of the tiles in hand) and by
+// 2^15, so that small p keep their low part.  The tensor core's additions
+// round towards zero, so a few tiles' products are added to the running
+// output in fp32.
+//
+// Rows of the tail are fp32: both operands are split into fp16 hi + lo,
+// scaled by powers of two, three products each.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -54,6 +59,20 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ uint32_t transposed8x8(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -67,15 +86,6 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   const float2 f = __half22float2(h);
   hi = as_u32(h);
   lo = as_u32(__floats2half2_rn(x - f.x, y - f.y));
-}
-
-// Two bytes (already flipped by 0x80: value + 128) to fp16: 0x6400 | u is
-// 1024 + u, less 1152.
-__device__ __forceinline__ uint32_t two_halves(uint32_t w, uint32_t sel) {
-  uint32_t r = __byte_perm(w, 0x64646464u, sel);
-  const __half2 v = __hsub2(*reinterpret_cast<__half2*>(&r),
-                            __half2half2(__ushort_as_half((unsigned short)0x6480)));
-  return as_u32(v);
 }
 
 // 2^-e and 2^e for a largest magnitude with these bits (finite).
@@ -92,21 +102,21 @@ __device__ __forceinline__ uint32_t finite_abs(float x) {
 
 // ---------------------------------------------------------------------------
 // Few rows (decode, drafts).  A row is a (new token, head of the group) pair.
-// Scores are held transposed, S^T = K Q^T: 16 keys are the M side of
-// mma.m16n8k16 and 8 rows the N side, so that no lane is padding for a group
-// of 8 heads.  Within a dot product the order of d is free: lane (g, t) reads
-// 16 contiguous bytes of key row g and lets them be its four k-steps, straight
-// from global memory in fragment order.  The output is held transposed too,
-// O^T = V^T P^T: the lane's V bytes of four keys are interleaved into fp16
-// pairs of keys, and the 8 x 8 blocks of P come from the scores' layout to the
-// B operand's by movmatrix.  Each warp walks its own 16-key tiles with its own
-// running maximum and sum; warps are joined in shared memory and the CTAs of a
-// cluster, over which one sequence's keys are spread, through distributed
-// shared memory: one launch, no workspace.
+// Scores are held transposed, S^T = K Q^T: 16 keys are the M side of an mma
+// and 8 rows the N side, so that no lane is padding for a group of 8 heads.
+// Within a dot product the order of d is free: lane (g, t) reads 16 contiguous
+// bytes of key row g, and they are its operand as they come from memory.  The
+// output is held transposed too, O^T = V^T P^T: the lane's V bytes of four keys
+// become fp16 pairs of keys, and the 8 x 8 blocks of P go from the scores'
+// layout to the B operand's by movmatrix.  Each warp walks its own groups of
+// tiles with its own running maximum and sum; warps are joined in shared
+// memory and the CTAs of a cluster, over which one sequence's keys are spread,
+// by stores into each other's shared memory: one launch, no workspace.
 //
-// What bounds it: the cache's bytes, 2 D + 8 / block a key and head; 16
-// products of 4096 operations for 16 keys of D = 64 are a third of the tensor
-// pipe's rate at full bandwidth.
+// What bounds it: the cache's bytes, 2 D + 8 / block a key and head, and close
+// behind the instructions, about 140 for 16 keys of D = 64 and 8 rows (48 of
+// them turn V into fp16).  So tiles that every row sees in full take a path
+// without masks, and the others, one by one, another.
 template <int D>
 struct Frag {                   // one 16-key tile of int8 K and V in registers
   uint4 k[2][D / 64];           // key rows g, g + 8
@@ -131,38 +141,46 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[NW], const void* p) {
 
 template <int D>
 struct Keys {
-  const int8_t* k8;
+  const int8_t* k8;    // at the lane's place in the first tile
   const int8_t* v8;
   const float* ks;
   const float* vs;
   const float* kt;
   const float* vt;
-  int shift;      // log2(block)
-  __device__ __forceinline__ void load_k(Frag<D>& f, int tile, int g, int t) const {
+  int shift;           // log2(block)
+  __device__ __forceinline__ Keys(const spx_kv8_cache& c, int64_t bh, int g, int t) {
+    shift = 31 - __clz(c.block);
+    k8 = c.k + bh * c.max_seq * D + g * D + 16 * t;
+    v8 = c.v + bh * c.max_seq * D + 2 * t * D + D / 8 * g;
+    ks = c.k_scale + bh * (c.max_seq >> shift);
+    vs = c.v_scale + bh * (c.max_seq >> shift);
+    kt = c.k_tail + bh * ((int64_t)D << shift);
+    vt = c.v_tail + bh * ((int64_t)D << shift);
+  }
+  __device__ __forceinline__ void load_k(Frag<D>& f, int tile) const {
+    const int8_t* p = k8 + (int64_t)tile * (16 * D);
 #pragma unroll
     for (int r = 0; r < 2; ++r)
 #pragma unroll
       for (int h = 0; h < D / 64; ++h)
-        f.k[r][h] = __ldg(reinterpret_cast<const uint4*>(
-            k8 + ((int64_t)tile * 16 + g + 8 * r) * D + 64 * h + 16 * t));
+        f.k[r][h] = __ldg(reinterpret_cast<const uint4*>(p + 8 * r * D + 64 * h));
     f.ks = __ldg(ks + ((tile * 16) >> shift));
   }
-  __device__ __forceinline__ void load_v(Frag<D>& f, int tile, int g, int t) const {
+  __device__ __forceinline__ void load_v(Frag<D>& f, int tile) const {
+    const int8_t* p = v8 + (int64_t)tile * (16 * D);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      load_words(f.v[i], v8 + ((int64_t)tile * 16 + 2 * t + (i & 1) + 8 * (i >> 1)) * D + D / 8 * g);
+    for (int i = 0; i < 4; ++i) load_words(f.v[i], p + ((i & 1) + 8 * (i >> 1)) * D);
     f.vs = __ldg(vs + ((tile * 16) >> shift));
   }
 };
 
-// Q of 8 rows as B fragments, hi and lo: [k-step][hi b0, b1, lo b0, b1], and
-// for the lane's two columns (rows 2t, 2t + 1) the factor that takes a product
-// to a score in units of log 2.
+// The lane's 16 values in each 64 of a row of q, and the row's largest finite
+// magnitude; `odd`: the row has a NaN or an infinity.
 template <int D>
-__device__ __forceinline__ void load_q(uint32_t (&qf)[D / 16][4], float (&qs)[2], const float* row,
-                                       float scale, int t) {
-  float x[D / 64][16];
+__device__ __forceinline__ uint32_t read_q(float (&x)[D / 64][16], bool& odd, const float* row,
+                                           int t) {
   uint32_t mx = 0;
+  odd = false;
 #pragma unroll
   for (int h = 0; h < D / 64; ++h)
 #pragma unroll
@@ -174,45 +192,73 @@ __device__ __forceinline__ void load_q(uint32_t (&qf)[D / 16][4], float (&qs)[2]
       x[h][4 * i + 2] = v.z;
       x[h][4 * i + 3] = v.w;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mx = max(mx, finite_abs(x[h][4 * i + e]));
+      for (int e = 0; e < 4; ++e) {
+        mx = max(mx, finite_abs(x[h][4 * i + e]));
+        odd |= (__float_as_uint(x[h][4 * i + e]) & 0x7f800000u) == 0x7f800000u;
+      }
     }
   mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
   mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-  float down, up;
-  pow2_scale(mx, down, up);
+  odd = __ballot_sync(0xffffffffu, odd) >> ((threadIdx.x & 28)) & 15u;
+  return mx;
+}
+
+// Q of 8 rows as B fragments, in digits: [k-step][digit][b0, b1], and for the
+// lane's two columns (rows 2t, 2t + 1) the factor that takes a product to a
+// score in units of log 2 (NaN for a row with a NaN or an infinity).
+template <int D>
+__device__ __forceinline__ void load_q(uint32_t (&qd)[D / 32][3][2], float (&qs)[2],
+                                       const float* row, float scale, int t) {
+  constexpr float kWhole = 8300000.0f;   // below 127 * (65536 + 256 + 1)
+  float x[D / 64][16];
+  bool odd;
+  const float amax = __uint_as_float(read_q<D>(x, odd, row, t));
+  const float inv = amax > 1e-30f ? copysignf(kWhole / amax, scale) : 0.0f;
 #pragma unroll
-  for (int h = 0; h < D / 64; ++h)
+  for (int i = 0; i < D / 16; ++i)       // four values: k-step i / 2, register i % 2
+    {
+      uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t* f = qf[4 * h + i];
-      split2(x[h][4 * i] * down, x[h][4 * i + 1] * down, f[0], f[2]);
-      split2(x[h][4 * i + 2] * down, x[h][4 * i + 3] * down, f[1], f[3]);
+      for (int e = 0; e < 4; ++e) {
+        // digits in [-128, 127]: the bytes of v + 0x808080, less 128 each
+        const float v = x[i / 4][4 * (i % 4) + e] * inv;
+        w[e] = ((uint32_t)__float2int_rn(odd ? 0.0f : v) + 0x808080u) ^ 0x808080u;
+      }
+      const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[2], w[3], 0x5140);
+      const uint32_t c = __byte_perm(w[0], w[1], 0x0062), d = __byte_perm(w[2], w[3], 0x0062);
+      qd[i / 2][0][i % 2] = __byte_perm(c, d, 0x5410);
+      qd[i / 2][1][i % 2] = __byte_perm(a, b, 0x7632);
+      qd[i / 2][2][i % 2] = __byte_perm(a, b, 0x5410);
     }
-  const float s = up * (scale * kLog2e);
+  const float s = odd ? __int_as_float(0x7fc00000)
+                      : amax * (1.0f / kWhole) * (fabsf(scale) * kLog2e);
   qs[0] = __shfl_sync(0xffffffffu, s, t * 8);
   qs[1] = __shfl_sync(0xffffffffu, s, t * 8 + 4);
 }
 
-// c += K Q^T of one int8 tile.
-template <int D, int NT>
-__device__ __forceinline__ void scores(float (&c)[NT][4], const Frag<D>& f,
-                                       const uint32_t (&qf)[NT][D / 16][4]) {
+// K Q^T of one int8 tile, before any scale.
+template <int D>
+__device__ __forceinline__ void products(float (&c)[4], const Frag<D>& f,
+                                         const uint32_t (&qd)[D / 32][3][2]) {
+  int hi[4] = {}, mid[4], lo[4];
+  auto sum = [&](int (&acc)[4], int digit) {
 #pragma unroll
-  for (int h = 0; h < D / 64; ++h) {
-    const uint32_t* r0 = reinterpret_cast<const uint32_t*>(&f.k[0][h]);
-    const uint32_t* r1 = reinterpret_cast<const uint32_t*>(&f.k[1][h]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t w0 = r0[i] ^ 0x80808080u, w1 = r1[i] ^ 0x80808080u;
-      const uint32_t a[4] = {two_halves(w0, 0x4140), two_halves(w1, 0x4140),
-                             two_halves(w0, 0x4342), two_halves(w1, 0x4342)};
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        mma16816(c[n], a, qf[n][4 * h + i][0], qf[n][4 * h + i][1]);
-        mma16816(c[n], a, qf[n][4 * h + i][2], qf[n][4 * h + i][3]);
-      }
+    for (int s = 0; s < D / 32; ++s) {
+      const uint32_t* r0 = reinterpret_cast<const uint32_t*>(&f.k[0][s / 2]) + 2 * (s % 2);
+      const uint32_t* r1 = reinterpret_cast<const uint32_t*>(&f.k[1][s / 2]) + 2 * (s % 2);
+      mma16832(acc, r0[0], r1[0], r0[1], r1[1], qd[s][digit][0], qd[s][digit][1]);
     }
-  }
+  };
+  sum(hi, 0);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) mid[e] = hi[e] * 256;     // at most 2^29
+  sum(mid, 1);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) lo[e] = 0x4b400000;       // as a float: 1.5 2^23 + the sum
+  sum(lo, 2);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    c[e] = fmaf((float)mid[e], 256.0f, __int_as_float(lo[e]) - 12582912.0f);
 }
 
 // The running softmax of one warp: lane (g, t) holds rows (columns) 2t, 2t+1
@@ -234,17 +280,29 @@ struct Running {
         for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
     }
   }
-  // New maxima for tile scores (log2 units); c becomes exp2(c - m), the sums
-  // take them, and `corr` is what the outputs so far have to be scaled by.
-  template <int KT>
-  __device__ __forceinline__ void weigh(float (&c)[KT][NT][4], float (&corr)[NT][2]) {
+  // New maxima for tile scores c f (f >= 0 the tile's factor of each column);
+  // c becomes exp2(c f - m), 0 where hidden, the sums take them, and `corr` is
+  // what the outputs so far have to be scaled by.
+  template <int KT, bool MASK>
+  __device__ __forceinline__ void weigh(float (&c)[KT][NT][4], const float (&f)[KT][NT][2],
+                                        float (&corr)[NT][2], uint32_t hidden) {
+    auto hides = [&](int k, int n, int e) {
+      return MASK && (hidden >> ((k * NT + n) * 4 + e) & 1u);
+    };
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float mt = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < KT; ++k) mt = fmaxf(mt, fmaxf(c[k][n][e], c[k][n][e + 2]));
+        for (int k = 0; k < KT; ++k) {
+          if (MASK) {
+            if (!hides(k, n, e)) mt = fmaxf(mt, c[k][n][e] * f[k][n][e]);
+            if (!hides(k, n, e + 2)) mt = fmaxf(mt, c[k][n][e + 2] * f[k][n][e]);
+          } else {
+            mt = fmaxf(mt, fmaxf(c[k][n][e], c[k][n][e + 2]) * f[k][n][e]);
+          }
+        }
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
         const float mn = fmaxf(m[n][e], mt), base = mn == -INFINITY ? 0.0f : mn;
@@ -252,11 +310,12 @@ struct Running {
         m[n][e] = mn;
         float sum = 0.0f;
 #pragma unroll
-        for (int k = 0; k < KT; ++k) {
-          c[k][n][e] = ex2(c[k][n][e] - base);
-          c[k][n][e + 2] = ex2(c[k][n][e + 2] - base);
-          sum += c[k][n][e] + c[k][n][e + 2];
-        }
+        for (int k = 0; k < KT; ++k)
+#pragma unroll
+          for (int i = e; i < 4; i += 2) {
+            c[k][n][i] = hides(k, n, i) ? 0.0f : ex2(fmaf(c[k][n][i], f[k][n][e], -base));
+            sum += c[k][n][i];
+          }
         l[n][e] = fmaf(l[n][e], corr[n][e], sum);
       }
   }
@@ -273,16 +332,94 @@ __device__ __forceinline__ void p_frags(uint32_t (&pf)[4], const float (&p)[4]) 
   pf[3] = transposed8x8(l1);
 }
 
-// One 16-key tile of the tail: fp32 rows, both operands split.
+// Bytes 0 and 2 of a word of two's complement bytes to fp16: with the sign bit
+// flipped under 0x64, they are 1024 + 128 + value.
+__device__ __forceinline__ uint32_t even_bytes(uint32_t w) {
+  uint32_t r = (w & 0x00ff00ffu) ^ 0x64806480u;
+  const __half2 v = __hsub2(*reinterpret_cast<__half2*>(&r),
+                            __half2half2(__ushort_as_half((unsigned short)0x6480)));
+  return as_u32(v);
+}
+
+constexpr float kPUp = 32768.0f;   // 2^15
+
+// O^T += V^T P^T over KT int8 tiles; c: exp2(score - m), zero where MASK hides.
+template <int D, int NT, int KT, bool MASK>
+__device__ __forceinline__ void add_values(Running<D, NT>& run, const Frag<D> (&f)[KT],
+                                           float (&c)[KT][NT][4], const float (&corr)[NT][2],
+                                           uint32_t hidden) {
+  float ref = 0.0f;
+  bool odd = false;                // a block with a NaN or an infinity
+#pragma unroll
+  for (int k = 0; k < KT; ++k) {
+    const bool fine = f[k].vs <= 3.4028234663852886e38f;
+    if (fine) ref = fmaxf(ref, f[k].vs);
+    odd |= !fine;
+  }
+  const float inv = ref > 0.0f ? kPUp / ref : 0.0f;
+  float o[NT][D / 16][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
+#pragma unroll
+  for (int k = 0; k < KT; ++k) {
+    const float share = f[k].vs * inv;
+    uint32_t pf[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[k][n][e] *= share;
+      if (odd) {
+        // its rows' weights become NaN, other rows' stay zero
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (!(f[k].vs <= 3.4028234663852886e38f)) c[k][n][e] = __int_as_float(0x7fc00000);
+          if (MASK && (hidden >> ((k * NT + n) * 4 + e) & 1u)) c[k][n][e] = 0.0f;
+        }
+      }
+      p_frags(pf[n], c[k][n]);
+    }
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        // d = 2 (2w + i) and + 1 of keys (2t, 2t + 1) and (2t + 8, 2t + 9)
+        const uint32_t sel = i ? 0x7632 : 0x5410;
+        const uint32_t x = __byte_perm(f[k].v[0][w], f[k].v[1][w], sel);
+        const uint32_t y = __byte_perm(f[k].v[2][w], f[k].v[3][w], sel);
+        const uint32_t av[4] = {even_bytes(x), even_bytes(x >> 8), even_bytes(y),
+                                even_bytes(y >> 8)};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma16816(o[n][2 * w + i], av, pf[n][0], pf[n][1]);
+          mma16816(o[n][2 * w + i], av, pf[n][2], pf[n][3]);
+        }
+      }
+  }
+  const float back = ref * (1.0f / kPUp);
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        run.o[n][i][e] = fmaf(run.o[n][i][e], corr[n][e & 1], back * o[n][i][e]);
+}
+
+// Scores of one 16-key tile of the tail: fp32 rows, both operands split; c f as
+// for weigh().  q: the rows of q that the lane's columns g stand for (null:
+// none).
 template <int D, int NT>
-__device__ __forceinline__ void tail_tile(Running<D, NT>& run, const Keys<D>& kv,
-                                          const uint32_t (&qf)[NT][D / 16][4],
-                                          const float (&qs)[NT][2], const int (&last)[NT][2],
-                                          int jb, int total, int g, int t) {
+__device__ __forceinline__ void tail_products(float (&c)[1][NT][4], float (&f)[1][NT][2],
+                                              const Keys<D>& kv, const float* const (&q)[NT],
+                                              float scale, int jb, int total, int g, int t) {
   const int blk_mask = (1 << kv.shift) - 1;
   // K rows g and g + 8
+  uint32_t a[D / 16][4], al[D / 16][4];
   float up_k, down;
-  float c[1][NT][4] = {};
   {
     float x[2][D / 64][16];
     uint32_t mx = 0;
@@ -306,31 +443,61 @@ __device__ __forceinline__ void tail_tile(Running<D, NT>& run, const Keys<D>& kv
     }
     pow2_scale(__reduce_max_sync(0xffffffffu, mx), down, up_k);
 #pragma unroll
-    for (int h = 0; h < D / 64; ++h)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t a[4], al[4];
-        split2(x[0][h][4 * i] * down, x[0][h][4 * i + 1] * down, a[0], al[0]);
-        split2(x[1][h][4 * i] * down, x[1][h][4 * i + 1] * down, a[1], al[1]);
-        split2(x[0][h][4 * i + 2] * down, x[0][h][4 * i + 3] * down, a[2], al[2]);
-        split2(x[1][h][4 * i + 2] * down, x[1][h][4 * i + 3] * down, a[3], al[3]);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const uint32_t* q = qf[n][4 * h + i];
-          mma16816(c[0][n], al, q[0], q[1]);
-          mma16816(c[0][n], a, q[2], q[3]);
-          mma16816(c[0][n], a, q[0], q[1]);
-        }
-      }
+    for (int k = 0; k < D / 16; ++k) {
+      const int h = k / 4, i = 4 * (k % 4);
+      split2(x[0][h][i] * down, x[0][h][i + 1] * down, a[k][0], al[k][0]);
+      split2(x[1][h][i] * down, x[1][h][i + 1] * down, a[k][1], al[k][1]);
+      split2(x[0][h][i + 2] * down, x[0][h][i + 3] * down, a[k][2], al[k][2]);
+      split2(x[1][h][i + 2] * down, x[1][h][i + 3] * down, a[k][3], al[k][3]);
+    }
   }
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float x[D / 64][16], up, dn;
+    bool odd;
+    pow2_scale(read_q<D>(x, odd, q[n], t), dn, up);
+    if (scale < 0.0f) dn = -dn;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[0][n][e] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      const int h = k / 4, i = 4 * (k % 4);
+      uint32_t h0, l0, h1, l1;
+      split2(x[h][i] * dn, x[h][i + 1] * dn, h0, l0);
+      split2(x[h][i + 2] * dn, x[h][i + 3] * dn, h1, l1);
+      mma16816(c[0][n], al[k], h0, h1);
+      mma16816(c[0][n], a[k], l0, l1);
+      mma16816(c[0][n], a[k], h0, h1);
+    }
+    const float s = up * up_k * (fabsf(scale) * kLog2e);
+    f[0][n][0] = __shfl_sync(0xffffffffu, s, t * 8);
+    f[0][n][1] = __shfl_sync(0xffffffffu, s, t * 8 + 4);
+  }
+}
+
+// Which of a tile's scores their columns do not see.
+template <int NT>
+__device__ __forceinline__ uint32_t hidden_in(int jb, const int (&last)[NT][2], int g) {
+  uint32_t hidden = 0;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      c[0][n][e] = jb + g + 8 * (e >> 1) <= last[n][e & 1] ? c[0][n][e] * (up_k * qs[n][e & 1])
-                                                           : -INFINITY;
-  float corr[NT][2];
-  run.weigh(c, corr);
+      hidden |= (jb + g + 8 * (e >> 1) > last[n][e & 1] ? 1u : 0u) << (n * 4 + e);
+  return hidden;
+}
+
+// One 16-key tile of the tail.
+template <int D, int NT>
+__device__ __forceinline__ void tail_tile(Running<D, NT>& run, const Keys<D>& kv,
+                                          const float* const (&q)[NT], float scale,
+                                          const int (&last)[NT][2], int jb, int total, int g,
+                                          int t) {
+  const int blk_mask = (1 << kv.shift) - 1;
+  float c[1][NT][4], f[1][NT][2], corr[NT][2];
+  tail_products<D, NT>(c, f, kv, q, scale, jb, total, g, t);
+  const uint32_t hidden = hidden_in<NT>(jb, last, g);
+  run.template weigh<1, true>(c, f, corr, hidden);
   // V rows 2t, 2t+1, 2t+8, 2t+9
   float y[4][D / 8];
   uint32_t mx = 0;
@@ -349,208 +516,198 @@ __device__ __forceinline__ void tail_tile(Running<D, NT>& run, const Keys<D>& kv
       y[i][4 * e + 2] = v.z;
       y[i][4 * e + 3] = v.w;
 #pragma unroll
-      for (int f = 0; f < 4; ++f) {
+      for (int z = 0; z < 4; ++z) {
         // A NaN or infinity would reach rows that do not see this key: it
         // goes into the key's weight instead, where the mask stops it.
-        float& z = y[i][4 * e + f];
-        if ((__float_as_uint(z) & 0x7f800000u) == 0x7f800000u) {
+        float& u = y[i][4 * e + z];
+        if ((__float_as_uint(u) & 0x7f800000u) == 0x7f800000u) {
           odd = true;
-          z = 0.0f;
+          u = 0.0f;
         }
-        mx = max(mx, __float_as_uint(z) & 0x7fffffffu);
+        mx = max(mx, __float_as_uint(u) & 0x7fffffffu);
       }
     }
     bad[i] = __ballot_sync(0xffffffffu, odd);
   }
-  float up_v;
+  float up_v, down;
   pow2_scale(__reduce_max_sync(0xffffffffu, mx), down, up_v);
   const uint32_t mine = 0x11111111u << (g >> 1);   // lanes with key g's (g + 8's) V
   const bool bad0 = (g & 1 ? bad[1] : bad[0]) & mine, bad1 = (g & 1 ? bad[3] : bad[2]) & mine;
+  uint32_t pf[NT][4];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if ((e < 2 ? bad0 : bad1) && jb + g + 8 * (e >> 1) <= last[n][e & 1])
+    for (int e = 0; e < 4; ++e) {
+      c[0][n][e] *= kPUp;
+      if ((e < 2 ? bad0 : bad1) && !(hidden >> (n * 4 + e) & 1u))
         c[0][n][e] = __int_as_float(0x7fc00000);
-    uint32_t pf[4];
-    p_frags(pf, c[0][n]);
+    }
+    p_frags(pf[n], c[0][n]);
+  }
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      uint32_t a[4], al[4];
-      split2(y[0][2 * i] * down, y[1][2 * i] * down, a[0], al[0]);
-      split2(y[0][2 * i + 1] * down, y[1][2 * i + 1] * down, a[1], al[1]);
-      split2(y[2][2 * i] * down, y[3][2 * i] * down, a[2], al[2]);
-      split2(y[2][2 * i + 1] * down, y[3][2 * i + 1] * down, a[3], al[3]);
+  for (int i = 0; i < D / 16; ++i) {
+    uint32_t a[4], al[4];
+    split2(y[0][2 * i] * down, y[1][2 * i] * down, a[0], al[0]);
+    split2(y[0][2 * i + 1] * down, y[1][2 * i + 1] * down, a[1], al[1]);
+    split2(y[2][2 * i] * down, y[3][2 * i] * down, a[2], al[2]);
+    split2(y[2][2 * i + 1] * down, y[3][2 * i + 1] * down, a[3], al[3]);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
       float o[4] = {};
-      mma16816(o, al, pf[0], pf[1]);
-      mma16816(o, a, pf[2], pf[3]);
-      mma16816(o, a, pf[0], pf[1]);
+      mma16816(o, al, pf[n][0], pf[n][1]);
+      mma16816(o, a, pf[n][2], pf[n][3]);
+      mma16816(o, a, pf[n][0], pf[n][1]);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        run.o[n][i][e] = fmaf(run.o[n][i][e], corr[n][e & 1], up_v * o[e]);
+        run.o[n][i][e] = fmaf(run.o[n][i][e], corr[n][e & 1], up_v * (1.0f / kPUp) * o[e]);
     }
   }
 }
 
+// Adds a slot's weight, summed over the four lanes that share it.
+__device__ __forceinline__ void put_weight(float* out, float w, int j, int len, int total, int t) {
+  w += __shfl_xor_sync(0xffffffffu, w, 1);
+  w += __shfl_xor_sync(0xffffffffu, w, 2);
+  if (t == 0 && j < total) out[j] = (j < len ? out[j] : 0.0f) + w;
+}
+// exp2(c f - z) of one tile, summed over the rows that see each key.
+template <int NT>
+__device__ __forceinline__ void add_weights(float* out, const float (&c)[1][NT][4],
+                                            const float (&f)[1][NT][2], const float (&z)[NT][2],
+                                            uint32_t hidden, int jb, int len, int total,
+                                            int lane) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float w = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (!(hidden >> (n * 4 + 2 * i + e) & 1u))
+          w += ex2(fmaf(c[0][n][2 * i + e], f[0][n][e], -z[n][e]));
+    put_weight(out, w, jb + (lane >> 2) + 8 * i, len, total, lane & 3);
+  }
+}
+
 constexpr int kFewMaxWarps = 8;
+constexpr int kMaxCluster = 8;
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kFewMaxWarps * 32, 1)
+struct FewShape {
+  static constexpr int KT = 2;                            // tiles of a group
+  static constexpr int R = 8 * NT;                        // rows
+  static constexpr int kBlocks = D == 64 && NT == 1 ? 2 : 1;   // of 8 warps an SM
+};
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
     attention_kv8_few_kernel(const AttnArgs a, int groups, int cluster) {
-  constexpr int KT = D == 64 ? 4 : 2;   // tiles in flight: 64 registers of K and V
-  constexpr int R = 8 * NT;
+  constexpr int KT = FewShape<D, NT>::KT, R = FewShape<D, NT>::R;
   extern __shared__ __align__(16) float smem[];
   const int W = blockDim.x >> 5;
-  float* part_m = smem;                 // [W][R]
+  float* part_o = smem;                 // [W][R][D]
+  float* recv_o = part_o + W * R * D;   // [cluster][R D / cluster]: this CTA's share
+  float* part_m = recv_o + R * D;       // [W][R]
   float* part_l = part_m + W * R;       // [W][R]
-  float* cta_m = part_l + W * R;        // [R]
-  float* cta_l = cta_m + R;             // [R]
-  float* part_o = cta_l + R;            // [W][R][D]; the CTA's own sum goes to warp 0's
+  float* recv_m = part_l + W * R;       // [cluster][R]
+  float* recv_l = recv_m + kMaxCluster * R;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rank = blockIdx.x % cluster;
   const int unit = blockIdx.x / cluster, grp = unit % groups, h = unit / groups, b = blockIdx.y;
   const int S = a.c.max_seq, Hkv = a.c.kv_heads, G = a.Hq / Hkv;
-  const int n_new = a.new_lens ? clamp_len(a.new_lens[b], a.T) : a.T;
-  const int rows = n_new * G, r0 = grp * R;
-  if (r0 >= rows) return;               // the whole cluster
-  const int len = clamp_len(a.c.lens[b], S), total = min(len + n_new, S);
-  const int shift = 31 - __clz(a.c.block);
-  const int closed = total >> shift << shift;
-  const int t_first = r0 / G, t_last = min(r0 + R, rows) - 1;   // rows; tokens below
-  const int lim = min(len + t_last / G + 1, S);                 // slots that some row sees
-  const int64_t bh = (int64_t)b * Hkv + h;
-  Keys<D> kv;
-  kv.k8 = a.c.k + bh * S * D;
-  kv.v8 = a.c.v + bh * S * D;
-  kv.ks = a.c.k_scale + bh * (S >> shift);
-  kv.vs = a.c.v_scale + bh * (S >> shift);
-  kv.kt = a.c.k_tail + bh * ((int64_t)D << shift);
-  kv.vt = a.c.v_tail + bh * ((int64_t)D << shift);
-  kv.shift = shift;
-
-  uint32_t qf[NT][D / 16][4];
-  float qs[NT][2];
-  int last[NT][2];                      // the last slot that a column sees
+  if (cluster > 1) cluster_arrive();    // waited for before stores into other CTAs
+  // What does not depend on the lengths is on its way before they are known.
+  const int n_arg = a.new_lens ? a.new_lens[b] : a.T, len_arg = a.c.lens[b];
+  const Keys<D> kv(a.c, (int64_t)b * Hkv + h, g, t);
+  const int first = (rank * W + warp) * KT, step = cluster * W * KT;
+  Frag<D> f[KT];
+  const bool ahead = (first + KT) * 16 <= S;
+  if (ahead) {
+#pragma unroll
+    for (int k = 0; k < KT; ++k) kv.load_k(f[k], first + k);
+#pragma unroll
+    for (int k = 0; k < KT; ++k) kv.load_v(f[k], first + k);
+  }
+  const int r0 = grp * R, all_rows = a.T * G;
   auto row_at = [&](int r) {            // [token][head] row of the group's row r
     return ((int64_t)b * a.T + r / G) * a.Hq + h * G + r % G;
   };
+  uint32_t qd[NT][D / 32][3][2];
+  float qs[NT][2];
+  const float* q_row[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int r = r0 + 8 * n + g;
-    load_q<D>(qf[n], qs[n], r < rows ? a.q + row_at(r) * D : nullptr, a.scale, t);
+    q_row[n] = r < all_rows ? a.q + row_at(r) * D : nullptr;
+    load_q<D>(qd[n], qs[n], q_row[n], a.scale, t);
+  }
+  const int n_new = clamp_len(n_arg, a.T), rows = n_new * G;
+  if (r0 >= rows) {                     // the whole cluster
+    if (cluster > 1) cluster_wait();
+    return;
+  }
+  const int len = clamp_len(len_arg, S), total = min(len + n_new, S);
+  const int closed = total >> kv.shift << kv.shift;
+  const int lim = min(len + min(r0 + R - 1, rows - 1) / G + 1, S);   // slots that some row sees
+  int last[NT][2];                      // the last slot that a column sees
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int e = 0; e < 2; ++e)
       last[n][e] = min(len + min(r0 + 8 * n + 2 * t + e, rows - 1) / G, total - 1);
-  }
   Running<D, NT> run;
   run.init();
 
+  // Groups of tiles that every row sees in full.
   const int tiles = (min(closed, lim) + 15) >> 4;
-  const int first = (rank * W + warp) * KT, step = cluster * W * KT;
-  Frag<D> f[KT];
-  auto load_k = [&](int base) {
+  const int whole = min(closed, len + r0 / G + 1) / (16 * KT) * KT;
+  if (!ahead && first < whole) {
 #pragma unroll
-    for (int k = 0; k < KT; ++k) kv.load_k(f[k], min(base + k, tiles - 1), g, t);
-  };
-  auto load_v = [&](int base) {
+    for (int k = 0; k < KT; ++k) kv.load_k(f[k], first + k);
 #pragma unroll
-    for (int k = 0; k < KT; ++k) kv.load_v(f[k], min(base + k, tiles - 1), g, t);
-  };
-  if (first < tiles) {
-    load_k(first);
-    load_v(first);
+    for (int k = 0; k < KT; ++k) kv.load_v(f[k], first + k);
   }
-  for (int base = first; base < tiles; base += step) {
-    float c[KT][NT][4];
-    // every key of these tiles is seen by every row of the group
-    const bool all = (base + KT) * 16 <= len + t_first / G + 1 && base + KT <= tiles;
-#pragma unroll
-    for (int k = 0; k < KT; ++k) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c[k][n][e] = 0.0f;
-      scores<D, NT>(c[k], f[k], qf);
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c[k][n][e] *= f[k].ks * qs[n][e & 1];
-      if (!all) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (base + k >= tiles || (base + k) * 16 + g + 8 * (e >> 1) > last[n][e & 1])
-              c[k][n][e] = -INFINITY;
-      }
-    }
-    const bool more = base + step < tiles;
-    if (more) load_k(base + step);
-    // Rows that do not see a key have to weigh it 0 whatever its scale is.
-    uint32_t hidden = 0;
-    if (!all) {
-#pragma unroll
-      for (int k = 0; k < KT; ++k)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            hidden |= (c[k][n][e] == -INFINITY ? 1u : 0u) << ((k * NT + n) * 4 + e);
-    }
-    float corr[NT][2];
-    run.weigh(c, corr);
-    float ref = 0.0f;
+  for (int base = first; base < whole; base += step) {
+    float c[KT][NT][4], fk[KT][NT][2], corr[NT][2];
 #pragma unroll
     for (int k = 0; k < KT; ++k)
-      if (f[k].vs <= 3.4028234663852886e38f) ref = fmaxf(ref, f[k].vs);
-    const float inv = ref > 0.0f ? 1.0f / ref : 0.0f;
-    float o[NT][D / 16][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
-#pragma unroll
-    for (int k = 0; k < KT; ++k) {
-      const float share = f[k].vs * inv;
-      uint32_t pf[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          c[k][n][e] = hidden >> ((k * NT + n) * 4 + e) & 1u ? 0.0f : c[k][n][e] * share;
-        p_frags(pf[n], c[k][n]);
+        products<D>(c[k][n], f[k], qd[n]);
+        fk[k][n][0] = f[k].ks * qs[n][0];
+        fk[k][n][1] = f[k].ks * qs[n][1];
       }
+    const bool more = base + step < whole;
+    if (more) {
 #pragma unroll
-      for (int w = 0; w < D / 32; ++w) {
-        const uint32_t v0 = f[k].v[0][w] ^ 0x80808080u, v1 = f[k].v[1][w] ^ 0x80808080u;
-        const uint32_t v2 = f[k].v[2][w] ^ 0x80808080u, v3 = f[k].v[3][w] ^ 0x80808080u;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t x = __byte_perm(v0, v1, i ? 0x7362 : 0x5140);
-          const uint32_t y = __byte_perm(v2, v3, i ? 0x7362 : 0x5140);
-          const uint32_t av[4] = {two_halves(x, 0x4140), two_halves(x, 0x4342),
-                                  two_halves(y, 0x4140), two_halves(y, 0x4342)};
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma16816(o[n][2 * w + i], av, pf[n][0], pf[n][1]);
-            mma16816(o[n][2 * w + i], av, pf[n][2], pf[n][3]);
-          }
-        }
-      }
+      for (int k = 0; k < KT; ++k) kv.load_k(f[k], base + step + k);
     }
-    if (more) load_v(base + step);
+    run.template weigh<KT, false>(c, fk, corr, 0u);
+    add_values<D, NT, KT, false>(run, f, c, corr, 0u);
+    if (more) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          run.o[n][i][e] = fmaf(run.o[n][i][e], corr[n][e & 1], ref * o[n][i][e]);
+      for (int k = 0; k < KT; ++k) kv.load_v(f[k], base + step + k);
+    }
   }
-  for (int i = rank * W + warp; closed + 16 * i < lim; i += cluster * W)
-    tail_tile<D, NT>(run, kv, qf, qs, last, closed + 16 * i, total, g, t);
+  // The other closed tiles, and the tail's, one by one, from the last warp on.
+  const int mine = cluster * W - 1 - (rank * W + warp);
+  for (int tile = whole + mine; tile < tiles; tile += cluster * W) {
+    Frag<D> one[1];
+    kv.load_k(one[0], tile);
+    kv.load_v(one[0], tile);
+    float c[1][NT][4], fk[1][NT][2], corr[NT][2];
+    const uint32_t hidden = hidden_in<NT>(tile * 16, last, g);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      products<D>(c[0][n], one[0], qd[n]);
+      fk[0][n][0] = one[0].ks * qs[n][0];
+      fk[0][n][1] = one[0].ks * qs[n][1];
+    }
+    run.template weigh<1, true>(c, fk, corr, hidden);
+    add_values<D, NT, 1, true>(run, one, c, corr, hidden);
+  }
+  for (int i = mine; closed + 16 * i < lim; i += cluster * W)
+    tail_tile<D, NT>(run, kv, q_row, a.scale, last, closed + 16 * i, total, g, t);
 
   // Join the warps, then the CTAs of the cluster.
 #pragma unroll
@@ -572,151 +729,195 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, 1)
     }
   }
   __syncthreads();
-  auto joined = [](float m, float to) { return m == -INFINITY ? 0.0f : ex2(m - to); };
-  for (int r = threadIdx.x; r < R; r += blockDim.x) {
-    float m = -INFINITY, l = 0.0f;
-    for (int w = 0; w < W; ++w) m = fmaxf(m, part_m[w * R + r]);
-    for (int w = 0; w < W; ++w) l += part_l[w * R + r] * joined(part_m[w * R + r], m);
-    cta_m[r] = m;
-    cta_l[r] = l;
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < R * D; e += blockDim.x) {
-    const int r = e / D;
-    float o = 0.0f;
-    for (int w = 0; w < W; ++w)
-      o += part_o[w * R * D + e] * joined(part_m[w * R + r], cta_m[r]);
-    part_o[e] = o;
-  }
-  auto emit = [&](int e, float o, float m, float l) {
-    const int r = e / D, row = r0 + r;
+  // Four outputs of one row from `parts` partial sums.
+  auto join = [](const float* m, const float* l, int ml_step, const float* o, int o_step,
+                 int parts, float& M, float& L) {
+    M = -INFINITY;
+    L = 0.0f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < parts; ++w) M = fmaxf(M, m[w * ml_step]);
+    for (int w = 0; w < parts; ++w) {
+      const float mw = m[w * ml_step], x = mw == -INFINITY ? 0.0f : ex2(mw - M);
+      const float4 v = *reinterpret_cast<const float4*>(o + w * o_step);
+      L = fmaf(l[w * ml_step], x, L);
+      sum.x = fmaf(v.x, x, sum.x);
+      sum.y = fmaf(v.y, x, sum.y);
+      sum.z = fmaf(v.z, x, sum.z);
+      sum.w = fmaf(v.w, x, sum.w);
+    }
+    return sum;
+  };
+  auto emit = [&](int e, float4 o, float M, float L) {
+    const int row = r0 + e / D;
     if (row >= rows) return;
     const int64_t at = row_at(row);
-    a.out[at * D + e % D] = o / l;
-    if (a.lse && e % D == 0) a.lse[at] = (m + log2f(l)) * kLn2;
+    const float inv = 1.0f / L;
+    *reinterpret_cast<float4*>(a.out + at * D + e % D) =
+        make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    if (a.lse && e % D == 0) a.lse[at] = (M + log2f(L)) * kLn2;
   };
-  if (cluster == 1) {
-    for (int e = threadIdx.x; e < R * D; e += blockDim.x)   // the thread's own sums
-      emit(e, part_o[e], cta_m[e / D], cta_l[e / D]);
-    return;
-  }
-  cg::cluster_group cl = cg::this_cluster();
-  cl.sync();
-  const int share = R * D / cluster;
-  for (int i = threadIdx.x; i < share; i += blockDim.x) {
-    const int e = rank * share + i, r = e / D;
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    for (int k = 0; k < cluster; ++k) m = fmaxf(m, *cl.map_shared_rank(cta_m + r, k));
-    for (int k = 0; k < cluster; ++k) {
-      const float f = joined(*cl.map_shared_rank(cta_m + r, k), m);
-      l = fmaf(*cl.map_shared_rank(cta_l + r, k), f, l);
-      o = fmaf(*cl.map_shared_rank(part_o + e, k), f, o);
+  const int share = R * D / cluster;    // whole rows
+  const float *m_of = part_m, *l_of = part_l;
+  int parts = W;
+  if (cluster > 1) {
+    cg::cluster_group cl = cg::this_cluster();
+    cluster_wait();                     // every CTA of the cluster has started
+    for (int e = threadIdx.x * 4; e < R * D; e += blockDim.x * 4) {
+      float M, L;
+      const float4 o = join(part_m + e / D, part_l + e / D, R, part_o + e, R * D, W, M, L);
+      *reinterpret_cast<float4*>(cl.map_shared_rank(recv_o, e / share) + rank * share +
+                                 e % share) = o;
+      if (e % D == 0)
+        for (int k = 0; k < cluster; ++k) {
+          cl.map_shared_rank(recv_m, k)[rank * R + e / D] = M;
+          cl.map_shared_rank(recv_l, k)[rank * R + e / D] = L;
+        }
     }
-    emit(e, o, m, l);
+    cl.sync();
+    m_of = recv_m;
+    l_of = recv_l;
+    parts = cluster;
   }
-  cl.sync();
+  const float* o_of = cluster > 1 ? recv_o : part_o;
+  for (int i = threadIdx.x * 4; i < share; i += blockDim.x * 4) {
+    const int e = rank * share + i;
+    float M, L;
+    const float4 o = join(m_of + e / D, l_of + e / D, R, o_of + i, share, parts, M, L);
+    emit(e, o, M, L);
+  }
+  if (!a.weights || groups > 1) return;
+  // The weights of this warp's keys, which are in a cache near by, now that
+  // the sums are known.
+  float z[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = 8 * n + 2 * t + e;
+      float M = -INFINITY, L = 0.0f;
+      for (int w = 0; w < parts; ++w) M = fmaxf(M, m_of[w * R + r]);
+      for (int w = 0; w < parts; ++w) {
+        const float mw = m_of[w * R + r];
+        L = fmaf(l_of[w * R + r], mw == -INFINITY ? 0.0f : ex2(mw - M), L);
+      }
+      z[n][e] = M + log2f(L);
+      if (r >= rows) last[n][e] = -1;   // sees nothing
+    }
+  float* w_out = a.weights + ((int64_t)b * Hkv + h) * S;
+  auto weights_of = [&](float (&c)[1][NT][4], const float (&fk)[1][NT][2], int jb) {
+    const uint32_t hidden = hidden_in<NT>(jb, last, g);
+    add_weights(w_out, c, fk, z, hidden, jb, len, total, lane);
+  };
+  for (int tile = rank * W + warp; tile < tiles; tile += cluster * W) {
+    Frag<D> one;
+    kv.load_k(one, tile);
+    float c[1][NT][4], fk[1][NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      products<D>(c[0][n], one, qd[n]);
+      fk[0][n][0] = one.ks * qs[n][0];
+      fk[0][n][1] = one.ks * qs[n][1];
+    }
+    weights_of(c, fk, tile * 16);
+  }
+  for (int i = mine; closed + 16 * i < lim; i += cluster * W) {
+    float c[1][NT][4], fk[1][NT][2];
+    tail_products<D, NT>(c, fk, kv, q_row, a.scale, closed + 16 * i, total, g, t);
+    weights_of(c, fk, closed + 16 * i);
+  }
 }
 
 // ---------------------------------------------------------------------------
-// Weights: S^T again, now with the softmax sums known.  A warp keeps the keys
-// of one 16-key tile and walks the rows that see them.
+// Weights for more rows: a warp keeps the keys of two 16-key tiles, the CTA
+// turns 64 rows of q at a time into digits in shared memory, eight a warp.
 template <int D>
-__global__ void __launch_bounds__(128) kv8_weights_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(256) kv8_weights_kernel(const AttnArgs a) {
+  __shared__ uint32_t q_s[8][D / 32][3][2][32];
+  __shared__ float qs_s[8][2][32], z_s[8][8];
+  __shared__ int last_s[8][8];
   const int S = a.c.max_seq, G = a.Hq / a.c.kv_heads;
   const int bh = blockIdx.y, b = bh / a.c.kv_heads, h = bh % a.c.kv_heads;
   const int n_new = a.new_lens ? clamp_len(a.new_lens[b], a.T) : a.T;
   const int len = clamp_len(a.c.lens[b], S), total = min(len + n_new, S);
-  const int shift = 31 - __clz(a.c.block), closed = total >> shift << shift;
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int tile = blockIdx.x * 4 + (threadIdx.x >> 5), jb = tile * 16;
-  if (n_new == 0 || jb >= total) return;
-  const bool tail = jb >= closed;
-  uint32_t ka[D / 16][4], kl[D / 16][4];   // A fragments, hi and lo (tail only)
-  float up;
-  if (!tail) {
-    Keys<D> kv;
-    kv.k8 = a.c.k + (int64_t)bh * S * D;
-    kv.ks = a.c.k_scale + (int64_t)bh * (S >> shift);
-    kv.shift = shift;
-    Frag<D> f;
-    kv.load_k(f, tile, g, t);
-    up = f.ks;
-#pragma unroll
-    for (int k = 0; k < D / 16; ++k) {
-      const uint32_t w0 = reinterpret_cast<const uint32_t*>(&f.k[0][k / 4])[k % 4] ^ 0x80808080u;
-      const uint32_t w1 = reinterpret_cast<const uint32_t*>(&f.k[1][k / 4])[k % 4] ^ 0x80808080u;
-      ka[k][0] = two_halves(w0, 0x4140);
-      ka[k][1] = two_halves(w1, 0x4140);
-      ka[k][2] = two_halves(w0, 0x4342);
-      ka[k][3] = two_halves(w1, 0x4342);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) kl[k][e] = 0;
-    }
-  } else {
-    const float* kt = a.c.k_tail + (int64_t)bh * ((int64_t)D << shift);
-    float x[2][D / 64][16];
-    uint32_t mx = 0;
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int j = jb + g + 8 * r;
-      const float* row = kt + (int64_t)(j & (a.c.block - 1)) * D + 16 * t;
-#pragma unroll
-      for (int hh = 0; hh < D / 64; ++hh)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          x[r][hh][i] = j < total ? row[64 * hh + i] : 0.0f;
-          mx = max(mx, finite_abs(x[r][hh][i]));
-        }
-    }
-    float down;
-    pow2_scale(__reduce_max_sync(0xffffffffu, mx), down, up);
-#pragma unroll
-    for (int k = 0; k < D / 16; ++k) {
-      const int hh = k / 4, i = 4 * (k % 4);
-      split2(x[0][hh][i] * down, x[0][hh][i + 1] * down, ka[k][0], kl[k][0]);
-      split2(x[1][hh][i] * down, x[1][hh][i + 1] * down, ka[k][1], kl[k][1]);
-      split2(x[0][hh][i + 2] * down, x[0][hh][i + 3] * down, ka[k][2], kl[k][2]);
-      split2(x[1][hh][i + 2] * down, x[1][hh][i + 3] * down, ka[k][3], kl[k][3]);
-    }
-  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int j0 = blockIdx.x * 256;
+  if (n_new == 0 || j0 >= total) return;
+  const Keys<D> kv(a.c, bh, g, t);
+  const int closed = total >> kv.shift << kv.shift;
   const int rows = n_new * G;
-  float w[2] = {0.0f, 0.0f};
-  // rows of the tokens before the tile's first key see none of it
-  for (int r0 = max(0, jb - len) * G / 8 * 8; r0 < rows; r0 += 8) {
-    const int r = r0 + g;
-    uint32_t qf[D / 16][4];
-    float qs[2], z[2];
-    int last[2];
-    auto row_at = [&](int rr) { return ((int64_t)b * a.T + rr / G) * a.Hq + h * G + rr % G; };
-    load_q<D>(qf, qs, r < rows ? a.q + row_at(r) * D : nullptr, a.scale, t);
+  float* w_out = a.weights + (int64_t)bh * S;
+  Frag<D> f[2];
+  float w[2][2] = {};
+  auto jb = [&](int k) { return j0 + (warp * 2 + k) * 16; };
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int col = r0 + 2 * t + e;
-      z[e] = col < rows ? a.lse[row_at(col)] * kLog2e : 0.0f;
-      last[e] = col < rows ? min(len + col / G, total - 1) : -1;
+  for (int k = 0; k < 2; ++k)
+    if (jb(k) < closed) kv.load_k(f[k], jb(k) >> 4);
+  auto row_at = [&](int r) { return ((int64_t)b * a.T + r / G) * a.Hq + h * G + r % G; };
+  // rows of the tokens before the chunk's first key see none of it
+  for (int r0 = max(0, j0 - len) * G / 64 * 64; r0 < rows; r0 += 64) {
+    __syncthreads();
+    {
+      const int r = r0 + 8 * warp + g;
+      const float* row = r < rows ? a.q + row_at(r) * D : nullptr;
+      uint32_t qd[D / 32][3][2];
+      float qs[2];
+      load_q<D>(qd, qs, row, a.scale, t);
+#pragma unroll
+      for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+        for (int d = 0; d < 3; ++d)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) q_s[warp][s][d][i][lane] = qd[s][d][i];
+      qs_s[warp][0][lane] = qs[0];
+      qs_s[warp][1][lane] = qs[1];
+      if (t == 0) {
+        z_s[warp][g] = r < rows ? a.lse[row_at(r)] * kLog2e : 0.0f;
+        last_s[warp][g] = r < rows ? min(len + r / G, total - 1) : -1;
+      }
     }
-    float c[4] = {};
+    __syncthreads();
+    for (int grp = 0; grp < 8 && r0 + 8 * grp < rows; ++grp) {
+      uint32_t qd[D / 32][3][2];
 #pragma unroll
-    for (int k = 0; k < D / 16; ++k) {
-      if (tail) mma16816(c, kl[k], qf[k][0], qf[k][1]);
-      mma16816(c, ka[k], qf[k][2], qf[k][3]);
-      mma16816(c, ka[k], qf[k][0], qf[k][1]);
+      for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+        for (int d = 0; d < 3; ++d)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) qd[s][d][i] = q_s[grp][s][d][i][lane];
+      const float qs0 = qs_s[grp][0][lane], qs1 = qs_s[grp][1][lane];
+      const float z0 = z_s[grp][2 * t], z1 = z_s[grp][2 * t + 1];
+      const int last0 = last_s[grp][2 * t], last1 = last_s[grp][2 * t + 1];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (jb(k) >= total) continue;
+        float c[4], f0, f1;
+        if (jb(k) < closed) {
+          products<D>(c, f[k], qd);
+          f0 = f[k].ks * qs0;
+          f1 = f[k].ks * qs1;
+        } else {
+          const int r = r0 + 8 * grp + g;
+          const float* const row[1] = {r < rows ? a.q + row_at(r) * D : nullptr};
+          float cc[1][1][4], ff[1][1][2];
+          tail_products<D, 1>(cc, ff, kv, row, a.scale, jb(k), total, g, t);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[e] = cc[0][0][e];
+          f0 = ff[0][0][0];
+          f1 = ff[0][0][1];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int j = jb(k) + g + 8 * i;
+          if (j <= last0) w[k][i] += ex2(fmaf(c[2 * i], f0, -z0));
+          if (j <= last1) w[k][i] += ex2(fmaf(c[2 * i + 1], f1, -z1));
+        }
+      }
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (jb + g + 8 * (e >> 1) <= last[e & 1])
-        w[e >> 1] += ex2(fmaf(c[e], up * qs[e & 1], -z[e & 1]));
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    w[i] += __shfl_xor_sync(0xffffffffu, w[i], 1);
-    w[i] += __shfl_xor_sync(0xffffffffu, w[i], 2);
-    const int j = jb + g + 8 * i;
-    if (t == 0 && j < total) {
-      float* p = a.weights + (int64_t)bh * S + j;
-      *p = (j < len ? *p : 0.0f) + w[i];
-    }
-  }
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) put_weight(w_out, w[k][i], jb(k) + g + 8 * i, len, total, t);
 }
 
 template <int D, int NT>
@@ -724,23 +925,20 @@ int launch_few(cudaStream_t s, const AttnArgs& a) {
   constexpr int R = 8 * NT;
   const int groups = (int)ceil_div((int64_t)a.T * (a.Hq / a.c.kv_heads), R);
   const int64_t units = (int64_t)groups * a.c.kv_heads * a.c.batch;
-  // Spread a sequence's keys over warps while there are SMs without work and
-  // a warp still has a step of tiles; over CTAs before warps.
-  const int steps = (int)ceil_div(a.c.max_seq, D == 64 ? 64 : 32);
+  // Spread a sequence's keys over CTAs and warps while there are SMs without
+  // work and a warp still has a group of tiles.
+  const int steps = (int)ceil_div(a.c.max_seq, 16 * FewShape<D, NT>::KT);
   int W = 4, C = 1;
-  while (C < 16 && units * C * 2 <= 2 * kNumSms && C * 2 * W <= steps) C *= 2;
+  while (C < kMaxCluster && units * C * 2 <= 4 * kNumSms && C * 2 * W <= steps) C *= 2;
   while (W < kFewMaxWarps && units * C * W * 2 <= 16 * kNumSms && C * W * 2 <= steps) W *= 2;
-  const size_t smem = sizeof(float) * ((size_t)W * R * (2 + D) + 2 * R);
+  const size_t smem =
+      sizeof(float) * ((size_t)(W + 1) * R * D + 2 * W * R + 2 * kMaxCluster * R);
   auto kern = attention_kv8_few_kernel<D, NT>;
   int rc;
   if (smem > 48 * 1024 &&
       (rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                             (int)smem),
                        "attention_kv8: smem attribute")))
-    return rc;
-  if (C > 8 && (rc = check_cuda(cudaFuncSetAttribute(
-                                    kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
-                                "attention_kv8: cluster attribute")))
     return rc;
   if ((int64_t)groups * a.c.kv_heads * C > INT32_MAX || a.c.batch > 65535)
     return fail(SPX_ERR_UNSUPPORTED, "attention_kv8: grid too large");
@@ -776,18 +974,21 @@ int launch_attention_kv8(cudaStream_t s, int64_t* cnt, const float* q, const spx
   if ((int64_t)c->batch * T * Hq > INT32_MAX || bh > 65535)
     return fail(SPX_ERR_UNSUPPORTED, "attention_kv8: grid too large");
   const AttnArgs a{q, *c, new_lens, T, Hq, scale, out, lse, weights};
-  const bool wide = (int64_t)T * (Hq / c->kv_heads) > 8;
+  const int64_t rows = (int64_t)T * (Hq / c->kv_heads);
+  const bool wide = rows > 8;
+  // A group of rows that is alone adds its weights itself.
+  const bool apart = rows > (c->head_dim == 64 ? 16 : 8);
   if (c->head_dim == 64)
     rc = wide ? launch_few<64, 2>(s, a) : launch_few<64, 1>(s, a);
   else
     rc = launch_few<128, 1>(s, a);
   if (rc) return rc;
-  if ((rc = after_launch(cnt, "attention_kv8")) || !weights) return rc;
-  const dim3 wg((unsigned)ceil_div(c->max_seq, 64), (unsigned)bh);
+  if ((rc = after_launch(cnt, "attention_kv8")) || !weights || !apart) return rc;
+  const dim3 wg((unsigned)ceil_div(c->max_seq, 256), (unsigned)bh);
   if (c->head_dim == 64)
-    kv8_weights_kernel<64><<<wg, 128, 0, s>>>(a);
+    kv8_weights_kernel<64><<<wg, 256, 0, s>>>(a);
   else
-    kv8_weights_kernel<128><<<wg, 128, 0, s>>>(a);
+    kv8_weights_kernel<128><<<wg, 256, 0, s>>>(a);
   return after_launch(cnt, "attention_kv8: weights");
 }
 
