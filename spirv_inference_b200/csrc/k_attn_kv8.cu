@@ -35,15 +35,22 @@ __device__ __forceinline__ int clamp_len(int v, int hi) { return v < 0 ? 0 : v >
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+constexpr float kPUp = 32768.0f;   // 2^15
+
 struct AttnArgs {
   const float* q;
   spx_kv8_cache c;
   const int32_t* new_lens;
   int T, Hq;
+  uint32_t g_mul;   // ceil(2^32 / heads of a group)
   float scale;
   float* out;
   float* lse;
   float* weights;
+  // r / (heads of a group), exact while r times those is below 2^32
+  __device__ __forceinline__ int div_g(int r) const {
+    return g_mul ? (int)__umulhi((uint32_t)r, g_mul) : r;
+  }
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -51,21 +58,28 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                         uint32_t b1) {
+// d = a b + c.  (c apart from d: zeros and constants need no copy.)
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1, float c0, float c1, float c2, float c3) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      "{%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2),
+        "f"(c3));
 }
-__device__ __forceinline__ void mma16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  mma16816(c, a, b0, b1, c[0], c[1], c[2], c[3]);
+}
+__device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1, int c0, int c1,
+                                         int c2, int c3) {
   asm volatile(
       "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%0, %1, %2, %3};"
-      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+      "{%8, %9}, {%10, %11, %12, %13};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
 }
 __device__ __forceinline__ void cluster_arrive() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -73,19 +87,25 @@ __device__ __forceinline__ void cluster_arrive() {
 __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ uint32_t transposed8x8(uint32_t v) {
-  uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
+// Two differences in one instruction.
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) {
+  unsigned long long d;
+  b.x = -b.x;
+  b.y = -b.y;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)),
+        "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
 // (x, y) as packed fp16 hi and lo parts.
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
   const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
+  const float2 f = __half22float2(h), d = sub2(make_float2(x, y), f);
   hi = as_u32(h);
-  lo = as_u32(__floats2half2_rn(x - f.x, y - f.y));
+  lo = as_u32(__floats2half2_rn(d.x, d.y));
 }
 
 // 2^-e and 2^e for a largest magnitude with these bits (finite).
@@ -101,25 +121,29 @@ __device__ __forceinline__ uint32_t finite_abs(float x) {
 }
 
 // ---------------------------------------------------------------------------
-// Few rows (decode, drafts).  A row is a (new token, head of the group) pair.
-// Scores are held transposed, S^T = K Q^T: 16 keys are the M side of an mma
-// and 8 rows the N side, so that no lane is padding for a group of 8 heads.
-// Within a dot product the order of d is free: lane (g, t) reads 16 contiguous
-// bytes of key row g, and they are its operand as they come from memory.  The
-// output is held transposed too, O^T = V^T P^T: the lane's V bytes of four keys
-// become fp16 pairs of keys, and the 8 x 8 blocks of P go from the scores'
-// layout to the B operand's by movmatrix.  Each warp walks its own groups of
-// tiles with its own running maximum and sum; warps are joined in shared
-// memory and the CTAs of a cluster, over which one sequence's keys are spread,
-// by stores into each other's shared memory: one launch, no workspace.
+// Few rows (decode, drafts).  A row is a (new token, head of the group) pair;
+// a warp takes 8 of them, or 16, and walks its own groups of 16-key tiles with
+// its own running maxima and sums.
+//
+// Scores, S = Q K^T: the 16 rows of the A operand are the first and the second
+// digits of 8 rows of q (and in another product the third ones), the 8 columns
+// are keys.  Within a dot product the order of d is free, so lane (g, t) reads
+// 16 contiguous bytes of key g, and they are its B operand as they come from
+// memory.  Lane (g, t) then holds row g and keys 2t, 2t + 1, which is also how
+// O^T = V^T P^T wants P as its B operand.  There the lane's V bytes of four
+// keys become fp16 pairs of keys.
+//
+// Warps are joined in shared memory and the CTAs of a cluster, over which one
+// sequence's keys are spread, by stores into each other's shared memory: one
+// launch, no workspace.
 //
 // What bounds it: the cache's bytes, 2 D + 8 / block a key and head, and close
-// behind the instructions, about 140 for 16 keys of D = 64 and 8 rows (48 of
+// behind the instructions, about 150 for 16 keys of D = 64 and 8 rows (48 of
 // them turn V into fp16).  So tiles that every row sees in full take a path
 // without masks, and the others, one by one, another.
 template <int D>
 struct Frag {                   // one 16-key tile of int8 K and V in registers
-  uint4 k[2][D / 64];           // key rows g, g + 8
+  uint4 k[2][D / 64];           // keys g, g + 8
   uint32_t v[4][D / 32];        // keys 2t, 2t+1, 2t+8, 2t+9; d = D/8 g ...
   float ks, vs;
 };
@@ -157,20 +181,33 @@ struct Keys {
     kt = c.k_tail + bh * ((int64_t)D << shift);
     vt = c.v_tail + bh * ((int64_t)D << shift);
   }
-  __device__ __forceinline__ void load_k(Frag<D>& f, int tile) const {
+  // KT tiles from `tile` on (a multiple of KT: blocks of 32 and more hold two).
+  template <int KT>
+  __device__ __forceinline__ void load_k(Frag<D> (&f)[KT], int tile) const {
     const int8_t* p = k8 + (int64_t)tile * (16 * D);
+    const float* s = ks + ((tile * 16) >> shift);
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+    for (int k = 0; k < KT; ++k) {
 #pragma unroll
-      for (int h = 0; h < D / 64; ++h)
-        f.k[r][h] = __ldg(reinterpret_cast<const uint4*>(p + 8 * r * D + 64 * h));
-    f.ks = __ldg(ks + ((tile * 16) >> shift));
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h)
+          f[k].k[r][h] =
+              __ldg(reinterpret_cast<const uint4*>(p + k * 16 * D + 8 * r * D + 64 * h));
+      f[k].ks = __ldg(s + (k && shift == 4 ? k : 0));
+    }
   }
-  __device__ __forceinline__ void load_v(Frag<D>& f, int tile) const {
+  template <int KT>
+  __device__ __forceinline__ void load_v(Frag<D> (&f)[KT], int tile) const {
     const int8_t* p = v8 + (int64_t)tile * (16 * D);
+    const float* s = vs + ((tile * 16) >> shift);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load_words(f.v[i], p + ((i & 1) + 8 * (i >> 1)) * D);
-    f.vs = __ldg(vs + ((tile * 16) >> shift));
+    for (int k = 0; k < KT; ++k) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        load_words(f[k].v[i], p + k * 16 * D + ((i & 1) + 8 * (i >> 1)) * D);
+      f[k].vs = __ldg(s + (k && shift == 4 ? k : 0));
+    }
   }
 };
 
@@ -203,185 +240,222 @@ __device__ __forceinline__ uint32_t read_q(float (&x)[D / 64][16], bool& odd, co
   return mx;
 }
 
-// Q of 8 rows as B fragments, in digits: [k-step][digit][b0, b1], and for the
-// lane's two columns (rows 2t, 2t + 1) the factor that takes a product to a
-// score in units of log 2 (NaN for a row with a NaN or an infinity).
+// Digits of 8 rows of q as A fragments: [k-step][digit][4 + 4 values], and the
+// factor that takes a product of row g to a score in units of log 2 (NaN for a
+// row with a NaN or an infinity).
 template <int D>
-__device__ __forceinline__ void load_q(uint32_t (&qd)[D / 32][3][2], float (&qs)[2],
-                                       const float* row, float scale, int t) {
+__device__ __forceinline__ void load_q(uint32_t (&qd)[D / 32][3][2], float& qs, const float* row,
+                                       float scale, int t) {
   constexpr float kWhole = 8300000.0f;   // below 127 * (65536 + 256 + 1)
   float x[D / 64][16];
   bool odd;
   const float amax = __uint_as_float(read_q<D>(x, odd, row, t));
-  const float inv = amax > 1e-30f ? copysignf(kWhole / amax, scale) : 0.0f;
+  float inv = amax > 1e-30f ? copysignf(kWhole / amax, scale) : 0.0f;
+  qs = amax * (1.0f / kWhole) * (fabsf(scale) * kLog2e);
+  if (odd) qs = __int_as_float(0x7fc00000);
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i)       // four values: k-step i / 2, register i % 2
-    {
-      uint32_t w[4];
+  for (int i = 0; i < D / 16; ++i) {     // four values: k-step i / 2, register i % 2
+    uint32_t w[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        // digits in [-128, 127]: the bytes of v + 0x808080, less 128 each
-        const float v = x[i / 4][4 * (i % 4) + e] * inv;
-        w[e] = ((uint32_t)__float2int_rn(odd ? 0.0f : v) + 0x808080u) ^ 0x808080u;
-      }
-      const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[2], w[3], 0x5140);
-      const uint32_t c = __byte_perm(w[0], w[1], 0x0062), d = __byte_perm(w[2], w[3], 0x0062);
-      qd[i / 2][0][i % 2] = __byte_perm(c, d, 0x5410);
-      qd[i / 2][1][i % 2] = __byte_perm(a, b, 0x7632);
-      qd[i / 2][2][i % 2] = __byte_perm(a, b, 0x5410);
-    }
-  const float s = odd ? __int_as_float(0x7fc00000)
-                      : amax * (1.0f / kWhole) * (fabsf(scale) * kLog2e);
-  qs[0] = __shfl_sync(0xffffffffu, s, t * 8);
-  qs[1] = __shfl_sync(0xffffffffu, s, t * 8 + 4);
+    for (int e = 0; e < 4; ++e)
+      // digits in [-128, 127]: the bytes of v + 0x808080, less 128 each (of a
+      // NaN or an infinity, any)
+      w[e] = ((uint32_t)__float2int_rn(x[i / 4][4 * (i % 4) + e] * inv) + 0x808080u) ^ 0x808080u;
+    const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[2], w[3], 0x5140);
+    const uint32_t c = __byte_perm(w[0], w[1], 0x0062), d = __byte_perm(w[2], w[3], 0x0062);
+    qd[i / 2][0][i % 2] = __byte_perm(c, d, 0x5410);
+    qd[i / 2][1][i % 2] = __byte_perm(a, b, 0x7632);
+    qd[i / 2][2][i % 2] = __byte_perm(a, b, 0x5410);
+  }
 }
 
-// K Q^T of one int8 tile, before any scale.
-template <int D>
-__device__ __forceinline__ void products(float (&c)[4], const Frag<D>& f,
-                                         const uint32_t (&qd)[D / 32][3][2]) {
-  int hi[4] = {}, mid[4], lo[4];
-  auto sum = [&](int (&acc)[4], int digit) {
+// Q K^T of 8 NT rows and one int8 tile, before any scale, plus kBias: row g,
+// keys 2t, 2t + 1, 2t + 8, 2t + 9.
+constexpr float kBias = 12582912.0f;   // 1.5 2^23, of scores of about 2^30
+template <int D, int NT>
+__device__ __forceinline__ void products(float (&c)[NT][4], const Frag<D>& f,
+                                         const uint32_t (&qd)[NT][D / 32][3][2]) {
+  constexpr int kOne = 0x4b400000;     // as a float, kBias; plus a sum, kBias + the sum
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    int hi[NT][4], lo[4];
 #pragma unroll
     for (int s = 0; s < D / 32; ++s) {
-      const uint32_t* r0 = reinterpret_cast<const uint32_t*>(&f.k[0][s / 2]) + 2 * (s % 2);
-      const uint32_t* r1 = reinterpret_cast<const uint32_t*>(&f.k[1][s / 2]) + 2 * (s % 2);
-      mma16832(acc, r0[0], r1[0], r0[1], r1[1], qd[s][digit][0], qd[s][digit][1]);
+      const uint32_t* k = reinterpret_cast<const uint32_t*>(&f.k[b][s / 2]) + 2 * (s % 2);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        if (s == 0)
+          mma16832(hi[n], qd[n][s][0][0], qd[n][s][1][0], qd[n][s][0][1], qd[n][s][1][1], k[0],
+                   k[1], 0, 0, 0, 0);
+        else
+          mma16832(hi[n], qd[n][s][0][0], qd[n][s][1][0], qd[n][s][0][1], qd[n][s][1][1], k[0],
+                   k[1], hi[n][0], hi[n][1], hi[n][2], hi[n][3]);
+      // third digits: of 8 rows and none, or of 16 rows
+      const uint32_t o0 = NT == 2 ? qd[NT - 1][s][2][0] : 0u;
+      const uint32_t o1 = NT == 2 ? qd[NT - 1][s][2][1] : 0u;
+      if (s == 0)
+        mma16832(lo, qd[0][s][2][0], o0, qd[0][s][2][1], o1, k[0], k[1], kOne, kOne, kOne, kOne);
+      else
+        mma16832(lo, qd[0][s][2][0], o0, qd[0][s][2][1], o1, k[0], k[1], lo[0], lo[1], lo[2],
+                 lo[3]);
     }
-  };
-  sum(hi, 0);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) mid[e] = hi[e] * 256;     // at most 2^29
-  sum(mid, 1);
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-  for (int e = 0; e < 4; ++e) lo[e] = 0x4b400000;       // as a float: 1.5 2^23 + the sum
-  sum(lo, 2);
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    c[e] = fmaf((float)mid[e], 256.0f, __int_as_float(lo[e]) - 12582912.0f);
+      for (int e = 0; e < 2; ++e)      // at most 2^29 in the inner sum
+        c[n][2 * b + e] = fmaf((float)(hi[n][e] * 256 + hi[n][e + 2]), 256.0f,
+                               __int_as_float(lo[2 * n + e]));
+  }
 }
 
-// The running softmax of one warp: lane (g, t) holds rows (columns) 2t, 2t+1
-// of each 8 and, of the output, d = D/8 g .. D/8 (g + 1) - 1.
+// The running softmax of one warp: lane (g, t) holds maximum and sum of row g
+// of each 8 and, of the output, rows 2t, 2t+1 and d = D/8 g .. D/8 (g + 1) - 1.
 template <int D, int NT>
 struct Running {
-  float m[NT][2], l[NT][2], o[NT][D / 16][4];
+  float m[NT], l[NT], o[NT][D / 16][4];   // o in units of `ref` / 2^15
+  float ref;                              // the largest v scale so far
   __device__ __forceinline__ void init() {
+    ref = 0.0f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        m[n][e] = -INFINITY;
-        l[n][e] = 0.0f;
-      }
+      m[n] = -INFINITY;
+      l[n] = 0.0f;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
     }
   }
-  // New maxima for tile scores c f (f >= 0 the tile's factor of each column);
-  // c becomes exp2(c f - m), 0 where hidden, the sums take them, and `corr` is
-  // what the outputs so far have to be scaled by.
+  // New maxima for tile scores (c - bias) f (f >= 0 the tile's factor of row
+  // g); c becomes exp2(score - m), 0 where hidden, the sums take them, and
+  // `corr` is what the outputs of the lane's two rows have to be scaled by.
   template <int KT, bool MASK>
-  __device__ __forceinline__ void weigh(float (&c)[KT][NT][4], const float (&f)[KT][NT][2],
-                                        float (&corr)[NT][2], uint32_t hidden) {
+  __device__ __forceinline__ void weigh(float (&c)[KT][NT][4], const float (&f)[KT][NT],
+                                        float bias, float (&corr)[NT][2], uint32_t hidden,
+                                        int t) {
     auto hides = [&](int k, int n, int e) {
       return MASK && (hidden >> ((k * NT + n) * 4 + e) & 1u);
     };
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n) {
+      float mt = -INFINITY, off[KT];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float mt = -INFINITY;
+      for (int k = 0; k < KT; ++k) {
+        off[k] = -bias * f[k][n];
+        if (MASK) {
 #pragma unroll
-        for (int k = 0; k < KT; ++k) {
-          if (MASK) {
-            if (!hides(k, n, e)) mt = fmaxf(mt, c[k][n][e] * f[k][n][e]);
-            if (!hides(k, n, e + 2)) mt = fmaxf(mt, c[k][n][e + 2] * f[k][n][e]);
-          } else {
-            mt = fmaxf(mt, fmaxf(c[k][n][e], c[k][n][e + 2]) * f[k][n][e]);
-          }
+          for (int e = 0; e < 4; ++e)
+            if (!hides(k, n, e)) mt = fmaxf(mt, fmaf(c[k][n][e], f[k][n], off[k]));
+        } else {
+          const float most = fmaxf(fmaxf(c[k][n][0], c[k][n][1]), fmaxf(c[k][n][2], c[k][n][3]));
+          mt = fmaxf(mt, fmaf(most, f[k][n], off[k]));
         }
-#pragma unroll
-        for (int x = 4; x < 32; x <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
-        const float mn = fmaxf(m[n][e], mt), base = mn == -INFINITY ? 0.0f : mn;
-        corr[n][e] = ex2(m[n][e] - base);
-        m[n][e] = mn;
-        float sum = 0.0f;
-#pragma unroll
-        for (int k = 0; k < KT; ++k)
-#pragma unroll
-          for (int i = e; i < 4; i += 2) {
-            c[k][n][i] = hides(k, n, i) ? 0.0f : ex2(fmaf(c[k][n][i], f[k][n][e], -base));
-            sum += c[k][n][i];
-          }
-        l[n][e] = fmaf(l[n][e], corr[n][e], sum);
       }
+      mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+      mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
+      const float mn = fmaxf(m[n], mt), base = mn == -INFINITY ? 0.0f : mn;
+      const float down = ex2(m[n] - base);
+      m[n] = mn;
+      float sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KT; ++k) {
+        const float to = off[k] - base;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          c[k][n][e] = hides(k, n, e) ? 0.0f : ex2(fmaf(c[k][n][e], f[k][n], to));
+          sum += c[k][n][e];
+        }
+      }
+      l[n] = fmaf(l[n], down, sum);
+      corr[n][0] = __shfl_sync(0xffffffffu, down, t * 8);
+      corr[n][1] = __shfl_sync(0xffffffffu, down, t * 8 + 4);
+    }
   }
 };
 
-// P (rows of 16 keys, already scaled) as B fragments: hi b0, b1, lo b0, b1.
+// P (row g, 16 keys, already scaled) as B fragments: hi b0, b1, lo b0, b1.
 __device__ __forceinline__ void p_frags(uint32_t (&pf)[4], const float (&p)[4]) {
-  uint32_t h0, l0, h1, l1;
-  split2(p[0], p[1], h0, l0);
-  split2(p[2], p[3], h1, l1);
-  pf[0] = transposed8x8(h0);
-  pf[1] = transposed8x8(h1);
-  pf[2] = transposed8x8(l0);
-  pf[3] = transposed8x8(l1);
+  split2(p[0], p[1], pf[0], pf[2]);
+  split2(p[2], p[3], pf[1], pf[3]);
 }
 
 // Bytes 0 and 2 of a word of two's complement bytes to fp16: with the sign bit
-// flipped under 0x64, they are 1024 + 128 + value.
-__device__ __forceinline__ uint32_t even_bytes(uint32_t w) {
-  uint32_t r = (w & 0x00ff00ffu) ^ 0x64806480u;
+// flipped under 0x64, they are 1024 + 128 + value.  (mask: 0x00ff00ff in a
+// register, for one instruction: a lop3 takes one constant of its own.)
+__device__ __forceinline__ uint32_t even_bytes(uint32_t w, uint32_t mask) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, 0x64806480, 0x6a;" : "=r"(r) : "r"(w), "r"(mask));   // (w & mask) ^ c
   const __half2 v = __hsub2(*reinterpret_cast<__half2*>(&r),
                             __half2half2(__ushort_as_half((unsigned short)0x6480)));
   return as_u32(v);
 }
 
-constexpr float kPUp = 32768.0f;   // 2^15
+// The factor that takes a tile's v scale to its share of 2^15, after `ref` has
+// grown to the largest (finite) scale of KT tiles; `corr` takes what the change
+// means for the outputs so far.
+template <int D, int NT>
+__device__ __forceinline__ float share_of(Running<D, NT>& run, float largest,
+                                          float (&corr)[NT][2]) {
+  if (largest > run.ref) {               // the same in every lane
+    const float down = run.ref / largest;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      corr[n][0] *= down;
+      corr[n][1] *= down;
+    }
+    run.ref = largest;
+  }
+  return run.ref > 0.0f ? kPUp / run.ref : 0.0f;
+}
 
 // O^T += V^T P^T over KT int8 tiles; c: exp2(score - m), zero where MASK hides.
 template <int D, int NT, int KT, bool MASK>
 __device__ __forceinline__ void add_values(Running<D, NT>& run, const Frag<D> (&f)[KT],
-                                           float (&c)[KT][NT][4], const float (&corr)[NT][2],
+                                           float (&c)[KT][NT][4], float (&corr)[NT][2],
                                            uint32_t hidden) {
-  float ref = 0.0f;
-  bool odd = false;                // a block with a NaN or an infinity
+  float most = 0.0f, sum = 0.0f;
 #pragma unroll
   for (int k = 0; k < KT; ++k) {
-    const bool fine = f[k].vs <= 3.4028234663852886e38f;
-    if (fine) ref = fmaxf(ref, f[k].vs);
-    odd |= !fine;
+    most = fmaxf(most, f[k].vs);
+    sum += f[k].vs;
   }
-  const float inv = ref > 0.0f ? kPUp / ref : 0.0f;
-  float o[NT][D / 16][4];
+  const bool odd = !(sum <= 3.4028234663852886e38f);   // a block with a NaN or an infinity
+  if (odd) {
+    most = 0.0f;
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
+    for (int k = 0; k < KT; ++k)
+      if (f[k].vs <= 3.4028234663852886e38f) most = fmaxf(most, f[k].vs);
+  }
+  const float inv = share_of<D, NT>(run, most, corr);
 #pragma unroll
   for (int k = 0; k < KT; ++k) {
     const float share = f[k].vs * inv;
-    uint32_t pf[NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) c[k][n][e] *= share;
-      if (odd) {
-        // its rows' weights become NaN, other rows' stay zero
+  }
+  if (odd) {
+    // The weights of that block's keys become NaN, hidden ones stay zero.
+    asm volatile("");              // a branch, not selects
+#pragma unroll
+    for (int k = 0; k < KT; ++k)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if (!(f[k].vs <= 3.4028234663852886e38f)) c[k][n][e] = __int_as_float(0x7fc00000);
           if (MASK && (hidden >> ((k * NT + n) * 4 + e) & 1u)) c[k][n][e] = 0.0f;
         }
-      }
-      p_frags(pf[n], c[k][n]);
-    }
+  }
+  uint32_t mask;
+  asm volatile("mov.b32 %0, 0x00ff00ff;" : "=r"(mask));
+  float o[NT][D / 16][4];
+#pragma unroll
+  for (int k = 0; k < KT; ++k) {
+    uint32_t pf[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) p_frags(pf[n], c[k][n]);
 #pragma unroll
     for (int w = 0; w < D / 32; ++w)
 #pragma unroll
@@ -390,35 +464,37 @@ __device__ __forceinline__ void add_values(Running<D, NT>& run, const Frag<D> (&
         const uint32_t sel = i ? 0x7632 : 0x5410;
         const uint32_t x = __byte_perm(f[k].v[0][w], f[k].v[1][w], sel);
         const uint32_t y = __byte_perm(f[k].v[2][w], f[k].v[3][w], sel);
-        const uint32_t av[4] = {even_bytes(x), even_bytes(x >> 8), even_bytes(y),
-                                even_bytes(y >> 8)};
+        const uint32_t av[4] = {even_bytes(x, mask), even_bytes(x >> 8, mask),
+                                even_bytes(y, mask), even_bytes(y >> 8, mask)};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          mma16816(o[n][2 * w + i], av, pf[n][0], pf[n][1]);
-          mma16816(o[n][2 * w + i], av, pf[n][2], pf[n][3]);
+          float(&acc)[4] = o[n][2 * w + i];
+          if (k == 0)
+            mma16816(acc, av, pf[n][0], pf[n][1], 0.f, 0.f, 0.f, 0.f);
+          else
+            mma16816(acc, av, pf[n][0], pf[n][1]);
+          mma16816(acc, av, pf[n][2], pf[n][3]);
         }
       }
   }
-  const float back = ref * (1.0f / kPUp);
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        run.o[n][i][e] = fmaf(run.o[n][i][e], corr[n][e & 1], back * o[n][i][e]);
+        run.o[n][i][e] = fmaf(run.o[n][i][e], corr[n][e & 1], o[n][i][e]);
 }
 
 // Scores of one 16-key tile of the tail: fp32 rows, both operands split; c f as
-// for weigh().  q: the rows of q that the lane's columns g stand for (null:
-// none).
+// for weigh().  The A operand's rows are q hi and q lo.  q: row g of each 8
+// (null: none).
 template <int D, int NT>
-__device__ __forceinline__ void tail_products(float (&c)[1][NT][4], float (&f)[1][NT][2],
+__device__ __forceinline__ void tail_products(float (&c)[1][NT][4], float (&f)[1][NT],
                                               const Keys<D>& kv, const float* const (&q)[NT],
                                               float scale, int jb, int total, int g, int t) {
   const int blk_mask = (1 << kv.shift) - 1;
-  // K rows g and g + 8
-  uint32_t a[D / 16][4], al[D / 16][4];
+  uint32_t kh[2][D / 16][2], kl[2][D / 16][2];   // keys g and g + 8
   float up_k, down;
   {
     float x[2][D / 64][16];
@@ -443,13 +519,13 @@ __device__ __forceinline__ void tail_products(float (&c)[1][NT][4], float (&f)[1
     }
     pow2_scale(__reduce_max_sync(0xffffffffu, mx), down, up_k);
 #pragma unroll
-    for (int k = 0; k < D / 16; ++k) {
-      const int h = k / 4, i = 4 * (k % 4);
-      split2(x[0][h][i] * down, x[0][h][i + 1] * down, a[k][0], al[k][0]);
-      split2(x[1][h][i] * down, x[1][h][i + 1] * down, a[k][1], al[k][1]);
-      split2(x[0][h][i + 2] * down, x[0][h][i + 3] * down, a[k][2], al[k][2]);
-      split2(x[1][h][i + 2] * down, x[1][h][i + 3] * down, a[k][3], al[k][3]);
-    }
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const int h = k / 4, i = 4 * (k % 4);
+        split2(x[r][h][i] * down, x[r][h][i + 1] * down, kh[r][k][0], kl[r][k][0]);
+        split2(x[r][h][i + 2] * down, x[r][h][i + 3] * down, kh[r][k][1], kl[r][k][1]);
+      }
   }
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -457,33 +533,36 @@ __device__ __forceinline__ void tail_products(float (&c)[1][NT][4], float (&f)[1
     bool odd;
     pow2_scale(read_q<D>(x, odd, q[n], t), dn, up);
     if (scale < 0.0f) dn = -dn;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) c[0][n][e] = 0.0f;
+    float s[2][4] = {};
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
       const int h = k / 4, i = 4 * (k % 4);
-      uint32_t h0, l0, h1, l1;
-      split2(x[h][i] * dn, x[h][i + 1] * dn, h0, l0);
-      split2(x[h][i + 2] * dn, x[h][i + 3] * dn, h1, l1);
-      mma16816(c[0][n], al[k], h0, h1);
-      mma16816(c[0][n], a[k], l0, l1);
-      mma16816(c[0][n], a[k], h0, h1);
+      uint32_t a[4];
+      split2(x[h][i] * dn, x[h][i + 1] * dn, a[0], a[1]);
+      split2(x[h][i + 2] * dn, x[h][i + 3] * dn, a[2], a[3]);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        mma16816(s[r], a, kl[r][k][0], kl[r][k][1]);
+        mma16816(s[r], a, kh[r][k][0], kh[r][k][1]);
+      }
     }
-    const float s = up * up_k * (fabsf(scale) * kLog2e);
-    f[0][n][0] = __shfl_sync(0xffffffffu, s, t * 8);
-    f[0][n][1] = __shfl_sync(0xffffffffu, s, t * 8 + 4);
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) c[0][n][2 * r + e] = s[r][e] + s[r][e + 2];
+    f[0][n] = up * up_k * (fabsf(scale) * kLog2e);
   }
 }
 
-// Which of a tile's scores their columns do not see.
+// Which of a tile's scores their rows do not see.
 template <int NT>
-__device__ __forceinline__ uint32_t hidden_in(int jb, const int (&last)[NT][2], int g) {
+__device__ __forceinline__ uint32_t hidden_in(int jb, const int (&last)[NT], int t) {
   uint32_t hidden = 0;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      hidden |= (jb + g + 8 * (e >> 1) > last[n][e & 1] ? 1u : 0u) << (n * 4 + e);
+      hidden |= (jb + 2 * t + (e & 1) + 8 * (e >> 1) > last[n] ? 1u : 0u) << (n * 4 + e);
   return hidden;
 }
 
@@ -491,13 +570,13 @@ __device__ __forceinline__ uint32_t hidden_in(int jb, const int (&last)[NT][2], 
 template <int D, int NT>
 __device__ __forceinline__ void tail_tile(Running<D, NT>& run, const Keys<D>& kv,
                                           const float* const (&q)[NT], float scale,
-                                          const int (&last)[NT][2], int jb, int total, int g,
+                                          const int (&last)[NT], int jb, int total, int g,
                                           int t) {
   const int blk_mask = (1 << kv.shift) - 1;
-  float c[1][NT][4], f[1][NT][2], corr[NT][2];
+  float c[1][NT][4], f[1][NT], corr[NT][2];
   tail_products<D, NT>(c, f, kv, q, scale, jb, total, g, t);
-  const uint32_t hidden = hidden_in<NT>(jb, last, g);
-  run.template weigh<1, true>(c, f, corr, hidden);
+  const uint32_t hidden = hidden_in<NT>(jb, last, t);
+  run.template weigh<1, true>(c, f, 0.0f, corr, hidden, t);
   // V rows 2t, 2t+1, 2t+8, 2t+9
   float y[4][D / 8];
   uint32_t mx = 0;
@@ -531,15 +610,16 @@ __device__ __forceinline__ void tail_tile(Running<D, NT>& run, const Keys<D>& kv
   }
   float up_v, down;
   pow2_scale(__reduce_max_sync(0xffffffffu, mx), down, up_v);
-  const uint32_t mine = 0x11111111u << (g >> 1);   // lanes with key g's (g + 8's) V
-  const bool bad0 = (g & 1 ? bad[1] : bad[0]) & mine, bad1 = (g & 1 ? bad[3] : bad[2]) & mine;
+  // The tile's sums are in units of up_v / 2^15, the running ones of ref / 2^15.
+  const float back = up_v * (1.0f / kPUp) * share_of<D, NT>(run, up_v, corr);
   uint32_t pf[NT][4];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       c[0][n][e] *= kPUp;
-      if ((e < 2 ? bad0 : bad1) && !(hidden >> (n * 4 + e) & 1u))
+      // some lane of those with this t holds a bad value of the key
+      if ((bad[e] >> t & 0x11111111u) && !(hidden >> (n * 4 + e) & 1u))
         c[0][n][e] = __int_as_float(0x7fc00000);
     }
     p_frags(pf[n], c[0][n]);
@@ -559,33 +639,34 @@ __device__ __forceinline__ void tail_tile(Running<D, NT>& run, const Keys<D>& kv
       mma16816(o, a, pf[n][0], pf[n][1]);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        run.o[n][i][e] = fmaf(run.o[n][i][e], corr[n][e & 1], up_v * (1.0f / kPUp) * o[e]);
+        run.o[n][i][e] = fmaf(run.o[n][i][e], corr[n][e & 1], back * o[e]);
     }
   }
 }
 
-// Adds a slot's weight, summed over the four lanes that share it.
-__device__ __forceinline__ void put_weight(float* out, float w, int j, int len, int total, int t) {
-  w += __shfl_xor_sync(0xffffffffu, w, 1);
-  w += __shfl_xor_sync(0xffffffffu, w, 2);
-  if (t == 0 && j < total) out[j] = (j < len ? out[j] : 0.0f) + w;
+// Adds the weights of a tile's keys: w of keys 2t, 2t + 1, 2t + 8, 2t + 9,
+// summed over the lanes with the same t.
+__device__ __forceinline__ void put_weights(float* out, float (&w)[4], int jb, int len, int total,
+                                            int g, int t) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+#pragma unroll
+    for (int x = 4; x < 32; x <<= 1) w[e] += __shfl_xor_sync(0xffffffffu, w[e], x);
+    const int j = jb + 2 * t + (e & 1) + 8 * (e >> 1);
+    if (g == e && j < total) out[j] = (j < len ? out[j] : 0.0f) + w[e];
+  }
 }
-// exp2(c f - z) of one tile, summed over the rows that see each key.
+// w += exp2((c - bias) f - z) of row g of each 8, where it sees the key.
 template <int NT>
-__device__ __forceinline__ void add_weights(float* out, const float (&c)[1][NT][4],
-                                            const float (&f)[1][NT][2], const float (&z)[NT][2],
-                                            uint32_t hidden, int jb, int len, int total,
-                                            int lane) {
+__device__ __forceinline__ void add_weights(float (&w)[4], const float (&c)[1][NT][4],
+                                            const float (&f)[1][NT], float bias,
+                                            const float (&z)[NT], uint32_t hidden) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    float w = 0.0f;
+  for (int n = 0; n < NT; ++n) {
+    const float to = fmaf(-bias, f[0][n], -z[n]);
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if (!(hidden >> (n * 4 + 2 * i + e) & 1u))
-          w += ex2(fmaf(c[0][n][2 * i + e], f[0][n][e], -z[n][e]));
-    put_weight(out, w, jb + (lane >> 2) + 8 * i, len, total, lane & 3);
+    for (int e = 0; e < 4; ++e)
+      if (!(hidden >> (n * 4 + e) & 1u)) w[e] += ex2(fmaf(c[0][n][e], f[0][n], to));
   }
 }
 
@@ -623,17 +704,16 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
   Frag<D> f[KT];
   const bool ahead = (first + KT) * 16 <= S;
   if (ahead) {
-#pragma unroll
-    for (int k = 0; k < KT; ++k) kv.load_k(f[k], first + k);
-#pragma unroll
-    for (int k = 0; k < KT; ++k) kv.load_v(f[k], first + k);
+    kv.load_k(f, first);
+    kv.load_v(f, first);
   }
   const int r0 = grp * R, all_rows = a.T * G;
   auto row_at = [&](int r) {            // [token][head] row of the group's row r
-    return ((int64_t)b * a.T + r / G) * a.Hq + h * G + r % G;
+    const int tk = a.div_g(r);
+    return ((int64_t)b * a.T + tk) * a.Hq + h * G + (r - tk * G);
   };
   uint32_t qd[NT][D / 32][3][2];
-  float qs[NT][2];
+  float qs[NT];
   const float* q_row[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -648,85 +728,71 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
   }
   const int len = clamp_len(len_arg, S), total = min(len + n_new, S);
   const int closed = total >> kv.shift << kv.shift;
-  const int lim = min(len + min(r0 + R - 1, rows - 1) / G + 1, S);   // slots that some row sees
-  int last[NT][2];                      // the last slot that a column sees
+  // slots that some row sees
+  const int lim = min(len + a.div_g(min(r0 + R - 1, rows - 1)) + 1, S);
+  int last[NT];                         // the last slot that row g sees
 #pragma unroll
   for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      last[n][e] = min(len + min(r0 + 8 * n + 2 * t + e, rows - 1) / G, total - 1);
+    last[n] = min(len + a.div_g(min(r0 + 8 * n + g, rows - 1)), total - 1);
   Running<D, NT> run;
   run.init();
 
   // Groups of tiles that every row sees in full.
   const int tiles = (min(closed, lim) + 15) >> 4;
-  const int whole = min(closed, len + r0 / G + 1) / (16 * KT) * KT;
+  const int whole = min(closed, len + a.div_g(r0) + 1) / (16 * KT) * KT;
   if (!ahead && first < whole) {
-#pragma unroll
-    for (int k = 0; k < KT; ++k) kv.load_k(f[k], first + k);
-#pragma unroll
-    for (int k = 0; k < KT; ++k) kv.load_v(f[k], first + k);
+    kv.load_k(f, first);
+    kv.load_v(f, first);
   }
   for (int base = first; base < whole; base += step) {
-    float c[KT][NT][4], fk[KT][NT][2], corr[NT][2];
+    float c[KT][NT][4], fk[KT][NT], corr[NT][2];
 #pragma unroll
-    for (int k = 0; k < KT; ++k)
+    for (int k = 0; k < KT; ++k) {
+      products<D, NT>(c[k], f[k], qd);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        products<D>(c[k][n], f[k], qd[n]);
-        fk[k][n][0] = f[k].ks * qs[n][0];
-        fk[k][n][1] = f[k].ks * qs[n][1];
-      }
+      for (int n = 0; n < NT; ++n) fk[k][n] = f[k].ks * qs[n];
+    }
     const bool more = base + step < whole;
-    if (more) {
-#pragma unroll
-      for (int k = 0; k < KT; ++k) kv.load_k(f[k], base + step + k);
-    }
-    run.template weigh<KT, false>(c, fk, corr, 0u);
+    if (more) kv.load_k(f, base + step);
+    run.template weigh<KT, false>(c, fk, kBias, corr, 0u, t);
     add_values<D, NT, KT, false>(run, f, c, corr, 0u);
-    if (more) {
-#pragma unroll
-      for (int k = 0; k < KT; ++k) kv.load_v(f[k], base + step + k);
-    }
+    if (more) kv.load_v(f, base + step);
   }
   // The other closed tiles, and the tail's, one by one, from the last warp on.
   const int mine = cluster * W - 1 - (rank * W + warp);
   for (int tile = whole + mine; tile < tiles; tile += cluster * W) {
     Frag<D> one[1];
-    kv.load_k(one[0], tile);
-    kv.load_v(one[0], tile);
-    float c[1][NT][4], fk[1][NT][2], corr[NT][2];
-    const uint32_t hidden = hidden_in<NT>(tile * 16, last, g);
+    kv.load_k(one, tile);
+    kv.load_v(one, tile);
+    float c[1][NT][4], fk[1][NT], corr[NT][2];
+    const uint32_t hidden = hidden_in<NT>(tile * 16, last, t);
+    products<D, NT>(c[0], one[0], qd);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      products<D>(c[0][n], one[0], qd[n]);
-      fk[0][n][0] = one[0].ks * qs[n][0];
-      fk[0][n][1] = one[0].ks * qs[n][1];
-    }
-    run.template weigh<1, true>(c, fk, corr, hidden);
+    for (int n = 0; n < NT; ++n) fk[0][n] = one[0].ks * qs[n];
+    run.template weigh<1, true>(c, fk, kBias, corr, hidden, t);
     add_values<D, NT, 1, true>(run, one, c, corr, hidden);
   }
   for (int i = mine; closed + 16 * i < lim; i += cluster * W)
     tail_tile<D, NT>(run, kv, q_row, a.scale, last, closed + 16 * i, total, g, t);
 
   // Join the warps, then the CTAs of the cluster.
+  const float o_unit = run.ref * (1.0f / kPUp);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
+    float l = run.l[n];
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (t == 0) {
+      part_m[warp * R + 8 * n + g] = run.m[n];
+      part_l[warp * R + 8 * n + g] = l;
+    }
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float l = run.l[n][e];
-#pragma unroll
-      for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-      if (g == 0) {
-        part_m[warp * R + 8 * n + 2 * t + e] = run.m[n][e];
-        part_l[warp * R + 8 * n + 2 * t + e] = l;
-      }
+    for (int e = 0; e < 2; ++e)
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
         *reinterpret_cast<float2*>(part_o + ((warp * R + 8 * n + 2 * t + e) * D + D / 8 * g +
                                              2 * i)) =
-            make_float2(run.o[n][i][e], run.o[n][i][e + 2]);
-    }
+            make_float2(run.o[n][i][e] * o_unit, run.o[n][i][e + 2] * o_unit);
   }
   __syncthreads();
   // Four outputs of one row from `parts` partial sums.
@@ -788,42 +854,35 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
   if (!a.weights || groups > 1) return;
   // The weights of this warp's keys, which are in a cache near by, now that
   // the sums are known.
-  float z[NT][2];
+  float z[NT];
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = 8 * n + 2 * t + e;
-      float M = -INFINITY, L = 0.0f;
-      for (int w = 0; w < parts; ++w) M = fmaxf(M, m_of[w * R + r]);
-      for (int w = 0; w < parts; ++w) {
-        const float mw = m_of[w * R + r];
-        L = fmaf(l_of[w * R + r], mw == -INFINITY ? 0.0f : ex2(mw - M), L);
-      }
-      z[n][e] = M + log2f(L);
-      if (r >= rows) last[n][e] = -1;   // sees nothing
+  for (int n = 0; n < NT; ++n) {
+    const int r = 8 * n + g;
+    float M = -INFINITY, L = 0.0f;
+    for (int w = 0; w < parts; ++w) M = fmaxf(M, m_of[w * R + r]);
+    for (int w = 0; w < parts; ++w) {
+      const float mw = m_of[w * R + r];
+      L = fmaf(l_of[w * R + r], mw == -INFINITY ? 0.0f : ex2(mw - M), L);
     }
+    z[n] = M + log2f(L);
+    if (r >= rows) last[n] = -1;        // sees nothing
+  }
   float* w_out = a.weights + ((int64_t)b * Hkv + h) * S;
-  auto weights_of = [&](float (&c)[1][NT][4], const float (&fk)[1][NT][2], int jb) {
-    const uint32_t hidden = hidden_in<NT>(jb, last, g);
-    add_weights(w_out, c, fk, z, hidden, jb, len, total, lane);
-  };
   for (int tile = rank * W + warp; tile < tiles; tile += cluster * W) {
-    Frag<D> one;
+    Frag<D> one[1];
     kv.load_k(one, tile);
-    float c[1][NT][4], fk[1][NT][2];
+    float c[1][NT][4], fk[1][NT], w[4] = {};
+    products<D, NT>(c[0], one[0], qd);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      products<D>(c[0][n], one, qd[n]);
-      fk[0][n][0] = one.ks * qs[n][0];
-      fk[0][n][1] = one.ks * qs[n][1];
-    }
-    weights_of(c, fk, tile * 16);
+    for (int n = 0; n < NT; ++n) fk[0][n] = one[0].ks * qs[n];
+    add_weights<NT>(w, c, fk, kBias, z, hidden_in<NT>(tile * 16, last, t));
+    put_weights(w_out, w, tile * 16, len, total, g, t);
   }
   for (int i = mine; closed + 16 * i < lim; i += cluster * W) {
-    float c[1][NT][4], fk[1][NT][2];
+    float c[1][NT][4], fk[1][NT], w[4] = {};
     tail_products<D, NT>(c, fk, kv, q_row, a.scale, closed + 16 * i, total, g, t);
-    weights_of(c, fk, closed + 16 * i);
+    add_weights<NT>(w, c, fk, 0.0f, z, hidden_in<NT>(closed + 16 * i, last, t));
+    put_weights(w_out, w, closed + 16 * i, len, total, g, t);
   }
 }
 
@@ -831,9 +890,9 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
 // Weights for more rows: a warp keeps the keys of two 16-key tiles, the CTA
 // turns 64 rows of q at a time into digits in shared memory, eight a warp.
 template <int D>
-__global__ void __launch_bounds__(256) kv8_weights_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(256, D == 64 ? 2 : 1) kv8_weights_kernel(const AttnArgs a) {
   __shared__ uint32_t q_s[8][D / 32][3][2][32];
-  __shared__ float qs_s[8][2][32], z_s[8][8];
+  __shared__ float qs_s[8][8], z_s[8][8];
   __shared__ int last_s[8][8];
   const int S = a.c.max_seq, G = a.Hq / a.c.kv_heads;
   const int bh = blockIdx.y, b = bh / a.c.kv_heads, h = bh % a.c.kv_heads;
@@ -845,14 +904,16 @@ __global__ void __launch_bounds__(256) kv8_weights_kernel(const AttnArgs a) {
   const Keys<D> kv(a.c, bh, g, t);
   const int closed = total >> kv.shift << kv.shift;
   const int rows = n_new * G;
-  float* w_out = a.weights + (int64_t)bh * S;
-  Frag<D> f[2];
-  float w[2][2] = {};
+  Frag<D> f[2][1];
+  float w[2][4] = {};
   auto jb = [&](int k) { return j0 + (warp * 2 + k) * 16; };
 #pragma unroll
   for (int k = 0; k < 2; ++k)
     if (jb(k) < closed) kv.load_k(f[k], jb(k) >> 4);
-  auto row_at = [&](int r) { return ((int64_t)b * a.T + r / G) * a.Hq + h * G + r % G; };
+  auto row_at = [&](int r) {
+    const int tk = a.div_g(r);
+    return ((int64_t)b * a.T + tk) * a.Hq + h * G + (r - tk * G);
+  };
   // rows of the tokens before the chunk's first key see none of it
   for (int r0 = max(0, j0 - len) * G / 64 * 64; r0 < rows; r0 += 64) {
     __syncthreads();
@@ -860,7 +921,7 @@ __global__ void __launch_bounds__(256) kv8_weights_kernel(const AttnArgs a) {
       const int r = r0 + 8 * warp + g;
       const float* row = r < rows ? a.q + row_at(r) * D : nullptr;
       uint32_t qd[D / 32][3][2];
-      float qs[2];
+      float qs;
       load_q<D>(qd, qs, row, a.scale, t);
 #pragma unroll
       for (int s = 0; s < D / 32; ++s)
@@ -868,56 +929,43 @@ __global__ void __launch_bounds__(256) kv8_weights_kernel(const AttnArgs a) {
         for (int d = 0; d < 3; ++d)
 #pragma unroll
           for (int i = 0; i < 2; ++i) q_s[warp][s][d][i][lane] = qd[s][d][i];
-      qs_s[warp][0][lane] = qs[0];
-      qs_s[warp][1][lane] = qs[1];
       if (t == 0) {
+        qs_s[warp][g] = qs;
         z_s[warp][g] = r < rows ? a.lse[row_at(r)] * kLog2e : 0.0f;
-        last_s[warp][g] = r < rows ? min(len + r / G, total - 1) : -1;
+        last_s[warp][g] = r < rows ? min(len + a.div_g(r), total - 1) : -1;
       }
     }
     __syncthreads();
     for (int grp = 0; grp < 8 && r0 + 8 * grp < rows; ++grp) {
-      uint32_t qd[D / 32][3][2];
+      uint32_t qd[1][D / 32][3][2];
 #pragma unroll
       for (int s = 0; s < D / 32; ++s)
 #pragma unroll
         for (int d = 0; d < 3; ++d)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) qd[s][d][i] = q_s[grp][s][d][i][lane];
-      const float qs0 = qs_s[grp][0][lane], qs1 = qs_s[grp][1][lane];
-      const float z0 = z_s[grp][2 * t], z1 = z_s[grp][2 * t + 1];
-      const int last0 = last_s[grp][2 * t], last1 = last_s[grp][2 * t + 1];
+          for (int i = 0; i < 2; ++i) qd[0][s][d][i] = q_s[grp][s][d][i][lane];
+      const float qs = qs_s[grp][g], z[1] = {z_s[grp][g]};
+      const int last[1] = {last_s[grp][g]};
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         if (jb(k) >= total) continue;
-        float c[4], f0, f1;
+        float c[1][1][4], fk[1][1];
         if (jb(k) < closed) {
-          products<D>(c, f[k], qd);
-          f0 = f[k].ks * qs0;
-          f1 = f[k].ks * qs1;
+          products<D, 1>(c[0], f[k][0], qd);
+          fk[0][0] = f[k][0].ks * qs;
+          add_weights<1>(w[k], c, fk, kBias, z, hidden_in<1>(jb(k), last, t));
         } else {
           const int r = r0 + 8 * grp + g;
           const float* const row[1] = {r < rows ? a.q + row_at(r) * D : nullptr};
-          float cc[1][1][4], ff[1][1][2];
-          tail_products<D, 1>(cc, ff, kv, row, a.scale, jb(k), total, g, t);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) c[e] = cc[0][0][e];
-          f0 = ff[0][0][0];
-          f1 = ff[0][0][1];
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int j = jb(k) + g + 8 * i;
-          if (j <= last0) w[k][i] += ex2(fmaf(c[2 * i], f0, -z0));
-          if (j <= last1) w[k][i] += ex2(fmaf(c[2 * i + 1], f1, -z1));
+          tail_products<D, 1>(c, fk, kv, row, a.scale, jb(k), total, g, t);
+          add_weights<1>(w[k], c, fk, 0.0f, z, hidden_in<1>(jb(k), last, t));
         }
       }
     }
   }
 #pragma unroll
   for (int k = 0; k < 2; ++k)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) put_weight(w_out, w[k][i], jb(k) + g + 8 * i, len, total, t);
+    put_weights(a.weights + (int64_t)bh * S, w[k], jb(k), len, total, g, t);
 }
 
 template <int D, int NT>
@@ -973,8 +1021,11 @@ int launch_attention_kv8(cudaStream_t s, int64_t* cnt, const float* q, const spx
   const int64_t bh = (int64_t)c->batch * c->kv_heads;
   if ((int64_t)c->batch * T * Hq > INT32_MAX || bh > 65535)
     return fail(SPX_ERR_UNSUPPORTED, "attention_kv8: grid too large");
-  const AttnArgs a{q, *c, new_lens, T, Hq, scale, out, lse, weights};
-  const int64_t rows = (int64_t)T * (Hq / c->kv_heads);
+  const int G = Hq / c->kv_heads;
+  const int64_t rows = (int64_t)T * G;
+  if (rows * G > UINT32_MAX) return fail(SPX_ERR_UNSUPPORTED, "attention_kv8: too many rows");
+  const uint32_t g_mul = G > 1 ? (uint32_t)(((1ull << 32) + G - 1) / G) : 0u;
+  const AttnArgs a{q, *c, new_lens, T, Hq, g_mul, scale, out, lse, weights};
   const bool wide = rows > 8;
   // A group of rows that is alone adds its weights itself.
   const bool apart = rows > (c->head_dim == 64 ? 16 : 8);
