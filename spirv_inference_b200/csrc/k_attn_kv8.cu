@@ -23,6 +23,8 @@
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "spx_internal.cuh"
 
 namespace spx {
@@ -127,11 +129,14 @@ __device__ __forceinline__ uint32_t finite_abs(float x) {
 //
 // Scores, S = Q K^T: the 16 rows of the A operand are the first and the second
 // digits of 8 rows of q (and in another product the third ones), the 8 columns
-// are keys.  Within a dot product the order of d is free, so lane (g, t) reads
-// 16 contiguous bytes of key g, and they are its B operand as they come from
-// memory.  Lane (g, t) then holds row g and keys 2t, 2t + 1, which is also how
-// O^T = V^T P^T wants P as its B operand.  There the lane's V bytes of four
+// are keys.  Within a dot product the order of d is free, so lane (g, t) takes
+// 16 contiguous bytes of a key, and they are its B operand as they come from
+// memory.  Lane (g, t) then holds row g and two keys of eight, which is also
+// how O^T = V^T P^T wants P as its B operand.  There the lane's V bytes of four
 // keys become fp16 pairs of keys.
+//
+// A warp copies its next groups of 32 keys to shared memory for itself, three
+// ahead (64 D bytes each, 192 KB an SM), with no barrier but its own.
 //
 // Warps are joined in shared memory and the CTAs of a cluster, over which one
 // sequence's keys are spread, by stores into each other's shared memory: one
@@ -141,72 +146,155 @@ __device__ __forceinline__ uint32_t finite_abs(float x) {
 // behind the instructions, about 150 for 16 keys of D = 64 and 8 rows (48 of
 // them turn V into fp16).  So tiles that every row sees in full take a path
 // without masks, and the others, one by one, another.
+// Which key of eight stands in column n: the order in which lanes' reads of K
+// (keys_at(g), 16 bytes at t) and of V (keys_at(2t), keys_at(2t + 1), 8 bytes
+// at g) meet no bank of shared memory twice.
+__device__ __forceinline__ int key_at(int n) { return n & 1 ? ((n >> 1) ^ 1) + 4 : n >> 1; }
+// The key of 16 that score e of a lane belongs to.
+__device__ __forceinline__ int key_of(int e, int t) {
+  return 8 * (e >> 1) + (e & 1 ? (t ^ 1) + 4 : t);
+}
+// 16-byte pieces of a row are exchanged by this in shared memory.
+template <int D>
+__device__ __forceinline__ int row_swap(int row) {
+  return (D == 128 ? 4 * (row & 1) : 0) + (row & 2);
+}
+
 template <int D>
 struct Frag {                   // one 16-key tile of int8 K and V in registers
-  uint4 k[2][D / 64];           // keys g, g + 8
-  uint32_t v[4][D / 32];        // keys 2t, 2t+1, 2t+8, 2t+9; d = D/8 g ...
+  uint4 k[2][D / 64];           // keys key_at(g), + 8
+  uint32_t v[4][D / 32];        // keys key_of(0 .. 3); d = D/8 g ...
   float ks, vs;
 };
 
 template <int NW>
-__device__ __forceinline__ void load_words(uint32_t (&w)[NW], const void* p) {
-  if constexpr (NW == 2) {
-    const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
-    w[0] = x.x;
-    w[1] = x.y;
-  } else {
-    const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
-    w[0] = x.x;
-    w[1] = x.y;
-    w[2] = x.z;
-    w[3] = x.w;
-  }
+__device__ __forceinline__ void put_words(uint32_t (&w)[NW], uint2 x) {
+  w[0] = x.x;
+  w[1] = x.y;
+}
+template <int NW>
+__device__ __forceinline__ void put_words(uint32_t (&w)[NW], uint4 x) {
+  w[0] = x.x;
+  w[1] = x.y;
+  w[2] = x.z;
+  w[3] = x.w;
 }
 
 template <int D>
 struct Keys {
-  const int8_t* k8;    // at the lane's place in the first tile
+  using Words = typename std::conditional<D == 64, uint2, uint4>::type;
+  const int8_t* k8;
   const int8_t* v8;
   const float* ks;
   const float* vs;
   const float* kt;
   const float* vt;
   int shift;           // log2(block)
-  __device__ __forceinline__ Keys(const spx_kv8_cache& c, int64_t bh, int g, int t) {
+  __device__ __forceinline__ Keys(const spx_kv8_cache& c, int64_t bh) {
     shift = 31 - __clz(c.block);
-    k8 = c.k + bh * c.max_seq * D + g * D + 16 * t;
-    v8 = c.v + bh * c.max_seq * D + 2 * t * D + D / 8 * g;
+    k8 = c.k + bh * c.max_seq * D;
+    v8 = c.v + bh * c.max_seq * D;
     ks = c.k_scale + bh * (c.max_seq >> shift);
     vs = c.v_scale + bh * (c.max_seq >> shift);
     kt = c.k_tail + bh * ((int64_t)D << shift);
     vt = c.v_tail + bh * ((int64_t)D << shift);
   }
-  // KT tiles from `tile` on (a multiple of KT: blocks of 32 and more hold two).
-  template <int KT>
-  __device__ __forceinline__ void load_k(Frag<D> (&f)[KT], int tile) const {
-    const int8_t* p = k8 + (int64_t)tile * (16 * D);
-    const float* s = ks + ((tile * 16) >> shift);
+  // One tile from global memory.
+  __device__ __forceinline__ void load_k(Frag<D>& f, int tile, int g, int t) const {
+    const int8_t* p = k8 + (int64_t)tile * (16 * D) + key_at(g) * D + 16 * t;
 #pragma unroll
-    for (int k = 0; k < KT; ++k) {
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
+      for (int h = 0; h < D / 64; ++h)
+        f.k[r][h] = __ldg(reinterpret_cast<const uint4*>(p + 8 * r * D + 64 * h));
+    f.ks = __ldg(ks + ((tile * 16) >> shift));
+  }
+  __device__ __forceinline__ void load_v(Frag<D>& f, int tile, int g, int t) const {
+    const int8_t* p = v8 + (int64_t)tile * (16 * D) + D / 8 * g;
 #pragma unroll
-        for (int h = 0; h < D / 64; ++h)
-          f[k].k[r][h] =
-              __ldg(reinterpret_cast<const uint4*>(p + k * 16 * D + 8 * r * D + 64 * h));
-      f[k].ks = __ldg(s + (k && shift == 4 ? k : 0));
+    for (int e = 0; e < 4; ++e)
+      put_words(f.v[e], __ldg(reinterpret_cast<const Words*>(p + key_of(e, t) * D)));
+    f.vs = __ldg(vs + ((tile * 16) >> shift));
+  }
+};
+
+// A warp's ring of groups of 32 keys in shared memory.
+template <int D>
+struct Ring {
+  static constexpr int kSlots = 3, kGroup = 32 * D, kSlot = 2 * kGroup;   // bytes: K, then V
+  uint32_t here;          // the lane's place in the ring, as it copies
+  uint32_t k_at[D / 64];  // the lane's bytes of K and V in a slot
+  uint32_t v_at[2];
+  __device__ __forceinline__ Ring(uint8_t* mem, int lane, int g, int t) {
+    const uint32_t base = (uint32_t)__cvta_generic_to_shared(mem);
+    constexpr int kPieces = D / 16;
+    const int row = lane / kPieces;
+    here = base + row * D + ((lane % kPieces) ^ row_swap<D>(row)) * 16;
+    const int k = key_at(g);
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h)
+      k_at[h] = base + k * D + ((t + 4 * h) ^ row_swap<D>(k)) * 16;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int v = key_of(e, t);
+      v_at[e] = base + kGroup + v * D +
+                (D == 64 ? ((g >> 1) ^ row_swap<D>(v)) * 16 + (g & 1) * 8
+                         : (g ^ row_swap<D>(v)) * 16);
     }
   }
-  template <int KT>
-  __device__ __forceinline__ void load_v(Frag<D> (&f)[KT], int tile) const {
-    const int8_t* p = v8 + (int64_t)tile * (16 * D);
-    const float* s = vs + ((tile * 16) >> shift);
+  // Starts the copies of the 32 keys from tile `tile` on, if any.
+  __device__ __forceinline__ void start(int slot, const Keys<D>& kv, int tile, bool any,
+                                        bool with_v, int lane) const {
+    if (any) {
+      const int64_t from = (int64_t)tile * (16 * D) + lane * 16;
+      const uint32_t to = here + slot * kSlot;
 #pragma unroll
-    for (int k = 0; k < KT; ++k) {
+      for (int i = 0; i < kGroup / 512; ++i)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * 512),
+                     "l"(kv.k8 + from + i * 512)
+                     : "memory");
+      if (with_v) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        load_words(f[k].v[i], p + k * 16 * D + ((i & 1) + 8 * (i >> 1)) * D);
-      f[k].vs = __ldg(s + (k && shift == 4 ? k : 0));
+        for (int i = 0; i < kGroup / 512; ++i)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + kGroup + i * 512),
+                       "l"(kv.v8 + from + i * 512)
+                       : "memory");
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // Until the oldest of kSlots groups is there, for the whole warp.
+  __device__ __forceinline__ void wait() const {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 1) : "memory");
+    __syncwarp();
+  }
+  __device__ __forceinline__ void drain() const {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
+  }
+  __device__ __forceinline__ void read_k(Frag<D>& f, int slot, int k) const {
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int h = 0; h < D / 64; ++h) {
+        uint4& x = f.k[r][h];
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                     : "r"(k_at[h] + slot * kSlot + (16 * k + 8 * r) * D));
+      }
+  }
+  __device__ __forceinline__ void read_v(Frag<D>& f, int slot, int k) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t at = v_at[e & 1] + slot * kSlot + (16 * k + 8 * (e >> 1)) * D;
+      if constexpr (D == 64)
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                     : "=r"(f.v[e][0]), "=r"(f.v[e][1])
+                     : "r"(at));
+      else
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(f.v[e][0]), "=r"(f.v[e][1]), "=r"(f.v[e][2]), "=r"(f.v[e][3])
+                     : "r"(at));
     }
   }
 };
@@ -270,7 +358,7 @@ __device__ __forceinline__ void load_q(uint32_t (&qd)[D / 32][3][2], float& qs, 
 }
 
 // Q K^T of 8 NT rows and one int8 tile, before any scale, plus kBias: row g,
-// keys 2t, 2t + 1, 2t + 8, 2t + 9.
+// keys key_of(0 .. 3).
 constexpr float kBias = 12582912.0f;   // 1.5 2^23, of scores of about 2^30
 template <int D, int NT>
 __device__ __forceinline__ void products(float (&c)[NT][4], const Frag<D>& f,
@@ -460,7 +548,7 @@ __device__ __forceinline__ void add_values(Running<D, NT>& run, const Frag<D> (&
     for (int w = 0; w < D / 32; ++w)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        // d = 2 (2w + i) and + 1 of keys (2t, 2t + 1) and (2t + 8, 2t + 9)
+        // d = 2 (2w + i) and + 1 of keys key_of(0, 1) and key_of(2, 3)
         const uint32_t sel = i ? 0x7632 : 0x5410;
         const uint32_t x = __byte_perm(f[k].v[0][w], f[k].v[1][w], sel);
         const uint32_t y = __byte_perm(f[k].v[2][w], f[k].v[3][w], sel);
@@ -494,14 +582,14 @@ __device__ __forceinline__ void tail_products(float (&c)[1][NT][4], float (&f)[1
                                               const Keys<D>& kv, const float* const (&q)[NT],
                                               float scale, int jb, int total, int g, int t) {
   const int blk_mask = (1 << kv.shift) - 1;
-  uint32_t kh[2][D / 16][2], kl[2][D / 16][2];   // keys g and g + 8
+  uint32_t kh[2][D / 16][2], kl[2][D / 16][2];   // keys key_at(g), + 8
   float up_k, down;
   {
     float x[2][D / 64][16];
     uint32_t mx = 0;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int j = jb + g + 8 * r;
+      const int j = jb + key_at(g) + 8 * r;
       const float* row = kv.kt + (int64_t)(j & blk_mask) * D + 16 * t;
 #pragma unroll
       for (int h = 0; h < D / 64; ++h)
@@ -562,7 +650,7 @@ __device__ __forceinline__ uint32_t hidden_in(int jb, const int (&last)[NT], int
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      hidden |= (jb + 2 * t + (e & 1) + 8 * (e >> 1) > last[n] ? 1u : 0u) << (n * 4 + e);
+      hidden |= (jb + key_of(e, t) > last[n] ? 1u : 0u) << (n * 4 + e);
   return hidden;
 }
 
@@ -577,13 +665,13 @@ __device__ __forceinline__ void tail_tile(Running<D, NT>& run, const Keys<D>& kv
   tail_products<D, NT>(c, f, kv, q, scale, jb, total, g, t);
   const uint32_t hidden = hidden_in<NT>(jb, last, t);
   run.template weigh<1, true>(c, f, 0.0f, corr, hidden, t);
-  // V rows 2t, 2t+1, 2t+8, 2t+9
+  // V of keys key_of(0 .. 3)
   float y[4][D / 8];
   uint32_t mx = 0;
   uint32_t bad[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int j = jb + 2 * t + (i & 1) + 8 * (i >> 1);
+    const int j = jb + key_of(i, t);
     const float* row = kv.vt + (int64_t)(j & blk_mask) * D + D / 8 * g;
     bool odd = false;
 #pragma unroll
@@ -644,17 +732,17 @@ __device__ __forceinline__ void tail_tile(Running<D, NT>& run, const Keys<D>& kv
   }
 }
 
-// Adds the weights of a tile's keys: w of keys 2t, 2t + 1, 2t + 8, 2t + 9,
-// summed over the lanes with the same t.
-__device__ __forceinline__ void put_weights(float* out, float (&w)[4], int jb, int len, int total,
-                                            int g, int t) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-#pragma unroll
-    for (int x = 4; x < 32; x <<= 1) w[e] += __shfl_xor_sync(0xffffffffu, w[e], x);
-    const int j = jb + 2 * t + (e & 1) + 8 * (e >> 1);
-    if (g == e && j < total) out[j] = (j < len ? out[j] : 0.0f) + w[e];
-  }
+// Adds the weights of a tile's keys: w of keys key_of(0 .. 3), summed over the
+// lanes with the same t (each step leaves a lane half of the values).
+__device__ __forceinline__ void put_weights(float* out, const float (&w)[4], int jb, int len,
+                                            int total, int g, int t) {
+  const bool up = g & 4, right = g & 2;
+  const float a = (up ? w[2] : w[0]) + __shfl_xor_sync(0xffffffffu, up ? w[0] : w[2], 16);
+  const float b = (up ? w[3] : w[1]) + __shfl_xor_sync(0xffffffffu, up ? w[1] : w[3], 16);
+  float sum = (right ? b : a) + __shfl_xor_sync(0xffffffffu, right ? a : b, 8);
+  sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+  const int j = jb + key_of((up ? 2 : 0) + (right ? 1 : 0), t);
+  if (!(g & 1) && j < total) out[j] = (j < len ? out[j] : 0.0f) + sum;
 }
 // w += exp2((c - bias) f - z) of row g of each 8, where it sees the key.
 template <int NT>
@@ -675,19 +763,29 @@ constexpr int kMaxCluster = 8;
 
 template <int D, int NT>
 struct FewShape {
-  static constexpr int KT = 2;                            // tiles of a group
-  static constexpr int R = 8 * NT;                        // rows
-  static constexpr int kBlocks = D == 64 && NT == 1 ? 2 : 1;   // of 8 warps an SM
+  static constexpr int KT = 2;          // tiles of a group of 32 keys
+  static constexpr int R = 8 * NT;      // rows
+  // Warps an SM that the rings leave room for: 16, or 8 of D = 128.
+  static constexpr int kBlocks = D == 64 && NT == 1 ? 2 : 1;   // of 8 warps
+  // Shared memory in floats: the warps' rings (later their partial outputs),
+  // then what the others of the cluster send, then maxima and sums.
+  static constexpr int kRing = Ring<D>::kSlots * Ring<D>::kSlot / 4;
+  static_assert(R * D <= kRing, "partial outputs fit a ring");
+  static constexpr size_t smem(int W) {
+    return sizeof(float) * ((size_t)W * kRing + R * D + 2 * W * R + 2 * kMaxCluster * R);
+  }
 };
 
 template <int D, int NT>
 __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
     attention_kv8_few_kernel(const AttnArgs a, int groups, int cluster) {
-  constexpr int KT = FewShape<D, NT>::KT, R = FewShape<D, NT>::R;
+  using Shape = FewShape<D, NT>;
+  constexpr int KT = Shape::KT, R = Shape::R, kRing = Shape::kRing;
+  constexpr int kSlots = Ring<D>::kSlots;
   extern __shared__ __align__(16) float smem[];
   const int W = blockDim.x >> 5;
-  float* part_o = smem;                 // [W][R][D]
-  float* recv_o = part_o + W * R * D;   // [cluster][R D / cluster]: this CTA's share
+  float* part_o = smem;                 // [W][kRing], the first R D of each
+  float* recv_o = part_o + W * kRing;   // [cluster][R D / cluster]: this CTA's share
   float* part_m = recv_o + R * D;       // [W][R]
   float* part_l = part_m + W * R;       // [W][R]
   float* recv_m = part_l + W * R;       // [cluster][R]
@@ -699,14 +797,12 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
   if (cluster > 1) cluster_arrive();    // waited for before stores into other CTAs
   // What does not depend on the lengths is on its way before they are known.
   const int n_arg = a.new_lens ? a.new_lens[b] : a.T, len_arg = a.c.lens[b];
-  const Keys<D> kv(a.c, (int64_t)b * Hkv + h, g, t);
+  const Keys<D> kv(a.c, (int64_t)b * Hkv + h);
+  const Ring<D> ring(reinterpret_cast<uint8_t*>(part_o + warp * kRing), lane, g, t);
   const int first = (rank * W + warp) * KT, step = cluster * W * KT;
-  Frag<D> f[KT];
-  const bool ahead = (first + KT) * 16 <= S;
-  if (ahead) {
-    kv.load_k(f, first);
-    kv.load_v(f, first);
-  }
+#pragma unroll
+  for (int s = 0; s < kSlots; ++s)
+    ring.start(s, kv, first + s * step, (first + s * step + KT) * 16 <= S, true, lane);
   const int r0 = grp * R, all_rows = a.T * G;
   auto row_at = [&](int r) {            // [token][head] row of the group's row r
     const int tk = a.div_g(r);
@@ -723,6 +819,7 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
   }
   const int n_new = clamp_len(n_arg, a.T), rows = n_new * G;
   if (r0 >= rows) {                     // the whole cluster
+    ring.drain();
     if (cluster > 1) cluster_wait();
     return;
   }
@@ -740,30 +837,50 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
   // Groups of tiles that every row sees in full.
   const int tiles = (min(closed, lim) + 15) >> 4;
   const int whole = min(closed, len + a.div_g(r0) + 1) / (16 * KT) * KT;
-  if (!ahead && first < whole) {
-    kv.load_k(f, first);
-    kv.load_v(f, first);
-  }
+  // (a block of 32 keys or more holds both tiles of a group)
+  const int second = kv.shift == 4 ? 1 : 0;
+  auto scales = [&](float (&s)[2 * KT], int base) {
+    if (base >= whole) return;
+    const int blk = (base * 16) >> kv.shift;
+    s[0] = __ldg(kv.ks + blk);
+    s[1] = __ldg(kv.ks + blk + second);
+    s[2] = __ldg(kv.vs + blk);
+    s[3] = __ldg(kv.vs + blk + second);
+  };
+  float sc[2 * KT], sc_next[2 * KT] = {};
+  scales(sc_next, first);
+  int slot = 0;
   for (int base = first; base < whole; base += step) {
     float c[KT][NT][4], fk[KT][NT], corr[NT][2];
+    Frag<D> f[KT];
+#pragma unroll
+    for (int i = 0; i < 2 * KT; ++i) sc[i] = sc_next[i];
+    scales(sc_next, base + step);
+    ring.wait();
 #pragma unroll
     for (int k = 0; k < KT; ++k) {
+      ring.read_k(f[k], slot, k);
       products<D, NT>(c[k], f[k], qd);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) fk[k][n] = f[k].ks * qs[n];
+      for (int n = 0; n < NT; ++n) fk[k][n] = sc[k] * qs[n];
+      f[k].vs = sc[KT + k];
     }
-    const bool more = base + step < whole;
-    if (more) kv.load_k(f, base + step);
     run.template weigh<KT, false>(c, fk, kBias, corr, 0u, t);
+#pragma unroll
+    for (int k = 0; k < KT; ++k) ring.read_v(f[k], slot, k);
     add_values<D, NT, KT, false>(run, f, c, corr, 0u);
-    if (more) kv.load_v(f, base + step);
+    __syncwarp();                       // all lanes have read the slot
+    const int ahead = base + kSlots * step;
+    ring.start(slot, kv, ahead, ahead < whole, true, lane);
+    slot = slot == kSlots - 1 ? 0 : slot + 1;
   }
+  ring.drain();
   // The other closed tiles, and the tail's, one by one, from the last warp on.
   const int mine = cluster * W - 1 - (rank * W + warp);
   for (int tile = whole + mine; tile < tiles; tile += cluster * W) {
     Frag<D> one[1];
-    kv.load_k(one, tile);
-    kv.load_v(one, tile);
+    kv.load_k(one[0], tile, g, t);
+    kv.load_v(one[0], tile, g, t);
     float c[1][NT][4], fk[1][NT], corr[NT][2];
     const uint32_t hidden = hidden_in<NT>(tile * 16, last, t);
     products<D, NT>(c[0], one[0], qd);
@@ -790,8 +907,8 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
     for (int e = 0; e < 2; ++e)
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
-        *reinterpret_cast<float2*>(part_o + ((warp * R + 8 * n + 2 * t + e) * D + D / 8 * g +
-                                             2 * i)) =
+        *reinterpret_cast<float2*>(part_o + warp * kRing + (8 * n + 2 * t + e) * D + D / 8 * g +
+                                   2 * i) =
             make_float2(run.o[n][i][e] * o_unit, run.o[n][i][e + 2] * o_unit);
   }
   __syncthreads();
@@ -830,7 +947,7 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
     cluster_wait();                     // every CTA of the cluster has started
     for (int e = threadIdx.x * 4; e < R * D; e += blockDim.x * 4) {
       float M, L;
-      const float4 o = join(part_m + e / D, part_l + e / D, R, part_o + e, R * D, W, M, L);
+      const float4 o = join(part_m + e / D, part_l + e / D, R, part_o + e, kRing, W, M, L);
       *reinterpret_cast<float4*>(cl.map_shared_rank(recv_o, e / share) + rank * share +
                                  e % share) = o;
       if (e % D == 0)
@@ -845,10 +962,11 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
     parts = cluster;
   }
   const float* o_of = cluster > 1 ? recv_o : part_o;
+  const int o_step = cluster > 1 ? share : kRing;
   for (int i = threadIdx.x * 4; i < share; i += blockDim.x * 4) {
     const int e = rank * share + i;
     float M, L;
-    const float4 o = join(m_of + e / D, l_of + e / D, R, o_of + i, share, parts, M, L);
+    const float4 o = join(m_of + e / D, l_of + e / D, R, o_of + i, o_step, parts, M, L);
     emit(e, o, M, L);
   }
   if (!a.weights || groups > 1) return;
@@ -868,13 +986,45 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
     if (r >= rows) last[n] = -1;        // sees nothing
   }
   float* w_out = a.weights + ((int64_t)b * Hkv + h) * S;
-  for (int tile = rank * W + warp; tile < tiles; tile += cluster * W) {
-    Frag<D> one[1];
-    kv.load_k(one, tile);
-    float c[1][NT][4], fk[1][NT], w[4] = {};
-    products<D, NT>(c[0], one[0], qd);
+  // (the partial outputs in the ring have been read: every thread of the CTA
+  // is past its share before the next copies)
+  __syncthreads();
 #pragma unroll
-    for (int n = 0; n < NT; ++n) fk[0][n] = one[0].ks * qs[n];
+  for (int s = 0; s < kSlots; ++s)
+    ring.start(s, kv, first + s * step, first + s * step < whole, false, lane);
+  scales(sc_next, first);
+  slot = 0;
+  for (int base = first; base < whole; base += step) {
+    float keep[KT];
+#pragma unroll
+    for (int k = 0; k < KT; ++k) keep[k] = sc_next[k];
+    scales(sc_next, base + step);
+    ring.wait();
+#pragma unroll
+    for (int k = 0; k < KT; ++k) {
+      Frag<D> one;
+      ring.read_k(one, slot, k);
+      float c[1][NT][4], fk[1][NT], w[4] = {};
+      products<D, NT>(c[0], one, qd);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) fk[0][n] = keep[k] * qs[n];
+      // (rows past the last see nothing, the others all of a whole group)
+      add_weights<NT>(w, c, fk, kBias, z, hidden_in<NT>((base + k) * 16, last, t));
+      put_weights(w_out, w, (base + k) * 16, len, total, g, t);
+    }
+    __syncwarp();
+    const int ahead = base + kSlots * step;
+    ring.start(slot, kv, ahead, ahead < whole, false, lane);
+    slot = slot == kSlots - 1 ? 0 : slot + 1;
+  }
+  ring.drain();
+  for (int tile = whole + mine; tile < tiles; tile += cluster * W) {
+    Frag<D> one;
+    kv.load_k(one, tile, g, t);
+    float c[1][NT][4], fk[1][NT], w[4] = {};
+    products<D, NT>(c[0], one, qd);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) fk[0][n] = one.ks * qs[n];
     add_weights<NT>(w, c, fk, kBias, z, hidden_in<NT>(tile * 16, last, t));
     put_weights(w_out, w, tile * 16, len, total, g, t);
   }
@@ -901,15 +1051,15 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) kv8_weights_kernel(const
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int j0 = blockIdx.x * 256;
   if (n_new == 0 || j0 >= total) return;
-  const Keys<D> kv(a.c, bh, g, t);
+  const Keys<D> kv(a.c, bh);
   const int closed = total >> kv.shift << kv.shift;
   const int rows = n_new * G;
-  Frag<D> f[2][1];
+  Frag<D> f[2];
   float w[2][4] = {};
   auto jb = [&](int k) { return j0 + (warp * 2 + k) * 16; };
 #pragma unroll
   for (int k = 0; k < 2; ++k)
-    if (jb(k) < closed) kv.load_k(f[k], jb(k) >> 4);
+    if (jb(k) < closed) kv.load_k(f[k], jb(k) >> 4, g, t);
   auto row_at = [&](int r) {
     const int tk = a.div_g(r);
     return ((int64_t)b * a.T + tk) * a.Hq + h * G + (r - tk * G);
@@ -951,8 +1101,8 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) kv8_weights_kernel(const
         if (jb(k) >= total) continue;
         float c[1][1][4], fk[1][1];
         if (jb(k) < closed) {
-          products<D, 1>(c[0], f[k][0], qd);
-          fk[0][0] = f[k][0].ks * qs;
+          products<D, 1>(c[0], f[k], qd);
+          fk[0][0] = f[k].ks * qs;
           add_weights<1>(w[k], c, fk, kBias, z, hidden_in<1>(jb(k), last, t));
         } else {
           const int r = r0 + 8 * grp + g;
@@ -979,8 +1129,7 @@ int launch_few(cudaStream_t s, const AttnArgs& a) {
   int W = 4, C = 1;
   while (C < kMaxCluster && units * C * 2 <= 4 * kNumSms && C * 2 * W <= steps) C *= 2;
   while (W < kFewMaxWarps && units * C * W * 2 <= 16 * kNumSms && C * W * 2 <= steps) W *= 2;
-  const size_t smem =
-      sizeof(float) * ((size_t)(W + 1) * R * D + 2 * W * R + 2 * kMaxCluster * R);
+  const size_t smem = FewShape<D, NT>::smem(W);
   auto kern = attention_kv8_few_kernel<D, NT>;
   int rc;
   if (smem > 48 * 1024 &&
