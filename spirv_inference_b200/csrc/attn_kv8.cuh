@@ -1,0 +1,89 @@
+// What the kernels of attention over the 8-bit key / value cache share.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "spx_internal.cuh"
+
+namespace spx {
+
+struct AttnArgs {
+  const float* q;
+  spx_kv8_cache c;
+  const int32_t* new_lens;
+  int T, Hq;
+  uint32_t g_mul;   // ceil(2^32 / heads of a group)
+  float scale;
+  float* out;
+  float* lse;
+  float* weights;
+  // r / (heads of a group), exact while r times those is below 2^32
+  __device__ __forceinline__ int div_g(int r) const {
+    return g_mul ? (int)__umulhi((uint32_t)r, g_mul) : r;
+  }
+};
+
+namespace {
+
+__device__ __forceinline__ int clamp_len(int v, int hi) { return v < 0 ? 0 : v > hi ? hi : v; }
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+constexpr float kPUp = 32768.0f;   // 2^15
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+
+// Two differences in one instruction.
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) {
+  unsigned long long d;
+  b.x = -b.x;
+  b.y = -b.y;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)),
+        "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+// (x, y) as packed fp16 hi and lo parts.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h), d = sub2(make_float2(x, y), f);
+  hi = as_u32(h);
+  lo = as_u32(__floats2half2_rn(d.x, d.y));
+}
+
+// 2^-e and 2^e for a largest magnitude with these bits (finite).
+__device__ __forceinline__ void pow2_scale(uint32_t amax_bits, float& down, float& up) {
+  int e = (int)(amax_bits >> 23);
+  e = e < 1 ? 1 : e > 253 ? 253 : e;
+  down = __uint_as_float((uint32_t)(254 - e) << 23);
+  up = __uint_as_float((uint32_t)e << 23);
+}
+__device__ __forceinline__ uint32_t finite_abs(float x) {
+  const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+  return b >= 0x7f800000u ? 0u : b;
+}
+
+// Bytes 0 and 2 of a word of two's complement bytes to fp16: with the sign bit
+// flipped under 0x64, they are 1024 + 128 + value.  (mask: 0x00ff00ff in a
+// register, for one instruction: a lop3 takes one constant of its own.)
+__device__ __forceinline__ uint32_t even_bytes(uint32_t w, uint32_t mask) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, 0x64806480, 0x6a;" : "=r"(r) : "r"(w), "r"(mask));   // (w & mask) ^ c
+  const __half2 v = __hsub2(*reinterpret_cast<__half2*>(&r),
+                            __half2half2(__ushort_as_half((unsigned short)0x6480)));
+  return as_u32(v);
+}
+
+}  // namespace
+
+// Many rows (k_attn_kv8_tc.cu).
+int launch_attention_kv8_tc(cudaStream_t s, const AttnArgs& a);
+
+}  // namespace spx

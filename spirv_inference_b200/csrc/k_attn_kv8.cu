@@ -25,41 +25,13 @@
 
 #include <type_traits>
 
-#include "spx_internal.cuh"
+#include "attn_kv8.cuh"
 
 namespace spx {
 namespace {
 
 namespace cg = cooperative_groups;
 
-__device__ __forceinline__ int clamp_len(int v, int hi) { return v < 0 ? 0 : v > hi ? hi : v; }
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-
-constexpr float kPUp = 32768.0f;   // 2^15
-
-struct AttnArgs {
-  const float* q;
-  spx_kv8_cache c;
-  const int32_t* new_lens;
-  int T, Hq;
-  uint32_t g_mul;   // ceil(2^32 / heads of a group)
-  float scale;
-  float* out;
-  float* lse;
-  float* weights;
-  // r / (heads of a group), exact while r times those is below 2^32
-  __device__ __forceinline__ int div_g(int r) const {
-    return g_mul ? (int)__umulhi((uint32_t)r, g_mul) : r;
-  }
-};
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // d = a b + c.  (c apart from d: zeros and constants need no copy.)
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1, float c0, float c1, float c2, float c3) {
@@ -89,39 +61,6 @@ __device__ __forceinline__ void cluster_arrive() {
 __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-
-// Two differences in one instruction.
-__device__ __forceinline__ float2 sub2(float2 a, float2 b) {
-  unsigned long long d;
-  b.x = -b.x;
-  b.y = -b.y;
-  asm("add.rn.f32x2 %0, %1, %2;"
-      : "=l"(d)
-      : "l"(*reinterpret_cast<unsigned long long*>(&a)),
-        "l"(*reinterpret_cast<unsigned long long*>(&b)));
-  return *reinterpret_cast<float2*>(&d);
-}
-// (x, y) as packed fp16 hi and lo parts.
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h), d = sub2(make_float2(x, y), f);
-  hi = as_u32(h);
-  lo = as_u32(__floats2half2_rn(d.x, d.y));
-}
-
-// 2^-e and 2^e for a largest magnitude with these bits (finite).
-__device__ __forceinline__ void pow2_scale(uint32_t amax_bits, float& down, float& up) {
-  int e = (int)(amax_bits >> 23);
-  e = e < 1 ? 1 : e > 253 ? 253 : e;
-  down = __uint_as_float((uint32_t)(254 - e) << 23);
-  up = __uint_as_float((uint32_t)e << 23);
-}
-__device__ __forceinline__ uint32_t finite_abs(float x) {
-  const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
-  return b >= 0x7f800000u ? 0u : b;
-}
-
 // ---------------------------------------------------------------------------
 // Few rows (decode, drafts).  A row is a (new token, head of the group) pair;
 // a warp takes 8 of them, or 16, and walks its own groups of 16-key tiles with
@@ -465,17 +404,6 @@ struct Running {
 __device__ __forceinline__ void p_frags(uint32_t (&pf)[4], const float (&p)[4]) {
   split2(p[0], p[1], pf[0], pf[2]);
   split2(p[2], p[3], pf[1], pf[3]);
-}
-
-// Bytes 0 and 2 of a word of two's complement bytes to fp16: with the sign bit
-// flipped under 0x64, they are 1024 + 128 + value.  (mask: 0x00ff00ff in a
-// register, for one instruction: a lop3 takes one constant of its own.)
-__device__ __forceinline__ uint32_t even_bytes(uint32_t w, uint32_t mask) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, 0x64806480, 0x6a;" : "=r"(r) : "r"(w), "r"(mask));   // (w & mask) ^ c
-  const __half2 v = __hsub2(*reinterpret_cast<__half2*>(&r),
-                            __half2half2(__ushort_as_half((unsigned short)0x6480)));
-  return as_u32(v);
 }
 
 // The factor that takes a tile's v scale to its share of 2^15, after `ref` has
@@ -1118,17 +1046,21 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) kv8_weights_kernel(const
     put_weights(a.weights + (int64_t)bh * S, w[k], jb(k), len, total, g, t);
 }
 
+// From so many rows of a sequence on, tcgen05.
+constexpr int kTcRows = 128;
+
 template <int D, int NT>
 int launch_few(cudaStream_t s, const AttnArgs& a) {
   constexpr int R = 8 * NT;
   const int groups = (int)ceil_div((int64_t)a.T * (a.Hq / a.c.kv_heads), R);
   const int64_t units = (int64_t)groups * a.c.kv_heads * a.c.batch;
-  // Spread a sequence's keys over CTAs and warps while there are SMs without
-  // work and a warp still has a group of tiles.
+  // Spread a sequence's keys over a CTA's warps, then over CTAs, while that does
+  // not make more warps than are resident at a time (16 an SM) and a warp still
+  // has a group of tiles.
   const int steps = (int)ceil_div(a.c.max_seq, 16 * FewShape<D, NT>::KT);
   int W = 4, C = 1;
-  while (C < kMaxCluster && units * C * 2 <= 4 * kNumSms && C * 2 * W <= steps) C *= 2;
-  while (W < kFewMaxWarps && units * C * W * 2 <= 16 * kNumSms && C * W * 2 <= steps) W *= 2;
+  while (W < kFewMaxWarps && units * W * 2 <= 16 * kNumSms && W * 2 <= steps) W *= 2;
+  while (C < kMaxCluster && units * C * W * 2 <= 16 * kNumSms && C * W * 2 <= steps) C *= 2;
   const size_t smem = FewShape<D, NT>::smem(W);
   auto kern = attention_kv8_few_kernel<D, NT>;
   int rc;
@@ -1178,7 +1110,9 @@ int launch_attention_kv8(cudaStream_t s, int64_t* cnt, const float* q, const spx
   const bool wide = rows > 8;
   // A group of rows that is alone adds its weights itself.
   const bool apart = rows > (c->head_dim == 64 ? 16 : 8);
-  if (c->head_dim == 64)
+  if (rows >= kTcRows)
+    rc = launch_attention_kv8_tc(s, a);
+  else if (c->head_dim == 64)
     rc = wide ? launch_few<64, 2>(s, a) : launch_few<64, 1>(s, a);
   else
     rc = launch_few<128, 1>(s, a);

@@ -1,0 +1,631 @@
+// Attention over the 8-bit cache for many rows (prompts), on tcgen05.
+//
+// A CTA takes 128 rows, (new token, head of the group) pairs of one sequence
+// and kv head, and walks the keys they see in tiles of 128:
+//
+//   four warps turn a tile's K and V into fp16 (int8 is exact there) in shared
+//     memory, one key a thread, two tiles ahead;
+//   S = Q K^T goes into TMEM, q as fp16 hi + lo, two products;
+//   four warps, one row a thread, read S, take the softmax step, and write P,
+//     as fp16 hi + lo, over the part of S that they have just read;
+//   O = P V, two products with P from TMEM, each tile into a fresh accumulator;
+//     one thread of these warps issues it, and then the next tile's S;
+//   the row's thread adds O to its output in registers, in fp32 (the tensor
+//     core's sums round towards zero: over a whole prompt that shows).
+//
+// K and V rows are 128 bytes of 64 values under the 128-byte swizzle: K is a
+// K-major operand, V, whose keys are the reduction, an MN-major one of the same
+// layout.  Turning bytes into fp16 leaves each four values in the order 0, 2,
+// 1, 3: q is stored in that order too, and the output comes out in it.
+//
+// A tile with rows of the tail (fp32) is two tiles: the hi parts, scaled by a
+// power of two for 16 keys, and the lo parts, whose products with the hi parts
+// of q and p are added.
+//
+// What bounds it: the softmax warps' instructions, about 20 a score; the
+// tensor core needs half of that time.  Two CTAs an SM (D = 64) overlap them.
+#include <cuda.h>
+
+#include "attn_kv8.cuh"
+#include "sm100_prims.cuh"
+
+namespace spx {
+
+__device__ int g_at_status = 0;
+
+namespace {
+
+using namespace sm100;
+
+constexpr int kRows = 128, kTile = 128;
+constexpr int kThreads = 256;             // softmax, conversion
+constexpr uint32_t kAtom = 128 * 128;     // 128 rows of 128 bytes
+constexpr unsigned long long kWaitNs = 2000000000ull;
+constexpr float kMaxFloat = 3.4028234663852886e38f;
+
+template <int D>
+struct TcShape {
+  static constexpr int kAtoms = D / 64;
+  static constexpr uint32_t kQ = kAtoms * kAtom;         // hi or lo
+  static constexpr uint32_t kSlot = 2 * kAtoms * kAtom;  // K, V
+  static constexpr uint32_t kTmem = 256;                 // S / P: 128 columns, O: D
+  static constexpr int kBlocks = D == 64 ? 2 : 1;        // CTAs an SM
+  // Two CTAs an SM leave 128 registers a thread; the conversion warps give
+  // some of theirs to the softmax warps, which hold a row of the output.
+  static constexpr int kRegs = 128, kSoftmaxRegs = 184, kConvertRegs = 72;
+  static_assert(kSoftmaxRegs + kConvertRegs <= 2 * kRegs, "within what the launch has");
+};
+
+struct Aux {                   // of the two slots
+  float k_scale[2][8];         // of 16 keys
+  float v_raw[2][8];
+  float share[2][8];
+  float back[2];
+  alignas(16) uint8_t bad[2][kTile];   // the key's V has a NaN or an infinity (tail)
+  uint64_t full[2], empty[2], q_full, s_ready, done;
+  uint32_t tmem;
+  int abort_flag;
+};
+
+// fp16 A and B, fp32 sums; b_mn: B's rows are the reduction.
+__host__ __device__ constexpr uint32_t idesc_f16(int m, int n, int b_mn) {
+  return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+// The same with A in TMEM.
+__device__ __forceinline__ void mma_f16_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+// MN-major operand in the same layout as sw128_desc's: 64 values a row, 8-row
+// groups of the reduction 1024 bytes apart, the next 64 values an atom away.
+__device__ __forceinline__ uint64_t mn_desc(uint32_t saddr) {
+  return (sw128_desc(saddr) & ~(0x3fffull << 16)) | ((uint64_t)(kAtom >> 4) << 16);
+}
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(
+          r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+      "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+// Barrier of 128 threads; whether all of them came with `ok`.
+__device__ __forceinline__ bool vote(int id, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, %2, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)ok), "r"(id)
+      : "memory");
+  return r != 0;
+}
+
+// 16 bytes of piece `c` (eight values) of row `r` of an operand.
+__device__ __forceinline__ uint4* piece(uint8_t* base, int r, int c) {
+  return reinterpret_cast<uint4*>(base + (c >> 3) * kAtom + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+// Eight int8 values as fp16, each four in the order 0, 2, 1, 3.
+__device__ __forceinline__ uint4 eight(uint32_t a, uint32_t b, uint32_t mask) {
+  return make_uint4(even_bytes(a, mask), even_bytes(a >> 8, mask), even_bytes(b, mask),
+                    even_bytes(b >> 8, mask));
+}
+// Eight fp32 values times `by` as fp16 hi and lo, in that order.
+__device__ __forceinline__ void eight_split(const float4 x, const float4 y, float by, uint4& hi,
+                                            uint4& lo) {
+  split2(x.x * by, x.z * by, hi.x, lo.x);
+  split2(x.y * by, x.w * by, hi.y, lo.y);
+  split2(y.x * by, y.z * by, hi.z, lo.z);
+  split2(y.y * by, y.w * by, hi.w, lo.w);
+}
+__device__ __forceinline__ bool odd_bits(float x) {
+  return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u;
+}
+__device__ __forceinline__ float4 finite4(float4 v, bool& odd) {
+  if (odd_bits(v.x)) odd = true, v.x = 0.f;
+  if (odd_bits(v.y)) odd = true, v.y = 0.f;
+  if (odd_bits(v.z)) odd = true, v.z = 0.f;
+  if (odd_bits(v.w)) odd = true, v.w = 0.f;
+  return v;
+}
+
+// What every role knows of the CTA's work.
+template <int D>
+struct Unit {
+  int h, b, r0, rows, len, total, closed, lim, tiles, G;
+  __device__ __forceinline__ Unit(const AttnArgs& a) {
+    G = a.Hq / a.c.kv_heads;
+    h = blockIdx.y;
+    b = blockIdx.z;
+    // the last rows see the most keys: first
+    r0 = (int)(gridDim.x - 1 - blockIdx.x) * kRows;
+    const int n_new = a.new_lens ? clamp_len(a.new_lens[b], a.T) : a.T;
+    rows = n_new * G;
+    len = clamp_len(a.c.lens[b], a.c.max_seq);
+    total = min(len + n_new, a.c.max_seq);
+    closed = total / a.c.block * a.c.block;
+    lim = min(len + a.div_g(min(r0 + kRows, rows) - 1) + 1, a.c.max_seq);
+    tiles = (lim + kTile - 1) / kTile;
+  }
+  __device__ __forceinline__ int64_t row_at(const AttnArgs& a, int r) const {
+    const int tk = a.div_g(r);
+    return ((int64_t)b * a.T + tk) * a.Hq + h * G + (r - tk * G);
+  }
+  __device__ __forceinline__ bool has_tail(int tile) const {
+    return closed < lim && (tile + 1) * kTile > closed;
+  }
+};
+
+// ---- conversion: one row of Q, K and V a thread ------------------------------
+template <int D>
+__device__ __forceinline__ void convert_q(const AttnArgs& a, const Unit<D>& u, uint8_t* q_hi,
+                                          uint8_t* q_lo, float* q_scale, int x) {
+  const int r = u.r0 + x;
+  const float4* row =
+      r < u.rows ? reinterpret_cast<const float4*>(a.q + u.row_at(a, r) * D) : nullptr;
+  uint32_t mx = 0;
+  bool odd = false;
+  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < D / 4; ++i) {
+    const float4 v = row ? __ldg(row + i) : zero;
+    mx = max(max(mx, finite_abs(v.x)), max(finite_abs(v.y), max(finite_abs(v.z),
+                                                                finite_abs(v.w))));
+    odd |= odd_bits(v.x) || odd_bits(v.y) || odd_bits(v.z) || odd_bits(v.w);
+  }
+  float down, up;
+  pow2_scale(mx, down, up);
+  if (a.scale < 0.0f) down = -down;
+#pragma unroll 4
+  for (int c = 0; c < D / 8; ++c) {
+    uint4 hi, lo;
+    eight_split(row ? __ldg(row + 2 * c) : zero, row ? __ldg(row + 2 * c + 1) : zero, down, hi, lo);
+    *piece(q_hi, x, c) = hi;
+    *piece(q_lo, x, c) = lo;
+  }
+  q_scale[x] = odd ? __int_as_float(0x7fc00000) : up * (fabsf(a.scale) * kLog2e);
+}
+
+template <int D>
+__device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& u, uint8_t* slots,
+                                              Aux& aux, int x) {
+  using S = TcShape<D>;
+  const int64_t bh = (int64_t)u.b * a.c.kv_heads + u.h;
+  const int8_t* k8 = a.c.k + bh * a.c.max_seq * D;
+  const int8_t* v8 = a.c.v + bh * a.c.max_seq * D;
+  const int blk = a.c.block;
+  const float* ks = a.c.k_scale + bh * (a.c.max_seq / blk);
+  const float* vs = a.c.v_scale + bh * (a.c.max_seq / blk);
+  const float* kt = a.c.k_tail + bh * blk * D;
+  const float* vt = a.c.v_tail + bh * blk * D;
+  uint32_t mask;
+  asm volatile("mov.b32 %0, 0x00ff00ff;" : "=r"(mask));
+  int n = 0;                   // slots used
+  for (int tile = 0; tile < u.tiles; ++tile, ++n) {
+    const int key = tile * kTile + x, s = n & 1;
+    const bool closed = key < u.closed, in_tail = !closed && key < u.total;
+    const bool tail = u.has_tail(tile);
+    // The rows' bytes, and the scales, are on their way while the slot drains.
+    uint4 kr[D / 16], vr[D / 16];
+    float k_sc = 0.0f, v_sc = 0.0f;
+    if (closed) {
+      const uint4* kp = reinterpret_cast<const uint4*>(k8 + (int64_t)key * D);
+      const uint4* vp = reinterpret_cast<const uint4*>(v8 + (int64_t)key * D);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) kr[i] = __ldg(kp + i);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) vr[i] = __ldg(vp + i);
+      k_sc = __ldg(ks + key / blk);
+      v_sc = __ldg(vs + key / blk);
+    }
+    float k_down = 0.0f, v_down = 0.0f;
+    const float4* kf = reinterpret_cast<const float4*>(kt + (int64_t)(key & (blk - 1)) * D);
+    const float4* vf = reinterpret_cast<const float4*>(vt + (int64_t)(key & (blk - 1)) * D);
+    bool odd = false, unused = false;
+    if (tail) {                // the tail's 16-key groups: powers of two
+      uint32_t mk = 0, mv = 0;
+      if (in_tail)
+        for (int i = 0; i < D / 4; ++i) {
+          const float4 p = kf[i], q = finite4(vf[i], odd);
+          mk = max(max(mk, finite_abs(p.x)),
+                   max(finite_abs(p.y), max(finite_abs(p.z), finite_abs(p.w))));
+          mv = max(max(mv, finite_abs(q.x)),
+                   max(finite_abs(q.y), max(finite_abs(q.z), finite_abs(q.w))));
+        }
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) {
+        mk = max(mk, __shfl_xor_sync(0xffffffffu, mk, o));
+        mv = max(mv, __shfl_xor_sync(0xffffffffu, mv, o));
+      }
+      if (!closed) {
+        pow2_scale(mk, k_down, k_sc);
+        pow2_scale(mv, v_down, v_sc);
+      }
+    }
+    const bool drained =
+        mb_wait(&aux.empty[s], ((n >> 1) & 1) ^ 1, &aux.abort_flag, &g_at_status, kWaitNs, 64);
+    if (drained && (x & 15) == 0) {
+      aux.k_scale[s][x >> 4] = k_sc;
+      aux.v_raw[s][x >> 4] = v_sc;
+    }
+    if (drained) aux.bad[s][x] = odd;
+    if (!vote(1, drained)) return;
+    if (x < 8) {
+      float ref = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float v = aux.v_raw[s][i];
+        if (v <= kMaxFloat) ref = fmaxf(ref, v);
+      }
+      aux.share[s][x] = ref > 0.0f ? aux.v_raw[s][x] * (kPUp / ref) : aux.v_raw[s][x];
+      if (x == 0) aux.back[s] = ref * (1.0f / kPUp);
+    }
+    uint8_t* k_to = slots + s * S::kSlot;
+    uint8_t* v_to = k_to + S::kAtoms * kAtom;
+    if (closed) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        *piece(k_to, x, 2 * i) = eight(kr[i].x, kr[i].y, mask);
+        *piece(k_to, x, 2 * i + 1) = eight(kr[i].z, kr[i].w, mask);
+        *piece(v_to, x, 2 * i) = eight(vr[i].x, vr[i].y, mask);
+        *piece(v_to, x, 2 * i + 1) = eight(vr[i].z, vr[i].w, mask);
+      }
+    } else {
+      for (int c = 0; c < D / 8; ++c) {
+        uint4 hi = make_uint4(0, 0, 0, 0), lo, vh = hi;
+        if (in_tail) {
+          eight_split(kf[2 * c], kf[2 * c + 1], k_down, hi, lo);
+          eight_split(finite4(vf[2 * c], unused), finite4(vf[2 * c + 1], unused), v_down, vh, lo);
+        }
+        *piece(k_to, x, c) = hi;
+        *piece(v_to, x, c) = vh;
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    mb_arrive(&aux.full[s]);
+    if (!tail) continue;
+    ++n;
+    const int s2 = n & 1;
+    if (!vote(1, mb_wait(&aux.empty[s2], ((n >> 1) & 1) ^ 1, &aux.abort_flag, &g_at_status,
+                         kWaitNs, 64)))
+      return;
+    k_to = slots + s2 * S::kSlot;
+    v_to = k_to + S::kAtoms * kAtom;
+    for (int c = 0; c < D / 8; ++c) {
+      uint4 hi, lo = make_uint4(0, 0, 0, 0), vl = lo;
+      if (in_tail) {
+        eight_split(kf[2 * c], kf[2 * c + 1], k_down, hi, lo);
+        eight_split(finite4(vf[2 * c], unused), finite4(vf[2 * c + 1], unused), v_down, hi, vl);
+      }
+      *piece(k_to, x, c) = lo;
+      *piece(v_to, x, c) = vl;
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    mb_arrive(&aux.full[s2]);
+  }
+}
+
+// ---- products, issued by one thread ----------------------------------------------
+template <int D>
+struct Issue {
+  using S = TcShape<D>;
+  static constexpr uint32_t kS = idesc_f16(kRows, kTile, 0), kO = idesc_f16(kRows, D, 1);
+  uint32_t q_hi, q_lo, slots, tmem;
+  // Q (from q) K^T (from slot s) over D.
+  __device__ __forceinline__ void scores(uint32_t q, int s, bool more) const {
+    const uint32_t k = slots + s * S::kSlot;
+#pragma unroll 1
+    for (int i = 0; i < D / 16; ++i) {
+      const uint32_t at = (i >> 2) * kAtom + (i & 3) * 32;
+      mma_f16(tmem, sw128_desc(q + at), sw128_desc(k + at), kS, more || i ? 1u : 0u);
+    }
+  }
+  // P (hi: part 0, lo: part 16 columns into each 32) V (from slot s) over the keys.
+  __device__ __forceinline__ void values(uint32_t part, int s, bool more) const {
+    const uint32_t v = slots + s * S::kSlot + S::kAtoms * kAtom;
+#pragma unroll 1
+    for (int i = 0; i < kTile / 16; ++i)
+      mma_f16_ta(tmem + kTile, tmem + (i >> 1) * 32 + part + (i & 1) * 8, mn_desc(v + i * 2048),
+                 kO, more || i ? 1u : 0u);
+  }
+  // S of the tile in slot n (and n + 1), once it is there.
+  __device__ __forceinline__ void tile_scores(Aux& aux, int n, bool tail) const {
+    auto wait = [&](int k) {
+      return mb_wait(&aux.full[k & 1], (k >> 1) & 1, &aux.abort_flag, &g_at_status, kWaitNs, 32);
+    };
+    if (!wait(n)) return;
+    tc_after();
+    scores(q_lo, n & 1, false);
+    scores(q_hi, n & 1, true);
+    if (tail) {
+      if (!wait(n + 1)) return;
+      tc_after();
+      scores(q_hi, (n + 1) & 1, true);
+    }
+    mma_commit(&aux.s_ready);
+  }
+  __device__ __forceinline__ void tile_values(Aux& aux, int n, bool tail) const {
+    tc_after();
+    values(16, n & 1, false);
+    values(0, n & 1, true);
+    if (tail) values(0, (n + 1) & 1, true);
+    mma_commit(&aux.empty[n & 1]);
+    if (tail) mma_commit(&aux.empty[(n + 1) & 1]);
+  }
+};
+
+// ---- softmax: one row a thread -------------------------------------------------
+template <int D>
+__device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& u, Aux& aux,
+                                              const float* q_scale, const Issue<D>& issue, int x,
+                                              float (&o)[D], float& m, float& l) {
+  const uint32_t tmem = issue.tmem;
+  const uint32_t lanes = (uint32_t)((x >> 5) * 32) << 16;
+  const uint32_t t_s = tmem + lanes, t_o = tmem + lanes + kTile;
+  auto wait = [&](uint64_t* b, int parity) {
+    return mb_wait(b, parity, &aux.abort_flag, &g_at_status, kWaitNs, 32);
+  };
+  // Exits are by vote: no warp is left alone at a barrier.
+  if (!vote(2, wait(&aux.q_full, 0))) return false;
+  if (x == 0) issue.tile_scores(aux, 0, u.has_tail(0));
+  const float qs = q_scale[x];
+  const int last = min(u.len + a.div_g(min(u.r0 + x, u.rows - 1)), u.total - 1);
+  const int last_of_first = min(u.len + a.div_g(u.r0), u.total - 1);
+  m = -INFINITY;
+  l = 0.0f;
+  float corr = 0.0f, back = 0.0f;   // of the tile before
+  // o = o corr + back * (P V of the tile before)
+  auto take_output = [&]() {
+    tc_after();
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      float v[32];
+      tmem_ld_32x32(t_o + c * 32, v);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[c * 32 + e] = fmaf(o[c * 32 + e], corr, back * v[e]);
+    }
+  };
+  int n = 0;
+  for (int tile = 0; tile < u.tiles; ++tile, ++n) {
+    const int s = n & 1, j0 = tile * kTile;
+    const bool tail = u.has_tail(tile);
+    // (the slot for its scales)
+    if (!vote(2, wait(&aux.full[s], (n >> 1) & 1) && wait(&aux.s_ready, tile & 1))) return false;
+    tc_after();
+    const bool mask = j0 + kTile - 1 > last_of_first;
+    const int seen = last - j0;         // the last column that the row sees
+    float mt = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      float v[32];
+      tmem_ld_32x32(t_s + c * 32, v);
+      if (mask) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (c * 32 + e > seen) v[e] = -INFINITY;
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const float f = aux.k_scale[s][c * 2 + half] * qs;
+        float most = v[half * 16];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) most = fmaxf(most, v[half * 16 + e]);
+        // (a factor of 0 or NaN would make NaN of -inf, which fmaxf passes over)
+        mt = fmaxf(mt, most * f);
+      }
+    }
+    const float mn = fmaxf(m, mt), base = mn == -INFINITY ? 0.0f : mn;
+    // The output of the tile before is relative to the old maximum.
+    if (tile > 0) take_output();
+    corr = ex2(m - base);
+    m = mn;
+    bool any_bad = false;
+    if (tail) {
+#pragma unroll 1
+      for (int i = 0; i < kTile / 16; ++i) {
+        const uint4 w = reinterpret_cast<const uint4*>(aux.bad[s])[i];
+        any_bad |= (w.x | w.y | w.z | w.w) != 0;
+      }
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      float v[32];
+      tmem_ld_32x32(t_s + c * 32, v);
+      uint32_t p[32];
+      float part = 0.0f;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const float f = aux.k_scale[s][c * 2 + half] * qs, share = aux.share[s][c * 2 + half];
+#pragma unroll
+        for (int e = half * 16; e < half * 16 + 16; ++e) {
+          float w = ex2(fmaf(v[e], f, -base));
+          if (mask && c * 32 + e > seen) w = 0.0f;
+          part += w;
+          w *= share;
+          if (mask && c * 32 + e > seen) w = 0.0f;
+          v[e] = w;
+        }
+      }
+      if (any_bad) {
+#pragma unroll 1
+        for (int e = 0; e < 32; ++e) {
+          const bool hit = aux.bad[s][c * 32 + e] && c * 32 + e <= seen;
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (i == e && hit) v[i] = __int_as_float(0x7fc00000);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) split2(v[2 * e], v[2 * e + 1], p[e], p[16 + e]);
+      sum += part;
+      tmem_st_32x32(t_s + c * 32, p);
+    }
+    l = fmaf(l, corr, sum);
+    back = aux.back[s];
+    tmem_wait_st();
+    tc_before();
+    vote(2, true);                      // all of P is there
+    const int now = n;
+    if (tail) ++n;
+    if (x == 0) {
+      issue.tile_values(aux, now, tail);
+      if (tile + 1 < u.tiles)
+        issue.tile_scores(aux, n + 1, u.has_tail(tile + 1));
+      else
+        mma_commit(&aux.done);
+    }
+  }
+  if (!vote(2, wait(&aux.done, 0))) return false;
+  take_output();
+  return true;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
+    attention_kv8_tc_kernel(const AttnArgs a) {
+  using S = TcShape<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* q_hi = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* q_lo = q_hi + S::kQ;
+  uint8_t* slots = q_lo + S::kQ;
+  __shared__ Aux aux;
+  __shared__ float q_scale[kRows];
+  const int warp = threadIdx.x >> 5;
+  const Unit<D> u(a);
+  if (u.r0 >= u.rows) return;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mb_init(&aux.full[i], 128);
+      mb_init(&aux.empty[i], 1);
+    }
+    mb_init(&aux.q_full, 128);
+    mb_init(&aux.s_ready, 1);
+    mb_init(&aux.done, 1);
+    aux.abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 4) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     sa(&aux.tmem)),
+                 "r"(S::kTmem));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = aux.tmem;
+  if (warp < 4) {
+    if constexpr (D == 64)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftmaxRegs));
+    const int x = threadIdx.x;
+    const Issue<D> issue{sa(q_hi), sa(q_lo), sa(slots), tmem};
+    float o[D], m, l;
+#pragma unroll
+    for (int i = 0; i < D; ++i) o[i] = 0.0f;
+    const bool ok = softmax_tiles<D>(a, u, aux, q_scale, issue, x, o, m, l);
+    if (!ok && x == 0) {
+      // The products in flight end before shared memory and TMEM are given up.
+      volatile int never = 0;
+      mma_commit(&aux.done);
+      mb_wait(&aux.done, 0, &never, &g_at_status, 200000000ull, 64);
+    }
+    const int r = u.r0 + x;
+    if (ok && r < u.rows) {
+      const int64_t at = u.row_at(a, r);
+      const float inv = 1.0f / l;
+      float4* out = reinterpret_cast<float4*>(a.out + at * D);
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i)   // each four came as 0, 2, 1, 3
+        out[i] = make_float4(o[4 * i] * inv, o[4 * i + 2] * inv, o[4 * i + 1] * inv,
+                             o[4 * i + 3] * inv);
+      if (a.lse) a.lse[at] = (m + log2f(l)) * kLn2;
+    }
+  } else {
+    if constexpr (D == 64)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kConvertRegs));
+    const int x = threadIdx.x - 128;
+    convert_q<D>(a, u, q_hi, q_lo, q_scale, x);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    mb_arrive(&aux.q_full);
+    convert_tiles<D>(a, u, slots, aux, x);
+  }
+  tc_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(S::kTmem));
+  }
+}
+
+template <int D>
+int launch_tc(cudaStream_t s, const AttnArgs& a) {
+  using S = TcShape<D>;
+  const int64_t row_tiles = ceil_div((int64_t)a.T * (a.Hq / a.c.kv_heads), kRows);
+  if (row_tiles > INT32_MAX || a.c.kv_heads > 65535 || a.c.batch > 65535)
+    return fail(SPX_ERR_UNSUPPORTED, "attention_kv8: grid too large");
+  const size_t smem = 1024 + 2 * S::kQ + 2 * S::kSlot;
+  int rc = check_cuda(cudaFuncSetAttribute(attention_kv8_tc_kernel<D>,
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+                      "attention_kv8: smem attribute");
+  if (rc) return rc;
+  if constexpr (D == 64) {
+    // setmaxnreg draws on the registers that the launch has: with fewer than
+    // it was written for, it would wait for good.
+    cudaFuncAttributes f;
+    if ((rc = check_cuda(cudaFuncGetAttributes(&f, attention_kv8_tc_kernel<D>),
+                         "attention_kv8: attributes")))
+      return rc;
+    if (f.numRegs < S::kRegs)
+      return fail(SPX_ERR_UNSUPPORTED, "attention_kv8: built with %d registers a thread",
+                  f.numRegs);
+  }
+  const dim3 grid((unsigned)row_tiles, (unsigned)a.c.kv_heads, (unsigned)a.c.batch);
+  attention_kv8_tc_kernel<D><<<grid, kThreads, smem, s>>>(a);
+  return SPX_OK;
+}
+
+}  // namespace
+
+int launch_attention_kv8_tc(cudaStream_t s, const AttnArgs& a) {
+  return a.c.head_dim == 64 ? launch_tc<64>(s, a) : launch_tc<128>(s, a);
+}
+
+int at_take_status() {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_at_status, sizeof(int)) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  if (v) {
+    int zero = 0;
+    cudaMemcpyToSymbol(g_at_status, &zero, sizeof(int));
+  }
+  return v;
+}
+
+}  // namespace spx

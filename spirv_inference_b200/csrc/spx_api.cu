@@ -591,6 +591,9 @@ static int device_status(const char* what) {
   if (tc_take_status())
     return fail(SPX_ERR_CUDA, "%s: a tensor-core pipeline wait timed out; tiles were abandoned",
                 what);
+  if (at_take_status())
+    return fail(SPX_ERR_CUDA, "%s: an attention pipeline wait timed out; rows were abandoned",
+                what);
   if (ar_take_status())
     return fail(SPX_ERR_CUDA,
                 "%s: an all-reduce waited %lld us for a peer rank and gave up; reset the "

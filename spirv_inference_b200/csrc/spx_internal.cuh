@@ -331,6 +331,7 @@ int launch_stem_tc(cudaStream_t s, int64_t* cnt, const float* x, const float* w_
 int launch_dw_project(cudaStream_t s, int64_t* cnt, const float* x, const float* wd,
                       const float* bd, const float* w_hi, const float* w_lo, const float* bp,
                       const float* res, float* y, const spx_dwproj_params* q, bool dry_run);
+int at_take_status();   // attention over the 8-bit cache
 int ar_take_status();
 
 // Process-wide dense-contraction path: 0 auto, 1 SIMT only, 2 tensor cores
