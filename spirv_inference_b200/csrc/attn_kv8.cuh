@@ -85,5 +85,6 @@ __device__ __forceinline__ uint32_t even_bytes(uint32_t w, uint32_t mask) {
 
 // Many rows (k_attn_kv8_tc.cu).
 int launch_attention_kv8_tc(cudaStream_t s, const AttnArgs& a);
+int launch_weights_kv8_tc(cudaStream_t s, const AttnArgs& a);
 
 }  // namespace spx

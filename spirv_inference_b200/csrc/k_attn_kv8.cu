@@ -1118,11 +1118,15 @@ int launch_attention_kv8(cudaStream_t s, int64_t* cnt, const float* q, const spx
     rc = launch_few<128, 1>(s, a);
   if (rc) return rc;
   if ((rc = after_launch(cnt, "attention_kv8")) || !weights || !apart) return rc;
-  const dim3 wg((unsigned)ceil_div(c->max_seq, 256), (unsigned)bh);
-  if (c->head_dim == 64)
-    kv8_weights_kernel<64><<<wg, 256, 0, s>>>(a);
-  else
-    kv8_weights_kernel<128><<<wg, 256, 0, s>>>(a);
+  if (rows >= kTcRows) {
+    if ((rc = launch_weights_kv8_tc(s, a))) return rc;
+  } else {
+    const dim3 wg((unsigned)ceil_div(c->max_seq, 256), (unsigned)bh);
+    if (c->head_dim == 64)
+      kv8_weights_kernel<64><<<wg, 256, 0, s>>>(a);
+    else
+      kv8_weights_kernel<128><<<wg, 256, 0, s>>>(a);
+  }
   return after_launch(cnt, "attention_kv8: weights");
 }
 

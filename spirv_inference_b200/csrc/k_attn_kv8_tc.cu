@@ -24,6 +24,7 @@
 //
 // What bounds it: the softmax warps' instructions, about 20 a score; the
 // tensor core needs half of that time.  Two CTAs an SM (D = 64) overlap them.
+#include <cooperative_groups.h>
 #include <cuda.h>
 
 #include "attn_kv8.cuh"
@@ -36,6 +37,7 @@ __device__ int g_at_status = 0;
 namespace {
 
 using namespace sm100;
+namespace cg = cooperative_groups;
 
 constexpr int kRows = 128, kTile = 128;
 constexpr int kThreads = 256;             // softmax, conversion
@@ -180,33 +182,35 @@ struct Unit {
 };
 
 // ---- conversion: one row of Q, K and V a thread ------------------------------
+// Row x of an operand from a row of q (null: zeros), hi and lo; returns the
+// factor that takes its products to scores in units of log 2 (NaN for a row
+// with a NaN or an infinity).
 template <int D>
-__device__ __forceinline__ void convert_q(const AttnArgs& a, const Unit<D>& u, uint8_t* q_hi,
-                                          uint8_t* q_lo, float* q_scale, int x) {
-  const int r = u.r0 + x;
-  const float4* row =
-      r < u.rows ? reinterpret_cast<const float4*>(a.q + u.row_at(a, r) * D) : nullptr;
+__device__ __forceinline__ float convert_q(const float* row, float scale, uint8_t* q_hi,
+                                           uint8_t* q_lo, int x) {
+  const float4* from = reinterpret_cast<const float4*>(row);
   uint32_t mx = 0;
   bool odd = false;
   const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int i = 0; i < D / 4; ++i) {
-    const float4 v = row ? __ldg(row + i) : zero;
+    const float4 v = row ? __ldg(from + i) : zero;
     mx = max(max(mx, finite_abs(v.x)), max(finite_abs(v.y), max(finite_abs(v.z),
                                                                 finite_abs(v.w))));
     odd |= odd_bits(v.x) || odd_bits(v.y) || odd_bits(v.z) || odd_bits(v.w);
   }
   float down, up;
   pow2_scale(mx, down, up);
-  if (a.scale < 0.0f) down = -down;
+  if (scale < 0.0f) down = -down;
 #pragma unroll 4
   for (int c = 0; c < D / 8; ++c) {
     uint4 hi, lo;
-    eight_split(row ? __ldg(row + 2 * c) : zero, row ? __ldg(row + 2 * c + 1) : zero, down, hi, lo);
+    eight_split(row ? __ldg(from + 2 * c) : zero, row ? __ldg(from + 2 * c + 1) : zero, down, hi,
+                lo);
     *piece(q_hi, x, c) = hi;
     *piece(q_lo, x, c) = lo;
   }
-  q_scale[x] = odd ? __int_as_float(0x7fc00000) : up * (fabsf(a.scale) * kLog2e);
+  return odd ? __int_as_float(0x7fc00000) : up * (fabsf(scale) * kLog2e);
 }
 
 template <int D>
@@ -568,7 +572,9 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
     if constexpr (D == 64)
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kConvertRegs));
     const int x = threadIdx.x - 128;
-    convert_q<D>(a, u, q_hi, q_lo, q_scale, x);
+    const int r = u.r0 + x;
+    q_scale[x] =
+        convert_q<D>(r < u.rows ? a.q + u.row_at(a, r) * D : nullptr, a.scale, q_hi, q_lo, x);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mb_arrive(&aux.q_full);
     convert_tiles<D>(a, u, slots, aux, x);
@@ -579,6 +585,214 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
     tc_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "r"(S::kTmem));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Weights for many rows: S^T = K Q^T, 128 keys on the lanes, which stay, and
+// 128 rows at a time on the columns.  Four warps turn rows of q into operands,
+// two tiles ahead; four, one key a thread, add exp(score - lse) over a tile's
+// rows while the next tile's products run into the other half of TMEM.  The
+// row tiles are dealt to a cluster's CTAs, whose sums are added in order.
+// About 5 instructions a score, and as many again for q.
+constexpr int kWeightCluster = 4;
+
+struct WeightAux {
+  float2 row[2][kRows];        // the row's factor, and its lse in units of log 2
+  float got[kWeightCluster][kTile];
+  uint64_t full[2], empty[2], k_full, s_ready[2], done;
+  uint32_t tmem;
+  int abort_flag;
+};
+
+template <int D>
+struct WeightShape {
+  static constexpr uint32_t kK = D / 64 * kAtom;       // hi or lo
+  static constexpr uint32_t kSlot = 2 * D / 64 * kAtom;  // q hi, lo
+  static constexpr size_t kSmem = 1024 + 2 * kK + 2 * kSlot;
+};
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
+    kv8_weights_tc_kernel(const AttnArgs a, int cluster) {
+  using S = WeightShape<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* k_hi = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* k_lo = k_hi + S::kK;
+  uint8_t* slots = k_lo + S::kK;
+  __shared__ WeightAux aux;
+  const int warp = threadIdx.x >> 5, x = threadIdx.x & 127;
+  const int rank = blockIdx.x % cluster, j0 = blockIdx.x / cluster * kTile;
+  const int h = blockIdx.y, b = blockIdx.z, G = a.Hq / a.c.kv_heads, blk = a.c.block;
+  const int n_new = a.new_lens ? clamp_len(a.new_lens[b], a.T) : a.T;
+  const int len = clamp_len(a.c.lens[b], a.c.max_seq), total = min(len + n_new, a.c.max_seq);
+  if (n_new == 0 || j0 >= total) return;      // the whole cluster
+  const int closed = total / blk * blk, rows = n_new * G;
+  const bool tail = j0 + kTile > closed && closed < total;
+  // Rows of tokens before the first key see none of these.
+  const int first = max(0, j0 - len) * G / kRows, last = (rows + kRows - 1) / kRows;
+  const int tiles = max(0, (last - first - rank + cluster - 1) / cluster);
+  auto row0 = [&](int i) { return (first + rank + i * cluster) * kRows; };
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mb_init(&aux.full[i], 128);
+      mb_init(&aux.empty[i], 129);     // the products, and the threads that read `row`
+      mb_init(&aux.s_ready[i], 1);
+    }
+    mb_init(&aux.k_full, 128);
+    mb_init(&aux.done, 1);
+    aux.abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 4) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     sa(&aux.tmem)),
+                 "r"(256));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  if (cluster > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  const uint32_t tmem = aux.tmem;
+  auto wait = [&](uint64_t* bar, int parity) {
+    return mb_wait(bar, parity, &aux.abort_flag, &g_at_status, kWaitNs, 32);
+  };
+  float w = 0.0f;
+  if (warp >= 4) {
+    auto row_at = [&](int r) {
+      const int tk = a.div_g(r);
+      return ((int64_t)b * a.T + tk) * a.Hq + h * G + (r - tk * G);
+    };
+    for (int i = 0; i < tiles; ++i) {
+      const int s = i & 1, r = row0(i) + x;
+      if (!wait(&aux.empty[s], ((i >> 1) & 1) ^ 1)) break;
+      uint8_t* to = slots + s * S::kSlot;
+      const int64_t at = r < rows ? row_at(r) : 0;
+      const float f =
+          convert_q<D>(r < rows ? a.q + at * D : nullptr, a.scale, to, to + S::kSlot / 2, x);
+      // (a row that is none weighs nothing)
+      aux.row[s][x] = make_float2(f, r < rows ? a.lse[at] * kLog2e : INFINITY);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mb_arrive(&aux.full[s]);
+    }
+  } else {
+    // The key's row, and its scale.
+    const int key = j0 + x;
+    const int64_t bh = (int64_t)b * a.c.kv_heads + h;
+    float ks = 0.0f;
+    if (key < closed) {
+      const uint4* kp = reinterpret_cast<const uint4*>(a.c.k + (bh * a.c.max_seq + key) * D);
+      uint32_t mask;
+      asm volatile("mov.b32 %0, 0x00ff00ff;" : "=r"(mask));
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const uint4 v = __ldg(kp + i);
+        *piece(k_hi, x, 2 * i) = eight(v.x, v.y, mask);
+        *piece(k_hi, x, 2 * i + 1) = eight(v.z, v.w, mask);
+        *piece(k_lo, x, 2 * i) = *piece(k_lo, x, 2 * i + 1) = make_uint4(0, 0, 0, 0);
+      }
+      ks = __ldg(a.c.k_scale + bh * (a.c.max_seq / blk) + key / blk);
+    } else {
+      // a row of the tail on its own: any power of two does
+      const float* row =
+          key < total ? a.c.k_tail + (bh * blk + (key & (blk - 1))) * D : nullptr;
+      const float4* from = reinterpret_cast<const float4*>(row);
+      const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+      uint32_t mx = 0;
+      for (int i = 0; i < D / 4; ++i) {
+        const float4 v = row ? from[i] : zero;
+        mx = max(max(mx, finite_abs(v.x)),
+                 max(finite_abs(v.y), max(finite_abs(v.z), finite_abs(v.w))));
+      }
+      float down;
+      pow2_scale(mx, down, ks);
+      for (int c = 0; c < D / 8; ++c) {
+        uint4 hi, lo;
+        eight_split(row ? from[2 * c] : zero, row ? from[2 * c + 1] : zero, down, hi, lo);
+        *piece(k_hi, x, c) = hi;
+        *piece(k_lo, x, c) = lo;
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    mb_arrive(&aux.k_full);
+    const uint32_t kh = sa(k_hi), kl = sa(k_lo);
+    constexpr uint32_t kDesc = idesc_f16(kTile, kRows, 0);
+    auto products = [&](uint32_t k, uint32_t q, uint32_t to, bool more) {
+#pragma unroll 1
+      for (int i = 0; i < D / 16; ++i) {
+        const uint32_t at = (i >> 2) * kAtom + (i & 3) * 32;
+        mma_f16(to, sw128_desc(k + at), sw128_desc(q + at), kDesc, more || i ? 1u : 0u);
+      }
+    };
+    auto issue = [&](int i) {                 // by one thread
+      const int s = i & 1;
+      if (!wait(&aux.full[s], (i >> 1) & 1)) return;
+      tc_after();
+      const uint32_t qh = sa(slots) + s * S::kSlot, ql = qh + S::kSlot / 2, to = tmem + s * kRows;
+      products(kh, ql, to, false);
+      if (tail) products(kl, qh, to, true);
+      products(kh, qh, to, true);
+      mma_commit(&aux.empty[s]);
+      mma_commit(&aux.s_ready[s]);
+    };
+    bool ok = vote(2, wait(&aux.k_full, 0));
+    if (ok && x == 0 && tiles > 0) issue(0);
+    // The key's first row, and whether a tile has any before that of some key.
+    const int r_min = max(0, key - len) * G, r_all = max(0, j0 + kTile - 1 - len) * G;
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    for (int i = 0; ok && i < tiles; ++i) {
+      const int s = i & 1;
+      if (x == 0 && i + 1 < tiles) issue(i + 1);
+      ok = vote(2, wait(&aux.s_ready[s], (i >> 1) & 1) && wait(&aux.full[s], (i >> 1) & 1));
+      if (!ok) break;
+      tc_after();
+      const bool mask = row0(i) < r_all;
+      const int from = r_min - row0(i);       // the first column that the key is seen by
+#pragma unroll 1
+      for (int c = 0; c < kRows / 32; ++c) {
+        float v[32];
+        tmem_ld_32x32(tmem + s * kRows + lanes + c * 32, v);
+        float part = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float2 r = aux.row[s][c * 32 + e];
+          const float p = ex2(fmaf(v[e], ks * r.x, -r.y));
+          part += mask && c * 32 + e < from ? 0.0f : p;
+        }
+        w += part;
+      }
+      tc_before();
+      mb_arrive(&aux.empty[s]);
+      vote(2, true);                          // this half of TMEM has been read
+    }
+    if (!ok && x == 0) {
+      // The products in flight end before shared memory and TMEM are given up.
+      volatile int never = 0;
+      mma_commit(&aux.done);
+      mb_wait(&aux.done, 0, &never, &g_at_status, 200000000ull, 64);
+    }
+  }
+  __syncwarp();
+  const bool good = !aux.abort_flag;
+  if (cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cg::cluster_group cl = cg::this_cluster();
+  if (warp < 4) cl.map_shared_rank(&aux.got[rank][0], 0)[x] = good ? w : __int_as_float(0x7fc00000);
+  if (cluster > 1)
+    cl.sync();
+  else
+    __syncthreads();
+  if (rank == 0 && warp < 4 && j0 + x < total) {
+    float sum = 0.0f;
+    for (int i = 0; i < cluster; ++i) sum += aux.got[i][x];
+    float* out = a.weights + ((int64_t)b * a.c.kv_heads + h) * a.c.max_seq + j0 + x;
+    *out = (j0 + x < len ? *out : 0.0f) + sum;
+  }
+  tc_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256));
   }
 }
 
@@ -609,7 +823,39 @@ int launch_tc(cudaStream_t s, const AttnArgs& a) {
   return SPX_OK;
 }
 
+template <int D>
+int launch_weights_tc(cudaStream_t s, const AttnArgs& a) {
+  const int64_t row_tiles = ceil_div((int64_t)a.T * (a.Hq / a.c.kv_heads), kRows);
+  int cluster = 1;
+  while (cluster < kWeightCluster && cluster * 2 <= row_tiles) cluster *= 2;
+  const int64_t grid = ceil_div(a.c.max_seq, kTile) * cluster;
+  if (grid > INT32_MAX) return fail(SPX_ERR_UNSUPPORTED, "attention_kv8: grid too large");
+  auto kern = kv8_weights_tc_kernel<D>;
+  constexpr size_t smem = WeightShape<D>::kSmem;
+  int rc = check_cuda(
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+      "attention_kv8: smem attribute");
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid, (unsigned)a.c.kv_heads, (unsigned)a.c.batch);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, a, cluster), "attention_kv8: weights");
+}
+
 }  // namespace
+
+int launch_weights_kv8_tc(cudaStream_t s, const AttnArgs& a) {
+  return a.c.head_dim == 64 ? launch_weights_tc<64>(s, a) : launch_weights_tc<128>(s, a);
+}
 
 int launch_attention_kv8_tc(cudaStream_t s, const AttnArgs& a) {
   return a.c.head_dim == 64 ? launch_tc<64>(s, a) : launch_tc<128>(s, a);
