@@ -39,21 +39,31 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
-// Two differences in one instruction.
-__device__ __forceinline__ float2 sub2(float2 a, float2 b) {
+// Two fp32 operations in one instruction, each rounded as the single one is.
+__device__ __forceinline__ unsigned long long f2_bits(float2 v) {
+  return *reinterpret_cast<unsigned long long*>(&v);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
   unsigned long long d;
-  b.x = -b.x;
-  b.y = -b.y;
-  asm("add.rn.f32x2 %0, %1, %2;"
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
       : "=l"(d)
-      : "l"(*reinterpret_cast<unsigned long long*>(&a)),
-        "l"(*reinterpret_cast<unsigned long long*>(&b)));
+      : "l"(f2_bits(a)), "l"(f2_bits(b)), "l"(f2_bits(c)));
   return *reinterpret_cast<float2*>(&d);
 }
 // (x, y) as packed fp16 hi and lo parts.
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
   const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h), d = sub2(make_float2(x, y), f);
+  const float2 f = __half22float2(h), d = add2(make_float2(x, y), make_float2(-f.x, -f.y));
   hi = as_u32(h);
   lo = as_u32(__floats2half2_rn(d.x, d.y));
 }

@@ -27,6 +27,8 @@
 #include <cooperative_groups.h>
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "attn_kv8.cuh"
 #include "sm100_prims.cuh"
 
@@ -95,6 +97,10 @@ __device__ __forceinline__ void mma_f16_ta(uint32_t d, uint32_t a, uint64_t b, u
 // groups of the reduction 1024 bytes apart, the next 64 values an atom away.
 __device__ __forceinline__ uint64_t mn_desc(uint32_t saddr) {
   return (sw128_desc(saddr) & ~(0x3fffull << 16)) | ((uint64_t)(kAtom >> 4) << 16);
+}
+// What k-step i of a K-major operand adds to its descriptor.
+__host__ __device__ constexpr uint64_t k_step(int i) {
+  return ((uint64_t)(i >> 2) * kAtom + (i & 3) * 32) >> 4;
 }
 __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -182,36 +188,46 @@ struct Unit {
 };
 
 // ---- conversion: one row of Q, K and V a thread ------------------------------
-// Row x of an operand from a row of q (null: zeros), hi and lo; returns the
-// factor that takes its products to scores in units of log 2 (NaN for a row
-// with a NaN or an infinity).
 template <int D>
-__device__ __forceinline__ float convert_q(const float* row, float scale, uint8_t* q_hi,
-                                           uint8_t* q_lo, int x) {
-  const float4* from = reinterpret_cast<const float4*>(row);
-  uint32_t mx = 0;
-  bool odd = false;
-  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = 0; i < D / 4; ++i) {
-    const float4 v = row ? __ldg(from + i) : zero;
-    mx = max(max(mx, finite_abs(v.x)), max(finite_abs(v.y), max(finite_abs(v.z),
-                                                                finite_abs(v.w))));
-    odd |= odd_bits(v.x) || odd_bits(v.y) || odd_bits(v.z) || odd_bits(v.w);
+struct Row {                   // a row of q, or zeros
+  float4 v[D / 4];
+  __device__ __forceinline__ void load(const float* row) {
+    const float4* from = reinterpret_cast<const float4*>(row);
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i)
+      v[i] = row ? __ldg(from + i) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  float down, up;
-  pow2_scale(mx, down, up);
-  if (scale < 0.0f) down = -down;
-#pragma unroll 4
-  for (int c = 0; c < D / 8; ++c) {
-    uint4 hi, lo;
-    eight_split(row ? __ldg(from + 2 * c) : zero, row ? __ldg(from + 2 * c + 1) : zero, down, hi,
-                lo);
-    *piece(q_hi, x, c) = hi;
-    *piece(q_lo, x, c) = lo;
+  // Row x of an operand, hi and lo; returns the factor that takes its products
+  // to scores in units of log 2 (NaN for a row with a NaN or an infinity).
+  __device__ __forceinline__ float convert(float scale, uint8_t* hi_to, uint8_t* lo_to,
+                                           int x) const {
+    uint32_t mx = 0;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) {
+      const uint32_t m = max(max(__float_as_uint(v[i].x) & 0x7fffffffu,
+                                 __float_as_uint(v[i].y) & 0x7fffffffu),
+                             max(__float_as_uint(v[i].z) & 0x7fffffffu,
+                                 __float_as_uint(v[i].w) & 0x7fffffffu));
+      mx = max(mx, m);
+    }
+    if (mx >= 0x7f800000u) {
+      odd = true;
+      mx = 0x3f800000u;
+    }
+    float down, up;
+    pow2_scale(mx, down, up);
+    if (scale < 0.0f) down = -down;
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c) {
+      uint4 hi, lo;
+      eight_split(v[2 * c], v[2 * c + 1], down, hi, lo);
+      *piece(hi_to, x, c) = hi;
+      *piece(lo_to, x, c) = lo;
+    }
+    return odd ? __int_as_float(0x7fc00000) : up * (fabsf(scale) * kLog2e);
   }
-  return odd ? __int_as_float(0x7fc00000) : up * (fabsf(scale) * kLog2e);
-}
+};
 
 template <int D>
 __device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& u, uint8_t* slots,
@@ -337,23 +353,27 @@ template <int D>
 struct Issue {
   using S = TcShape<D>;
   static constexpr uint32_t kS = idesc_f16(kRows, kTile, 0), kO = idesc_f16(kRows, D, 1);
-  uint32_t q_hi, q_lo, slots, tmem;
+  uint64_t q_hi, q_lo, k, v;     // descriptors; k and v of slot 0
+  uint32_t tmem;
+  __device__ __forceinline__ Issue(uint32_t q_hi_at, uint32_t q_lo_at, uint32_t slots, uint32_t t)
+      : q_hi(sw128_desc(q_hi_at)), q_lo(sw128_desc(q_lo_at)), k(sw128_desc(slots)),
+        v(mn_desc(slots + S::kAtoms * kAtom)), tmem(t) {}
   // Q (from q) K^T (from slot s) over D.
-  __device__ __forceinline__ void scores(uint32_t q, int s, bool more) const {
-    const uint32_t k = slots + s * S::kSlot;
-#pragma unroll 1
-    for (int i = 0; i < D / 16; ++i) {
-      const uint32_t at = (i >> 2) * kAtom + (i & 3) * 32;
-      mma_f16(tmem, sw128_desc(q + at), sw128_desc(k + at), kS, more || i ? 1u : 0u);
-    }
+  template <bool MORE>
+  __device__ __forceinline__ void scores(uint64_t q, int s) const {
+    const uint64_t from = k + (uint64_t)s * (S::kSlot >> 4);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+      mma_f16(tmem, q + k_step(i), from + k_step(i), kS, MORE || i ? 1u : 0u);
   }
-  // P (hi: part 0, lo: part 16 columns into each 32) V (from slot s) over the keys.
-  __device__ __forceinline__ void values(uint32_t part, int s, bool more) const {
-    const uint32_t v = slots + s * S::kSlot + S::kAtoms * kAtom;
-#pragma unroll 1
+  // P (hi: PART 0, lo: PART 16 columns into each 32) V (from slot s) over the keys.
+  template <int PART, bool MORE>
+  __device__ __forceinline__ void values(int s) const {
+    const uint64_t from = v + (uint64_t)s * (S::kSlot >> 4);
+#pragma unroll
     for (int i = 0; i < kTile / 16; ++i)
-      mma_f16_ta(tmem + kTile, tmem + (i >> 1) * 32 + part + (i & 1) * 8, mn_desc(v + i * 2048),
-                 kO, more || i ? 1u : 0u);
+      mma_f16_ta(tmem + kTile, tmem + (i >> 1) * 32 + PART + (i & 1) * 8, from + i * (2048 >> 4),
+                 kO, MORE || i ? 1u : 0u);
   }
   // S of the tile in slot n (and n + 1), once it is there.
   __device__ __forceinline__ void tile_scores(Aux& aux, int n, bool tail) const {
@@ -362,20 +382,20 @@ struct Issue {
     };
     if (!wait(n)) return;
     tc_after();
-    scores(q_lo, n & 1, false);
-    scores(q_hi, n & 1, true);
+    scores<false>(q_lo, n & 1);
+    scores<true>(q_hi, n & 1);
     if (tail) {
       if (!wait(n + 1)) return;
       tc_after();
-      scores(q_hi, (n + 1) & 1, true);
+      scores<true>(q_hi, (n + 1) & 1);
     }
     mma_commit(&aux.s_ready);
   }
   __device__ __forceinline__ void tile_values(Aux& aux, int n, bool tail) const {
     tc_after();
-    values(16, n & 1, false);
-    values(0, n & 1, true);
-    if (tail) values(0, (n + 1) & 1, true);
+    values<16, false>(n & 1);
+    values<0, true>(n & 1);
+    if (tail) values<0, true>((n + 1) & 1);
     mma_commit(&aux.empty[n & 1]);
     if (tail) mma_commit(&aux.empty[(n + 1) & 1]);
   }
@@ -409,7 +429,13 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
       float v[32];
       tmem_ld_32x32(t_o + c * 32, v);
 #pragma unroll
-      for (int e = 0; e < 32; ++e) o[c * 32 + e] = fmaf(o[c * 32 + e], corr, back * v[e]);
+      for (int e = 0; e < 32; e += 2) {
+        const float2 r = fma2(make_float2(o[c * 32 + e], o[c * 32 + e + 1]),
+                              make_float2(corr, corr),
+                              mul2(make_float2(v[e], v[e + 1]), make_float2(back, back)));
+        o[c * 32 + e] = r.x;
+        o[c * 32 + e + 1] = r.y;
+      }
     }
   };
   int n = 0;
@@ -454,41 +480,48 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
         any_bad |= (w.x | w.y | w.z | w.w) != 0;
       }
     }
-    float sum = 0.0f;
+    float2 sum = make_float2(0.f, 0.f);
+    auto weigh = [&](auto tag) {
+      constexpr bool masked = decltype(tag)::value;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      float v[32];
-      tmem_ld_32x32(t_s + c * 32, v);
-      uint32_t p[32];
-      float part = 0.0f;
+      for (int c = 0; c < 4; ++c) {
+        float v[32];
+        tmem_ld_32x32(t_s + c * 32, v);
+        uint32_t p[32];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const float f = aux.k_scale[s][c * 2 + half] * qs, share = aux.share[s][c * 2 + half];
+        for (int half = 0; half < 2; ++half) {
+          const float f = aux.k_scale[s][c * 2 + half] * qs, share = aux.share[s][c * 2 + half];
 #pragma unroll
-        for (int e = half * 16; e < half * 16 + 16; ++e) {
-          float w = ex2(fmaf(v[e], f, -base));
-          if (mask && c * 32 + e > seen) w = 0.0f;
-          part += w;
-          w *= share;
-          if (mask && c * 32 + e > seen) w = 0.0f;
-          v[e] = w;
+          for (int e = half * 16; e < half * 16 + 16; e += 2) {
+            float2 w = fma2(make_float2(v[e], v[e + 1]), make_float2(f, f),
+                            make_float2(-base, -base));
+            w = make_float2(ex2(w.x), ex2(w.y));
+            if (masked) {
+              if (c * 32 + e > seen) w.x = 0.0f;
+              if (c * 32 + e + 1 > seen) w.y = 0.0f;
+            }
+            sum = add2(sum, w);
+            w = mul2(w, make_float2(share, share));
+            if (masked) {              // (a share may be NaN)
+              if (c * 32 + e > seen) w.x = 0.0f;
+              if (c * 32 + e + 1 > seen) w.y = 0.0f;
+            }
+            if (masked && any_bad) {
+              if (c * 32 + e <= seen && aux.bad[s][c * 32 + e]) w.x = __int_as_float(0x7fc00000);
+              if (c * 32 + e + 1 <= seen && aux.bad[s][c * 32 + e + 1])
+                w.y = __int_as_float(0x7fc00000);
+            }
+            split2(w.x, w.y, p[e / 2], p[16 + e / 2]);
+          }
         }
+        tmem_st_32x32(t_s + c * 32, p);
       }
-      if (any_bad) {
-#pragma unroll 1
-        for (int e = 0; e < 32; ++e) {
-          const bool hit = aux.bad[s][c * 32 + e] && c * 32 + e <= seen;
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (i == e && hit) v[i] = __int_as_float(0x7fc00000);
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) split2(v[2 * e], v[2 * e + 1], p[e], p[16 + e]);
-      sum += part;
-      tmem_st_32x32(t_s + c * 32, p);
-    }
-    l = fmaf(l, corr, sum);
+    };
+    if (mask || any_bad)
+      weigh(std::true_type());
+    else
+      weigh(std::false_type());
+    l = fmaf(l, corr, sum.x + sum.y);
     back = aux.back[s];
     tmem_wait_st();
     tc_before();
@@ -546,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
     if constexpr (D == 64)
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftmaxRegs));
     const int x = threadIdx.x;
-    const Issue<D> issue{sa(q_hi), sa(q_lo), sa(slots), tmem};
+    const Issue<D> issue(sa(q_hi), sa(q_lo), sa(slots), tmem);
     float o[D], m, l;
 #pragma unroll
     for (int i = 0; i < D; ++i) o[i] = 0.0f;
@@ -573,8 +606,11 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kConvertRegs));
     const int x = threadIdx.x - 128;
     const int r = u.r0 + x;
-    q_scale[x] =
-        convert_q<D>(r < u.rows ? a.q + u.row_at(a, r) * D : nullptr, a.scale, q_hi, q_lo, x);
+    {
+      Row<D> row;
+      row.load(r < u.rows ? a.q + u.row_at(a, r) * D : nullptr);
+      q_scale[x] = row.convert(a.scale, q_hi, q_lo, x);
+    }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mb_arrive(&aux.q_full);
     convert_tiles<D>(a, u, slots, aux, x);
@@ -598,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
 constexpr int kWeightCluster = 4;
 
 struct WeightAux {
-  float2 row[2][kRows];        // the row's factor, and its lse in units of log 2
+  alignas(16) float2 row[2][kRows];   // the row's factor, and its lse in units of log 2
   float got[kWeightCluster][kTile];
   uint64_t full[2], empty[2], k_full, s_ready[2], done;
   uint32_t tmem;
@@ -664,15 +700,24 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
       const int tk = a.div_g(r);
       return ((int64_t)b * a.T + tk) * a.Hq + h * G + (r - tk * G);
     };
+    Row<D> row;
+    float z = INFINITY;                // (a row that is none weighs nothing)
+    auto load = [&](int i) {
+      const int r = row0(i) + x;
+      const bool is = i < tiles && r < rows;
+      const int64_t at = is ? row_at(r) : 0;
+      row.load(is ? a.q + at * D : nullptr);
+      z = is ? a.lse[at] * kLog2e : INFINITY;
+    };
+    load(0);
     for (int i = 0; i < tiles; ++i) {
-      const int s = i & 1, r = row0(i) + x;
-      if (!wait(&aux.empty[s], ((i >> 1) & 1) ^ 1)) break;
+      const int s = i & 1;
+      if (!mb_wait(&aux.empty[s], ((i >> 1) & 1) ^ 1, &aux.abort_flag, &g_at_status, kWaitNs, 128))
+        break;
       uint8_t* to = slots + s * S::kSlot;
-      const int64_t at = r < rows ? row_at(r) : 0;
-      const float f =
-          convert_q<D>(r < rows ? a.q + at * D : nullptr, a.scale, to, to + S::kSlot / 2, x);
-      // (a row that is none weighs nothing)
-      aux.row[s][x] = make_float2(f, r < rows ? a.lse[at] * kLog2e : INFINITY);
+      const float f = row.convert(a.scale, to, to + S::kSlot / 2, x);
+      aux.row[s][x] = make_float2(f, z);
+      load(i + 1);                     // on its way while the slot is used
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mb_arrive(&aux.full[s]);
     }
@@ -716,23 +761,23 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mb_arrive(&aux.k_full);
-    const uint32_t kh = sa(k_hi), kl = sa(k_lo);
+    const uint64_t kh = sw128_desc(sa(k_hi)), kl = sw128_desc(sa(k_lo));
+    const uint64_t q0 = sw128_desc(sa(slots));
     constexpr uint32_t kDesc = idesc_f16(kTile, kRows, 0);
-    auto products = [&](uint32_t k, uint32_t q, uint32_t to, bool more) {
-#pragma unroll 1
-      for (int i = 0; i < D / 16; ++i) {
-        const uint32_t at = (i >> 2) * kAtom + (i & 3) * 32;
-        mma_f16(to, sw128_desc(k + at), sw128_desc(q + at), kDesc, more || i ? 1u : 0u);
-      }
+    auto products = [&](uint64_t k, uint64_t q, uint32_t to, uint32_t more) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+        mma_f16(to, k + k_step(i), q + k_step(i), kDesc, i ? 1u : more);
     };
     auto issue = [&](int i) {                 // by one thread
       const int s = i & 1;
       if (!wait(&aux.full[s], (i >> 1) & 1)) return;
       tc_after();
-      const uint32_t qh = sa(slots) + s * S::kSlot, ql = qh + S::kSlot / 2, to = tmem + s * kRows;
-      products(kh, ql, to, false);
-      if (tail) products(kl, qh, to, true);
-      products(kh, qh, to, true);
+      const uint64_t qh = q0 + (uint64_t)s * (S::kSlot >> 4), ql = qh + (S::kSlot >> 5);
+      const uint32_t to = tmem + s * kRows;
+      products(kh, ql, to, 0u);
+      if (tail) products(kl, qh, to, 1u);
+      products(kh, qh, to, 1u);
       mma_commit(&aux.empty[s]);
       mma_commit(&aux.s_ready[s]);
     };
@@ -749,19 +794,34 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
       tc_after();
       const bool mask = row0(i) < r_all;
       const int from = r_min - row0(i);       // the first column that the key is seen by
-#pragma unroll 1
-      for (int c = 0; c < kRows / 32; ++c) {
-        float v[32];
-        tmem_ld_32x32(tmem + s * kRows + lanes + c * 32, v);
-        float part = 0.0f;
+      auto add = [&](auto tag) {
+        constexpr bool masked = decltype(tag)::value;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float2 r = aux.row[s][c * 32 + e];
-          const float p = ex2(fmaf(v[e], ks * r.x, -r.y));
-          part += mask && c * 32 + e < from ? 0.0f : p;
+        for (int c = 0; c < kRows / 32; ++c) {
+          float v[32];
+          tmem_ld_32x32(tmem + s * kRows + lanes + c * 32, v);
+          float2 part = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            // factor and lse of two rows
+            const float4 r = *reinterpret_cast<const float4*>(&aux.row[s][c * 32 + e]);
+            float2 p = fma2(make_float2(v[e], v[e + 1]),
+                            mul2(make_float2(r.x, r.z), make_float2(ks, ks)),
+                            make_float2(-r.y, -r.w));
+            p = make_float2(ex2(p.x), ex2(p.y));
+            if (masked) {
+              if (c * 32 + e < from) p.x = 0.0f;
+              if (c * 32 + e + 1 < from) p.y = 0.0f;
+            }
+            part = add2(part, p);
+          }
+          w += part.x + part.y;
         }
-        w += part;
-      }
+      };
+      if (mask)
+        add(std::true_type());
+      else
+        add(std::false_type());
       tc_before();
       mb_arrive(&aux.empty[s]);
       vote(2, true);                          // this half of TMEM has been read
