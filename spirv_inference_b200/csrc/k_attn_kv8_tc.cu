@@ -1,17 +1,21 @@
 // Attention over the 8-bit cache for many rows (prompts), on tcgen05.
 //
 // A CTA takes 128 rows, (new token, head of the group) pairs of one sequence
-// and kv head, and walks the keys they see in tiles of 128:
+// and kv head, and walks the keys they see in tiles of 64:
 //
 //   four warps turn a tile's K and V into fp16 (int8 is exact there) in shared
-//     memory, one key a thread, two tiles ahead;
+//     memory, a row of K or V a thread;
 //   S = Q K^T goes into TMEM, q as fp16 hi + lo, two products;
 //   four warps, one row a thread, read S, take the softmax step, and write P,
-//     as fp16 hi + lo, over the part of S that they have just read;
+//     as fp16 hi + lo, over S;
 //   O = P V, two products with P from TMEM, each tile into a fresh accumulator;
-//     one thread of these warps issues it, and then the next tile's S;
 //   the row's thread adds O to its output in registers, in fp32 (the tensor
 //     core's sums round towards zero: over a whole prompt that shows).
+//
+// S and O have two buffers each, so that the products of a tile run under the
+// softmax of its neighbours; one thread of the conversion warps issues them.
+// (With tiles of 128 keys, one buffer and the issue on a softmax thread, a tile
+// of 128 took 10.7 thousand cycles, 3.3 of them issuing and 5.3 of softmax.)
 //
 // K and V rows are 128 bytes of 64 values under the 128-byte swizzle: K is a
 // K-major operand, V, whose keys are the reduction, an MN-major one of the same
@@ -22,8 +26,8 @@
 // power of two for 16 keys, and the lo parts, whose products with the hi parts
 // of q and p are added.
 //
-// What bounds it: the softmax warps' instructions, about 20 a score; the
-// tensor core needs half of that time.  Two CTAs an SM (D = 64) overlap them.
+// What bounds it: the softmax warps' instructions, about 9 a score, at two CTAs
+// an SM (D = 64).
 #include <cooperative_groups.h>
 #include <cuda.h>
 
@@ -41,7 +45,7 @@ namespace {
 using namespace sm100;
 namespace cg = cooperative_groups;
 
-constexpr int kRows = 128, kTile = 128;
+constexpr int kRows = 128, kTile = 64, kGroups = kTile / 16;
 constexpr int kThreads = 256;             // softmax, conversion
 constexpr uint32_t kAtom = 128 * 128;     // 128 rows of 128 bytes
 constexpr unsigned long long kWaitNs = 2000000000ull;
@@ -50,9 +54,11 @@ constexpr float kMaxFloat = 3.4028234663852886e38f;
 template <int D>
 struct TcShape {
   static constexpr int kAtoms = D / 64;
+  static constexpr int kSlots = 4;
   static constexpr uint32_t kQ = kAtoms * kAtom;         // hi or lo
-  static constexpr uint32_t kSlot = 2 * kAtoms * kAtom;  // K, V
-  static constexpr uint32_t kTmem = 256;                 // S / P: 128 columns, O: D
+  static constexpr uint32_t kHalf = kAtoms * kTile * 128;  // K or V of a slot
+  static constexpr uint32_t kSlot = 2 * kHalf;
+  static constexpr uint32_t kTmem = D == 64 ? 256 : 512;   // S / P: 2 x 64 columns, O: 2 x D
   static constexpr int kBlocks = D == 64 ? 2 : 1;        // CTAs an SM
   // Two CTAs an SM leave 128 registers a thread; the conversion warps give
   // some of theirs to the softmax warps, which hold a row of the output.
@@ -60,13 +66,13 @@ struct TcShape {
   static_assert(kSoftmaxRegs + kConvertRegs <= 2 * kRegs, "within what the launch has");
 };
 
-struct Aux {                   // of the two slots
-  float k_scale[2][8];         // of 16 keys
-  float v_raw[2][8];
-  float share[2][8];
-  float back[2];
-  alignas(16) uint8_t bad[2][kTile];   // the key's V has a NaN or an infinity (tail)
-  uint64_t full[2], empty[2], q_full, s_ready, done;
+struct Aux {                   // of the slots
+  float k_scale[4][kGroups];   // of 16 keys
+  float v_raw[4][kGroups];
+  float share[4][kGroups];
+  float back[4];
+  alignas(16) uint8_t bad[4][kTile];   // the key's V has a NaN or an infinity (tail)
+  uint64_t full[4], empty[4], q_full, s_ready[2], p_ready[2], done;
   uint32_t tmem;
   int abort_flag;
 };
@@ -96,11 +102,11 @@ __device__ __forceinline__ void mma_f16_ta(uint32_t d, uint32_t a, uint64_t b, u
 // MN-major operand in the same layout as sw128_desc's: 64 values a row, 8-row
 // groups of the reduction 1024 bytes apart, the next 64 values an atom away.
 __device__ __forceinline__ uint64_t mn_desc(uint32_t saddr) {
-  return (sw128_desc(saddr) & ~(0x3fffull << 16)) | ((uint64_t)(kAtom >> 4) << 16);
+  return (sw128_desc(saddr) & ~(0x3fffull << 16)) | ((uint64_t)((kTile * 128) >> 4) << 16);
 }
-// What k-step i of a K-major operand adds to its descriptor.
-__host__ __device__ constexpr uint64_t k_step(int i) {
-  return ((uint64_t)(i >> 2) * kAtom + (i & 3) * 32) >> 4;
+// What k-step i of a K-major operand of `rows` rows adds to its descriptor.
+__host__ __device__ constexpr uint64_t k_step(int i, int rows) {
+  return ((uint64_t)(i >> 2) * rows * 128 + (i & 3) * 32) >> 4;
 }
 __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -132,9 +138,11 @@ __device__ __forceinline__ bool vote(int id, bool ok) {
   return r != 0;
 }
 
-// 16 bytes of piece `c` (eight values) of row `r` of an operand.
+// 16 bytes of piece `c` (eight values) of row `r` of an operand of ROWS rows.
+template <int ROWS>
 __device__ __forceinline__ uint4* piece(uint8_t* base, int r, int c) {
-  return reinterpret_cast<uint4*>(base + (c >> 3) * kAtom + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+  return reinterpret_cast<uint4*>(base + (c >> 3) * (ROWS * 128) + r * 128 +
+                                  (((c & 7) ^ (r & 7)) << 4));
 }
 // Eight int8 values as fp16, each four in the order 0, 2, 1, 3.
 __device__ __forceinline__ uint4 eight(uint32_t a, uint32_t b, uint32_t mask) {
@@ -222,131 +230,12 @@ struct Row {                   // a row of q, or zeros
     for (int c = 0; c < D / 8; ++c) {
       uint4 hi, lo;
       eight_split(v[2 * c], v[2 * c + 1], down, hi, lo);
-      *piece(hi_to, x, c) = hi;
-      *piece(lo_to, x, c) = lo;
+      *piece<kRows>(hi_to, x, c) = hi;
+      *piece<kRows>(lo_to, x, c) = lo;
     }
     return odd ? __int_as_float(0x7fc00000) : up * (fabsf(scale) * kLog2e);
   }
 };
-
-template <int D>
-__device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& u, uint8_t* slots,
-                                              Aux& aux, int x) {
-  using S = TcShape<D>;
-  const int64_t bh = (int64_t)u.b * a.c.kv_heads + u.h;
-  const int8_t* k8 = a.c.k + bh * a.c.max_seq * D;
-  const int8_t* v8 = a.c.v + bh * a.c.max_seq * D;
-  const int blk = a.c.block;
-  const float* ks = a.c.k_scale + bh * (a.c.max_seq / blk);
-  const float* vs = a.c.v_scale + bh * (a.c.max_seq / blk);
-  const float* kt = a.c.k_tail + bh * blk * D;
-  const float* vt = a.c.v_tail + bh * blk * D;
-  uint32_t mask;
-  asm volatile("mov.b32 %0, 0x00ff00ff;" : "=r"(mask));
-  int n = 0;                   // slots used
-  for (int tile = 0; tile < u.tiles; ++tile, ++n) {
-    const int key = tile * kTile + x, s = n & 1;
-    const bool closed = key < u.closed, in_tail = !closed && key < u.total;
-    const bool tail = u.has_tail(tile);
-    // The rows' bytes, and the scales, are on their way while the slot drains.
-    uint4 kr[D / 16], vr[D / 16];
-    float k_sc = 0.0f, v_sc = 0.0f;
-    if (closed) {
-      const uint4* kp = reinterpret_cast<const uint4*>(k8 + (int64_t)key * D);
-      const uint4* vp = reinterpret_cast<const uint4*>(v8 + (int64_t)key * D);
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) kr[i] = __ldg(kp + i);
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) vr[i] = __ldg(vp + i);
-      k_sc = __ldg(ks + key / blk);
-      v_sc = __ldg(vs + key / blk);
-    }
-    float k_down = 0.0f, v_down = 0.0f;
-    const float4* kf = reinterpret_cast<const float4*>(kt + (int64_t)(key & (blk - 1)) * D);
-    const float4* vf = reinterpret_cast<const float4*>(vt + (int64_t)(key & (blk - 1)) * D);
-    bool odd = false, unused = false;
-    if (tail) {                // the tail's 16-key groups: powers of two
-      uint32_t mk = 0, mv = 0;
-      if (in_tail)
-        for (int i = 0; i < D / 4; ++i) {
-          const float4 p = kf[i], q = finite4(vf[i], odd);
-          mk = max(max(mk, finite_abs(p.x)),
-                   max(finite_abs(p.y), max(finite_abs(p.z), finite_abs(p.w))));
-          mv = max(max(mv, finite_abs(q.x)),
-                   max(finite_abs(q.y), max(finite_abs(q.z), finite_abs(q.w))));
-        }
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) {
-        mk = max(mk, __shfl_xor_sync(0xffffffffu, mk, o));
-        mv = max(mv, __shfl_xor_sync(0xffffffffu, mv, o));
-      }
-      if (!closed) {
-        pow2_scale(mk, k_down, k_sc);
-        pow2_scale(mv, v_down, v_sc);
-      }
-    }
-    const bool drained =
-        mb_wait(&aux.empty[s], ((n >> 1) & 1) ^ 1, &aux.abort_flag, &g_at_status, kWaitNs, 64);
-    if (drained && (x & 15) == 0) {
-      aux.k_scale[s][x >> 4] = k_sc;
-      aux.v_raw[s][x >> 4] = v_sc;
-    }
-    if (drained) aux.bad[s][x] = odd;
-    if (!vote(1, drained)) return;
-    if (x < 8) {
-      float ref = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float v = aux.v_raw[s][i];
-        if (v <= kMaxFloat) ref = fmaxf(ref, v);
-      }
-      aux.share[s][x] = ref > 0.0f ? aux.v_raw[s][x] * (kPUp / ref) : aux.v_raw[s][x];
-      if (x == 0) aux.back[s] = ref * (1.0f / kPUp);
-    }
-    uint8_t* k_to = slots + s * S::kSlot;
-    uint8_t* v_to = k_to + S::kAtoms * kAtom;
-    if (closed) {
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        *piece(k_to, x, 2 * i) = eight(kr[i].x, kr[i].y, mask);
-        *piece(k_to, x, 2 * i + 1) = eight(kr[i].z, kr[i].w, mask);
-        *piece(v_to, x, 2 * i) = eight(vr[i].x, vr[i].y, mask);
-        *piece(v_to, x, 2 * i + 1) = eight(vr[i].z, vr[i].w, mask);
-      }
-    } else {
-      for (int c = 0; c < D / 8; ++c) {
-        uint4 hi = make_uint4(0, 0, 0, 0), lo, vh = hi;
-        if (in_tail) {
-          eight_split(kf[2 * c], kf[2 * c + 1], k_down, hi, lo);
-          eight_split(finite4(vf[2 * c], unused), finite4(vf[2 * c + 1], unused), v_down, vh, lo);
-        }
-        *piece(k_to, x, c) = hi;
-        *piece(v_to, x, c) = vh;
-      }
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    mb_arrive(&aux.full[s]);
-    if (!tail) continue;
-    ++n;
-    const int s2 = n & 1;
-    if (!vote(1, mb_wait(&aux.empty[s2], ((n >> 1) & 1) ^ 1, &aux.abort_flag, &g_at_status,
-                         kWaitNs, 64)))
-      return;
-    k_to = slots + s2 * S::kSlot;
-    v_to = k_to + S::kAtoms * kAtom;
-    for (int c = 0; c < D / 8; ++c) {
-      uint4 hi, lo = make_uint4(0, 0, 0, 0), vl = lo;
-      if (in_tail) {
-        eight_split(kf[2 * c], kf[2 * c + 1], k_down, hi, lo);
-        eight_split(finite4(vf[2 * c], unused), finite4(vf[2 * c + 1], unused), v_down, hi, vl);
-      }
-      *piece(k_to, x, c) = lo;
-      *piece(v_to, x, c) = vl;
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    mb_arrive(&aux.full[s2]);
-  }
-}
 
 // ---- products, issued by one thread ----------------------------------------------
 template <int D>
@@ -357,77 +246,195 @@ struct Issue {
   uint32_t tmem;
   __device__ __forceinline__ Issue(uint32_t q_hi_at, uint32_t q_lo_at, uint32_t slots, uint32_t t)
       : q_hi(sw128_desc(q_hi_at)), q_lo(sw128_desc(q_lo_at)), k(sw128_desc(slots)),
-        v(mn_desc(slots + S::kAtoms * kAtom)), tmem(t) {}
-  // Q (from q) K^T (from slot s) over D.
+        v(mn_desc(slots + S::kHalf)), tmem(t) {}
+  // Q (from q) K^T (from slot s) over D, to S buffer `to`.
   template <bool MORE>
-  __device__ __forceinline__ void scores(uint64_t q, int s) const {
+  __device__ __forceinline__ void scores(uint64_t q, int s, int to) const {
     const uint64_t from = k + (uint64_t)s * (S::kSlot >> 4);
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
-      mma_f16(tmem, q + k_step(i), from + k_step(i), kS, MORE || i ? 1u : 0u);
+      mma_f16(tmem + to * kTile, q + k_step(i, kRows), from + k_step(i, kTile), kS,
+              MORE || i ? 1u : 0u);
   }
-  // P (hi: PART 0, lo: PART 16 columns into each 32) V (from slot s) over the keys.
+  // P (of S buffer `to`; hi: PART 0, lo: PART 16 columns into each 32) V (from
+  // slot s) over the keys, to O buffer `to`.
   template <int PART, bool MORE>
-  __device__ __forceinline__ void values(int s) const {
+  __device__ __forceinline__ void values(int s, int to) const {
     const uint64_t from = v + (uint64_t)s * (S::kSlot >> 4);
 #pragma unroll
     for (int i = 0; i < kTile / 16; ++i)
-      mma_f16_ta(tmem + kTile, tmem + (i >> 1) * 32 + PART + (i & 1) * 8, from + i * (2048 >> 4),
-                 kO, MORE || i ? 1u : 0u);
+      mma_f16_ta(tmem + 2 * kTile + to * D, tmem + to * kTile + (i >> 1) * 32 + PART + (i & 1) * 8,
+                 from + i * (2048 >> 4), kO, MORE || i ? 1u : 0u);
   }
-  // S of the tile in slot n (and n + 1), once it is there.
-  __device__ __forceinline__ void tile_scores(Aux& aux, int n, bool tail) const {
+  // S of a tile whose rows are in slot n (and n + 1), once they are there.
+  __device__ __forceinline__ void tile_scores(Aux& aux, int tile, int n, bool tail) const {
     auto wait = [&](int k) {
-      return mb_wait(&aux.full[k & 1], (k >> 1) & 1, &aux.abort_flag, &g_at_status, kWaitNs, 32);
+      return mb_wait(&aux.full[k & 3], (k >> 2) & 1, &aux.abort_flag, &g_at_status, kWaitNs, 32);
     };
     if (!wait(n)) return;
     tc_after();
-    scores<false>(q_lo, n & 1);
-    scores<true>(q_hi, n & 1);
+    scores<false>(q_lo, n & 3, tile & 1);
+    scores<true>(q_hi, n & 3, tile & 1);
     if (tail) {
       if (!wait(n + 1)) return;
       tc_after();
-      scores<true>(q_hi, (n + 1) & 1);
+      scores<true>(q_hi, (n + 1) & 3, tile & 1);
     }
-    mma_commit(&aux.s_ready);
+    mma_commit(&aux.s_ready[tile & 1]);
   }
-  __device__ __forceinline__ void tile_values(Aux& aux, int n, bool tail) const {
+  // O of a tile, once P is there.
+  __device__ __forceinline__ void tile_values(Aux& aux, int tile, int n, bool tail) const {
+    if (!mb_wait(&aux.p_ready[tile & 1], (tile >> 1) & 1, &aux.abort_flag, &g_at_status, kWaitNs,
+                 32))
+      return;
     tc_after();
-    values<16, false>(n & 1);
-    values<0, true>(n & 1);
-    if (tail) values<0, true>((n + 1) & 1);
-    mma_commit(&aux.empty[n & 1]);
-    if (tail) mma_commit(&aux.empty[(n + 1) & 1]);
+    values<16, false>(n & 3, tile & 1);
+    values<0, true>(n & 3, tile & 1);
+    if (tail) values<0, true>((n + 1) & 3, tile & 1);
+    mma_commit(&aux.empty[n & 3]);
+    if (tail) mma_commit(&aux.empty[(n + 1) & 3]);
   }
 };
+
+// ---- conversion: a row of K (threads 0 .. 63) or V a thread; thread 0 issues ------
+template <int D>
+__device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& u, uint8_t* slots,
+                                              Aux& aux, const Issue<D>& issue, int x) {
+  using S = TcShape<D>;
+  const int64_t bh = (int64_t)u.b * a.c.kv_heads + u.h;
+  const bool is_v = x >= kTile;
+  const int r = x & (kTile - 1), blk = a.c.block;
+  const int8_t* from8 = (is_v ? a.c.v : a.c.k) + bh * a.c.max_seq * D;
+  const float* scales = (is_v ? a.c.v_scale : a.c.k_scale) + bh * (a.c.max_seq / blk);
+  const float* tails = (is_v ? a.c.v_tail : a.c.k_tail) + bh * blk * D;
+  float(*raw)[kGroups] = is_v ? aux.v_raw : aux.k_scale;
+  uint32_t mask;
+  asm volatile("mov.b32 %0, 0x00ff00ff;" : "=r"(mask));
+  // Step j: the products P V of tile j - 2, the rows of tile j, its S.
+  int n = 0, n1 = 0, n2 = 0;   // the slots of tiles j, j - 1, j - 2
+  for (int j = 0; j < u.tiles + 2; ++j) {
+    const int key = j * kTile + r;
+    const bool closed = key < u.closed, in_tail = !closed && key < u.total;
+    const bool tail = u.has_tail(j);
+    // The row's bytes, and its scale, are on their way meanwhile.
+    uint4 row[D / 16];
+    float sc = 0.0f;
+    if (j < u.tiles && closed) {
+      const uint4* p = reinterpret_cast<const uint4*>(from8 + (int64_t)key * D);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) row[i] = __ldg(p + i);
+      sc = __ldg(scales + key / blk);
+    }
+    if (x == 0 && j >= 2) {
+      issue.tile_values(aux, j - 2, n2, u.has_tail(j - 2));
+      if (j == u.tiles + 1) mma_commit(&aux.done);
+    }
+    __syncwarp();
+    if (j >= u.tiles) {
+      n2 = n1;
+      continue;
+    }
+    float down = 0.0f;
+    const float4* rf = reinterpret_cast<const float4*>(tails + (int64_t)(key & (blk - 1)) * D);
+    bool odd = false, unused = false;
+    if (tail) {                // the tail's 16-key groups: powers of two
+      uint32_t mx = 0;
+      if (in_tail)
+        for (int i = 0; i < D / 4; ++i) {
+          float4 p = rf[i];
+          if (is_v) p = finite4(p, odd);
+          mx = max(max(mx, finite_abs(p.x)),
+                   max(finite_abs(p.y), max(finite_abs(p.z), finite_abs(p.w))));
+        }
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      if (!closed) pow2_scale(mx, down, sc);
+    }
+    const int s = n & 3;
+    const bool drained = mb_wait(&aux.empty[s], ((n >> 2) & 1) ^ 1, &aux.abort_flag, &g_at_status,
+                                 kWaitNs, 64);
+    if (drained) {
+      if ((r & 15) == 0) raw[s][r >> 4] = sc;
+      if (is_v) aux.bad[s][r] = odd;
+    }
+    if (!vote(1, drained)) return;
+    if (x < kGroups) {
+      float ref = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) {
+        const float v = aux.v_raw[s][i];
+        if (v <= kMaxFloat) ref = fmaxf(ref, v);
+      }
+      aux.share[s][x] = ref > 0.0f ? aux.v_raw[s][x] * (kPUp / ref) : aux.v_raw[s][x];
+      if (x == 0) aux.back[s] = ref * (1.0f / kPUp);
+    }
+    uint8_t* to = slots + s * S::kSlot + (is_v ? S::kHalf : 0);
+    auto put_tail = [&](uint8_t* base, bool low) {
+      for (int c = 0; c < D / 8; ++c) {
+        uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+        if (in_tail) {
+          float4 p = rf[2 * c], q = rf[2 * c + 1];
+          if (is_v) {
+            p = finite4(p, unused);
+            q = finite4(q, unused);
+          }
+          eight_split(p, q, down, hi, lo);
+        }
+        *piece<kTile>(base, r, c) = low ? lo : hi;
+      }
+    };
+    if (closed) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        *piece<kTile>(to, r, 2 * i) = eight(row[i].x, row[i].y, mask);
+        *piece<kTile>(to, r, 2 * i + 1) = eight(row[i].z, row[i].w, mask);
+      }
+    } else {
+      put_tail(to, false);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    mb_arrive(&aux.full[s]);
+    if (tail) {
+      const int s2 = (n + 1) & 3;
+      if (!vote(1, mb_wait(&aux.empty[s2], (((n + 1) >> 2) & 1) ^ 1, &aux.abort_flag,
+                           &g_at_status, kWaitNs, 64)))
+        return;
+      put_tail(slots + s2 * S::kSlot + (is_v ? S::kHalf : 0), true);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mb_arrive(&aux.full[s2]);
+    }
+    if (x == 0) issue.tile_scores(aux, j, n, tail);
+    __syncwarp();
+    n2 = n1;
+    n1 = n;
+    n += tail ? 2 : 1;
+  }
+}
 
 // ---- softmax: one row a thread -------------------------------------------------
 template <int D>
 __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& u, Aux& aux,
-                                              const float* q_scale, const Issue<D>& issue, int x,
+                                              const float* q_scale, uint32_t tmem, int x,
                                               float (&o)[D], float& m, float& l) {
-  const uint32_t tmem = issue.tmem;
-  const uint32_t lanes = (uint32_t)((x >> 5) * 32) << 16;
-  const uint32_t t_s = tmem + lanes, t_o = tmem + lanes + kTile;
+  const uint32_t lanes = tmem + ((uint32_t)((x >> 5) * 32) << 16);
   auto wait = [&](uint64_t* b, int parity) {
-    return mb_wait(b, parity, &aux.abort_flag, &g_at_status, kWaitNs, 32);
+    const bool ok = mb_wait(b, parity, &aux.abort_flag, &g_at_status, kWaitNs, 32);
+    return __all_sync(0xffffffffu, ok) != 0;   // a warp goes on or ends as one
   };
-  // Exits are by vote: no warp is left alone at a barrier.
-  if (!vote(2, wait(&aux.q_full, 0))) return false;
-  if (x == 0) issue.tile_scores(aux, 0, u.has_tail(0));
+  if (!wait(&aux.q_full, 0)) return false;
   const float qs = q_scale[x];
   const int last = min(u.len + a.div_g(min(u.r0 + x, u.rows - 1)), u.total - 1);
   const int last_of_first = min(u.len + a.div_g(u.r0), u.total - 1);
   m = -INFINITY;
   l = 0.0f;
-  float corr = 0.0f, back = 0.0f;   // of the tile before
-  // o = o corr + back * (P V of the tile before)
-  auto take_output = [&]() {
-    tc_after();
+  // of the tile before, and of the one before that, whose output comes next
+  float corr1 = 0.0f, back1 = 0.0f, corr2 = 0.0f, back2 = 0.0f;
+  // o = o corr + back * (P V of `tile`)
+  auto take_output = [&](int tile, float corr, float back) {
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
       float v[32];
-      tmem_ld_32x32(t_o + c * 32, v);
+      tmem_ld_32x32(lanes + 2 * kTile + (tile & 1) * D + c * 32, v);
 #pragma unroll
       for (int e = 0; e < 32; e += 2) {
         const float2 r = fma2(make_float2(o[c * 32 + e], o[c * 32 + e + 1]),
@@ -439,38 +446,41 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
     }
   };
   int n = 0;
-  for (int tile = 0; tile < u.tiles; ++tile, ++n) {
-    const int s = n & 1, j0 = tile * kTile;
+  for (int tile = 0; tile < u.tiles; ++tile) {
+    const int s = n & 3, j0 = tile * kTile;
     const bool tail = u.has_tail(tile);
     // (the slot for its scales)
-    if (!vote(2, wait(&aux.full[s], (n >> 1) & 1) && wait(&aux.s_ready, tile & 1))) return false;
+    if (!wait(&aux.full[s], (n >> 2) & 1)) return false;
+    if (!wait(&aux.s_ready[tile & 1], (tile >> 1) & 1)) return false;
+    n += tail ? 2 : 1;
     tc_after();
+    const uint32_t t_s = lanes + (tile & 1) * kTile;
+    // The products before this tile's S are done, P V of two tiles back too.
+    if (tile >= 2) take_output(tile - 2, corr2, back2);
     const bool mask = j0 + kTile - 1 > last_of_first;
     const int seen = last - j0;         // the last column that the row sees
-    float mt = -INFINITY;
+    float v[kTile];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      float v[32];
-      tmem_ld_32x32(t_s + c * 32, v);
-      if (mask) {
+    for (int c = 0; c < kTile / 32; ++c)
+      tmem_ld_32x32_async(t_s + c * 32, reinterpret_cast<uint32_t(&)[32]>(v[c * 32]));
+    tmem_wait_ld();
+    float f[kGroups], mt = -INFINITY;
+    if (mask) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e)
-          if (c * 32 + e > seen) v[e] = -INFINITY;
-      }
+      for (int e = 0; e < kTile; ++e)
+        if (e > seen) v[e] = -INFINITY;
+    }
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const float f = aux.k_scale[s][c * 2 + half] * qs;
-        float most = v[half * 16];
+    for (int i = 0; i < kGroups; ++i) {
+      f[i] = aux.k_scale[s][i] * qs;
+      float most = v[i * 16];
 #pragma unroll
-        for (int e = 1; e < 16; ++e) most = fmaxf(most, v[half * 16 + e]);
-        // (a factor of 0 or NaN would make NaN of -inf, which fmaxf passes over)
-        mt = fmaxf(mt, most * f);
-      }
+      for (int e = 1; e < 16; ++e) most = fmaxf(most, v[i * 16 + e]);
+      // (a factor of 0 or NaN would make NaN of -inf, which fmaxf passes over)
+      mt = fmaxf(mt, most * f[i]);
     }
     const float mn = fmaxf(m, mt), base = mn == -INFINITY ? 0.0f : mn;
-    // The output of the tile before is relative to the old maximum.
-    if (tile > 0) take_output();
-    corr = ex2(m - base);
+    const float corr = ex2(m - base);
     m = mn;
     bool any_bad = false;
     if (tail) {
@@ -484,35 +494,30 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
     auto weigh = [&](auto tag) {
       constexpr bool masked = decltype(tag)::value;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float v[32];
-        tmem_ld_32x32(t_s + c * 32, v);
+      for (int c = 0; c < kTile / 32; ++c) {
         uint32_t p[32];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const float f = aux.k_scale[s][c * 2 + half] * qs, share = aux.share[s][c * 2 + half];
-#pragma unroll
-          for (int e = half * 16; e < half * 16 + 16; e += 2) {
-            float2 w = fma2(make_float2(v[e], v[e + 1]), make_float2(f, f),
-                            make_float2(-base, -base));
-            w = make_float2(ex2(w.x), ex2(w.y));
-            if (masked) {
-              if (c * 32 + e > seen) w.x = 0.0f;
-              if (c * 32 + e + 1 > seen) w.y = 0.0f;
-            }
-            sum = add2(sum, w);
-            w = mul2(w, make_float2(share, share));
-            if (masked) {              // (a share may be NaN)
-              if (c * 32 + e > seen) w.x = 0.0f;
-              if (c * 32 + e + 1 > seen) w.y = 0.0f;
-            }
-            if (masked && any_bad) {
-              if (c * 32 + e <= seen && aux.bad[s][c * 32 + e]) w.x = __int_as_float(0x7fc00000);
-              if (c * 32 + e + 1 <= seen && aux.bad[s][c * 32 + e + 1])
-                w.y = __int_as_float(0x7fc00000);
-            }
-            split2(w.x, w.y, p[e / 2], p[16 + e / 2]);
+        for (int e = 0; e < 32; e += 2) {
+          const int k = c * 32 + e;
+          const float share = aux.share[s][k / 16];
+          float2 w = fma2(make_float2(v[k], v[k + 1]), make_float2(f[k / 16], f[k / 16]),
+                          make_float2(-base, -base));
+          w = make_float2(ex2(w.x), ex2(w.y));
+          if (masked) {
+            if (k > seen) w.x = 0.0f;
+            if (k + 1 > seen) w.y = 0.0f;
           }
+          sum = add2(sum, w);
+          w = mul2(w, make_float2(share, share));
+          if (masked) {                // (a share may be NaN)
+            if (k > seen) w.x = 0.0f;
+            if (k + 1 > seen) w.y = 0.0f;
+            if (any_bad) {
+              if (k <= seen && aux.bad[s][k]) w.x = __int_as_float(0x7fc00000);
+              if (k + 1 <= seen && aux.bad[s][k + 1]) w.y = __int_as_float(0x7fc00000);
+            }
+          }
+          split2(w.x, w.y, p[e / 2], p[16 + e / 2]);
         }
         tmem_st_32x32(t_s + c * 32, p);
       }
@@ -522,22 +527,18 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
     else
       weigh(std::false_type());
     l = fmaf(l, corr, sum.x + sum.y);
-    back = aux.back[s];
+    corr2 = corr1;
+    back2 = back1;
+    corr1 = corr;
+    back1 = aux.back[s];
     tmem_wait_st();
     tc_before();
-    vote(2, true);                      // all of P is there
-    const int now = n;
-    if (tail) ++n;
-    if (x == 0) {
-      issue.tile_values(aux, now, tail);
-      if (tile + 1 < u.tiles)
-        issue.tile_scores(aux, n + 1, u.has_tail(tile + 1));
-      else
-        mma_commit(&aux.done);
-    }
+    mb_arrive(&aux.p_ready[tile & 1]);
   }
-  if (!vote(2, wait(&aux.done, 0))) return false;
-  take_output();
+  if (!wait(&aux.done, 0)) return false;
+  tc_after();
+  if (u.tiles >= 2) take_output(u.tiles - 2, corr2, back2);
+  take_output(u.tiles - 1, corr1, back1);
   return true;
 }
 
@@ -555,12 +556,15 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
   const Unit<D> u(a);
   if (u.r0 >= u.rows) return;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < S::kSlots; ++i) {
       mb_init(&aux.full[i], 128);
       mb_init(&aux.empty[i], 1);
     }
+    for (int i = 0; i < 2; ++i) {
+      mb_init(&aux.s_ready[i], 1);
+      mb_init(&aux.p_ready[i], 128);
+    }
     mb_init(&aux.q_full, 128);
-    mb_init(&aux.s_ready, 1);
     mb_init(&aux.done, 1);
     aux.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -579,17 +583,10 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
     if constexpr (D == 64)
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftmaxRegs));
     const int x = threadIdx.x;
-    const Issue<D> issue(sa(q_hi), sa(q_lo), sa(slots), tmem);
     float o[D], m, l;
 #pragma unroll
     for (int i = 0; i < D; ++i) o[i] = 0.0f;
-    const bool ok = softmax_tiles<D>(a, u, aux, q_scale, issue, x, o, m, l);
-    if (!ok && x == 0) {
-      // The products in flight end before shared memory and TMEM are given up.
-      volatile int never = 0;
-      mma_commit(&aux.done);
-      mb_wait(&aux.done, 0, &never, &g_at_status, 200000000ull, 64);
-    }
+    const bool ok = softmax_tiles<D>(a, u, aux, q_scale, tmem, x, o, m, l);
     const int r = u.r0 + x;
     if (ok && r < u.rows) {
       const int64_t at = u.row_at(a, r);
@@ -613,7 +610,14 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mb_arrive(&aux.q_full);
-    convert_tiles<D>(a, u, slots, aux, x);
+    const Issue<D> issue(sa(q_hi), sa(q_lo), sa(slots), tmem);
+    convert_tiles<D>(a, u, slots, aux, issue, x);
+    if (x == 0 && aux.abort_flag) {
+      // The products in flight end before shared memory and TMEM are given up.
+      volatile int never = 0;
+      mma_commit(&aux.done);
+      mb_wait(&aux.done, 0, &never, &g_at_status, 200000000ull, 64);
+    }
   }
   tc_before();
   __syncthreads();
@@ -631,11 +635,11 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
 // rows while the next tile's products run into the other half of TMEM.  The
 // row tiles are dealt to a cluster's CTAs, whose sums are added in order.
 // About 5 instructions a score, and as many again for q.
-constexpr int kWeightCluster = 4;
+constexpr int kWeightCluster = 4, kKeys = 128;
 
 struct WeightAux {
   alignas(16) float2 row[2][kRows];   // the row's factor, and its lse in units of log 2
-  float got[kWeightCluster][kTile];
+  float got[kWeightCluster][kKeys];
   uint64_t full[2], empty[2], k_full, s_ready[2], done;
   uint32_t tmem;
   int abort_flag;
@@ -658,13 +662,13 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
   uint8_t* slots = k_lo + S::kK;
   __shared__ WeightAux aux;
   const int warp = threadIdx.x >> 5, x = threadIdx.x & 127;
-  const int rank = blockIdx.x % cluster, j0 = blockIdx.x / cluster * kTile;
+  const int rank = blockIdx.x % cluster, j0 = blockIdx.x / cluster * kKeys;
   const int h = blockIdx.y, b = blockIdx.z, G = a.Hq / a.c.kv_heads, blk = a.c.block;
   const int n_new = a.new_lens ? clamp_len(a.new_lens[b], a.T) : a.T;
   const int len = clamp_len(a.c.lens[b], a.c.max_seq), total = min(len + n_new, a.c.max_seq);
   if (n_new == 0 || j0 >= total) return;      // the whole cluster
   const int closed = total / blk * blk, rows = n_new * G;
-  const bool tail = j0 + kTile > closed && closed < total;
+  const bool tail = j0 + kKeys > closed && closed < total;
   // Rows of tokens before the first key see none of these.
   const int first = max(0, j0 - len) * G / kRows, last = (rows + kRows - 1) / kRows;
   const int tiles = max(0, (last - first - rank + cluster - 1) / cluster);
@@ -733,9 +737,9 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
         const uint4 v = __ldg(kp + i);
-        *piece(k_hi, x, 2 * i) = eight(v.x, v.y, mask);
-        *piece(k_hi, x, 2 * i + 1) = eight(v.z, v.w, mask);
-        *piece(k_lo, x, 2 * i) = *piece(k_lo, x, 2 * i + 1) = make_uint4(0, 0, 0, 0);
+        *piece<kKeys>(k_hi, x, 2 * i) = eight(v.x, v.y, mask);
+        *piece<kKeys>(k_hi, x, 2 * i + 1) = eight(v.z, v.w, mask);
+        *piece<kKeys>(k_lo, x, 2 * i) = *piece<kKeys>(k_lo, x, 2 * i + 1) = make_uint4(0, 0, 0, 0);
       }
       ks = __ldg(a.c.k_scale + bh * (a.c.max_seq / blk) + key / blk);
     } else {
@@ -755,19 +759,19 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
       for (int c = 0; c < D / 8; ++c) {
         uint4 hi, lo;
         eight_split(row ? from[2 * c] : zero, row ? from[2 * c + 1] : zero, down, hi, lo);
-        *piece(k_hi, x, c) = hi;
-        *piece(k_lo, x, c) = lo;
+        *piece<kKeys>(k_hi, x, c) = hi;
+        *piece<kKeys>(k_lo, x, c) = lo;
       }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mb_arrive(&aux.k_full);
     const uint64_t kh = sw128_desc(sa(k_hi)), kl = sw128_desc(sa(k_lo));
     const uint64_t q0 = sw128_desc(sa(slots));
-    constexpr uint32_t kDesc = idesc_f16(kTile, kRows, 0);
+    constexpr uint32_t kDesc = idesc_f16(kKeys, kRows, 0);
     auto products = [&](uint64_t k, uint64_t q, uint32_t to, uint32_t more) {
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
-        mma_f16(to, k + k_step(i), q + k_step(i), kDesc, i ? 1u : more);
+        mma_f16(to, k + k_step(i, kKeys), q + k_step(i, kRows), kDesc, i ? 1u : more);
     };
     auto issue = [&](int i) {                 // by one thread
       const int s = i & 1;
@@ -784,7 +788,7 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
     bool ok = vote(2, wait(&aux.k_full, 0));
     if (ok && x == 0 && tiles > 0) issue(0);
     // The key's first row, and whether a tile has any before that of some key.
-    const int r_min = max(0, key - len) * G, r_all = max(0, j0 + kTile - 1 - len) * G;
+    const int r_min = max(0, key - len) * G, r_all = max(0, j0 + kKeys - 1 - len) * G;
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     for (int i = 0; ok && i < tiles; ++i) {
       const int s = i & 1;
@@ -862,7 +866,7 @@ int launch_tc(cudaStream_t s, const AttnArgs& a) {
   const int64_t row_tiles = ceil_div((int64_t)a.T * (a.Hq / a.c.kv_heads), kRows);
   if (row_tiles > INT32_MAX || a.c.kv_heads > 65535 || a.c.batch > 65535)
     return fail(SPX_ERR_UNSUPPORTED, "attention_kv8: grid too large");
-  const size_t smem = 1024 + 2 * S::kQ + 2 * S::kSlot;
+  const size_t smem = 1024 + 2 * S::kQ + S::kSlots * S::kSlot;
   int rc = check_cuda(cudaFuncSetAttribute(attention_kv8_tc_kernel<D>,
                                            cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
                       "attention_kv8: smem attribute");
@@ -888,7 +892,7 @@ int launch_weights_tc(cudaStream_t s, const AttnArgs& a) {
   const int64_t row_tiles = ceil_div((int64_t)a.T * (a.Hq / a.c.kv_heads), kRows);
   int cluster = 1;
   while (cluster < kWeightCluster && cluster * 2 <= row_tiles) cluster *= 2;
-  const int64_t grid = ceil_div(a.c.max_seq, kTile) * cluster;
+  const int64_t grid = ceil_div(a.c.max_seq, kKeys) * cluster;
   if (grid > INT32_MAX) return fail(SPX_ERR_UNSUPPORTED, "attention_kv8: grid too large");
   auto kern = kv8_weights_tc_kernel<D>;
   constexpr size_t smem = WeightShape<D>::kSmem;
