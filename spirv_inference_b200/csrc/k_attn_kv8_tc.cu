@@ -3,8 +3,8 @@
 // A CTA takes 128 rows, (new token, head of the group) pairs of one sequence
 // and kv head, and walks the keys they see in tiles of 64:
 //
-//   four warps turn a tile's K and V into fp16 (int8 is exact there) in shared
-//     memory, a row of K or V a thread;
+//   two warps turn a tile's K and V into fp16 (int8 is exact there) in shared
+//     memory, a key a thread;
 //   S = Q K^T goes into TMEM, q as fp16 hi + lo, two products;
 //   four warps, one row a thread, read S, take the softmax step, and write P,
 //     as fp16 hi + lo, over S;
@@ -13,9 +13,9 @@
 //     core's sums round towards zero: over a whole prompt that shows).
 //
 // S and O have two buffers each, so that the products of a tile run under the
-// softmax of its neighbours; one thread of the conversion warps issues them.
-// (With tiles of 128 keys, one buffer and the issue on a softmax thread, a tile
-// of 128 took 10.7 thousand cycles, 3.3 of them issuing and 5.3 of softmax.)
+// softmax of its neighbours; one more warp issues them.  (With tiles of 128
+// keys, one buffer and the issue on a softmax thread, 128 keys took 10.7
+// thousand cycles, 3.3 of them issuing and 5.3 of softmax.)
 //
 // K and V rows are 128 bytes of 64 values under the 128-byte swizzle: K is a
 // K-major operand, V, whose keys are the reduction, an MN-major one of the same
@@ -124,18 +124,35 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
-// Barrier of 128 threads; whether all of them came with `ok`.
-__device__ __forceinline__ bool vote(int id, bool ok) {
+// Barrier of so many threads; whether all of them came with `ok`.
+__device__ __forceinline__ bool vote(int id, int threads, bool ok) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.and.pred q, %2, 128, p;\n\t"
+      "barrier.cta.red.and.pred q, %2, %3, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"((uint32_t)ok), "r"(id)
+      : "r"((uint32_t)ok), "r"(id), "r"(threads)
       : "memory");
   return r != 0;
+}
+
+// One lane of a converged warp, and a value that all lanes have as the compiler
+// can see: descriptors then stay in uniform registers, and a product is issued
+// in a tenth of the 110 cycles that it takes to move them there each time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+template <class T>
+__device__ __forceinline__ T uniform(T v) {
+  return __shfl_sync(0xffffffffu, v, 0);
 }
 
 // 16 bytes of piece `c` (eight values) of row `r` of an operand of ROWS rows.
@@ -174,10 +191,12 @@ struct Unit {
   int h, b, r0, rows, len, total, closed, lim, tiles, G;
   __device__ __forceinline__ Unit(const AttnArgs& a) {
     G = a.Hq / a.c.kv_heads;
-    h = blockIdx.y;
-    b = blockIdx.z;
-    // the last rows see the most keys: first
-    r0 = (int)(gridDim.x - 1 - blockIdx.x) * kRows;
+    // the last rows see the most keys: first, and those of all heads
+    const int heads = a.c.batch * a.c.kv_heads, at = blockIdx.x / heads;
+    const int bh = blockIdx.x - at * heads;
+    b = bh / a.c.kv_heads;
+    h = bh - b * a.c.kv_heads;
+    r0 = (int)(gridDim.x / heads - 1 - at) * kRows;
     const int n_new = a.new_lens ? clamp_len(a.new_lens[b], a.T) : a.T;
     rows = n_new * G;
     len = clamp_len(a.c.lens[b], a.c.max_seq);
@@ -195,49 +214,57 @@ struct Unit {
   }
 };
 
-// ---- conversion: one row of Q, K and V a thread ------------------------------
+// ---- conversion of rows of q -----------------------------------------------------
+// kRows rows by 128 threads.  Threads next to each other take 8 values each of
+// one row, so that a warp reads whole lines (a row a thread took four times as
+// long for the loads: each touched 32 lines).
 template <int D>
-struct Row {                   // a row of q, or zeros
-  float4 v[D / 4];
-  __device__ __forceinline__ void load(const float* row) {
-    const float4* from = reinterpret_cast<const float4*>(row);
+struct Rows {
+  static constexpr int L = D / 8, PER = 128 / L, N = kRows / PER;
+  float4 v[N][2];
+  // row_of: the row's values, or null for zeros
+  template <class F>
+  __device__ __forceinline__ void load(int x, F row_of) {
 #pragma unroll
-    for (int i = 0; i < D / 4; ++i)
-      v[i] = row ? __ldg(from + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < N; ++i) {
+      const float4* from = reinterpret_cast<const float4*>(row_of(i * PER + x / L)) + x % L * 2;
+      const bool is = row_of(i * PER + x / L) != nullptr;
+      v[i][0] = is ? __ldg(from) : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[i][1] = is ? __ldg(from + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
   }
-  // Row x of an operand, hi and lo; returns the factor that takes its products
-  // to scores in units of log 2 (NaN for a row with a NaN or an infinity).
-  __device__ __forceinline__ float convert(float scale, uint8_t* hi_to, uint8_t* lo_to,
-                                           int x) const {
-    uint32_t mx = 0;
-    bool odd = false;
+  // put(row, the factor that takes its products to scores in units of log 2:
+  // NaN for a row with a NaN or an infinity)
+  template <class F>
+  __device__ __forceinline__ void convert(int x, float scale, uint8_t* hi_to, uint8_t* lo_to,
+                                          F put) const {
 #pragma unroll
-    for (int i = 0; i < D / 4; ++i) {
-      const uint32_t m = max(max(__float_as_uint(v[i].x) & 0x7fffffffu,
-                                 __float_as_uint(v[i].y) & 0x7fffffffu),
-                             max(__float_as_uint(v[i].z) & 0x7fffffffu,
-                                 __float_as_uint(v[i].w) & 0x7fffffffu));
-      mx = max(mx, m);
-    }
-    if (mx >= 0x7f800000u) {
-      odd = true;
-      mx = 0x3f800000u;
-    }
-    float down, up;
-    pow2_scale(mx, down, up);
-    if (scale < 0.0f) down = -down;
+    for (int i = 0; i < N; ++i) {
+      uint32_t mx = 0;
 #pragma unroll
-    for (int c = 0; c < D / 8; ++c) {
+      for (int e = 0; e < 2; ++e)
+        mx = max(max(max(__float_as_uint(v[i][e].x) & 0x7fffffffu,
+                         __float_as_uint(v[i][e].y) & 0x7fffffffu),
+                     max(__float_as_uint(v[i][e].z) & 0x7fffffffu,
+                         __float_as_uint(v[i][e].w) & 0x7fffffffu)),
+                 mx);
+#pragma unroll
+      for (int o = 1; o < L; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const bool odd = mx >= 0x7f800000u;
+      float down, up;
+      pow2_scale(odd ? 0x3f800000u : mx, down, up);
+      if (scale < 0.0f) down = -down;
       uint4 hi, lo;
-      eight_split(v[2 * c], v[2 * c + 1], down, hi, lo);
-      *piece<kRows>(hi_to, x, c) = hi;
-      *piece<kRows>(lo_to, x, c) = lo;
+      eight_split(v[i][0], v[i][1], down, hi, lo);
+      const int r = i * PER + x / L;
+      *piece<kRows>(hi_to, r, x % L) = hi;
+      *piece<kRows>(lo_to, r, x % L) = lo;
+      if (x % L == 0) put(r, odd ? __int_as_float(0x7fc00000) : up * (fabsf(scale) * kLog2e));
     }
-    return odd ? __int_as_float(0x7fc00000) : up * (fabsf(scale) * kLog2e);
   }
 };
 
-// ---- products, issued by one thread ----------------------------------------------
+// ---- products, issued by a warp ---------------------------------------------------
 template <int D>
 struct Issue {
   using S = TcShape<D>;
@@ -246,168 +273,238 @@ struct Issue {
   uint32_t tmem;
   __device__ __forceinline__ Issue(uint32_t q_hi_at, uint32_t q_lo_at, uint32_t slots, uint32_t t)
       : q_hi(sw128_desc(q_hi_at)), q_lo(sw128_desc(q_lo_at)), k(sw128_desc(slots)),
-        v(mn_desc(slots + S::kHalf)), tmem(t) {}
-  // Q (from q) K^T (from slot s) over D, to S buffer `to`.
+        v(mn_desc(slots + S::kHalf)), tmem(uniform(t)) {}
+  // (What the elected lane uses is made before, by the whole warp: made under
+  // elect_one(), descriptors came out wrong in one build.)
+  // Q (from q) K^T (from a slot's k) over D, to the S buffer at `to`.
   template <bool MORE>
-  __device__ __forceinline__ void scores(uint64_t q, int s, int to) const {
-    const uint64_t from = k + (uint64_t)s * (S::kSlot >> 4);
+  static __device__ __forceinline__ void scores(uint64_t q, uint64_t from, uint32_t to) {
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
-      mma_f16(tmem + to * kTile, q + k_step(i, kRows), from + k_step(i, kTile), kS,
+      mma_f16(to, q + k_step(i, kRows), from + k_step(i, kTile), kS,
               MORE || i ? 1u : 0u);
   }
-  // P (of S buffer `to`; hi: PART 0, lo: PART 16 columns into each 32) V (from
-  // slot s) over the keys, to O buffer `to`.
+  // P (at `p`; hi: PART 0, lo: PART 16 columns into each 32) V (from a slot's v)
+  // over the keys, to the O buffer at `to`.
   template <int PART, bool MORE>
-  __device__ __forceinline__ void values(int s, int to) const {
-    const uint64_t from = v + (uint64_t)s * (S::kSlot >> 4);
+  static __device__ __forceinline__ void values(uint32_t p, uint64_t from, uint32_t to) {
 #pragma unroll
     for (int i = 0; i < kTile / 16; ++i)
-      mma_f16_ta(tmem + 2 * kTile + to * D, tmem + to * kTile + (i >> 1) * 32 + PART + (i & 1) * 8,
+      mma_f16_ta(to, p + (i >> 1) * 32 + PART + (i & 1) * 8,
                  from + i * (2048 >> 4), kO, MORE || i ? 1u : 0u);
   }
-  // S of a tile whose rows are in slot n (and n + 1), once they are there.
-  __device__ __forceinline__ void tile_scores(Aux& aux, int tile, int n, bool tail) const {
-    auto wait = [&](int k) {
-      return mb_wait(&aux.full[k & 3], (k >> 2) & 1, &aux.abort_flag, &g_at_status, kWaitNs, 32);
-    };
-    if (!wait(n)) return;
+  static __device__ __forceinline__ bool wait(Aux& aux, uint64_t* bar, int parity) {
+    const bool ok = mb_wait(bar, parity, &aux.abort_flag, &g_at_status, kWaitNs, 32);
+    if (!__all_sync(0xffffffffu, ok)) return false;
     tc_after();
-    scores<false>(q_lo, n & 3, tile & 1);
-    scores<true>(q_hi, n & 3, tile & 1);
-    if (tail) {
-      if (!wait(n + 1)) return;
-      tc_after();
-      scores<true>(q_hi, (n + 1) & 3, tile & 1);
+    return true;
+  }
+  // S of a tile whose rows are in slot n (and n + 1), once they are there.
+  __device__ __forceinline__ bool tile_scores(Aux& aux, int tile, int n, bool tail) const {
+    const int s = uniform(n & 3), s2 = uniform((n + 1) & 3), j = uniform(tile & 1);
+    const uint64_t from = k + (uint64_t)s * (S::kSlot >> 4);
+    const uint64_t from2 = k + (uint64_t)s2 * (S::kSlot >> 4);
+    const uint32_t to = tmem + j * kTile;
+    if (!wait(aux, &aux.full[s], (n >> 2) & 1)) return false;
+    if (elect_one()) {
+      scores<false>(q_lo, from, to);
+      scores<true>(q_hi, from, to);
+      if (!tail) mma_commit(&aux.s_ready[j]);
     }
-    mma_commit(&aux.s_ready[tile & 1]);
+    __syncwarp();
+    if (!tail) return true;
+    if (!wait(aux, &aux.full[s2], ((n + 1) >> 2) & 1)) return false;
+    if (elect_one()) {
+      scores<true>(q_hi, from2, to);
+      mma_commit(&aux.s_ready[j]);
+    }
+    __syncwarp();
+    return true;
   }
   // O of a tile, once P is there.
-  __device__ __forceinline__ void tile_values(Aux& aux, int tile, int n, bool tail) const {
-    if (!mb_wait(&aux.p_ready[tile & 1], (tile >> 1) & 1, &aux.abort_flag, &g_at_status, kWaitNs,
-                 32))
-      return;
-    tc_after();
-    values<16, false>(n & 3, tile & 1);
-    values<0, true>(n & 3, tile & 1);
-    if (tail) values<0, true>((n + 1) & 3, tile & 1);
-    mma_commit(&aux.empty[n & 3]);
-    if (tail) mma_commit(&aux.empty[(n + 1) & 3]);
+  __device__ __forceinline__ bool tile_values(Aux& aux, int tile, int n, bool tail) const {
+    const int s = uniform(n & 3), s2 = uniform((n + 1) & 3), j = uniform(tile & 1);
+    const uint64_t from = v + (uint64_t)s * (S::kSlot >> 4);
+    const uint64_t from2 = v + (uint64_t)s2 * (S::kSlot >> 4);
+    const uint32_t p = tmem + j * kTile, to = tmem + 2 * kTile + j * D;
+    if (!wait(aux, &aux.p_ready[j], (tile >> 1) & 1)) return false;
+    if (elect_one()) {
+      values<16, false>(p, from, to);
+      values<0, true>(p, from, to);
+      if (tail) values<0, true>(p, from2, to);
+      mma_commit(&aux.empty[s]);
+      if (tail) mma_commit(&aux.empty[s2]);
+    }
+    __syncwarp();
+    return true;
   }
 };
 
-// ---- conversion: a row of K (threads 0 .. 63) or V a thread; thread 0 issues ------
+// All products of the tiles.  (elect_one gives the same lane each time, so a
+// commit follows all that was issued before it.)
+template <int D>
+__device__ __forceinline__ void issue_tiles(const Unit<D>& u, Aux& aux, const Issue<D>& issue) {
+  bool ok = Issue<D>::wait(aux, &aux.q_full, 0);
+  int n = 0, n1 = 0, n2 = 0;   // the slots of tiles j, j - 1, j - 2
+  for (int j = 0; ok && j < u.tiles + 2; ++j) {
+    if (j >= 2) ok = issue.tile_values(aux, j - 2, n2, u.has_tail(j - 2));
+    n2 = n1;
+    if (!ok || j >= u.tiles) continue;
+    const bool tail = u.has_tail(j);
+    ok = issue.tile_scores(aux, j, n, tail);
+    n1 = n;
+    n += tail ? 2 : 1;
+  }
+  if (elect_one()) {
+    mma_commit(&aux.done);
+    if (!ok) {
+      // The products in flight end before shared memory and TMEM are given up.
+      volatile int never = 0;
+      mb_wait(&aux.done, 0, &never, &g_at_status, 200000000ull, 64);
+    }
+  }
+  __syncwarp();
+}
+
+// ---- conversion of keys and values ------------------------------------------------
+// A row of the tail as its hi or lo part (x its scale); zeros where there is none.
+template <int D, bool V>
+__device__ __forceinline__ void put_tail(uint8_t* base, int r, const float* row, float down,
+                                         bool low) {
+  const float4* from = reinterpret_cast<const float4*>(row);
+  bool unused = false;
+  for (int c = 0; c < D / 8; ++c) {
+    uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+    if (row) {
+      float4 p = from[2 * c], q = from[2 * c + 1];
+      if (V) {
+        p = finite4(p, unused);
+        q = finite4(q, unused);
+      }
+      eight_split(p, q, down, hi, lo);
+    }
+    *piece<kTile>(base, r, c) = low ? lo : hi;
+  }
+}
+
 template <int D>
 __device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& u, uint8_t* slots,
-                                              Aux& aux, const Issue<D>& issue, int x) {
+                                              Aux& aux, int r) {
   using S = TcShape<D>;
   const int64_t bh = (int64_t)u.b * a.c.kv_heads + u.h;
-  const bool is_v = x >= kTile;
-  const int r = x & (kTile - 1), blk = a.c.block;
-  const int8_t* from8 = (is_v ? a.c.v : a.c.k) + bh * a.c.max_seq * D;
-  const float* scales = (is_v ? a.c.v_scale : a.c.k_scale) + bh * (a.c.max_seq / blk);
-  const float* tails = (is_v ? a.c.v_tail : a.c.k_tail) + bh * blk * D;
-  float(*raw)[kGroups] = is_v ? aux.v_raw : aux.k_scale;
+  const int blk = a.c.block;
+  const int8_t* k8 = a.c.k + bh * a.c.max_seq * D;
+  const int8_t* v8 = a.c.v + bh * a.c.max_seq * D;
+  const float* ks = a.c.k_scale + bh * (a.c.max_seq / blk);
+  const float* vs = a.c.v_scale + bh * (a.c.max_seq / blk);
+  const float* kt = a.c.k_tail + bh * blk * D;
+  const float* vt = a.c.v_tail + bh * blk * D;
   uint32_t mask;
   asm volatile("mov.b32 %0, 0x00ff00ff;" : "=r"(mask));
-  // Step j: the products P V of tile j - 2, the rows of tile j, its S.
-  int n = 0, n1 = 0, n2 = 0;   // the slots of tiles j, j - 1, j - 2
-  for (int j = 0; j < u.tiles + 2; ++j) {
-    const int key = j * kTile + r;
-    const bool closed = key < u.closed, in_tail = !closed && key < u.total;
-    const bool tail = u.has_tail(j);
-    // The row's bytes, and its scale, are on their way meanwhile.
-    uint4 row[D / 16];
-    float sc = 0.0f;
-    if (j < u.tiles && closed) {
-      const uint4* p = reinterpret_cast<const uint4*>(from8 + (int64_t)key * D);
+  // Rows of closed blocks: 16 bytes of a row a thread, a warp's next to each
+  // other.  Scales and rows of the tail: a key a thread.
+  constexpr int L = D / 16, PER = kTile / L;
+  const int r16 = r / L, c16 = r % L;
+  uint4 kr[L], vr[L];
+  float k_sc = 0.0f, v_sc = 0.0f;
+  auto load = [&](int tile) {
+    const int key = tile * kTile + r, key16 = tile * kTile + r16;
+    k_sc = v_sc = 0.0f;
+    if (tile >= u.tiles) return;
+    const uint4* kp = reinterpret_cast<const uint4*>(k8 + (int64_t)key16 * D) + c16;
+    const uint4* vp = reinterpret_cast<const uint4*>(v8 + (int64_t)key16 * D) + c16;
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) row[i] = __ldg(p + i);
-      sc = __ldg(scales + key / blk);
+    for (int i = 0; i < L; ++i)
+      if (key16 + i * PER < u.closed) kr[i] = __ldg(kp + i * PER * L);
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+      if (key16 + i * PER < u.closed) vr[i] = __ldg(vp + i * PER * L);
+    if (key < u.closed) {
+      k_sc = __ldg(ks + key / blk);
+      v_sc = __ldg(vs + key / blk);
     }
-    if (x == 0 && j >= 2) {
-      issue.tile_values(aux, j - 2, n2, u.has_tail(j - 2));
-      if (j == u.tiles + 1) mma_commit(&aux.done);
-    }
-    __syncwarp();
-    if (j >= u.tiles) {
-      n2 = n1;
-      continue;
-    }
-    float down = 0.0f;
-    const float4* rf = reinterpret_cast<const float4*>(tails + (int64_t)(key & (blk - 1)) * D);
-    bool odd = false, unused = false;
+  };
+  load(0);
+  int n = 0;                   // the tile's slot
+  for (int tile = 0; tile < u.tiles; ++tile) {
+    const int key = tile * kTile + r;
+    const bool closed = key < u.closed, in_tail = !closed && key < u.total;
+    const bool tail = u.has_tail(tile);
+    const float* kf = in_tail ? kt + (int64_t)(key & (blk - 1)) * D : nullptr;
+    const float* vf = in_tail ? vt + (int64_t)(key & (blk - 1)) * D : nullptr;
+    float k_down = 0.0f, v_down = 0.0f;
+    bool odd = false;
     if (tail) {                // the tail's 16-key groups: powers of two
-      uint32_t mx = 0;
+      uint32_t mk = 0, mv = 0;
       if (in_tail)
         for (int i = 0; i < D / 4; ++i) {
-          float4 p = rf[i];
-          if (is_v) p = finite4(p, odd);
-          mx = max(max(mx, finite_abs(p.x)),
+          const float4 p = reinterpret_cast<const float4*>(kf)[i];
+          const float4 q = finite4(reinterpret_cast<const float4*>(vf)[i], odd);
+          mk = max(max(mk, finite_abs(p.x)),
                    max(finite_abs(p.y), max(finite_abs(p.z), finite_abs(p.w))));
+          mv = max(max(mv, finite_abs(q.x)),
+                   max(finite_abs(q.y), max(finite_abs(q.z), finite_abs(q.w))));
         }
 #pragma unroll
-      for (int o = 1; o < 16; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      if (!closed) pow2_scale(mx, down, sc);
+      for (int o = 1; o < 16; o <<= 1) {
+        mk = max(mk, __shfl_xor_sync(0xffffffffu, mk, o));
+        mv = max(mv, __shfl_xor_sync(0xffffffffu, mv, o));
+      }
+      if (!closed) {
+        pow2_scale(mk, k_down, k_sc);
+        pow2_scale(mv, v_down, v_sc);
+      }
     }
     const int s = n & 3;
     const bool drained = mb_wait(&aux.empty[s], ((n >> 2) & 1) ^ 1, &aux.abort_flag, &g_at_status,
                                  kWaitNs, 64);
     if (drained) {
-      if ((r & 15) == 0) raw[s][r >> 4] = sc;
-      if (is_v) aux.bad[s][r] = odd;
+      if ((r & 15) == 0) {
+        aux.k_scale[s][r >> 4] = k_sc;
+        aux.v_raw[s][r >> 4] = v_sc;
+      }
+      aux.bad[s][r] = odd;
     }
-    if (!vote(1, drained)) return;
-    if (x < kGroups) {
+    if (!vote(1, kTile, drained)) return;
+    if (r < kGroups) {
       float ref = 0.0f;
 #pragma unroll
       for (int i = 0; i < kGroups; ++i) {
         const float v = aux.v_raw[s][i];
         if (v <= kMaxFloat) ref = fmaxf(ref, v);
       }
-      aux.share[s][x] = ref > 0.0f ? aux.v_raw[s][x] * (kPUp / ref) : aux.v_raw[s][x];
-      if (x == 0) aux.back[s] = ref * (1.0f / kPUp);
+      aux.share[s][r] = ref > 0.0f ? aux.v_raw[s][r] * (kPUp / ref) : aux.v_raw[s][r];
+      if (r == 0) aux.back[s] = ref * (1.0f / kPUp);
     }
-    uint8_t* to = slots + s * S::kSlot + (is_v ? S::kHalf : 0);
-    auto put_tail = [&](uint8_t* base, bool low) {
-      for (int c = 0; c < D / 8; ++c) {
-        uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-        if (in_tail) {
-          float4 p = rf[2 * c], q = rf[2 * c + 1];
-          if (is_v) {
-            p = finite4(p, unused);
-            q = finite4(q, unused);
-          }
-          eight_split(p, q, down, hi, lo);
-        }
-        *piece<kTile>(base, r, c) = low ? lo : hi;
-      }
-    };
-    if (closed) {
+    uint8_t* k_to = slots + s * S::kSlot;
+    uint8_t* v_to = k_to + S::kHalf;
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        *piece<kTile>(to, r, 2 * i) = eight(row[i].x, row[i].y, mask);
-        *piece<kTile>(to, r, 2 * i + 1) = eight(row[i].z, row[i].w, mask);
-      }
-    } else {
-      put_tail(to, false);
+    for (int i = 0; i < L; ++i) {
+      const int to = i * PER + r16;
+      if (tile * kTile + to >= u.closed) break;
+      *piece<kTile>(k_to, to, 2 * c16) = eight(kr[i].x, kr[i].y, mask);
+      *piece<kTile>(k_to, to, 2 * c16 + 1) = eight(kr[i].z, kr[i].w, mask);
+      *piece<kTile>(v_to, to, 2 * c16) = eight(vr[i].x, vr[i].y, mask);
+      *piece<kTile>(v_to, to, 2 * c16 + 1) = eight(vr[i].z, vr[i].w, mask);
+    }
+    if (!closed) {
+      put_tail<D, false>(k_to, r, kf, k_down, false);
+      put_tail<D, true>(v_to, r, vf, v_down, false);
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mb_arrive(&aux.full[s]);
-    if (tail) {
-      const int s2 = (n + 1) & 3;
-      if (!vote(1, mb_wait(&aux.empty[s2], (((n + 1) >> 2) & 1) ^ 1, &aux.abort_flag,
-                           &g_at_status, kWaitNs, 64)))
-        return;
-      put_tail(slots + s2 * S::kSlot + (is_v ? S::kHalf : 0), true);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mb_arrive(&aux.full[s2]);
-    }
-    if (x == 0) issue.tile_scores(aux, j, n, tail);
-    __syncwarp();
-    n2 = n1;
-    n1 = n;
-    n += tail ? 2 : 1;
+    load(tile + 1);            // on its way while the next slot drains
+    ++n;
+    if (!tail) continue;
+    const int s2 = n & 3;
+    if (!vote(1, kTile, mb_wait(&aux.empty[s2], ((n >> 2) & 1) ^ 1, &aux.abort_flag, &g_at_status,
+                                kWaitNs, 64)))
+      return;
+    put_tail<D, false>(slots + s2 * S::kSlot, r, kf, k_down, true);
+    put_tail<D, true>(slots + s2 * S::kSlot + S::kHalf, r, vf, v_down, true);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    mb_arrive(&aux.full[s2]);
+    ++n;
   }
 }
 
@@ -557,7 +654,7 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
   if (u.r0 >= u.rows) return;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kSlots; ++i) {
-      mb_init(&aux.full[i], 128);
+      mb_init(&aux.full[i], kTile);
       mb_init(&aux.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -599,24 +696,23 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
       if (a.lse) a.lse[at] = (m + log2f(l)) * kLn2;
     }
   } else {
-    if constexpr (D == 64)
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kConvertRegs));
     const int x = threadIdx.x - 128;
-    const int r = u.r0 + x;
     {
-      Row<D> row;
-      row.load(r < u.rows ? a.q + u.row_at(a, r) * D : nullptr);
-      q_scale[x] = row.convert(a.scale, q_hi, q_lo, x);
+      Rows<D> rows;
+      rows.load(x, [&](int r) {
+        return u.r0 + r < u.rows ? a.q + u.row_at(a, u.r0 + r) * D : nullptr;
+      });
+      rows.convert(x, a.scale, q_hi, q_lo, [&](int r, float f) { q_scale[r] = f; });
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mb_arrive(&aux.q_full);
-    const Issue<D> issue(sa(q_hi), sa(q_lo), sa(slots), tmem);
-    convert_tiles<D>(a, u, slots, aux, issue, x);
-    if (x == 0 && aux.abort_flag) {
-      // The products in flight end before shared memory and TMEM are given up.
-      volatile int never = 0;
-      mma_commit(&aux.done);
-      mb_wait(&aux.done, 0, &never, &g_at_status, 200000000ull, 64);
+    if constexpr (D == 64)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kConvertRegs));
+    if (warp < 6) {
+      convert_tiles<D>(a, u, slots, aux, x);
+    } else if (warp == 6) {
+      const Issue<D> issue(sa(q_hi), sa(q_lo), sa(slots), tmem);
+      issue_tiles<D>(u, aux, issue);
     }
   }
   tc_before();
@@ -630,17 +726,19 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
 
 // ---------------------------------------------------------------------------
 // Weights for many rows: S^T = K Q^T, 128 keys on the lanes, which stay, and
-// 128 rows at a time on the columns.  Four warps turn rows of q into operands,
-// two tiles ahead; four, one key a thread, add exp(score - lse) over a tile's
-// rows while the next tile's products run into the other half of TMEM.  The
-// row tiles are dealt to a cluster's CTAs, whose sums are added in order.
-// About 5 instructions a score, and as many again for q.
-constexpr int kWeightCluster = 4, kKeys = 128;
+// 128 rows at a time on the columns.  Four warps turn rows of q into operands
+// one tile ahead; two groups of four take every other tile, each with a half of
+// TMEM, issue its products themselves and add exp(score - lse) over its rows, a
+// key a thread: while one waits for its products, the other adds.  The row
+// tiles are dealt to a cluster's CTAs, whose sums are added in order.  About 3
+// instructions a score, and 4 a value of q.
+constexpr int kWeightCluster = 4, kKeys = 128, kWeightThreads = 384;
 
 struct WeightAux {
   alignas(16) float2 row[2][kRows];   // the row's factor, and its lse in units of log 2
   float got[kWeightCluster][kKeys];
-  uint64_t full[2], empty[2], k_full, s_ready[2], done;
+  float k_scale[kKeys], odd_tiles[kKeys];
+  uint64_t full[2], empty[2], k_full, s_ready[2], done[2];
   uint32_t tmem;
   int abort_flag;
 };
@@ -653,7 +751,7 @@ struct WeightShape {
 };
 
 template <int D>
-__global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
+__global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
     kv8_weights_tc_kernel(const AttnArgs a, int cluster) {
   using S = WeightShape<D>;
   extern __shared__ uint8_t smem_raw[];
@@ -661,9 +759,11 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
   uint8_t* k_lo = k_hi + S::kK;
   uint8_t* slots = k_lo + S::kK;
   __shared__ WeightAux aux;
-  const int warp = threadIdx.x >> 5, x = threadIdx.x & 127;
-  const int rank = blockIdx.x % cluster, j0 = blockIdx.x / cluster * kKeys;
-  const int h = blockIdx.y, b = blockIdx.z, G = a.Hq / a.c.kv_heads, blk = a.c.block;
+  const int warp = threadIdx.x >> 5, x = threadIdx.x & 127;   // of the first four: a key
+  // the first keys are seen by the most rows: first, and those of all heads
+  const int heads = a.c.batch * a.c.kv_heads, rank = blockIdx.x % cluster;
+  const int unit = blockIdx.x / cluster, j0 = unit / heads * kKeys, bh = unit % heads;
+  const int b = bh / a.c.kv_heads, h = bh - b * a.c.kv_heads, G = a.Hq / a.c.kv_heads, blk = a.c.block;
   const int n_new = a.new_lens ? clamp_len(a.new_lens[b], a.T) : a.T;
   const int len = clamp_len(a.c.lens[b], a.c.max_seq), total = min(len + n_new, a.c.max_seq);
   if (n_new == 0 || j0 >= total) return;      // the whole cluster
@@ -678,9 +778,9 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
       mb_init(&aux.full[i], 128);
       mb_init(&aux.empty[i], 129);     // the products, and the threads that read `row`
       mb_init(&aux.s_ready[i], 1);
+      mb_init(&aux.done[i], 1);
     }
     mb_init(&aux.k_full, 128);
-    mb_init(&aux.done, 1);
     aux.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -699,72 +799,77 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
     return mb_wait(bar, parity, &aux.abort_flag, &g_at_status, kWaitNs, 32);
   };
   float w = 0.0f;
-  if (warp >= 4) {
+  if (warp >= 8) {
     auto row_at = [&](int r) {
       const int tk = a.div_g(r);
       return ((int64_t)b * a.T + tk) * a.Hq + h * G + (r - tk * G);
     };
-    Row<D> row;
+    Rows<D> q;
     float z = INFINITY;                // (a row that is none weighs nothing)
     auto load = [&](int i) {
-      const int r = row0(i) + x;
-      const bool is = i < tiles && r < rows;
-      const int64_t at = is ? row_at(r) : 0;
-      row.load(is ? a.q + at * D : nullptr);
-      z = is ? a.lse[at] * kLog2e : INFINITY;
+      if (i >= tiles) return;
+      const int r0 = row0(i);
+      q.load(x, [&](int r) { return r0 + r < rows ? a.q + row_at(r0 + r) * D : nullptr; });
+      z = r0 + x < rows ? a.lse[row_at(r0 + x)] * kLog2e : INFINITY;
     };
     load(0);
     for (int i = 0; i < tiles; ++i) {
       const int s = i & 1;
-      if (!mb_wait(&aux.empty[s], ((i >> 1) & 1) ^ 1, &aux.abort_flag, &g_at_status, kWaitNs, 128))
-        break;
+      const bool drained = mb_wait(&aux.empty[s], ((i >> 1) & 1) ^ 1, &aux.abort_flag,
+                                   &g_at_status, kWaitNs, 128);
+      if (!__all_sync(0xffffffffu, drained)) break;
       uint8_t* to = slots + s * S::kSlot;
-      const float f = row.convert(a.scale, to, to + S::kSlot / 2, x);
-      aux.row[s][x] = make_float2(f, z);
+      q.convert(x, a.scale, to, to + S::kSlot / 2,
+                [&](int r, float f) { aux.row[s][r].x = f; });
+      aux.row[s][x].y = z;
       load(i + 1);                     // on its way while the slot is used
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mb_arrive(&aux.full[s]);
     }
   } else {
-    // The key's row, and its scale.
-    const int key = j0 + x;
-    const int64_t bh = (int64_t)b * a.c.kv_heads + h;
-    float ks = 0.0f;
-    if (key < closed) {
-      const uint4* kp = reinterpret_cast<const uint4*>(a.c.k + (bh * a.c.max_seq + key) * D);
-      uint32_t mask;
-      asm volatile("mov.b32 %0, 0x00ff00ff;" : "=r"(mask));
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const uint4 v = __ldg(kp + i);
-        *piece<kKeys>(k_hi, x, 2 * i) = eight(v.x, v.y, mask);
-        *piece<kKeys>(k_hi, x, 2 * i + 1) = eight(v.z, v.w, mask);
-        *piece<kKeys>(k_lo, x, 2 * i) = *piece<kKeys>(k_lo, x, 2 * i + 1) = make_uint4(0, 0, 0, 0);
+    if (warp < 4) {
+      // The key's row, and its scale.
+      const int key = j0 + x;
+      float ks = 0.0f;
+      if (key < closed) {
+        const uint4* kp =
+            reinterpret_cast<const uint4*>(a.c.k + ((int64_t)bh * a.c.max_seq + key) * D);
+        uint32_t mask;
+        asm volatile("mov.b32 %0, 0x00ff00ff;" : "=r"(mask));
+  #pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          const uint4 v = __ldg(kp + i);
+          *piece<kKeys>(k_hi, x, 2 * i) = eight(v.x, v.y, mask);
+          *piece<kKeys>(k_hi, x, 2 * i + 1) = eight(v.z, v.w, mask);
+          *piece<kKeys>(k_lo, x, 2 * i) = make_uint4(0, 0, 0, 0);
+          *piece<kKeys>(k_lo, x, 2 * i + 1) = make_uint4(0, 0, 0, 0);
+        }
+        ks = __ldg(a.c.k_scale + (int64_t)bh * (a.c.max_seq / blk) + key / blk);
+      } else {
+        // a row of the tail on its own: any power of two does
+        const float* row =
+            key < total ? a.c.k_tail + ((int64_t)bh * blk + (key & (blk - 1))) * D : nullptr;
+        const float4* from = reinterpret_cast<const float4*>(row);
+        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+        uint32_t mx = 0;
+        for (int i = 0; i < D / 4; ++i) {
+          const float4 v = row ? from[i] : zero;
+          mx = max(max(mx, finite_abs(v.x)),
+                   max(finite_abs(v.y), max(finite_abs(v.z), finite_abs(v.w))));
+        }
+        float down;
+        pow2_scale(mx, down, ks);
+        for (int c = 0; c < D / 8; ++c) {
+          uint4 hi, lo;
+          eight_split(row ? from[2 * c] : zero, row ? from[2 * c + 1] : zero, down, hi, lo);
+          *piece<kKeys>(k_hi, x, c) = hi;
+          *piece<kKeys>(k_lo, x, c) = lo;
+        }
       }
-      ks = __ldg(a.c.k_scale + bh * (a.c.max_seq / blk) + key / blk);
-    } else {
-      // a row of the tail on its own: any power of two does
-      const float* row =
-          key < total ? a.c.k_tail + (bh * blk + (key & (blk - 1))) * D : nullptr;
-      const float4* from = reinterpret_cast<const float4*>(row);
-      const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-      uint32_t mx = 0;
-      for (int i = 0; i < D / 4; ++i) {
-        const float4 v = row ? from[i] : zero;
-        mx = max(max(mx, finite_abs(v.x)),
-                 max(finite_abs(v.y), max(finite_abs(v.z), finite_abs(v.w))));
-      }
-      float down;
-      pow2_scale(mx, down, ks);
-      for (int c = 0; c < D / 8; ++c) {
-        uint4 hi, lo;
-        eight_split(row ? from[2 * c] : zero, row ? from[2 * c + 1] : zero, down, hi, lo);
-        *piece<kKeys>(k_hi, x, c) = hi;
-        *piece<kKeys>(k_lo, x, c) = lo;
-      }
+      aux.k_scale[x] = ks;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mb_arrive(&aux.k_full);
     }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    mb_arrive(&aux.k_full);
     const uint64_t kh = sw128_desc(sa(k_hi)), kl = sw128_desc(sa(k_lo));
     const uint64_t q0 = sw128_desc(sa(slots));
     constexpr uint32_t kDesc = idesc_f16(kKeys, kRows, 0);
@@ -773,28 +878,32 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
       for (int i = 0; i < D / 16; ++i)
         mma_f16(to, k + k_step(i, kKeys), q + k_step(i, kRows), kDesc, i ? 1u : more);
     };
-    auto issue = [&](int i) {                 // by one thread
-      const int s = i & 1;
-      if (!wait(&aux.full[s], (i >> 1) & 1)) return;
-      tc_after();
-      const uint64_t qh = q0 + (uint64_t)s * (S::kSlot >> 4), ql = qh + (S::kSlot >> 5);
-      const uint32_t to = tmem + s * kRows;
-      products(kh, ql, to, 0u);
-      if (tail) products(kl, qh, to, 1u);
-      products(kh, qh, to, 1u);
-      mma_commit(&aux.empty[s]);
-      mma_commit(&aux.s_ready[s]);
+    const int s = uniform(warp >> 2), key = j0 + x;
+    const uint64_t qh = q0 + (uint64_t)s * (S::kSlot >> 4), ql = qh + (S::kSlot >> 5);
+    const uint32_t to = uniform(tmem) + s * kRows;
+    auto hold = [&](uint64_t* bar, int parity) {     // a warp goes on or ends as one
+      return __all_sync(0xffffffffu, wait(bar, parity)) != 0;
     };
-    bool ok = vote(2, wait(&aux.k_full, 0));
-    if (ok && x == 0 && tiles > 0) issue(0);
+    bool ok = hold(&aux.k_full, 0);
+    const float ks = aux.k_scale[x];
     // The key's first row, and whether a tile has any before that of some key.
     const int r_min = max(0, key - len) * G, r_all = max(0, j0 + kKeys - 1 - len) * G;
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    for (int i = 0; ok && i < tiles; ++i) {
-      const int s = i & 1;
-      if (x == 0 && i + 1 < tiles) issue(i + 1);
-      ok = vote(2, wait(&aux.s_ready[s], (i >> 1) & 1) && wait(&aux.full[s], (i >> 1) & 1));
-      if (!ok) break;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    for (int i = s; ok && i < tiles; i += 2) {
+      // (a slot is filled anew after the group has read its half of TMEM)
+      if (!(ok = hold(&aux.full[s], (i >> 1) & 1))) break;
+      if ((warp & 3) == 0) {
+        tc_after();
+        if (elect_one()) {
+          products(kh, ql, to, 0u);
+          if (tail) products(kl, qh, to, 1u);
+          products(kh, qh, to, 1u);
+          mma_commit(&aux.empty[s]);
+          mma_commit(&aux.s_ready[s]);
+        }
+        __syncwarp();
+      }
+      if (!(ok = hold(&aux.s_ready[s], (i >> 1) & 1))) break;
       tc_after();
       const bool mask = row0(i) < r_all;
       const int from = r_min - row0(i);       // the first column that the key is seen by
@@ -828,16 +937,17 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
         add(std::false_type());
       tc_before();
       mb_arrive(&aux.empty[s]);
-      vote(2, true);                          // this half of TMEM has been read
     }
-    if (!ok && x == 0) {
+    if (!ok && (warp & 3) == 0 && elect_one()) {
       // The products in flight end before shared memory and TMEM are given up.
       volatile int never = 0;
-      mma_commit(&aux.done);
-      mb_wait(&aux.done, 0, &never, &g_at_status, 200000000ull, 64);
+      mma_commit(&aux.done[s]);
+      mb_wait(&aux.done[s], 0, &never, &g_at_status, 200000000ull, 64);
     }
+    if (s == 1) aux.odd_tiles[x] = w;
   }
-  __syncwarp();
+  __syncthreads();
+  if (warp < 4) w += aux.odd_tiles[x];
   const bool good = !aux.abort_flag;
   if (cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   cg::cluster_group cl = cg::this_cluster();
@@ -864,8 +974,8 @@ template <int D>
 int launch_tc(cudaStream_t s, const AttnArgs& a) {
   using S = TcShape<D>;
   const int64_t row_tiles = ceil_div((int64_t)a.T * (a.Hq / a.c.kv_heads), kRows);
-  if (row_tiles > INT32_MAX || a.c.kv_heads > 65535 || a.c.batch > 65535)
-    return fail(SPX_ERR_UNSUPPORTED, "attention_kv8: grid too large");
+  const int64_t grid = row_tiles * a.c.kv_heads * a.c.batch;
+  if (grid > INT32_MAX) return fail(SPX_ERR_UNSUPPORTED, "attention_kv8: grid too large");
   const size_t smem = 1024 + 2 * S::kQ + S::kSlots * S::kSlot;
   int rc = check_cuda(cudaFuncSetAttribute(attention_kv8_tc_kernel<D>,
                                            cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
@@ -882,8 +992,7 @@ int launch_tc(cudaStream_t s, const AttnArgs& a) {
       return fail(SPX_ERR_UNSUPPORTED, "attention_kv8: built with %d registers a thread",
                   f.numRegs);
   }
-  const dim3 grid((unsigned)row_tiles, (unsigned)a.c.kv_heads, (unsigned)a.c.batch);
-  attention_kv8_tc_kernel<D><<<grid, kThreads, smem, s>>>(a);
+  attention_kv8_tc_kernel<D><<<(unsigned)grid, kThreads, smem, s>>>(a);
   return SPX_OK;
 }
 
@@ -892,7 +1001,7 @@ int launch_weights_tc(cudaStream_t s, const AttnArgs& a) {
   const int64_t row_tiles = ceil_div((int64_t)a.T * (a.Hq / a.c.kv_heads), kRows);
   int cluster = 1;
   while (cluster < kWeightCluster && cluster * 2 <= row_tiles) cluster *= 2;
-  const int64_t grid = ceil_div(a.c.max_seq, kKeys) * cluster;
+  const int64_t grid = ceil_div(a.c.max_seq, kKeys) * cluster * a.c.batch * a.c.kv_heads;
   if (grid > INT32_MAX) return fail(SPX_ERR_UNSUPPORTED, "attention_kv8: grid too large");
   auto kern = kv8_weights_tc_kernel<D>;
   constexpr size_t smem = WeightShape<D>::kSmem;
@@ -901,8 +1010,8 @@ int launch_weights_tc(cudaStream_t s, const AttnArgs& a) {
       "attention_kv8: smem attribute");
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid, (unsigned)a.c.kv_heads, (unsigned)a.c.batch);
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kWeightThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
