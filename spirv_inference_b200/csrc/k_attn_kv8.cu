@@ -660,17 +660,26 @@ __device__ __forceinline__ void tail_tile(Running<D, NT>& run, const Keys<D>& kv
   }
 }
 
-// Adds the weights of a tile's keys: w of keys key_of(0 .. 3), summed over the
-// lanes with the same t (each step leaves a lane half of the values).
-__device__ __forceinline__ void put_weights(float* out, const float (&w)[4], int jb, int len,
+// What this lane's key of a tile has gathered: nothing for a new token.
+__device__ __forceinline__ int own_key(int jb, int g, int t) {
+  return jb + key_of((g & 4 ? 2 : 0) + (g & 2 ? 1 : 0), t);
+}
+__device__ __forceinline__ float gathered(const float* out, int jb, int len, int g, int t) {
+  const int j = own_key(jb, g, t);
+  return !(g & 1) && j < len ? out[j] : 0.0f;
+}
+// Puts the weights of a tile's keys: w of keys key_of(0 .. 3), summed over the
+// lanes with the same t (each step leaves a lane half of the values), and what
+// they had.
+__device__ __forceinline__ void put_weights(float* out, const float (&w)[4], float had, int jb,
                                             int total, int g, int t) {
   const bool up = g & 4, right = g & 2;
   const float a = (up ? w[2] : w[0]) + __shfl_xor_sync(0xffffffffu, up ? w[0] : w[2], 16);
   const float b = (up ? w[3] : w[1]) + __shfl_xor_sync(0xffffffffu, up ? w[1] : w[3], 16);
   float sum = (right ? b : a) + __shfl_xor_sync(0xffffffffu, right ? a : b, 8);
   sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-  const int j = jb + key_of((up ? 2 : 0) + (right ? 1 : 0), t);
-  if (!(g & 1) && j < total) out[j] = (j < len ? out[j] : 0.0f) + sum;
+  const int j = own_key(jb, g, t);
+  if (!(g & 1) && j < total) out[j] = had + sum;
 }
 // w += exp2((c - bias) f - z) of row g of each 8, where it sees the key.
 template <int NT>
@@ -920,13 +929,24 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
 #pragma unroll
   for (int s = 0; s < kSlots; ++s)
     ring.start(s, kv, first + s * step, first + s * step < whole, false, lane);
+  float had_next[KT] = {};
+  auto had_of = [&](int base) {
+    if (base >= whole) return;
+#pragma unroll
+    for (int k = 0; k < KT; ++k) had_next[k] = gathered(w_out, (base + k) * 16, len, g, t);
+  };
   scales(sc_next, first);
+  had_of(first);
   slot = 0;
   for (int base = first; base < whole; base += step) {
-    float keep[KT];
+    float keep[KT], had[KT];
 #pragma unroll
-    for (int k = 0; k < KT; ++k) keep[k] = sc_next[k];
+    for (int k = 0; k < KT; ++k) {
+      keep[k] = sc_next[k];
+      had[k] = had_next[k];
+    }
     scales(sc_next, base + step);
+    had_of(base + step);
     ring.wait();
 #pragma unroll
     for (int k = 0; k < KT; ++k) {
@@ -938,7 +958,7 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
       for (int n = 0; n < NT; ++n) fk[0][n] = keep[k] * qs[n];
       // (rows past the last see nothing, the others all of a whole group)
       add_weights<NT>(w, c, fk, kBias, z, hidden_in<NT>((base + k) * 16, last, t));
-      put_weights(w_out, w, (base + k) * 16, len, total, g, t);
+      put_weights(w_out, w, had[k], (base + k) * 16, total, g, t);
     }
     __syncwarp();
     const int ahead = base + kSlots * step;
@@ -948,19 +968,21 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
   ring.drain();
   for (int tile = whole + mine; tile < tiles; tile += cluster * W) {
     Frag<D> one;
+    const float had = gathered(w_out, tile * 16, len, g, t);
     kv.load_k(one, tile, g, t);
     float c[1][NT][4], fk[1][NT], w[4] = {};
     products<D, NT>(c[0], one, qd);
 #pragma unroll
     for (int n = 0; n < NT; ++n) fk[0][n] = one.ks * qs[n];
     add_weights<NT>(w, c, fk, kBias, z, hidden_in<NT>(tile * 16, last, t));
-    put_weights(w_out, w, tile * 16, len, total, g, t);
+    put_weights(w_out, w, had, tile * 16, total, g, t);
   }
   for (int i = mine; closed + 16 * i < lim; i += cluster * W) {
+    const float had = gathered(w_out, closed + 16 * i, len, g, t);
     float c[1][NT][4], fk[1][NT], w[4] = {};
     tail_products<D, NT>(c, fk, kv, q_row, a.scale, closed + 16 * i, total, g, t);
     add_weights<NT>(w, c, fk, 0.0f, z, hidden_in<NT>(closed + 16 * i, last, t));
-    put_weights(w_out, w, closed + 16 * i, len, total, g, t);
+    put_weights(w_out, w, had, closed + 16 * i, total, g, t);
   }
 }
 
@@ -988,6 +1010,10 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) kv8_weights_kernel(const
 #pragma unroll
   for (int k = 0; k < 2; ++k)
     if (jb(k) < closed) kv.load_k(f[k], jb(k) >> 4, g, t);
+  float* out = a.weights + (int64_t)bh * S;
+  float had[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) had[k] = gathered(out, jb(k), len, g, t);
   auto row_at = [&](int r) {
     const int tk = a.div_g(r);
     return ((int64_t)b * a.T + tk) * a.Hq + h * G + (r - tk * G);
@@ -1043,7 +1069,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) kv8_weights_kernel(const
   }
 #pragma unroll
   for (int k = 0; k < 2; ++k)
-    put_weights(a.weights + (int64_t)bh * S, w[k], jb(k), len, total, g, t);
+    put_weights(out, w[k], had[k], jb(k), total, g, t);
 }
 
 // From so many rows of a sequence on, tcgen05.
