@@ -23,6 +23,7 @@
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
+#include <array>
 #include <type_traits>
 
 #include "attn_kv8.cuh"
@@ -696,7 +697,8 @@ __device__ __forceinline__ void add_weights(float (&w)[4], const float (&c)[1][N
 }
 
 constexpr int kFewMaxWarps = 8;
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 16;
+constexpr int kBigClusters[] = {16, 14, 12, 10};
 
 template <int D, int NT>
 struct FewShape {
@@ -709,7 +711,7 @@ struct FewShape {
   static constexpr int kRing = Ring<D>::kSlots * Ring<D>::kSlot / 4;
   static_assert(R * D <= kRing, "partial outputs fit a ring");
   static constexpr size_t smem(int W) {
-    return sizeof(float) * ((size_t)W * kRing + R * D + 2 * W * R + 2 * kMaxCluster * R);
+    return sizeof(float) * ((size_t)W * kRing + R * D + 4 * kMaxCluster + 2 * W * R + 2 * kMaxCluster * R);
   }
 };
 
@@ -722,8 +724,8 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
   extern __shared__ __align__(16) float smem[];
   const int W = blockDim.x >> 5;
   float* part_o = smem;                 // [W][kRing], the first R D of each
-  float* recv_o = part_o + W * kRing;   // [cluster][R D / cluster]: this CTA's share
-  float* part_m = recv_o + R * D;       // [W][R]
+  float* recv_o = part_o + W * kRing;   // [cluster][share]: of this CTA's outputs
+  float* part_m = recv_o + R * D + 4 * kMaxCluster;   // [W][R]
   float* part_l = part_m + W * R;       // [W][R]
   float* recv_m = part_l + W * R;       // [cluster][R]
   float* recv_l = recv_m + kMaxCluster * R;
@@ -876,7 +878,7 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
         make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     if (a.lse && e % D == 0) a.lse[at] = (M + log2f(L)) * kLn2;
   };
-  const int share = R * D / cluster;    // whole rows
+  const int share = (R * D / 4 + cluster - 1) / cluster * 4;
   const float *m_of = part_m, *l_of = part_l;
   int parts = W;
   if (cluster > 1) {
@@ -900,7 +902,7 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
   }
   const float* o_of = cluster > 1 ? recv_o : part_o;
   const int o_step = cluster > 1 ? share : kRing;
-  for (int i = threadIdx.x * 4; i < share; i += blockDim.x * 4) {
+  for (int i = threadIdx.x * 4; i < share && rank * share + i < R * D; i += blockDim.x * 4) {
     const int e = rank * share + i;
     float M, L;
     const float4 o = join(m_of + e / D, l_of + e / D, R, o_of + i, o_step, parts, M, L);
@@ -1086,7 +1088,7 @@ int launch_few(cudaStream_t s, const AttnArgs& a) {
   const int steps = (int)ceil_div(a.c.max_seq, 16 * FewShape<D, NT>::KT);
   int W = 4, C = 1;
   while (W < kFewMaxWarps && units * W * 2 <= 16 * kNumSms && W * 2 <= steps) W *= 2;
-  while (C < kMaxCluster && units * C * W * 2 <= 16 * kNumSms && C * W * 2 <= steps) C *= 2;
+  while (C < 8 && units * C * W * 2 <= 16 * kNumSms && C * W * 2 <= steps) C *= 2;
   const size_t smem = FewShape<D, NT>::smem(W);
   auto kern = attention_kv8_few_kernel<D, NT>;
   int rc;
@@ -1095,7 +1097,7 @@ int launch_few(cudaStream_t s, const AttnArgs& a) {
                                             (int)smem),
                        "attention_kv8: smem attribute")))
     return rc;
-  if ((int64_t)groups * a.c.kv_heads * C > INT32_MAX || a.c.batch > 65535)
+  if ((int64_t)groups * a.c.kv_heads * kMaxCluster > INT32_MAX || a.c.batch > 65535)
     return fail(SPX_ERR_UNSUPPORTED, "attention_kv8: grid too large");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(groups * a.c.kv_heads * C), (unsigned)a.c.batch);
@@ -1109,6 +1111,30 @@ int launch_few(cudaStream_t s, const AttnArgs& a) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  if (C == 8 && units * 10 <= FewShape<D, NT>::kBlocks * kNumSms) {
+    // Few sequences: larger clusters, of as many CTAs as the GPU has room for
+    // at a time (a cluster's SMs are neighbours: 8 clusters of 16 may not fit).
+    // At one sequence of 131 thousand tokens, 8 kv heads of 128, 8 CTAs each
+    // take 85 us.
+    static const std::array<int, 4> most = [&] {
+      std::array<int, 4> n = {};
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1))
+        cudaGetLastError();
+      for (size_t i = 0; i < n.size(); ++i) {
+        cudaLaunchConfig_t big = cfg;
+        cudaLaunchAttribute size = attr[0];
+        size.val.clusterDim.x = kBigClusters[i];
+        big.attrs = &size;
+        big.gridDim = dim3(kBigClusters[i]);
+        if (cudaOccupancyMaxActiveClusters(&n[i], kern, &big)) cudaGetLastError();
+      }
+      return n;
+    }();
+    for (size_t i = 0; i < most.size() && C == 8; ++i)
+      if (most[i] >= units && kBigClusters[i] * W <= steps) C = kBigClusters[i];
+    attr[0].val.clusterDim.x = (unsigned)C;
+    cfg.gridDim.x = (unsigned)(groups * a.c.kv_heads * C);
+  }
   return check_cuda(cudaLaunchKernelEx(&cfg, kern, a, groups, C), "attention_kv8");
 }
 

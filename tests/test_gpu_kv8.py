@@ -126,7 +126,7 @@ class Setup:
                 # (2^-22 each of the row's largest term), D + 8 roundings of
                 # 2^-24 of sum |q k|; of exp: that, and 4 roundings.
                 qk = np.abs(q[b, :n, hs]).astype(np.float64).max(-1) * np.abs(K).sum(-1).max()
-                ds = scale * qk.max() * (2.0 ** -21 + (D + 8) * 2.0 ** -24)
+                ds = abs(scale) * qk.max() * (2.0 ** -21 + (D + 8) * 2.0 ** -24)
                 dp = 2 * ds + 2.0 ** -20
                 assert np.abs(o[b, :n, hs] - ro).max() <= np.abs(V).max() * dp, (b, h)
                 assert np.all(np.abs(z[b, :n, hs] - rz) <= ds + 2.0 ** -21 * (1 + np.abs(rz)))
@@ -241,6 +241,26 @@ def test_attend_many_tokens(g, T, G, D, blk, lens):
     s = Setup(g, 2, 2, G, D, 512, blk, seed=T, lens=lens)
     d_q, q = s.append(T, [T, max(1, T - 3)])
     s.check_attention(d_q, q, lens)
+
+
+@pytest.mark.parametrize("B,Hkv,G,D,T,lens", [
+    (1, 1, 8, 64, 1, [8000]), (1, 2, 4, 128, 1, [7777]), (1, 2, 5, 64, 3, [6000]),
+    (2, 4, 2, 128, 1, [8100, 37]), (3, 3, 1, 64, 2, [0, 8190, 4097])])
+def test_attend_few_long_sequences(g, B, Hkv, G, D, T, lens):
+    """Keys of a sequence over large clusters, of sizes that do not divide the rows."""
+    s = Setup(g, B, Hkv, G, D, 8192, 64, seed=D, lens=lens)
+    d_q, q = s.append(T)
+    s.check_attention(d_q, q, lens)
+
+
+@pytest.mark.parametrize("T,G,D,blk,lens,scale", [
+    (300, 1, 64, 128, [0, 200], None), (400, 2, 64, 16, [3, 100], -0.1),
+    (150, 6, 128, 32, [350, 0], -0.07), (64, 2, 64, 64, [440, 448], 0.0)])
+def test_attend_many_tokens_scales(g, T, G, D, blk, lens, scale):
+    """Row tiles dealt to a cluster, keys that only some of them see, scales of any sign."""
+    s = Setup(g, 2, 2, G, D, 512, blk, seed=T, lens=lens)
+    d_q, q = s.append(T)
+    s.check_attention(d_q, q, lens, scale=scale)
 
 
 def test_attend_sharp_and_flat(g):
