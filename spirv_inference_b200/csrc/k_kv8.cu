@@ -15,7 +15,7 @@
 // as NaN: the fault stays visible.
 #include <cooperative_groups.h>
 
-#include "spx_internal.cuh"
+#include "attn_kv8.cuh"
 
 namespace spx {
 namespace {
@@ -48,8 +48,6 @@ __device__ __forceinline__ float scale_of(uint32_t amax_bits) {
   return a < kTinyAmax ? 0.0f : a / 127.0f;
 }
 __device__ __forceinline__ bool usable(float s) { return s > 0.0f && s <= 3.4028234663852886e38f; }
-
-__device__ __forceinline__ int clamp_len(int v, int hi) { return v < 0 ? 0 : v > hi ? hi : v; }
 
 struct KvView {
   int8_t* q8;     // int8 blocks of this (sequence, head)
@@ -418,14 +416,21 @@ __device__ __forceinline__ int requant(int q, float ratio, float rest) {
 __device__ __forceinline__ uint32_t requant4(uint32_t w, float ratio, float rest) {
   uint32_t r[4];
   float worst = 0.0f;
+  const uint32_t x = w ^ 0x80808080u;
+  const float2 by = make_float2(ratio, ratio);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 4; i += 2) {
     // bytes to fp32: 0x4b000000 | (q + 128) is 2^23 + 128 + q
-    const float q = __uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4b000000u, 0x7550 | i)) -
-                    8388736.0f;
-    const float p = q * ratio, k = p + 12582912.0f;            // 1.5 2^23: rounds to a whole
-    r[i] = __float_as_uint(k);
-    worst = fmaxf(worst, fabsf(p - (k - 12582912.0f)));
+    const float2 q = add2(make_float2(__uint_as_float(__byte_perm(x, 0x4b000000u, 0x7550 | i)),
+                                      __uint_as_float(__byte_perm(x, 0x4b000000u, 0x7551 | i))),
+                          make_float2(-8388736.0f, -8388736.0f));
+    // 1.5 2^23: rounds to a whole, half to even
+    const float2 k = fma2(q, by, make_float2(12582912.0f, 12582912.0f));
+    r[i] = __float_as_uint(k.x);
+    r[i + 1] = __float_as_uint(k.y);
+    const float2 whole = add2(k, make_float2(-12582912.0f, -12582912.0f));
+    const float2 off = fma2(q, by, make_float2(-whole.x, -whole.y));
+    worst = fmaxf(worst, fmaxf(fabsf(off.x), fabsf(off.y)));
   }
   if (worst > 0.4999f) {
 #pragma unroll
@@ -444,6 +449,7 @@ __global__ void __launch_bounds__(kGatherRows)
   __shared__ float row_scale[kGatherRows];
   __shared__ int row_src[kGatherRows];
   __shared__ uint32_t blk_scale[kGatherRows / 16];
+  __shared__ float2 row_by[kGatherRows];       // the new scale into the row's: ratio, rest
   const int blk = src.block, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x % cluster, unit = blockIdx.x / cluster;
   const int bh = unit >> 1, b = bh / src.kv_heads, h = bh % src.kv_heads;
@@ -496,11 +502,19 @@ __global__ void __launch_bounds__(kGatherRows)
       if (r < rows && row_src[r] < closed)
         out[k] = *reinterpret_cast<const uint4*>(s.q8 + (int64_t)row_src[r] * D + at);
     }
+    if (tid < rows) {
+      // (far from subnormal remainders)
+      const float ns = __uint_as_float(blk_scale[tid / blk]), sc = row_scale[tid];
+      const float up = ns < 0x1p-60f ? 0x1p64f : 1.0f, sn = sc * up, nn = ns * up;
+      const float ratio = sn / nn;
+      row_by[tid] = make_float2(ratio, fmaf(-ratio, nn, sn) / nn);
+    }
+    __syncthreads();
 #pragma unroll
     for (int k = 0; k < P; ++k) {
       const int e = tid + k * kGatherRows, r = e / P, at = (e % P) * 16;
       if (r >= rows) continue;
-      const float ns = __uint_as_float(blk_scale[r / blk]), sc = row_scale[r];
+      const float ns = __uint_as_float(blk_scale[r / blk]);
       uint32_t* o = reinterpret_cast<uint32_t*>(&out[k]);
       if (!usable(ns)) {
         out[k] = make_uint4(0, 0, 0, 0);
@@ -515,12 +529,10 @@ __global__ void __launch_bounds__(kGatherRows)
               (signed char)round_div(v.z, ns, inv), (signed char)round_div(v.w, ns, inv));
           o[i] = *reinterpret_cast<const uint32_t*>(&q);
         }
-      } else if (sc != ns) {
-        // (far from subnormal remainders)
-        const float up = ns < 0x1p-60f ? 0x1p64f : 1.0f, sn = sc * up, nn = ns * up;
-        const float ratio = sn / nn, rest = fmaf(-ratio, nn, sn) / nn;
+      } else if (row_by[r].x != 1.0f) {        // (of 1, each value is its own quotient)
+        const float2 by = row_by[r];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = requant4(o[i], ratio, rest);
+        for (int i = 0; i < 4; ++i) o[i] = requant4(o[i], by.x, by.y);
       }
     }
     if (in_place) {
