@@ -261,21 +261,46 @@ __global__ void __launch_bounds__(256)
   const KvView kv = view_of(c, b, h, is_v);
   float* out = (is_v ? v_out : k_out) + (int64_t)u * count * D;
   const int64_t all = (int64_t)count * D;
+  constexpr int N = kReadValues / 2048;
+  const int blk_shift = 31 - __clz(blk), d = threadIdx.x * 8 & (D - 1);
+  const int64_t e0 = (int64_t)chunk * kReadValues + threadIdx.x * 8;
+  uint2 q[N];
+  float s[N];
 #pragma unroll
-  for (int k = 0; k < kReadValues / 1024; ++k) {
-    const int64_t e = (int64_t)chunk * kReadValues + k * 1024 + threadIdx.x * 4;
-    if (e >= all) continue;
-    const int64_t slot = start + (e >> shift);
-    const int d = (int)(e & (D - 1));
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (slot >= 0 && slot < closed) {
-      const char4 q = __ldg(reinterpret_cast<const char4*>(kv.q8 + slot * D + d));
-      const float s = __ldg(kv.scale + slot / blk);
-      x = make_float4(q.x * s, q.y * s, q.z * s, q.w * s);
-    } else if (slot >= 0 && slot < len) {
-      x = __ldg(reinterpret_cast<const float4*>(kv.tail + (slot & (blk - 1)) * D + d));
+  for (int k = 0; k < N; ++k) {
+    const int64_t e = e0 + k * 2048, slot = start + (e >> shift);
+    q[k] = make_uint2(0x80808080u, 0x80808080u);
+    s[k] = 0.0f;
+    if (e < all && slot >= 0 && slot < closed) {
+      q[k] = __ldg(reinterpret_cast<const uint2*>(kv.q8 + slot * D + d));
+      q[k] = make_uint2(q[k].x ^ 0x80808080u, q[k].y ^ 0x80808080u);
+      s[k] = __ldg(kv.scale + (slot >> blk_shift));
     }
-    __stcs(reinterpret_cast<float4*>(out + e), x);
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int64_t e = e0 + k * 2048, slot = start + (e >> shift);
+    if (e >= all) continue;
+    float4* to = reinterpret_cast<float4*>(out + e);
+    if (slot >= closed && slot < len) {
+      const float4* x =
+          reinterpret_cast<const float4*>(kv.tail + (slot & (blk - 1)) * D + d);
+      __stcs(to, __ldg(x));
+      __stcs(to + 1, __ldg(x + 1));
+      continue;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t w = i ? q[k].y : q[k].x;
+      float2 v[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)          // 0x4b000000 | (value + 128) is 2^23 + 128 + value
+        v[j] = mul2(add2(make_float2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7550 | 2 * j)),
+                                     __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7551 | 2 * j))),
+                         make_float2(-8388736.0f, -8388736.0f)),
+                    make_float2(s[k], s[k]));
+      __stcs(to + i, make_float4(v[0].x, v[0].y, v[1].x, v[1].y));
+    }
   }
 }
 
@@ -716,8 +741,8 @@ int launch_kv8_evict(cudaStream_t s, int64_t* cnt, const spx_kv8_cache* src, con
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  rc = check_cuda(cudaLaunchKernelEx(&cfg, kern, *src, *dst, weights, dst_weights, (const int32_t*)idx,
-                                     keep, same ? 1 : 0, cluster),
+  rc = check_cuda(cudaLaunchKernelEx(&cfg, kern, *src, *dst, weights, dst_weights,
+                                     (const int32_t*)idx, keep, same ? 1 : 0, cluster),
                   "kv8_evict: gather");
   return rc ? rc : after_launch(cnt, "kv8_evict: gather");
 }
