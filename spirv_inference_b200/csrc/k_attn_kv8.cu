@@ -1114,12 +1114,14 @@ int launch_few(cudaStream_t s, const AttnArgs& a) {
   if (C == 8 && units * 10 <= FewShape<D, NT>::kBlocks * kNumSms) {
     // Few sequences: larger clusters, of as many CTAs as the GPU has room for
     // at a time (a cluster's SMs are neighbours: 8 clusters of 16 may not fit).
-    // At one sequence of 131 thousand tokens, 8 kv heads of 128, 8 CTAs each
-    // take 85 us.
+    // At one sequence of 131 thousand tokens, 8 kv heads of 128, 8 CTAs a head
+    // take 85 us, 10 take 71.
+    if ((rc = check_cuda(
+             cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
+             "attention_kv8: cluster attribute")))
+      return rc;
     static const std::array<int, 4> most = [&] {
       std::array<int, 4> n = {};
-      if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1))
-        cudaGetLastError();
       for (size_t i = 0; i < n.size(); ++i) {
         cudaLaunchConfig_t big = cfg;
         cudaLaunchAttribute size = attr[0];

@@ -47,6 +47,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kRows = 128, kTile = 64, kGroups = kTile / 16;
 constexpr int kThreads = 256;             // softmax, conversion
+constexpr int kMaxSplit = 8;              // CTAs that share a row tile's keys
 constexpr uint32_t kAtom = 128 * 128;     // 128 rows of 128 bytes
 constexpr unsigned long long kWaitNs = 2000000000ull;
 constexpr float kMaxFloat = 3.4028234663852886e38f;
@@ -188,29 +189,32 @@ __device__ __forceinline__ float4 finite4(float4 v, bool& odd) {
 // What every role knows of the CTA's work.
 template <int D>
 struct Unit {
-  int h, b, r0, rows, len, total, closed, lim, tiles, G;
-  __device__ __forceinline__ Unit(const AttnArgs& a) {
+  int h, b, r0, rows, len, total, closed, lim, first, tiles, G;
+  __device__ __forceinline__ Unit(const AttnArgs& a, int cluster) {
     G = a.Hq / a.c.kv_heads;
     // the last rows see the most keys: first, and those of all heads
-    const int heads = a.c.batch * a.c.kv_heads, at = blockIdx.x / heads;
-    const int bh = blockIdx.x - at * heads;
+    const int heads = a.c.batch * a.c.kv_heads, unit = blockIdx.x / cluster;
+    const int at = unit / heads, bh = unit - at * heads;
     b = bh / a.c.kv_heads;
     h = bh - b * a.c.kv_heads;
-    r0 = (int)(gridDim.x / heads - 1 - at) * kRows;
+    r0 = (int)(gridDim.x / cluster / heads - 1 - at) * kRows;
     const int n_new = a.new_lens ? clamp_len(a.new_lens[b], a.T) : a.T;
     rows = n_new * G;
     len = clamp_len(a.c.lens[b], a.c.max_seq);
     total = min(len + n_new, a.c.max_seq);
     closed = total / a.c.block * a.c.block;
     lim = min(len + a.div_g(min(r0 + kRows, rows) - 1) + 1, a.c.max_seq);
-    tiles = (lim + kTile - 1) / kTile;
+    // this CTA's tiles, `tiles` from `first` on
+    const int all = (lim + kTile - 1) / kTile, rank = blockIdx.x % cluster;
+    first = (int)((int64_t)all * rank / cluster);
+    tiles = (int)((int64_t)all * (rank + 1) / cluster) - first;
   }
   __device__ __forceinline__ int64_t row_at(const AttnArgs& a, int r) const {
     const int tk = a.div_g(r);
     return ((int64_t)b * a.T + tk) * a.Hq + h * G + (r - tk * G);
   }
   __device__ __forceinline__ bool has_tail(int tile) const {
-    return closed < lim && (tile + 1) * kTile > closed;
+    return closed < lim && (first + tile + 1) * kTile > closed;
   }
 };
 
@@ -408,7 +412,7 @@ __device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& 
   uint4 kr[L], vr[L];
   float k_sc = 0.0f, v_sc = 0.0f;
   auto load = [&](int tile) {
-    const int key = tile * kTile + r, key16 = tile * kTile + r16;
+    const int key = (u.first + tile) * kTile + r, key16 = (u.first + tile) * kTile + r16;
     k_sc = v_sc = 0.0f;
     if (tile >= u.tiles) return;
     const uint4* kp = reinterpret_cast<const uint4*>(k8 + (int64_t)key16 * D) + c16;
@@ -427,7 +431,7 @@ __device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& 
   load(0);
   int n = 0;                   // the tile's slot
   for (int tile = 0; tile < u.tiles; ++tile) {
-    const int key = tile * kTile + r;
+    const int key = (u.first + tile) * kTile + r;
     const bool closed = key < u.closed, in_tail = !closed && key < u.total;
     const bool tail = u.has_tail(tile);
     const float* kf = in_tail ? kt + (int64_t)(key & (blk - 1)) * D : nullptr;
@@ -481,7 +485,7 @@ __device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& 
 #pragma unroll
     for (int i = 0; i < L; ++i) {
       const int to = i * PER + r16;
-      if (tile * kTile + to >= u.closed) break;
+      if ((u.first + tile) * kTile + to >= u.closed) break;
       *piece<kTile>(k_to, to, 2 * c16) = eight(kr[i].x, kr[i].y, mask);
       *piece<kTile>(k_to, to, 2 * c16 + 1) = eight(kr[i].z, kr[i].w, mask);
       *piece<kTile>(v_to, to, 2 * c16) = eight(vr[i].x, vr[i].y, mask);
@@ -544,7 +548,7 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
   };
   int n = 0;
   for (int tile = 0; tile < u.tiles; ++tile) {
-    const int s = n & 3, j0 = tile * kTile;
+    const int s = n & 3, j0 = (u.first + tile) * kTile;
     const bool tail = u.has_tail(tile);
     // (the slot for its scales)
     if (!wait(&aux.full[s], (n >> 2) & 1)) return false;
@@ -635,13 +639,60 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
   if (!wait(&aux.done, 0)) return false;
   tc_after();
   if (u.tiles >= 2) take_output(u.tiles - 2, corr2, back2);
-  take_output(u.tiles - 1, corr1, back1);
+  if (u.tiles >= 1) take_output(u.tiles - 1, corr1, back1);
   return true;
 }
 
+// Joins the outputs that a cluster's CTAs have of the same 128 rows: each gets
+// an equal share of the rows from all, where its keys and values were.  By the
+// softmax threads; the others take part in the two barriers.
 template <int D>
+__device__ __forceinline__ void join(const AttnArgs& a, const Unit<D>& u, uint8_t* slots,
+                                     int cluster, int x, const float (&o)[D], float m, float l) {
+  static_assert(kRows * (D + 2) * 4 <= TcShape<D>::kSlots * TcShape<D>::kSlot, "fits");
+  cg::cluster_group cl = cg::this_cluster();
+  const int rank = blockIdx.x % cluster, per = kRows / cluster;
+  float* got = reinterpret_cast<float*>(slots);        // [CTA][row][D]
+  float2* got_ml = reinterpret_cast<float2*>(got + kRows * D);
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  const int at = rank * per + x % per;
+  float4* to = reinterpret_cast<float4*>(cl.map_shared_rank(got, x / per) + at * D);
+#pragma unroll
+  for (int i = 0; i < D / 4; ++i)     // each four came as 0, 2, 1, 3
+    to[i] = make_float4(o[4 * i], o[4 * i + 2], o[4 * i + 1], o[4 * i + 3]);
+  cl.map_shared_rank(got_ml, x / per)[at] = make_float2(m, m == m ? l : NAN);
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  const int row = x / cluster, part = x % cluster, r = u.r0 + rank * per + row;
+  if (r >= u.rows) return;
+  float most = -INFINITY, sum = 0.0f;
+  for (int k = 0; k < cluster; ++k) most = fmaxf(most, got_ml[k * per + row].x);
+  for (int k = 0; k < cluster; ++k) {
+    const float2 ml = got_ml[k * per + row];
+    sum = fmaf(ml.y, ml.x == -INFINITY ? 0.0f : ex2(ml.x - most), sum);
+  }
+  const int64_t out_row = u.row_at(a, r);
+  const float inv = 1.0f / sum;
+  for (int e = part * (D / cluster); e < (part + 1) * (D / cluster); e += 4) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < cluster; ++k) {
+      const float mk = got_ml[k * per + row].x, f = mk == -INFINITY ? 0.0f : ex2(mk - most);
+      const float4 w = *reinterpret_cast<const float4*>(got + (k * per + row) * D + e);
+      v = make_float4(fmaf(w.x, f, v.x), fmaf(w.y, f, v.y), fmaf(w.z, f, v.z), fmaf(w.w, f, v.w));
+    }
+    *reinterpret_cast<float4*>(a.out + out_row * D + e) =
+        make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+  }
+  if (a.lse && part == 0) a.lse[out_row] = (most + log2f(sum)) * kLn2;
+}
+
+// SPLIT: the keys are dealt to a cluster.  (Apart: the join costs the others
+// registers, 168 against 180 us over four prompts of 1024.)
+template <int D, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
-    attention_kv8_tc_kernel(const AttnArgs a) {
+    attention_kv8_tc_kernel(const AttnArgs a, int ctas) {
   using S = TcShape<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* q_hi = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -650,8 +701,9 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
   __shared__ Aux aux;
   __shared__ float q_scale[kRows];
   const int warp = threadIdx.x >> 5;
-  const Unit<D> u(a);
-  if (u.r0 >= u.rows) return;
+  const int cluster = SPLIT ? ctas : 1;
+  const Unit<D> u(a, cluster);
+  if (u.r0 >= u.rows) return;                 // the whole cluster
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kSlots; ++i) {
       mb_init(&aux.full[i], kTile);
@@ -685,7 +737,9 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
     for (int i = 0; i < D; ++i) o[i] = 0.0f;
     const bool ok = softmax_tiles<D>(a, u, aux, q_scale, tmem, x, o, m, l);
     const int r = u.r0 + x;
-    if (ok && r < u.rows) {
+    if (SPLIT) {
+      join<D>(a, u, slots, cluster, x, o, ok ? m : NAN, l);
+    } else if (ok && r < u.rows) {
       const int64_t at = u.row_at(a, r);
       const float inv = 1.0f / l;
       float4* out = reinterpret_cast<float4*>(a.out + at * D);
@@ -713,6 +767,13 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
     } else if (warp == 6) {
       const Issue<D> issue(sa(q_hi), sa(q_lo), sa(slots), tmem);
       issue_tiles<D>(u, aux, issue);
+    }
+    if (SPLIT) {                              // (of join)
+      __syncwarp();
+      for (int i = 0; i < 2; ++i) {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+      }
     }
   }
   tc_before();
@@ -763,7 +824,8 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
   // the first keys are seen by the most rows: first, and those of all heads
   const int heads = a.c.batch * a.c.kv_heads, rank = blockIdx.x % cluster;
   const int unit = blockIdx.x / cluster, j0 = unit / heads * kKeys, bh = unit % heads;
-  const int b = bh / a.c.kv_heads, h = bh - b * a.c.kv_heads, G = a.Hq / a.c.kv_heads, blk = a.c.block;
+  const int b = bh / a.c.kv_heads, h = bh - b * a.c.kv_heads;
+  const int G = a.Hq / a.c.kv_heads, blk = a.c.block;
   const int n_new = a.new_lens ? clamp_len(a.new_lens[b], a.T) : a.T;
   const int len = clamp_len(a.c.lens[b], a.c.max_seq), total = min(len + n_new, a.c.max_seq);
   if (n_new == 0 || j0 >= total) return;      // the whole cluster
@@ -974,26 +1036,43 @@ template <int D>
 int launch_tc(cudaStream_t s, const AttnArgs& a) {
   using S = TcShape<D>;
   const int64_t row_tiles = ceil_div((int64_t)a.T * (a.Hq / a.c.kv_heads), kRows);
-  const int64_t grid = row_tiles * a.c.kv_heads * a.c.batch;
+  // Few rows: their keys go to the CTAs of a cluster, as long as there are SMs
+  // without work and four tiles each.
+  const int64_t units = row_tiles * a.c.kv_heads * a.c.batch;
+  int cluster = 1;
+  while (cluster < kMaxSplit && units * cluster * 2 <= S::kBlocks * kNumSms &&
+         cluster * 2 * 4 <= a.c.max_seq / kTile)
+    cluster *= 2;
+  const int64_t grid = units * cluster;
   if (grid > INT32_MAX) return fail(SPX_ERR_UNSUPPORTED, "attention_kv8: grid too large");
   const size_t smem = 1024 + 2 * S::kQ + S::kSlots * S::kSlot;
-  int rc = check_cuda(cudaFuncSetAttribute(attention_kv8_tc_kernel<D>,
-                                           cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
-                      "attention_kv8: smem attribute");
+  auto kern = cluster > 1 ? attention_kv8_tc_kernel<D, true> : attention_kv8_tc_kernel<D, false>;
+  int rc = check_cuda(
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+      "attention_kv8: smem attribute");
   if (rc) return rc;
   if constexpr (D == 64) {
     // setmaxnreg draws on the registers that the launch has: with fewer than
     // it was written for, it would wait for good.
     cudaFuncAttributes f;
-    if ((rc = check_cuda(cudaFuncGetAttributes(&f, attention_kv8_tc_kernel<D>),
-                         "attention_kv8: attributes")))
-      return rc;
+    if ((rc = check_cuda(cudaFuncGetAttributes(&f, kern), "attention_kv8: attributes"))) return rc;
     if (f.numRegs < S::kRegs)
       return fail(SPX_ERR_UNSUPPORTED, "attention_kv8: built with %d registers a thread",
                   f.numRegs);
   }
-  attention_kv8_tc_kernel<D><<<(unsigned)grid, kThreads, smem, s>>>(a);
-  return SPX_OK;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, a, cluster), "attention_kv8");
 }
 
 template <int D>

@@ -263,6 +263,36 @@ def test_attend_many_tokens_scales(g, T, G, D, blk, lens, scale):
     s.check_attention(d_q, q, lens, scale=scale)
 
 
+@pytest.mark.parametrize("B,Hkv,G,D,T,S,lens", [
+    (1, 1, 8, 64, 16, 4096, [4000]), (2, 1, 4, 128, 40, 2048, [1999, 1]),
+    (3, 2, 16, 64, 17, 2048, [0, 64, 2031]), (1, 1, 1, 128, 260, 1024, [700]),
+    (2, 2, 32, 64, 4, 512, [508, 100])])
+def test_attend_rows_split_over_keys(g, B, Hkv, G, D, T, S, lens):
+    """Few row tiles: their keys over a cluster, some CTAs of which have none."""
+    s = Setup(g, B, Hkv, G, D, S, 32, seed=T, lens=lens)
+    d_q, q = s.append(T, [T] + [max(1, T - 5)] * (B - 1))
+    s.check_attention(d_q, q, lens)
+
+
+@pytest.mark.parametrize("T", [1, 24])
+def test_nan_rows_and_values_over_clusters(g, T):
+    """A NaN in a query or in an open V reaches the rows that see it, no others."""
+    s = Setup(g, 1, 2, 8, 64, 4096, 32, lens=[3000])
+    x = s.rng.standard_normal((1, T, 20 * 64)).astype(np.float32)
+    x[0, T - 1, 18 * 64 + 3] = np.nan       # V of kv head 0 of the last token
+    x[0, 0, 9 * 64] = np.nan                # q of head 9 (kv head 1) of the first
+    d_q, q = s.append(T, qkv=x)
+    out, lse = g.tensor(np.zeros((T, 16, 64), np.float32)), g.tensor(
+        np.zeros((T, 16), np.float32))
+    g.attention_kv8(d_q, s.cache, out, q_len=T, q_heads=16, scale=0.125, lse=lse)
+    o = out.download().reshape(T, 16, 64)
+    bad = np.zeros((T, 16), bool)
+    bad[T - 1, :8] = True
+    bad[0, 9] = True
+    assert np.isnan(o[bad]).all(axis=-1).all() and np.isfinite(o[~bad]).all()
+    assert np.isnan(lse.download().reshape(T, 16)[0, 9])
+
+
 def test_attend_sharp_and_flat(g):
     """Scores of +-100 and of 0: one slot takes everything; all are equal."""
     s = Setup(g, 1, 2, 4, 64, 256, 32, lens=[200])
