@@ -371,24 +371,61 @@ __device__ __forceinline__ void issue_tiles(const Unit<D>& u, Aux& aux, const Is
 }
 
 // ---- conversion of keys and values ------------------------------------------------
-// A row of the tail as its hi or lo part (x its scale); zeros where there is none.
+// 16 rows of the tail, `n` of them there, as hi and lo parts of the operand's
+// rows r0 on, by a warp: a row's lanes next to each other, four loads at a time
+// (more cost the loop over closed tiles its registers), once for the largest
+// value and once more.  Returns what takes them back, a power of two.  V: a NaN
+// or an infinity becomes zero and marks its key.
 template <int D, bool V>
-__device__ __forceinline__ void put_tail(uint8_t* base, int r, const float* row, float down,
-                                         bool low) {
-  const float4* from = reinterpret_cast<const float4*>(row);
-  bool unused = false;
-  for (int c = 0; c < D / 8; ++c) {
-    uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-    if (row) {
-      float4 p = from[2 * c], q = from[2 * c + 1];
-      if (V) {
-        p = finite4(p, unused);
-        q = finite4(q, unused);
-      }
-      eight_split(p, q, down, hi, lo);
+__device__ __forceinline__ float tail_group(uint8_t* hi_to, uint8_t* lo_to, int r0,
+                                            const float* rows, int n, uint8_t* bad, int lane) {
+  constexpr int L = D / 4, PER = 32 / L, N = 16 / PER;
+  const int c = lane % L, r = lane / L;
+  auto load = [&](float4 (&v)[4], int from) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = (from + i) * PER + r;
+      v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row < n) v[i] = reinterpret_cast<const float4*>(rows)[row * L + c];
     }
-    *piece<kTile>(base, r, c) = low ? lo : hi;
+  };
+  uint32_t mx = 0;
+#pragma unroll 1
+  for (int from = 0; from < N; from += 4) {
+    float4 v[4];
+    load(v, from);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (V) {
+        const uint32_t all = __ballot_sync(
+            0xffffffffu, odd_bits(v[i].x) || odd_bits(v[i].y) || odd_bits(v[i].z) ||
+                             odd_bits(v[i].w));
+        if (c == 0)
+          bad[r0 + (from + i) * PER + r] = (L == 32 ? all : all >> (r * L) & 0xffffu) != 0;
+      }
+      mx = max(max(mx, finite_abs(v[i].x)),
+               max(finite_abs(v[i].y), max(finite_abs(v[i].z), finite_abs(v[i].w))));
+    }
   }
+  float down, up;
+  pow2_scale(__reduce_max_sync(0xffffffffu, mx), down, up);
+#pragma unroll 1
+  for (int from = 0; from < N; from += 4) {
+    float4 v[4];
+    load(v, from);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      bool odd;
+      if (V) v[i] = finite4(v[i], odd);
+      uint2 hi, lo;
+      split2(v[i].x * down, v[i].z * down, hi.x, lo.x);
+      split2(v[i].y * down, v[i].w * down, hi.y, lo.y);
+      const int to = r0 + (from + i) * PER + r;
+      reinterpret_cast<uint2*>(piece<kTile>(hi_to, to, c >> 1))[c & 1] = hi;
+      reinterpret_cast<uint2*>(piece<kTile>(lo_to, to, c >> 1))[c & 1] = lo;
+    }
+  }
+  return up;
 }
 
 template <int D>
@@ -430,46 +467,70 @@ __device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& 
   };
   load(0);
   int n = 0;                   // the tile's slot
-  for (int tile = 0; tile < u.tiles; ++tile) {
-    const int key = (u.first + tile) * kTile + r;
-    const bool closed = key < u.closed, in_tail = !closed && key < u.total;
-    const bool tail = u.has_tail(tile);
-    const float* kf = in_tail ? kt + (int64_t)(key & (blk - 1)) * D : nullptr;
-    const float* vf = in_tail ? vt + (int64_t)(key & (blk - 1)) * D : nullptr;
-    float k_down = 0.0f, v_down = 0.0f;
-    bool odd = false;
-    if (tail) {                // the tail's 16-key groups: powers of two
-      uint32_t mk = 0, mv = 0;
-      if (in_tail)
-        for (int i = 0; i < D / 4; ++i) {
-          const float4 p = reinterpret_cast<const float4*>(kf)[i];
-          const float4 q = finite4(reinterpret_cast<const float4*>(vf)[i], odd);
-          mk = max(max(mk, finite_abs(p.x)),
-                   max(finite_abs(p.y), max(finite_abs(p.z), finite_abs(p.w))));
-          mv = max(max(mv, finite_abs(q.x)),
-                   max(finite_abs(q.y), max(finite_abs(q.z), finite_abs(q.w))));
-        }
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) {
-        mk = max(mk, __shfl_xor_sync(0xffffffffu, mk, o));
-        mv = max(mv, __shfl_xor_sync(0xffffffffu, mv, o));
-      }
-      if (!closed) {
-        pow2_scale(mk, k_down, k_sc);
-        pow2_scale(mv, v_down, v_sc);
-      }
+  auto zero = [&](uint8_t* k_to, uint8_t* v_to, int row) {   // 16 rows, by a warp
+    for (int i = r & 31; i < D * 2; i += 32) {
+      *piece<kTile>(k_to, row + i / (D / 8), i % (D / 8)) = make_uint4(0, 0, 0, 0);
+      *piece<kTile>(v_to, row + i / (D / 8), i % (D / 8)) = make_uint4(0, 0, 0, 0);
     }
-    const int s = n & 3;
-    const bool drained = mb_wait(&aux.empty[s], ((n >> 2) & 1) ^ 1, &aux.abort_flag, &g_at_status,
-                                 kWaitNs, 64);
-    if (drained) {
+  };
+  for (int tile = 0; tile < u.tiles; ++tile) {
+    const int j0 = (u.first + tile) * kTile;
+    const bool tail = u.has_tail(tile);
+    const int s = n & 3, s2 = (n + 1) & 3;
+    auto drained = [&](int slot, int m) {
+      return mb_wait(&aux.empty[slot], ((m >> 2) & 1) ^ 1, &aux.abort_flag, &g_at_status, kWaitNs,
+                     64);
+    };
+    bool ok = drained(s, n);
+    if (tail) ok = ok && drained(s2, n + 1);
+    ok = __all_sync(0xffffffffu, ok);
+    uint8_t* k_to = slots + s * S::kSlot;
+    uint8_t* v_to = k_to + S::kHalf;
+    if (ok) {
       if ((r & 15) == 0) {
         aux.k_scale[s][r >> 4] = k_sc;
         aux.v_raw[s][r >> 4] = v_sc;
       }
-      aux.bad[s][r] = odd;
+      aux.bad[s][r] = 0;
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+        const int to = i * PER + r16;
+        if (j0 + to >= u.closed) break;
+        *piece<kTile>(k_to, to, 2 * c16) = eight(kr[i].x, kr[i].y, mask);
+        *piece<kTile>(k_to, to, 2 * c16 + 1) = eight(kr[i].z, kr[i].w, mask);
+        *piece<kTile>(v_to, to, 2 * c16) = eight(vr[i].x, vr[i].y, mask);
+        *piece<kTile>(v_to, to, 2 * c16 + 1) = eight(vr[i].z, vr[i].w, mask);
+      }
     }
-    if (!vote(1, kTile, drained)) return;
+    if (ok && j0 + kTile > u.closed) {
+      // Groups of 16 keys, two of the tile's four a warp: closed ones have no
+      // lo part; the others come from the tail if some row sees it.
+      uint8_t* k_lo = slots + s2 * S::kSlot;
+      uint8_t* v_lo = k_lo + S::kHalf;
+      __syncwarp();
+#pragma unroll 1
+      for (int grp = r >> 5 << 1; grp < (r >> 5 << 1) + kGroups / 2; ++grp) {
+        const int key = j0 + grp * 16;
+        if (key < u.closed || !tail) {
+          if (tail)
+            zero(k_lo, v_lo, grp * 16);
+          else if (key >= u.closed)
+            zero(k_to, v_to, grp * 16);
+          continue;
+        }
+        const int64_t at = (int64_t)(key & (blk - 1)) * D;
+        const int rows = max(0, min(u.total - key, 16));
+        const float ku =
+            tail_group<D, false>(k_to, k_lo, grp * 16, kt + at, rows, nullptr, r & 31);
+        const float vu =
+            tail_group<D, true>(v_to, v_lo, grp * 16, vt + at, rows, aux.bad[s], r & 31);
+        if ((r & 31) == 0) {
+          aux.k_scale[s][grp] = ku;
+          aux.v_raw[s][grp] = vu;
+        }
+      }
+    }
+    if (!vote(1, kTile, ok)) return;
     if (r < kGroups) {
       float ref = 0.0f;
 #pragma unroll
@@ -480,35 +541,11 @@ __device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& 
       aux.share[s][r] = ref > 0.0f ? aux.v_raw[s][r] * (kPUp / ref) : aux.v_raw[s][r];
       if (r == 0) aux.back[s] = ref * (1.0f / kPUp);
     }
-    uint8_t* k_to = slots + s * S::kSlot;
-    uint8_t* v_to = k_to + S::kHalf;
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-      const int to = i * PER + r16;
-      if ((u.first + tile) * kTile + to >= u.closed) break;
-      *piece<kTile>(k_to, to, 2 * c16) = eight(kr[i].x, kr[i].y, mask);
-      *piece<kTile>(k_to, to, 2 * c16 + 1) = eight(kr[i].z, kr[i].w, mask);
-      *piece<kTile>(v_to, to, 2 * c16) = eight(vr[i].x, vr[i].y, mask);
-      *piece<kTile>(v_to, to, 2 * c16 + 1) = eight(vr[i].z, vr[i].w, mask);
-    }
-    if (!closed) {
-      put_tail<D, false>(k_to, r, kf, k_down, false);
-      put_tail<D, true>(v_to, r, vf, v_down, false);
-    }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mb_arrive(&aux.full[s]);
+    if (tail) mb_arrive(&aux.full[s2]);
     load(tile + 1);            // on its way while the next slot drains
-    ++n;
-    if (!tail) continue;
-    const int s2 = n & 3;
-    if (!vote(1, kTile, mb_wait(&aux.empty[s2], ((n >> 2) & 1) ^ 1, &aux.abort_flag, &g_at_status,
-                                kWaitNs, 64)))
-      return;
-    put_tail<D, false>(slots + s2 * S::kSlot, r, kf, k_down, true);
-    put_tail<D, true>(slots + s2 * S::kSlot + S::kHalf, r, vf, v_down, true);
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    mb_arrive(&aux.full[s2]);
-    ++n;
+    n += tail ? 2 : 1;
   }
 }
 
