@@ -18,10 +18,10 @@
 // tile that would overflow it (rising logits, ties) gives its k best one by
 // one.  Warps' and CTAs' lists are merged by binary searches.
 //
-// Bound by the logits' bytes; instructions come next (a maximum, a difference,
-// a product, ex2 and two sums a value), so pairs of values go through the
-// packed fp32 operations, and the rank is counted only in lanes whose maximum
-// exceeds the token's logit.
+// 4096 rows of 32000: 102 us, 5.1 TB/s.  Bound by the logits' bytes;
+// instructions come next (a maximum, a difference, a product, ex2 and two sums a
+// value), so pairs of values go through the packed fp32 operations, and the rank
+// is counted only in lanes whose maximum exceeds the token's logit.
 #include <cooperative_groups.h>
 
 #include "spx_internal.cuh"
@@ -510,15 +510,18 @@ int launch_token_logprobs(cudaStream_t s, int64_t* cnt, const float* x, int64_t 
     return fail(SPX_ERR_INVALID_ARGUMENT, "token_logprobs: top_k needs both outputs");
   if (cols > INT32_MAX - 16 * kLpWarps * kLpTile)
     return fail(SPX_ERR_UNSUPPORTED, "token_logprobs: too many columns");
-  // A warp a row when that gives two CTAs an SM of at least half their warps:
-  // as few warps as take the same number of rounds, so that they end together.
-  // Else a CTA a row, or several while there are fewer than two CTAs an SM and
-  // half of a CTA's warps still have a tile.
-  const bool row_per_warp = rows >= kLpPerSm * kNumSms * kLpWarps / 2;
+  // A warp a row from two warps a CTA on, four CTAs an SM: as few warps as take
+  // the same number of rounds, so that they end together.  Of 32000 columns, us
+  // with a CTA and with a warp a row: 600 rows 39, 56; 1200: 62, 59; 2368: 109,
+  // 71; 4096: 182, 102.  Else a CTA a row, or several while that makes no more
+  // than three an SM and half of a CTA's warps still have a tile: 1 row with 1,
+  // 2, 4, 8 CTAs: 14.5, 12.0, 8.2, 6.5; 64 rows: 15.9, 12.7, 9.8, 11.2; 148 rows:
+  // 16.3, 14.4, 17.5, 21.2; 200 rows: 19.1, 17.5, 20.4, 27.4.
+  const bool row_per_warp = rows >= kLpPerSm * kNumSms * 2;
   const int rounds = (int)ceil_div(rows, kLpPerSm * kNumSms * kLpWarps);
   const int warps = row_per_warp ? (int)ceil_div(rows, kLpPerSm * kNumSms * rounds) : kLpWarps;
   int cluster = 1;
-  while (cluster < kLpMaxCluster && (int64_t)rows * cluster < 2 * kNumSms &&
+  while (cluster < kLpMaxCluster && (int64_t)rows * cluster * 2 <= 3 * kNumSms &&
          cols / cluster > kLpWarps * kLpTile / 2)
     cluster *= 2;
   const int seg = (int)ceil_div(ceil_div(cols + 3, cluster), 4) * 4;
