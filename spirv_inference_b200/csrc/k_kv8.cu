@@ -422,9 +422,10 @@ __global__ void __launch_bounds__(kSelThreads)
 // chunks of 256 rows a CTA: all of a chunk into registers, a cluster barrier,
 // then out.  Slot i of the result comes from a slot >= i, so in that order it
 // also works in place, without a second buffer.  64 sequences of 1500 to 4096
-// cut to 2048, 4 kv heads of 64: 75 us for 134 MB (clusters of 4: 73, of 2: 75),
-// 20 at the rate of a copy; the chain of loads (slot, scale, row) before each
-// barrier and some 5 instructions a value that is rounded again bound it.
+// cut to 2048, 4 kv heads of 64: 70 us for 134 MB, 20 at the rate of a copy
+// (clusters of 4 and 2 took 73 and 75 when this took 75); the chain of loads
+// (slot, scale, row) before each barrier and the instructions of values that
+// are rounded again bound it.
 constexpr int kGatherRows = 256;
 
 // The int8 value nearest to q s / ns, halves to even, for |q s| <= 127 ns.
@@ -479,15 +480,16 @@ __global__ void __launch_bounds__(kGatherRows)
   __shared__ int row_src[kGatherRows];
   __shared__ uint32_t blk_scale[kGatherRows / 16];
   __shared__ float2 row_by[kGatherRows];       // the new scale into the row's: ratio, rest
-  const int blk = src.block, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int blk = src.block, shift = 31 - __clz(blk);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x % cluster, unit = blockIdx.x / cluster;
   const int bh = unit >> 1, b = bh / src.kv_heads, h = bh % src.kv_heads;
   const bool is_v = unit & 1;
   const int n = clamp_len(src.lens[b], src.max_seq);
-  const int kept = min(n, keep), full = kept / blk * blk;
+  const int kept = min(n, keep), full = kept >> shift << shift;
   if (in_place && n <= keep) return;           // the whole cluster
   const KvView s = view_of(src, b, h, is_v), d = view_of(dst, b, h, is_v);
-  const int closed = n / blk * blk;
+  const int closed = n >> shift << shift;
   const int32_t* from = idx + (int64_t)bh * keep;
   for (int base = 0; base < kept; base += cluster * kGatherRows) {
     const int lo = base + rank * kGatherRows;  // this CTA's rows, whole blocks
@@ -504,9 +506,9 @@ __global__ void __launch_bounds__(kGatherRows)
       row_src[tid] = j;
       in_tail = j >= closed;
       if (!in_tail) {
-        const float sc = s.scale[j / blk];
+        const float sc = s.scale[j >> shift];
         row_scale[tid] = sc;
-        atomicMax(&blk_scale[tid / blk], abs_bits(sc));
+        atomicMax(&blk_scale[tid >> shift], abs_bits(sc));
       }
     }
     for (uint32_t todo = __ballot_sync(0xffffffffu, in_tail); todo; todo &= todo - 1) {
@@ -519,7 +521,7 @@ __global__ void __launch_bounds__(kGatherRows)
       const float sc = scale_of(__reduce_max_sync(0xffffffffu, mx));
       if (lane == 0) {
         row_scale[r] = sc;
-        atomicMax(&blk_scale[r / blk], abs_bits(sc));
+        atomicMax(&blk_scale[r >> shift], abs_bits(sc));
       }
     }
     __syncthreads();
@@ -533,7 +535,7 @@ __global__ void __launch_bounds__(kGatherRows)
     }
     if (tid < rows) {
       // (far from subnormal remainders)
-      const float ns = __uint_as_float(blk_scale[tid / blk]), sc = row_scale[tid];
+      const float ns = __uint_as_float(blk_scale[tid >> shift]), sc = row_scale[tid];
       const float up = ns < 0x1p-60f ? 0x1p64f : 1.0f, sn = sc * up, nn = ns * up;
       const float ratio = sn / nn;
       row_by[tid] = make_float2(ratio, fmaf(-ratio, nn, sn) / nn);
@@ -543,7 +545,7 @@ __global__ void __launch_bounds__(kGatherRows)
     for (int k = 0; k < P; ++k) {
       const int e = tid + k * kGatherRows, r = e / P, at = (e % P) * 16;
       if (r >= rows) continue;
-      const float ns = __uint_as_float(blk_scale[r / blk]);
+      const float ns = __uint_as_float(blk_scale[r >> shift]);
       uint32_t* o = reinterpret_cast<uint32_t*>(&out[k]);
       if (!usable(ns)) {
         out[k] = make_uint4(0, 0, 0, 0);
@@ -571,8 +573,8 @@ __global__ void __launch_bounds__(kGatherRows)
         __syncthreads();
     }
     if (has_w) w_dst[(int64_t)bh * dst.max_seq + lo + tid] = wv;
-    if (tid < rows && tid % blk == 0)
-      d.scale[(lo + tid) / blk] = __uint_as_float(blk_scale[tid / blk]);
+    if (tid < rows && (tid & (blk - 1)) == 0)
+      d.scale[(lo + tid) >> shift] = __uint_as_float(blk_scale[tid >> shift]);
 #pragma unroll
     for (int k = 0; k < P; ++k) {
       const int e = tid + k * kGatherRows;
@@ -586,7 +588,7 @@ __global__ void __launch_bounds__(kGatherRows)
   if (rank != 0 || full == kept) return;
   for (int e = tid; e < (kept - full) * D; e += kGatherRows) {
     const int j = from[full + e / D], x = e % D;
-    open_rows[e] = j < closed ? s.q8[(int64_t)j * D + x] * s.scale[j / blk]
+    open_rows[e] = j < closed ? s.q8[(int64_t)j * D + x] * s.scale[j >> shift]
                               : s.tail[(j & (blk - 1)) * D + x];
   }
   __syncthreads();
