@@ -596,7 +596,7 @@ int spx_op_rope_kv8_append(spx_graph* g, const float* qkv, int64_t ld_qkv, const
 /* Causal grouped-query attention of the new tokens over the cache, after their
  * append: the token in slot i sees the slots up to i, out = softmax(scale q
  * k^T) v in fp32 accuracy.  q and out are [batch * q_len][q_heads][head_dim],
- * 16-byte aligned.  lse (may be NULL): [batch * q_len][q_heads], the log of
+ * 16-byte aligned, and share no memory.  lse (may be NULL): [batch * q_len][q_heads], the log of
  * each softmax sum.  weights (may be NULL; needs lse): [batch][kv_heads]
  * [max_seq], to which each slot's attention weight, summed over the new tokens
  * and the heads of the group, is added; the new tokens' slots start from 0.

@@ -1162,6 +1162,9 @@ int launch_attention_kv8(cudaStream_t s, int64_t* cnt, const float* q, const spx
   if (((uintptr_t)q & 15) || ((uintptr_t)out & 15))
     return fail(SPX_ERR_INVALID_ARGUMENT, "attention_kv8: q and out must be 16-byte aligned");
   const int64_t bh = (int64_t)c->batch * c->kv_heads;
+  const uint64_t bytes = (uint64_t)c->batch * T * Hq * c->head_dim * 4;   // q is read to the end
+  if ((uintptr_t)q < (uintptr_t)out + bytes && (uintptr_t)out < (uintptr_t)q + bytes)
+    return fail(SPX_ERR_INVALID_ARGUMENT, "attention_kv8: q and out share memory");
   if ((int64_t)c->batch * T * Hq > INT32_MAX || bh > 65535)
     return fail(SPX_ERR_UNSUPPORTED, "attention_kv8: grid too large");
   const int G = Hq / c->kv_heads;

@@ -650,10 +650,12 @@ int launch_rope_kv8_append(cudaStream_t s, int64_t* cnt, const float* qkv, int64
   a.Hq = Hq;
   a.q_out = q_out;
   a.c = *c;
-  a.blocks = (T + 2 * c->block - 2) / c->block;   // the open block and what follows
+  // the open block and what follows
+  const int64_t blocks = ((int64_t)T + 2 * c->block - 2) / c->block;
   const int64_t q_ctas = (int64_t)c->batch * T;
-  const int64_t grid = q_ctas + (int64_t)c->batch * c->kv_heads * 2 * a.blocks;
+  const int64_t grid = q_ctas + (int64_t)c->batch * c->kv_heads * 2 * blocks;
   if (grid > INT32_MAX) return fail(SPX_ERR_UNSUPPORTED, "rope_kv8_append: grid too large");
+  a.blocks = (int)blocks;
   a.q_ctas = (int)q_ctas;
   a.vec = al16(qkv) && ld_qkv % 4 == 0 && al16(cos_t) && al16(sin_t);
   const int items = c->block * c->head_dim / 8;

@@ -469,6 +469,19 @@ def test_refusals(g):
     g.sync()
 
 
+def test_queries_and_outputs_apart(g):
+    """What a row writes, another may still have to read."""
+    s = Setup(g, 1, 1, 2, 64, 64, 32)
+    both = g.alloc((4, 2, 64))
+    for at in (0, 2 * 64):
+        with pytest.raises(_lib.SpxError) as e:
+            g.attention_kv8(both, s.cache, both.view((2, 2, 64), at), q_len=2, q_heads=2, scale=1.0)
+        assert e.value.code == _lib.SPX_ERR_INVALID_ARGUMENT
+    s.append(2)
+    g.attention_kv8(both, s.cache, both.view((2, 2, 64), 4 * 64), q_len=2, q_heads=2, scale=1.0)
+    g.sync()
+
+
 # -- together -----------------------------------------------------------------
 def test_captured_step(g):
     """Append, attention with weights, log probabilities of a made-up head and

@@ -85,6 +85,14 @@ def test_decoder_refuses_what_does_not_fit():
         llama.LlamaDecoder(cfg, W, 1, 60, 20, kv_cache="int8")
 
 
+@pytest.mark.parametrize("block", [0, 8, 24, 256])
+def test_decoder_refuses_blocks_of_other_sizes(block):
+    cfg = llama.LlamaConfig(hidden=128, layers=1, heads=2, kv_heads=1, ffn=64, vocab=50,
+                            max_seq=64)
+    with pytest.raises(ValueError, match="kv_block"):
+        llama.LlamaDecoder(cfg, {}, 1, 4, 4, kv_cache="int8", kv_block=block)
+
+
 def test_restatement_of_the_cache():
     rng = np.random.default_rng(0)
     x = rng.standard_normal((70, 64)).astype(np.float32)
