@@ -840,8 +840,7 @@ constexpr int kWeightCluster = 4, kKeys = 128, kWeightThreads = 384;
 struct WeightAux {
   alignas(16) float2 row[2][kRows];   // the row's factor, and its lse in units of log 2
   float got[kWeightCluster][kKeys];
-  float k_scale[kKeys], odd_tiles[kKeys];
-  uint64_t full[2], empty[2], k_full, s_ready[2], done[2];
+  uint64_t full[2], empty[2], k_full, s_ready[2], done;
   uint32_t tmem;
   int abort_flag;
 };
@@ -882,9 +881,9 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
       mb_init(&aux.full[i], 128);
       mb_init(&aux.empty[i], 129);     // the products, and the threads that read `row`
       mb_init(&aux.s_ready[i], 1);
-      mb_init(&aux.done[i], 1);
     }
     mb_init(&aux.k_full, 128);
+    mb_init(&aux.done, 1);
     aux.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -903,7 +902,7 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
     return mb_wait(bar, parity, &aux.abort_flag, &g_at_status, kWaitNs, 32);
   };
   float w = 0.0f;
-  if (warp >= 8) {
+  if (warp >= 4) {
     auto row_at = [&](int r) {
       const int tk = a.div_g(r);
       return ((int64_t)b * a.T + tk) * a.Hq + h * G + (r - tk * G);
@@ -914,66 +913,63 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
       if (i >= tiles) return;
       const int r0 = row0(i);
       q.load(x, [&](int r) { return r0 + r < rows ? a.q + row_at(r0 + r) * D : nullptr; });
-      z = r0 + x < rows ? a.lse[row_at(r0 + x)] * kLog2e : INFINITY;
+      z = r0 + x < rows ? a.lse[row_at(r0 + x)] : INFINITY;
     };
-    load(0);
-    for (int i = 0; i < tiles; ++i) {
-      const int s = i & 1;
+    const int s = uniform((warp - 4) >> 2);   // the group's slot, and its first tile
+    load(s);
+    for (int i = s; i < tiles; i += 2) {
       const bool drained = mb_wait(&aux.empty[s], ((i >> 1) & 1) ^ 1, &aux.abort_flag,
                                    &g_at_status, kWaitNs, 128);
       if (!__all_sync(0xffffffffu, drained)) break;
       uint8_t* to = slots + s * S::kSlot;
       q.convert(x, a.scale, to, to + S::kSlot / 2,
                 [&](int r, float f) { aux.row[s][r].x = f; });
-      aux.row[s][x].y = z;
-      load(i + 1);                     // on its way while the slot is used
+      aux.row[s][x].y = z * kLog2e;
+      load(i + 2);                     // on its way while the slot is used
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mb_arrive(&aux.full[s]);
     }
   } else {
-    if (warp < 4) {
-      // The key's row, and its scale.
-      const int key = j0 + x;
-      float ks = 0.0f;
-      if (key < closed) {
-        const uint4* kp =
-            reinterpret_cast<const uint4*>(a.c.k + ((int64_t)bh * a.c.max_seq + key) * D);
-        uint32_t mask;
-        asm volatile("mov.b32 %0, 0x00ff00ff;" : "=r"(mask));
-  #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          const uint4 v = __ldg(kp + i);
-          *piece<kKeys>(k_hi, x, 2 * i) = eight(v.x, v.y, mask);
-          *piece<kKeys>(k_hi, x, 2 * i + 1) = eight(v.z, v.w, mask);
-          *piece<kKeys>(k_lo, x, 2 * i) = make_uint4(0, 0, 0, 0);
-          *piece<kKeys>(k_lo, x, 2 * i + 1) = make_uint4(0, 0, 0, 0);
-        }
-        ks = __ldg(a.c.k_scale + (int64_t)bh * (a.c.max_seq / blk) + key / blk);
-      } else {
-        // a row of the tail on its own: any power of two does
-        const float* row =
-            key < total ? a.c.k_tail + ((int64_t)bh * blk + (key & (blk - 1))) * D : nullptr;
-        const float4* from = reinterpret_cast<const float4*>(row);
-        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-        uint32_t mx = 0;
-        for (int i = 0; i < D / 4; ++i) {
-          const float4 v = row ? from[i] : zero;
-          mx = max(max(mx, finite_abs(v.x)),
-                   max(finite_abs(v.y), max(finite_abs(v.z), finite_abs(v.w))));
-        }
-        float down;
-        pow2_scale(mx, down, ks);
-        for (int c = 0; c < D / 8; ++c) {
-          uint4 hi, lo;
-          eight_split(row ? from[2 * c] : zero, row ? from[2 * c + 1] : zero, down, hi, lo);
-          *piece<kKeys>(k_hi, x, c) = hi;
-          *piece<kKeys>(k_lo, x, c) = lo;
-        }
+    // The key's row, and its scale.
+    const int key = j0 + x;
+    float ks = 0.0f;
+    if (key < closed) {
+      const uint4* kp =
+          reinterpret_cast<const uint4*>(a.c.k + ((int64_t)bh * a.c.max_seq + key) * D);
+      uint32_t mask;
+      asm volatile("mov.b32 %0, 0x00ff00ff;" : "=r"(mask));
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const uint4 v = __ldg(kp + i);
+        *piece<kKeys>(k_hi, x, 2 * i) = eight(v.x, v.y, mask);
+        *piece<kKeys>(k_hi, x, 2 * i + 1) = eight(v.z, v.w, mask);
+        *piece<kKeys>(k_lo, x, 2 * i) = make_uint4(0, 0, 0, 0);
+        *piece<kKeys>(k_lo, x, 2 * i + 1) = make_uint4(0, 0, 0, 0);
       }
-      aux.k_scale[x] = ks;
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mb_arrive(&aux.k_full);
+      ks = __ldg(a.c.k_scale + (int64_t)bh * (a.c.max_seq / blk) + key / blk);
+    } else {
+      // a row of the tail on its own: any power of two does
+      const float* row =
+          key < total ? a.c.k_tail + ((int64_t)bh * blk + (key & (blk - 1))) * D : nullptr;
+      const float4* from = reinterpret_cast<const float4*>(row);
+      const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+      uint32_t mx = 0;
+      for (int i = 0; i < D / 4; ++i) {
+        const float4 v = row ? from[i] : zero;
+        mx = max(max(mx, finite_abs(v.x)),
+                 max(finite_abs(v.y), max(finite_abs(v.z), finite_abs(v.w))));
+      }
+      float down;
+      pow2_scale(mx, down, ks);
+      for (int c = 0; c < D / 8; ++c) {
+        uint4 hi, lo;
+        eight_split(row ? from[2 * c] : zero, row ? from[2 * c + 1] : zero, down, hi, lo);
+        *piece<kKeys>(k_hi, x, c) = hi;
+        *piece<kKeys>(k_lo, x, c) = lo;
+      }
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    mb_arrive(&aux.k_full);
     const uint64_t kh = sw128_desc(sa(k_hi)), kl = sw128_desc(sa(k_lo));
     const uint64_t q0 = sw128_desc(sa(slots));
     constexpr uint32_t kDesc = idesc_f16(kKeys, kRows, 0);
@@ -982,21 +978,21 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
       for (int i = 0; i < D / 16; ++i)
         mma_f16(to, k + k_step(i, kKeys), q + k_step(i, kRows), kDesc, i ? 1u : more);
     };
-    const int s = uniform(warp >> 2), key = j0 + x;
-    const uint64_t qh = q0 + (uint64_t)s * (S::kSlot >> 4), ql = qh + (S::kSlot >> 5);
-    const uint32_t to = uniform(tmem) + s * kRows;
+    const uint32_t base = uniform(tmem);
     auto hold = [&](uint64_t* bar, int parity) {     // a warp goes on or ends as one
       return __all_sync(0xffffffffu, wait(bar, parity)) != 0;
     };
     bool ok = hold(&aux.k_full, 0);
-    const float ks = aux.k_scale[x];
     // The key's first row, and whether a tile has any before that of some key.
     const int r_min = max(0, key - len) * G, r_all = max(0, j0 + kKeys - 1 - len) * G;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    for (int i = s; ok && i < tiles; i += 2) {
-      // (a slot is filled anew after the group has read its half of TMEM)
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    for (int i = 0; ok && i < tiles; ++i) {
+      const int s = uniform(i & 1);
+      const uint64_t qh = q0 + (uint64_t)s * (S::kSlot >> 4), ql = qh + (S::kSlot >> 5);
+      const uint32_t to = base + s * kRows;
+      // (a slot is filled anew after all four have read its half of TMEM)
       if (!(ok = hold(&aux.full[s], (i >> 1) & 1))) break;
-      if ((warp & 3) == 0) {
+      if (warp == 0) {
         tc_after();
         if (elect_one()) {
           products(kh, ql, to, 0u);
@@ -1042,16 +1038,14 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
       tc_before();
       mb_arrive(&aux.empty[s]);
     }
-    if (!ok && (warp & 3) == 0 && elect_one()) {
+    if (!ok && warp == 0 && elect_one()) {
       // The products in flight end before shared memory and TMEM are given up.
       volatile int never = 0;
-      mma_commit(&aux.done[s]);
-      mb_wait(&aux.done[s], 0, &never, &g_at_status, 200000000ull, 64);
+      mma_commit(&aux.done);
+      mb_wait(&aux.done, 0, &never, &g_at_status, 200000000ull, 64);
     }
-    if (s == 1) aux.odd_tiles[x] = w;
   }
   __syncthreads();
-  if (warp < 4) w += aux.odd_tiles[x];
   const bool good = !aux.abort_flag;
   if (cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   cg::cluster_group cl = cg::this_cluster();
