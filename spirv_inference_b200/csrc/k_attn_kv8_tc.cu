@@ -226,17 +226,18 @@ struct Unit {
 // kRows rows by 128 threads.  Threads next to each other take 8 values each of
 // one row, so that a warp reads whole lines (a row a thread took four times as
 // long for the loads: each touched 32 lines).
-template <int D>
-struct Rows {
-  static constexpr int L = D / 8, PER = 128 / L, N = kRows / PER;
+template <int D, int PARTS>
+struct Rows {                  // 1 / PARTS of them at a time
+  static constexpr int L = D / 8, PER = 128 / L, N = kRows / PER / PARTS;
   float4 v[N][2];
   // row_of: the row's values, or null for zeros
   template <class F>
-  __device__ __forceinline__ void load(int x, F row_of) {
+  __device__ __forceinline__ void load(int x, int part, F row_of) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float4* from = reinterpret_cast<const float4*>(row_of(i * PER + x / L)) + x % L * 2;
-      const bool is = row_of(i * PER + x / L) != nullptr;
+      const float* row = row_of((part * N + i) * PER + x / L);
+      const float4* from = reinterpret_cast<const float4*>(row) + x % L * 2;
+      const bool is = row != nullptr;
       v[i][0] = is ? __ldg(from) : make_float4(0.f, 0.f, 0.f, 0.f);
       v[i][1] = is ? __ldg(from + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
@@ -244,8 +245,8 @@ struct Rows {
   // put(row, the factor that takes its products to scores in units of log 2:
   // NaN for a row with a NaN or an infinity)
   template <class F>
-  __device__ __forceinline__ void convert(int x, float scale, uint8_t* hi_to, uint8_t* lo_to,
-                                          F put) const {
+  __device__ __forceinline__ void convert(int x, int part, float scale, uint8_t* hi_to,
+                                          uint8_t* lo_to, F put) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       uint32_t mx = 0;
@@ -264,7 +265,7 @@ struct Rows {
       if (scale < 0.0f) down = -down;
       uint4 hi, lo;
       eight_split(v[i][0], v[i][1], down, hi, lo);
-      const int r = i * PER + x / L;
+      const int r = (part * N + i) * PER + x / L;
       *piece<kRows>(hi_to, r, x % L) = hi;
       *piece<kRows>(lo_to, r, x % L) = lo;
       if (x % L == 0) put(r, odd ? __int_as_float(0x7fc00000) : up * (fabsf(scale) * kLog2e));
@@ -793,11 +794,11 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
   } else {
     const int x = threadIdx.x - 128;
     {
-      Rows<D> rows;
-      rows.load(x, [&](int r) {
+      Rows<D, 1> rows;
+      rows.load(x, 0, [&](int r) {
         return u.r0 + r < u.rows ? a.q + u.row_at(a, u.r0 + r) * D : nullptr;
       });
-      rows.convert(x, a.scale, q_hi, q_lo, [&](int r, float f) { q_scale[r] = f; });
+      rows.convert(x, 0, a.scale, q_hi, q_lo, [&](int r, float f) { q_scale[r] = f; });
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mb_arrive(&aux.q_full);
@@ -907,25 +908,28 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
       const int tk = a.div_g(r);
       return ((int64_t)b * a.T + tk) * a.Hq + h * G + (r - tk * G);
     };
-    Rows<D> q;
+    // (rows of q in two parts: all at once took registers that were not there)
+    Rows<D, 2> q;
     float z = INFINITY;                // (a row that is none weighs nothing)
-    auto load = [&](int i) {
+    auto load = [&](int i, int part) {
       if (i >= tiles) return;
       const int r0 = row0(i);
-      q.load(x, [&](int r) { return r0 + r < rows ? a.q + row_at(r0 + r) * D : nullptr; });
-      z = r0 + x < rows ? a.lse[row_at(r0 + x)] : INFINITY;
+      q.load(x, part, [&](int r) { return r0 + r < rows ? a.q + row_at(r0 + r) * D : nullptr; });
+      if (part == 0) z = r0 + x < rows ? a.lse[row_at(r0 + x)] : INFINITY;
     };
     const int s = uniform((warp - 4) >> 2);   // the group's slot, and its first tile
-    load(s);
+    uint8_t* to = slots + s * S::kSlot;
+    auto put = [&](int r, float f) { aux.row[s][r].x = f; };
+    load(s, 0);
     for (int i = s; i < tiles; i += 2) {
       const bool drained = mb_wait(&aux.empty[s], ((i >> 1) & 1) ^ 1, &aux.abort_flag,
                                    &g_at_status, kWaitNs, 128);
       if (!__all_sync(0xffffffffu, drained)) break;
-      uint8_t* to = slots + s * S::kSlot;
-      q.convert(x, a.scale, to, to + S::kSlot / 2,
-                [&](int r, float f) { aux.row[s][r].x = f; });
+      q.convert(x, 0, a.scale, to, to + S::kSlot / 2, put);
+      load(i, 1);
       aux.row[s][x].y = z * kLog2e;
-      load(i + 2);                     // on its way while the slot is used
+      q.convert(x, 1, a.scale, to, to + S::kSlot / 2, put);
+      load(i + 2, 0);                  // on its way while the slot is used
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mb_arrive(&aux.full[s]);
     }
