@@ -67,7 +67,7 @@ struct TcShape {
   static constexpr int kBlocks = D == 64 ? 2 : 1;        // CTAs an SM
   // Two CTAs an SM leave 128 registers a thread; the conversion warps give
   // some of theirs to the softmax warps, which hold a row of the output.
-  static constexpr int kRegs = 128, kSoftmaxRegs = 184, kConvertRegs = 72;
+  static constexpr int kRegs = 128, kSoftmaxRegs = 168, kConvertRegs = 88;
   static_assert(kSoftmaxRegs + kConvertRegs <= 2 * kRegs, "within what the launch has");
 };
 
@@ -437,98 +437,120 @@ template <int D>
 __device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& u, uint8_t* slots,
                                               Aux& aux, int r) {
   using S = TcShape<D>;
+  // (few values are kept: registers are short)
   const int64_t bh = (int64_t)u.b * a.c.kv_heads + u.h;
-  const int blk = a.c.block;
-  const int8_t* k8 = a.c.k + bh * a.c.max_seq * D;
-  const int8_t* v8 = a.c.v + bh * a.c.max_seq * D;
-  const float* ks = a.c.k_scale + bh * (a.c.max_seq / blk);
-  const float* vs = a.c.v_scale + bh * (a.c.max_seq / blk);
-  const float* kt = a.c.k_tail + bh * blk * D;
-  const float* vt = a.c.v_tail + bh * blk * D;
+  const int shift = 31 - __clz(a.c.block);
   uint32_t mask;
   asm volatile("mov.b32 %0, 0x00ff00ff;" : "=r"(mask));
   // Rows of closed blocks: 16 bytes of a row a thread, a warp's next to each
-  // other.  Scales and rows of the tail: a key a thread.
+  // other.  Scales: by the first four lanes, of a group each.
   constexpr int L = D / 16, PER = kTile / L;
   const int r16 = r / L, c16 = r % L;
   uint4 kr[L], vr[L];
   float k_sc = 0.0f, v_sc = 0.0f;
   auto load = [&](int tile) {
-    const int key = (u.first + tile) * kTile + r, key16 = (u.first + tile) * kTile + r16;
+    const int j0 = (u.first + tile) * kTile, left = u.closed - j0 - r16;
+    const int64_t at = (bh * a.c.max_seq + j0 + r16) * D + c16 * 16;
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+      if (i * PER < left) kr[i] = __ldg(reinterpret_cast<const uint4*>(a.c.k + at) + i * PER * L);
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+      if (i * PER < left) vr[i] = __ldg(reinterpret_cast<const uint4*>(a.c.v + at) + i * PER * L);
+    const int key = j0 + r * 16;
     k_sc = v_sc = 0.0f;
-    if (tile >= u.tiles) return;
-    const uint4* kp = reinterpret_cast<const uint4*>(k8 + (int64_t)key16 * D) + c16;
-    const uint4* vp = reinterpret_cast<const uint4*>(v8 + (int64_t)key16 * D) + c16;
-#pragma unroll
-    for (int i = 0; i < L; ++i)
-      if (key16 + i * PER < u.closed) kr[i] = __ldg(kp + i * PER * L);
-#pragma unroll
-    for (int i = 0; i < L; ++i)
-      if (key16 + i * PER < u.closed) vr[i] = __ldg(vp + i * PER * L);
-    if (key < u.closed) {
-      k_sc = __ldg(ks + key / blk);
-      v_sc = __ldg(vs + key / blk);
+    if (r < kGroups && key < u.closed) {
+      const int64_t blk = ((bh * a.c.max_seq) >> shift) + (key >> shift);
+      k_sc = __ldg(a.c.k_scale + blk);
+      v_sc = __ldg(a.c.v_scale + blk);
     }
   };
-  load(0);
+  auto store = [&](uint8_t* k_to, uint8_t* v_to, int left) {
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      const int to = i * PER + r16;
+      if (to >= left) break;
+      *piece<kTile>(k_to, to, 2 * c16) = eight(kr[i].x, kr[i].y, mask);
+      *piece<kTile>(k_to, to, 2 * c16 + 1) = eight(kr[i].z, kr[i].w, mask);
+      *piece<kTile>(v_to, to, 2 * c16) = eight(vr[i].x, vr[i].y, mask);
+      *piece<kTile>(v_to, to, 2 * c16 + 1) = eight(vr[i].z, vr[i].w, mask);
+    }
+  };
+  auto shares = [&](int s) {                 // by the first warp, lane i with group i's v_sc
+    float ref = v_sc <= kMaxFloat ? v_sc : 0.0f;
+#pragma unroll
+    for (int o = 1; o < kGroups; o <<= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
+    if (r < kGroups) aux.share[s][r] = ref > 0.0f ? v_sc * (kPUp / ref) : v_sc;
+    if (r == 0) aux.back[s] = ref * (1.0f / kPUp);
+  };
+  auto drained = [&](int slot, int m) {
+    return mb_wait(&aux.empty[slot], ((m >> 2) & 1) ^ 1, &aux.abort_flag, &g_at_status, kWaitNs,
+                   64);
+  };
+  // (Apart from the others, whose code cost this loop its registers: 172
+  // against 132 us over four prompts.)
+  // Tiles of closed blocks only, each one's bytes on their way while the one
+  // before drains.
+  const int whole = max(0, min(u.tiles, u.closed / kTile - u.first));
+  if (whole > 0) load(0);
   int n = 0;                   // the tile's slot
-  auto zero = [&](uint8_t* k_to, uint8_t* v_to, int row) {   // 16 rows, by a warp
-    for (int i = r & 31; i < D * 2; i += 32) {
-      *piece<kTile>(k_to, row + i / (D / 8), i % (D / 8)) = make_uint4(0, 0, 0, 0);
-      *piece<kTile>(v_to, row + i / (D / 8), i % (D / 8)) = make_uint4(0, 0, 0, 0);
+  for (; n < whole; ++n) {
+    const int s = n & 3;
+    if (!__all_sync(0xffffffffu, drained(s, n))) {
+      if (whole < u.tiles) vote(1, kTile, false);   // the other warp waits there
+      return;
     }
-  };
-  for (int tile = 0; tile < u.tiles; ++tile) {
+    uint8_t* k_to = slots + s * S::kSlot;
+    store(k_to, k_to + S::kHalf, kTile);
+    if (r < 32) {
+      if (r < kGroups) aux.k_scale[s][r] = k_sc;
+      shares(s);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    mb_arrive(&aux.full[s]);
+    if (n + 1 < whole) load(n + 1);
+  }
+  // The others.
+  for (int tile = whole; tile < u.tiles; ++tile) {
     const int j0 = (u.first + tile) * kTile;
     const bool tail = u.has_tail(tile);
     const int s = n & 3, s2 = (n + 1) & 3;
-    auto drained = [&](int slot, int m) {
-      return mb_wait(&aux.empty[slot], ((m >> 2) & 1) ^ 1, &aux.abort_flag, &g_at_status, kWaitNs,
-                     64);
-    };
+    load(tile);
     bool ok = drained(s, n);
     if (tail) ok = ok && drained(s2, n + 1);
     ok = __all_sync(0xffffffffu, ok);
     uint8_t* k_to = slots + s * S::kSlot;
     uint8_t* v_to = k_to + S::kHalf;
+    uint8_t* k_lo = slots + s2 * S::kSlot;
+    uint8_t* v_lo = k_lo + S::kHalf;
     if (ok) {
-      if ((r & 15) == 0) {
-        aux.k_scale[s][r >> 4] = k_sc;
-        aux.v_raw[s][r >> 4] = v_sc;
+      if (r < kGroups && (!tail || j0 + r * 16 < u.closed)) {
+        aux.k_scale[s][r] = k_sc;
+        aux.v_raw[s][r] = v_sc;
       }
       aux.bad[s][r] = 0;
-#pragma unroll
-      for (int i = 0; i < L; ++i) {
-        const int to = i * PER + r16;
-        if (j0 + to >= u.closed) break;
-        *piece<kTile>(k_to, to, 2 * c16) = eight(kr[i].x, kr[i].y, mask);
-        *piece<kTile>(k_to, to, 2 * c16 + 1) = eight(kr[i].z, kr[i].w, mask);
-        *piece<kTile>(v_to, to, 2 * c16) = eight(vr[i].x, vr[i].y, mask);
-        *piece<kTile>(v_to, to, 2 * c16 + 1) = eight(vr[i].z, vr[i].w, mask);
-      }
-    }
-    if (ok && j0 + kTile > u.closed) {
+      store(k_to, v_to, u.closed - j0);
+      __syncwarp();
       // Groups of 16 keys, two of the tile's four a warp: closed ones have no
       // lo part; the others come from the tail if some row sees it.
-      uint8_t* k_lo = slots + s2 * S::kSlot;
-      uint8_t* v_lo = k_lo + S::kHalf;
-      __syncwarp();
 #pragma unroll 1
       for (int grp = r >> 5 << 1; grp < (r >> 5 << 1) + kGroups / 2; ++grp) {
         const int key = j0 + grp * 16;
         if (key < u.closed || !tail) {
-          if (tail)
-            zero(k_lo, v_lo, grp * 16);
-          else if (key >= u.closed)
-            zero(k_to, v_to, grp * 16);
+          if (tail || key >= u.closed)
+            for (int i = r & 31; i < D * 2; i += 32) {
+              const int row = grp * 16 + i / (D / 8), c = i % (D / 8);
+              *piece<kTile>(tail ? k_lo : k_to, row, c) = make_uint4(0, 0, 0, 0);
+              *piece<kTile>(tail ? v_lo : v_to, row, c) = make_uint4(0, 0, 0, 0);
+            }
           continue;
         }
-        const int64_t at = (int64_t)(key & (blk - 1)) * D;
+        const int64_t at = ((bh << shift) + (key & (a.c.block - 1))) * D;
         const int rows = max(0, min(u.total - key, 16));
-        const float ku =
-            tail_group<D, false>(k_to, k_lo, grp * 16, kt + at, rows, nullptr, r & 31);
-        const float vu =
-            tail_group<D, true>(v_to, v_lo, grp * 16, vt + at, rows, aux.bad[s], r & 31);
+        const float ku = tail_group<D, false>(k_to, k_lo, grp * 16, a.c.k_tail + at, rows, nullptr,
+                                              r & 31);
+        const float vu = tail_group<D, true>(v_to, v_lo, grp * 16, a.c.v_tail + at, rows,
+                                             aux.bad[s], r & 31);
         if ((r & 31) == 0) {
           aux.k_scale[s][grp] = ku;
           aux.v_raw[s][grp] = vu;
@@ -536,20 +558,13 @@ __device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& 
       }
     }
     if (!vote(1, kTile, ok)) return;
-    if (r < kGroups) {
-      float ref = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kGroups; ++i) {
-        const float v = aux.v_raw[s][i];
-        if (v <= kMaxFloat) ref = fmaxf(ref, v);
-      }
-      aux.share[s][r] = ref > 0.0f ? aux.v_raw[s][r] * (kPUp / ref) : aux.v_raw[s][r];
-      if (r == 0) aux.back[s] = ref * (1.0f / kPUp);
+    if (r < 32) {
+      v_sc = r < kGroups ? aux.v_raw[s][r] : 0.0f;
+      shares(s);
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mb_arrive(&aux.full[s]);
     if (tail) mb_arrive(&aux.full[s2]);
-    load(tile + 1);            // on its way while the next slot drains
     n += tail ? 2 : 1;
   }
 }
@@ -841,7 +856,8 @@ constexpr int kWeightCluster = 4, kKeys = 128, kWeightThreads = 384;
 struct WeightAux {
   alignas(16) float2 row[2][kRows];   // the row's factor, and its lse in units of log 2
   float got[kWeightCluster][kKeys];
-  uint64_t full[2], empty[2], k_full, s_ready[2], done;
+  float k_scale[kKeys], odd_tiles[kKeys];
+  uint64_t full[2], empty[2], k_full, s_ready[2], done[2];
   uint32_t tmem;
   int abort_flag;
 };
@@ -882,9 +898,9 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
       mb_init(&aux.full[i], 128);
       mb_init(&aux.empty[i], 129);     // the products, and the threads that read `row`
       mb_init(&aux.s_ready[i], 1);
+      mb_init(&aux.done[i], 1);
     }
     mb_init(&aux.k_full, 128);
-    mb_init(&aux.done, 1);
     aux.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -903,7 +919,7 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
     return mb_wait(bar, parity, &aux.abort_flag, &g_at_status, kWaitNs, 32);
   };
   float w = 0.0f;
-  if (warp >= 4) {
+  if (warp >= 8) {
     auto row_at = [&](int r) {
       const int tk = a.div_g(r);
       return ((int64_t)b * a.T + tk) * a.Hq + h * G + (r - tk * G);
@@ -917,11 +933,11 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
       q.load(x, part, [&](int r) { return r0 + r < rows ? a.q + row_at(r0 + r) * D : nullptr; });
       if (part == 0) z = r0 + x < rows ? a.lse[row_at(r0 + x)] : INFINITY;
     };
-    const int s = uniform((warp - 4) >> 2);   // the group's slot, and its first tile
-    uint8_t* to = slots + s * S::kSlot;
-    auto put = [&](int r, float f) { aux.row[s][r].x = f; };
-    load(s, 0);
-    for (int i = s; i < tiles; i += 2) {
+    load(0, 0);
+    for (int i = 0; i < tiles; ++i) {
+      const int s = i & 1;
+      uint8_t* to = slots + s * S::kSlot;
+      auto put = [&](int r, float f) { aux.row[s][r].x = f; };
       const bool drained = mb_wait(&aux.empty[s], ((i >> 1) & 1) ^ 1, &aux.abort_flag,
                                    &g_at_status, kWaitNs, 128);
       if (!__all_sync(0xffffffffu, drained)) break;
@@ -929,51 +945,54 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
       load(i, 1);
       aux.row[s][x].y = z * kLog2e;
       q.convert(x, 1, a.scale, to, to + S::kSlot / 2, put);
-      load(i + 2, 0);                  // on its way while the slot is used
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mb_arrive(&aux.full[s]);
+      load(i + 1, 0);                  // on its way while the slot is used
     }
   } else {
-    // The key's row, and its scale.
-    const int key = j0 + x;
-    float ks = 0.0f;
-    if (key < closed) {
-      const uint4* kp =
-          reinterpret_cast<const uint4*>(a.c.k + ((int64_t)bh * a.c.max_seq + key) * D);
-      uint32_t mask;
-      asm volatile("mov.b32 %0, 0x00ff00ff;" : "=r"(mask));
+    if (warp < 4) {
+      // The key's row, and its scale.
+      const int key = j0 + x;
+      float ks = 0.0f;
+      if (key < closed) {
+        const uint4* kp =
+            reinterpret_cast<const uint4*>(a.c.k + ((int64_t)bh * a.c.max_seq + key) * D);
+        uint32_t mask;
+        asm volatile("mov.b32 %0, 0x00ff00ff;" : "=r"(mask));
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const uint4 v = __ldg(kp + i);
-        *piece<kKeys>(k_hi, x, 2 * i) = eight(v.x, v.y, mask);
-        *piece<kKeys>(k_hi, x, 2 * i + 1) = eight(v.z, v.w, mask);
-        *piece<kKeys>(k_lo, x, 2 * i) = make_uint4(0, 0, 0, 0);
-        *piece<kKeys>(k_lo, x, 2 * i + 1) = make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < D / 16; ++i) {
+          const uint4 v = __ldg(kp + i);
+          *piece<kKeys>(k_hi, x, 2 * i) = eight(v.x, v.y, mask);
+          *piece<kKeys>(k_hi, x, 2 * i + 1) = eight(v.z, v.w, mask);
+          *piece<kKeys>(k_lo, x, 2 * i) = make_uint4(0, 0, 0, 0);
+          *piece<kKeys>(k_lo, x, 2 * i + 1) = make_uint4(0, 0, 0, 0);
+        }
+        ks = __ldg(a.c.k_scale + (int64_t)bh * (a.c.max_seq / blk) + key / blk);
+      } else {
+        // a row of the tail on its own: any power of two does
+        const float* row =
+            key < total ? a.c.k_tail + ((int64_t)bh * blk + (key & (blk - 1))) * D : nullptr;
+        const float4* from = reinterpret_cast<const float4*>(row);
+        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+        uint32_t mx = 0;
+        for (int i = 0; i < D / 4; ++i) {
+          const float4 v = row ? from[i] : zero;
+          mx = max(max(mx, finite_abs(v.x)),
+                   max(finite_abs(v.y), max(finite_abs(v.z), finite_abs(v.w))));
+        }
+        float down;
+        pow2_scale(mx, down, ks);
+        for (int c = 0; c < D / 8; ++c) {
+          uint4 hi, lo;
+          eight_split(row ? from[2 * c] : zero, row ? from[2 * c + 1] : zero, down, hi, lo);
+          *piece<kKeys>(k_hi, x, c) = hi;
+          *piece<kKeys>(k_lo, x, c) = lo;
+        }
       }
-      ks = __ldg(a.c.k_scale + (int64_t)bh * (a.c.max_seq / blk) + key / blk);
-    } else {
-      // a row of the tail on its own: any power of two does
-      const float* row =
-          key < total ? a.c.k_tail + ((int64_t)bh * blk + (key & (blk - 1))) * D : nullptr;
-      const float4* from = reinterpret_cast<const float4*>(row);
-      const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-      uint32_t mx = 0;
-      for (int i = 0; i < D / 4; ++i) {
-        const float4 v = row ? from[i] : zero;
-        mx = max(max(mx, finite_abs(v.x)),
-                 max(finite_abs(v.y), max(finite_abs(v.z), finite_abs(v.w))));
-      }
-      float down;
-      pow2_scale(mx, down, ks);
-      for (int c = 0; c < D / 8; ++c) {
-        uint4 hi, lo;
-        eight_split(row ? from[2 * c] : zero, row ? from[2 * c + 1] : zero, down, hi, lo);
-        *piece<kKeys>(k_hi, x, c) = hi;
-        *piece<kKeys>(k_lo, x, c) = lo;
-      }
+      aux.k_scale[x] = ks;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mb_arrive(&aux.k_full);
     }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    mb_arrive(&aux.k_full);
     const uint64_t kh = sw128_desc(sa(k_hi)), kl = sw128_desc(sa(k_lo));
     const uint64_t q0 = sw128_desc(sa(slots));
     constexpr uint32_t kDesc = idesc_f16(kKeys, kRows, 0);
@@ -982,21 +1001,21 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
       for (int i = 0; i < D / 16; ++i)
         mma_f16(to, k + k_step(i, kKeys), q + k_step(i, kRows), kDesc, i ? 1u : more);
     };
-    const uint32_t base = uniform(tmem);
+    const int s = uniform(warp >> 2), key = j0 + x;
+    const uint64_t qh = q0 + (uint64_t)s * (S::kSlot >> 4), ql = qh + (S::kSlot >> 5);
+    const uint32_t to = uniform(tmem) + s * kRows;
     auto hold = [&](uint64_t* bar, int parity) {     // a warp goes on or ends as one
       return __all_sync(0xffffffffu, wait(bar, parity)) != 0;
     };
     bool ok = hold(&aux.k_full, 0);
+    const float ks = aux.k_scale[x];
     // The key's first row, and whether a tile has any before that of some key.
     const int r_min = max(0, key - len) * G, r_all = max(0, j0 + kKeys - 1 - len) * G;
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    for (int i = 0; ok && i < tiles; ++i) {
-      const int s = uniform(i & 1);
-      const uint64_t qh = q0 + (uint64_t)s * (S::kSlot >> 4), ql = qh + (S::kSlot >> 5);
-      const uint32_t to = base + s * kRows;
-      // (a slot is filled anew after all four have read its half of TMEM)
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    for (int i = s; ok && i < tiles; i += 2) {
+      // (a slot is filled anew after the group has read its half of TMEM)
       if (!(ok = hold(&aux.full[s], (i >> 1) & 1))) break;
-      if (warp == 0) {
+      if ((warp & 3) == 0) {
         tc_after();
         if (elect_one()) {
           products(kh, ql, to, 0u);
@@ -1042,14 +1061,16 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
       tc_before();
       mb_arrive(&aux.empty[s]);
     }
-    if (!ok && warp == 0 && elect_one()) {
+    if (!ok && (warp & 3) == 0 && elect_one()) {
       // The products in flight end before shared memory and TMEM are given up.
       volatile int never = 0;
-      mma_commit(&aux.done);
-      mb_wait(&aux.done, 0, &never, &g_at_status, 200000000ull, 64);
+      mma_commit(&aux.done[s]);
+      mb_wait(&aux.done[s], 0, &never, &g_at_status, 200000000ull, 64);
     }
+    if (s == 1) aux.odd_tiles[x] = w;
   }
   __syncthreads();
+  if (warp < 4) w += aux.odd_tiles[x];
   const bool good = !aux.abort_flag;
   if (cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   cg::cluster_group cl = cg::this_cluster();
