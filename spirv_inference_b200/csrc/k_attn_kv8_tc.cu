@@ -143,22 +143,8 @@ __device__ __forceinline__ bool vote(int id, int threads, bool ok) {
   return r != 0;
 }
 
-// One lane of a converged warp, and a value that all lanes have as the compiler
-// can see: descriptors then stay in uniform registers, and a product is issued
-// in a tenth of the 110 cycles that it takes to move them there each time.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(r));
-  return r != 0;
-}
-template <class T>
-__device__ __forceinline__ T uniform(T v) {
-  return __shfl_sync(0xffffffffu, v, 0);
-}
+// Of a warp that goes together, the lane that issues.
+__device__ __forceinline__ bool first_lane() { return (threadIdx.x & 31) == 0; }
 
 // 16 bytes of piece `c` (eight values) of row `r` of an operand of ROWS rows.
 template <int ROWS>
@@ -282,9 +268,7 @@ struct Issue {
   uint32_t tmem;
   __device__ __forceinline__ Issue(uint32_t q_hi_at, uint32_t q_lo_at, uint32_t slots, uint32_t t)
       : q_hi(sw128_desc(q_hi_at)), q_lo(sw128_desc(q_lo_at)), k(sw128_desc(slots)),
-        v(mn_desc(slots + S::kHalf)), tmem(uniform(t)) {}
-  // (What the elected lane uses is made before, by the whole warp: made under
-  // elect_one(), descriptors came out wrong in one build.)
+        v(mn_desc(slots + S::kHalf)), tmem(t) {}
   // Q (from q) K^T (from a slot's k) over D, to the S buffer at `to`.
   template <bool MORE>
   static __device__ __forceinline__ void scores(uint64_t q, uint64_t from, uint32_t to) {
@@ -310,12 +294,12 @@ struct Issue {
   }
   // S of a tile whose rows are in slot n (and n + 1), once they are there.
   __device__ __forceinline__ bool tile_scores(Aux& aux, int tile, int n, bool tail) const {
-    const int s = uniform(n & 3), s2 = uniform((n + 1) & 3), j = uniform(tile & 1);
+    const int s = n & 3, s2 = (n + 1) & 3, j = tile & 1;
     const uint64_t from = k + (uint64_t)s * (S::kSlot >> 4);
     const uint64_t from2 = k + (uint64_t)s2 * (S::kSlot >> 4);
     const uint32_t to = tmem + j * kTile;
     if (!wait(aux, &aux.full[s], (n >> 2) & 1)) return false;
-    if (elect_one()) {
+    if (first_lane()) {
       scores<false>(q_lo, from, to);
       scores<true>(q_hi, from, to);
       if (!tail) mma_commit(&aux.s_ready[j]);
@@ -323,7 +307,7 @@ struct Issue {
     __syncwarp();
     if (!tail) return true;
     if (!wait(aux, &aux.full[s2], ((n + 1) >> 2) & 1)) return false;
-    if (elect_one()) {
+    if (first_lane()) {
       scores<true>(q_hi, from2, to);
       mma_commit(&aux.s_ready[j]);
     }
@@ -332,12 +316,12 @@ struct Issue {
   }
   // O of a tile, once P is there.
   __device__ __forceinline__ bool tile_values(Aux& aux, int tile, int n, bool tail) const {
-    const int s = uniform(n & 3), s2 = uniform((n + 1) & 3), j = uniform(tile & 1);
+    const int s = n & 3, s2 = (n + 1) & 3, j = tile & 1;
     const uint64_t from = v + (uint64_t)s * (S::kSlot >> 4);
     const uint64_t from2 = v + (uint64_t)s2 * (S::kSlot >> 4);
     const uint32_t p = tmem + j * kTile, to = tmem + 2 * kTile + j * D;
     if (!wait(aux, &aux.p_ready[j], (tile >> 1) & 1)) return false;
-    if (elect_one()) {
+    if (first_lane()) {
       values<16, false>(p, from, to);
       values<0, true>(p, from, to);
       if (tail) values<0, true>(p, from2, to);
@@ -349,8 +333,7 @@ struct Issue {
   }
 };
 
-// All products of the tiles.  (elect_one gives the same lane each time, so a
-// commit follows all that was issued before it.)
+// All products of the tiles, by one lane: a commit follows all issued before it.
 template <int D>
 __device__ __forceinline__ void issue_tiles(const Unit<D>& u, Aux& aux, const Issue<D>& issue) {
   bool ok = Issue<D>::wait(aux, &aux.q_full, 0);
@@ -364,7 +347,7 @@ __device__ __forceinline__ void issue_tiles(const Unit<D>& u, Aux& aux, const Is
     n1 = n;
     n += tail ? 2 : 1;
   }
-  if (elect_one()) {
+  if (first_lane()) {
     mma_commit(&aux.done);
     if (!ok) {
       // The products in flight end before shared memory and TMEM are given up.
@@ -1001,9 +984,9 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
       for (int i = 0; i < D / 16; ++i)
         mma_f16(to, k + k_step(i, kKeys), q + k_step(i, kRows), kDesc, i ? 1u : more);
     };
-    const int s = uniform(warp >> 2), key = j0 + x;
+    const int s = warp >> 2, key = j0 + x;
     const uint64_t qh = q0 + (uint64_t)s * (S::kSlot >> 4), ql = qh + (S::kSlot >> 5);
-    const uint32_t to = uniform(tmem) + s * kRows;
+    const uint32_t to = tmem + s * kRows;
     auto hold = [&](uint64_t* bar, int parity) {     // a warp goes on or ends as one
       return __all_sync(0xffffffffu, wait(bar, parity)) != 0;
     };
@@ -1017,7 +1000,7 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
       if (!(ok = hold(&aux.full[s], (i >> 1) & 1))) break;
       if ((warp & 3) == 0) {
         tc_after();
-        if (elect_one()) {
+        if (first_lane()) {
           products(kh, ql, to, 0u);
           if (tail) products(kl, qh, to, 1u);
           products(kh, qh, to, 1u);
@@ -1061,7 +1044,7 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
       tc_before();
       mb_arrive(&aux.empty[s]);
     }
-    if (!ok && (warp & 3) == 0 && elect_one()) {
+    if (!ok && (warp & 3) == 0 && first_lane()) {
       // The products in flight end before shared memory and TMEM are given up.
       volatile int never = 0;
       mma_commit(&aux.done[s]);
