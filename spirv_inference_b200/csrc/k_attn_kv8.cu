@@ -1075,13 +1075,13 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) kv8_weights_kernel(const
     put_weights(out, w[k], had[k], jb(k), total, g, t);
 }
 
-// From so many rows of a sequence and kv head on, tcgen05.  In us, this kernel
-// against that one, with weights, caches of 300 to 1500 tokens, 4 kv heads:
+// From so many rows of a sequence and kv head on, tcgen05.  In us, this file's
+// kernels against those, with weights, caches of 300 to 1500 tokens, 4 kv heads:
 //                  4 sequences of 64    32 of 64    4 of 128     32 of 128
-//    64 rows             37, 40          63, 93      49, 56      118, 152
-//    96 rows             46, 42          89, 92      61, 58      167, 152
-//   128 rows             56, 42         112, 97      77, 59      209, 157
-constexpr int kTcRows = 128;
+//    64 rows             37, 34          63, 74      49, 47      118, 130
+//    96 rows             46, 34          90, 74      62, 48      167, 134
+//   128 rows             56, 35         112, 76      77, 49      208, 137
+constexpr int kTcRows = 80;
 
 template <int D, int NT>
 int launch_few(cudaStream_t s, const AttnArgs& a) {

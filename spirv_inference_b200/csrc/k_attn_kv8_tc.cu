@@ -28,10 +28,10 @@
 // of q and p are added.
 //
 // Four prompts of 777 to 1024 tokens onto 0 to 1000, 32 heads of 64 on 4 kv
-// heads: 172 us, 0.34 PFLOP/s of fp16 products, the weights another 136.  What
-// bounds it: the softmax warps' instructions, about 9 a score, which issue in
-// 37 % of the cycles: two CTAs an SM (D = 64) are two such warps a scheduler, too
-// few to hide their waits for S and for the tensor memory.
+// heads: 140 us, 0.41 PFLOP/s of fp16 products, the weights another 102.  What
+// bounds it: the softmax warps' instructions, about 9 a score; two CTAs an SM (D
+// = 64) are two such warps a scheduler, which wait for each other's issue slots
+// and for the tensor memory.
 #include <cooperative_groups.h>
 #include <cuda.h>
 
@@ -470,8 +470,8 @@ __device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& 
     return mb_wait(&aux.empty[slot], ((m >> 2) & 1) ^ 1, &aux.abort_flag, &g_at_status, kWaitNs,
                    64);
   };
-  // (Apart from the others, whose code cost this loop its registers: 172
-  // against 132 us over four prompts.)
+  // (Apart from the others, whose code cost this loop its registers: 40 us of
+  // 172 over four prompts.)
   // Tiles of closed blocks only, each one's bytes on their way while the one
   // before drains.
   const int whole = max(0, min(u.tiles, u.closed / kTile - u.first));
@@ -832,8 +832,9 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
 // TMEM, issue its products themselves and add exp(score - lse) over its rows, a
 // key a thread: while one waits for its products, the other adds.  The row
 // tiles are dealt to a cluster's CTAs, whose sums are added in order.  About 3
-// instructions a score, and 4 a value of q, issued in 42 % of the cycles.
-// (Clusters of 2 and 8 in place of 4: 141 and 162 us against 137.)
+// instructions a score, and 4 a value of q.  Four prompts as above: 102 us (one
+// group adding and two converting: 106; clusters of 2 and 8 in place of 4, when
+// this took 137: 141 and 162).
 constexpr int kWeightCluster = 4, kKeys = 128, kWeightThreads = 384;
 
 struct WeightAux {
@@ -1082,7 +1083,7 @@ int launch_tc(cudaStream_t s, const AttnArgs& a) {
   const int64_t row_tiles = ceil_div((int64_t)a.T * (a.Hq / a.c.kv_heads), kRows);
   // Few rows: their keys go to the CTAs of a cluster, as long as there are SMs
   // without work and four tiles each.  16 tokens of 4 sequences of 300 to 1500,
-  // 4 kv heads of 64, with weights: 42 us, 63 without a cluster.
+  // 4 kv heads of 64, with weights: 42 us, 63 without a cluster (now 35).
   const int64_t units = row_tiles * a.c.kv_heads * a.c.batch;
   int cluster = 1;
   while (cluster < kMaxSplit && units * cluster * 2 <= S::kBlocks * kNumSms &&

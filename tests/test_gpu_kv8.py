@@ -253,6 +253,14 @@ def test_attend_few_long_sequences(g, B, Hkv, G, D, T, lens):
     s.check_attention(d_q, q, lens)
 
 
+@pytest.mark.parametrize("T,G", [(79, 1), (80, 1), (9, 8), (10, 8), (20, 4), (27, 3)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attend_from_few_rows_to_many(g, T, G, D):
+    s = Setup(g, 2, 1, G, D, 512, 32, seed=T, lens=[370, 33])
+    d_q, q = s.append(T, [T, T - 1])
+    s.check_attention(d_q, q, [370, 33])
+
+
 @pytest.mark.parametrize("T,G,D,blk,lens,scale", [
     (300, 1, 64, 128, [0, 200], None), (400, 2, 64, 16, [3, 100], -0.1),
     (150, 6, 128, 32, [350, 0], -0.07), (64, 2, 64, 64, [440, 448], 0.0)])
