@@ -557,6 +557,57 @@ def _attend_steps(s):
     return out.download()
 
 
+def test_chunks_captured_on_two_streams(gpu):
+    """Prompts taken in chunks of many rows: two graphs at once, of 64 and 128
+    values a head, each a captured chunk replayed while its lengths grow, equal
+    to the same calls one by one."""
+    T, S, Hkv, G = 24, 512, 2, 8
+    Hq = Hkv * G
+
+    class Run:
+        def __init__(self, g, D):
+            self.s, self.D = Setup(g, 2, Hkv, G, D, S, 32, lens=[5, 130], seed=D), D
+            ld = (Hq + 2 * Hkv) * D
+            self.qkv, self.q, self.out = (g.alloc((2 * T, n)) for n in (ld, Hq * D, Hq * D))
+            self.lse, self.w = g.alloc((2 * T, Hq)), g.alloc((2, Hkv, S))
+            g.zero(self.w)
+            self.xs = np.random.default_rng(D).standard_normal((6, 2 * T, ld)).astype(np.float32)
+
+        def step(self):
+            s, g = self.s, self.s.g
+            g.rope_kv8_append(self.qkv, self.qkv.shape[1], s.cos, s.sin, s.pos, self.q, s.cache,
+                              q_len=T, q_heads=Hq)
+            g.attention_kv8(self.q, s.cache, self.out, q_len=T, q_heads=Hq, scale=self.D ** -0.5,
+                            lse=self.lse, weights=self.w)
+            g.kv8_advance(s.cache, s.pos, q_len=T)
+
+        def results(self):
+            return [t.download() for t in (self.out, self.lse, self.w, self.s.cache.lens)]
+
+    alone = []
+    for D in (64, 128):
+        with Graph(gpu) as g:
+            r = Run(g, D)
+            for x in r.xs:
+                r.qkv.upload(x)
+                r.step()
+            alone.append(r.results())
+    with Graph(gpu) as g1, Graph(gpu) as g2:
+        runs = [Run(g1, 64), Run(g2, 128)]
+        for r in runs:
+            r.s.g.capture_begin()
+            r.step()
+            r.s.g.capture_end()
+        for i in range(6):
+            for r in runs:
+                r.qkv.upload(r.xs[i])
+            for r in runs:
+                r.s.g.replay()
+        for r, want in zip(runs, alone):
+            for x, y in zip(r.results(), want):
+                assert np.isfinite(y).all() and np.array_equal(x, y)
+
+
 # -- decoder ------------------------------------------------------------------
 def _logits_match(dec, cfg, W, prompt, toks, blk, **kw):
     rope = llama.rope_tables(cfg, max(cfg.max_seq, prompt.shape[1] + toks.shape[1]))
