@@ -344,6 +344,36 @@ def test_long_cache_offsets_pass_32_bits(g):
             assert np.abs(o[b, h] - want[0, 0]).max() <= 1e-5
 
 
+def test_long_cache_offsets_many_rows(g):
+    """The same, for the chunk itself: its attention, weights and read-back."""
+    B, Hkv, D, S, blk, T = 3, 8, 128, 1 << 20, 32, 100
+    new = [100, 3, 95]
+    s = Setup.__new__(Setup)
+    s.g, s.B, s.Hkv, s.G, s.D, s.S, s.blk, s.Hq = g, B, Hkv, 1, D, S, blk, Hkv
+    s.rng = np.random.default_rng(2)
+    s.cache = g.kv8_cache(B, Hkv, S, D, block=blk)
+    s.np = [[(N.Cache(128, blk, D), N.Cache(128, blk, D)) for _ in range(Hkv)] for _ in range(B)]
+    s.rows, s.tables = 256, _rope(256, D)
+    s.cos, s.sin = (g.tensor(t) for t in s.tables)
+    s.pos = g.tensor(np.zeros(B, np.int32), np.int32)
+    d_q, q = s.append(T, new)
+    out, lse, w = g.alloc((B * T, Hkv, D)), g.alloc((B * T, Hkv)), g.alloc((B, Hkv, S))
+    g.attention_kv8(d_q, s.cache, out, q_len=T, q_heads=Hkv, scale=0.1, new_lens=s.d_new, lse=lse,
+                    weights=w)
+    k, v = g.alloc((B, Hkv, 96, D)), g.alloc((B, Hkv, 96, D))
+    g.kv8_read(s.cache, k, v, count=96, q_len=T, new_lens=s.d_new)
+    o, got_k = out.download().reshape(B, T, Hkv, D), k.download()
+    last = w.view((S,), (B * Hkv - 1) * S).download()
+    for b in range(B):
+        n = new[b]
+        for h in range(Hkv):
+            K, V = (c.values() for c in s.np[b][h])
+            want, _, weights = N.attend(q[b, :n, h:h + 1], K, V, 0, 0.1)
+            assert np.abs(o[b, :n, h] - want[:, 0]).max() <= 1e-5
+            assert np.array_equal(got_k[b, h, :min(n, 96)], K[:96].astype(np.float32))
+    assert np.abs(last[:new[-1]] - weights).max() <= 1e-4
+
+
 def test_runs_are_equal_to_the_bit(g):
     for T in (1, 40):
         s = Setup(g, 4, 2, 8, 64, 1024, 32, lens=[900, 10, 512, 333])
