@@ -129,6 +129,12 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
+// After a wait for loads: their values are used behind it, not before.
+template <int N>
+__device__ __forceinline__ void settled(float (&v)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) asm volatile("" : "+f"(v[e]));
+}
 // Barrier of so many threads; whether all of them came with `ok`.
 __device__ __forceinline__ bool vote(int id, int threads, bool ok) {
   uint32_t r;
@@ -576,6 +582,7 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
     for (int c = 0; c < D / 32; ++c) {
       float v[32];
       tmem_ld_32x32(lanes + 2 * kTile + (tile & 1) * D + c * 32, v);
+      settled(v);
 #pragma unroll
       for (int e = 0; e < 32; e += 2) {
         const float2 r = fma2(make_float2(o[c * 32 + e], o[c * 32 + e + 1]),
@@ -605,6 +612,7 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
     for (int c = 0; c < kTile / 32; ++c)
       tmem_ld_32x32_async(t_s + c * 32, reinterpret_cast<uint32_t(&)[32]>(v[c * 32]));
     tmem_wait_ld();
+    settled(v);
     float f[kGroups], mt = -INFINITY;
     if (mask) {
 #pragma unroll
@@ -1020,6 +1028,7 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
         for (int c = 0; c < kRows / 32; ++c) {
           float v[32];
           tmem_ld_32x32(tmem + s * kRows + lanes + c * 32, v);
+          settled(v);
           float2 part = make_float2(0.f, 0.f);
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
