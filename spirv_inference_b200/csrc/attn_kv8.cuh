@@ -31,6 +31,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 constexpr float kPUp = 32768.0f;   // 2^15
+// v scales are taken against a reference of at least this: kPUp over it, and it
+// over kPUp, are normal numbers (a smaller one's quotient would be infinite, and
+// times values of zero NaN).
+constexpr float kMinRef = 0x1p-111f;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;

@@ -341,9 +341,9 @@ __device__ __forceinline__ void products(float (&c)[NT][4], const Frag<D>& f,
 template <int D, int NT>
 struct Running {
   float m[NT], l[NT], o[NT][D / 16][4];   // o in units of `ref` / 2^15
-  float ref;                              // the largest v scale so far
+  float ref;                              // the largest v scale so far, or kMinRef
   __device__ __forceinline__ void init() {
-    ref = 0.0f;
+    ref = kMinRef;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       m[n] = -INFINITY;
@@ -422,7 +422,7 @@ __device__ __forceinline__ float share_of(Running<D, NT>& run, float largest,
     }
     run.ref = largest;
   }
-  return run.ref > 0.0f ? kPUp / run.ref : 0.0f;
+  return kPUp / run.ref;
 }
 
 // O^T += V^T P^T over KT int8 tiles; c: exp2(score - m), zero where MASK hides.

@@ -1,0 +1,144 @@
+"""Attention over the 8-bit cache on values of unlike sizes, each row against
+bounds of its own: what a row does not see, or hardly weighs, takes no part in
+its accuracy."""
+import numpy as np
+import pytest
+
+import _kv8_np as N
+from spirv_inference_b200.graph import Graph
+from test_gpu_kv8 import Setup
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def g(gpu):
+    with Graph(gpu) as graph:
+        yield graph
+
+
+def _filled(g, lens, T, change, *, Hkv=2, G=8, D=64, S=512, blk=32, seed=0, new=None):
+    """A cache of lens[b] tokens and the queries of T new ones.  `change` edits
+    the tokens [B][max(lens) + T][heads q, k, v][D]; sequence b has slot i of them
+    at i."""
+    B = len(lens)
+    s = Setup(g, B, Hkv, G, D, S, blk, seed=seed)
+    x = s.rng.standard_normal((B, max(lens) + T, Hkv * (G + 2), D)).astype(np.float32)
+    change(x, Hkv * G, Hkv)
+    if max(lens):
+        s.append(max(lens), lens, qkv=np.ascontiguousarray(x[:, :max(lens)]).reshape(B, -1, x[0, 0].size))
+        s.advance(max(lens), lens)
+    last = np.stack([x[b, n:n + T] for b, n in enumerate(lens)])
+    d_q, q = s.append(T, new, qkv=np.ascontiguousarray(last).reshape(B, T, -1))
+    return s, d_q, q
+
+
+def _bounds(q, K, V, tops, len0, scale):
+    """What the rows q [T][G][D] may be off by: out, lse, weights.  K, V [n][D],
+    tops [n]: the largest key value of a slot's closed block, or of an open slot.
+
+    A score: an element of q, or of an open key, has 22 bits (both of them, and
+    the product of their last halves left out: 3 2^-22) or, with few rows, 2^-30 of
+    the row's largest; D + 8 sums that may be cut, 2^-23 each of sum |q k|; a
+    key of a block may carry 2^-30 of the row's largest times the block's.  An
+    exponent: the score, the largest score and their difference rounded.  A
+    weight: that, exp2 and two halves of 11 bits (2^-20), and, held beside
+    the tile's largest, 2^-40 of a value.  Sums: 64 cut ones of a tile, and one
+    a tile."""
+    T, G, D = q.shape
+    n = len(K)
+    q, aK, aV = q.astype(np.float64), np.abs(K), np.abs(V)
+    sc = np.einsum("tgd,sd->tgs", q, K) * scale
+    qk = np.einsum("tgd,sd->tgs", np.abs(q), aK)
+    ds = abs(scale) * (qk * (3 * 2.0 ** -22 + (D + 8) * 2.0 ** -23)
+                       + np.abs(q).max(-1)[..., None] * (aK.sum(-1) + tops) * 2.0 ** -30)
+    out, lse, w = np.zeros((T, G, D)), np.zeros((T, G)), np.zeros(n)
+    for t in range(T):
+        m = len0 + t + 1
+        s, d, v = sc[t, :, :m], ds[t, :, :m], aV[:m]
+        top = s.max(-1, keepdims=True)
+        e = np.exp(s - top)
+        p = e / e.sum(-1, keepdims=True)
+        z = top[:, 0] + np.log(e.sum(-1))
+        d = np.expm1(d + (np.abs(s) + np.abs(top)) * 2.0 ** -22)
+        all_d = (p * d).sum(-1, keepdims=True) + (m / 16 + 64) * 2.0 ** -24
+        assert all_d.max() < 0.1
+        rel = (d + all_d) / (1 - all_d) + 2.0 ** -20
+        out[t] = (p * (rel + 64 * 2.0 ** -23 + (m / 16) * 2.0 ** -24)) @ v
+        out[t] += m * 2.0 ** -40 * v.max() + 2.0 ** -140
+        lse[t] = all_d[:, 0] / (1 - all_d[:, 0]) + 2.0 ** -21 * (1 + np.abs(z))
+        w[:m] += (p * (rel + np.abs(z)[:, None] * 2.0 ** -22)).sum(0) + G * 2.0 ** -120
+    return out, lse, w
+
+
+def _check(s, d_q, q, len0, scale=None):
+    B, T, G, D, Hq, S = s.B, s.T, s.G, s.D, s.Hq, s.S
+    scale = D ** -0.5 if scale is None else scale
+    out, lse = s.g.tensor(np.zeros((B * T, Hq, D), np.float32)), s.g.tensor(
+        np.zeros((B * T, Hq), np.float32))
+    w0 = s.rng.uniform(0, 1, (B, s.Hkv, S)).astype(np.float32)
+    w = s.g.tensor(w0)
+    s.g.attention_kv8(d_q, s.cache, out, q_len=T, q_heads=Hq, scale=scale, new_lens=s.d_new,
+                      lse=lse, weights=w)
+    o, z, wd = out.download().reshape(B, T, Hq, D), lse.download().reshape(B, T, Hq), w.download()
+    for b in range(B):
+        n = s.new[b]
+        for h in range(s.Hkv):
+            hs = slice(h * G, (h + 1) * G)
+            kc, K, V = s.np[b][h][0], *(c.values() for c in s.np[b][h])
+            tops = 127 * kc.row_scales().astype(np.float64)
+            ro, rz, rw = N.attend(q[b, :n, hs], K, V, len0[b], scale)
+            bo, bz, bw = _bounds(q[b, :n, hs], K, V, tops, len0[b], scale)
+            for what, err, bound in (("out", np.abs(o[b, :n, hs] - ro), bo),
+                                     ("lse", np.abs(z[b, :n, hs] - rz), bz)):
+                worst = np.unravel_index(np.argmax(np.where(np.isnan(err), np.inf, err / bound)),
+                                         err.shape)
+                assert np.all(err <= bound), (what, b, h, worst, err[worst], bound[worst])
+            total = len(K)
+            want = np.where(np.arange(total) < len0[b], w0[b, h, :total], 0) + rw
+            err = np.abs(wd[b, h, :total] - want)
+            bw = bw + want * 2.0 ** -22 + n * G * 2.0 ** -24 * rw
+            assert np.all(err <= bw), ("weights", b, h, np.argmax(err / bw))
+    return o, z, wd
+
+
+ROWS = [(1, 1), (1, 8), (2, 8), (5, 8), (16, 8), (24, 8)]   # new tokens, heads of a group
+
+
+def _zero(x, q, kv):
+    x[:, :, q + kv:] = 0
+
+
+def _zero_late(x, q, kv):          # the open block and what closed before it
+    x[:, 20:, q + kv:] = 0
+
+
+def _zero_early(x, q, kv):         # a zero start, in an open block too
+    x[:, :40, q + kv:] = 0
+
+
+def _zero_head(x, q, kv):
+    x[:, :, q + kv] = 0
+
+
+def _tiny(size):
+    def change(x, q, kv):
+        x[:, :, q + kv:] *= np.float32(size)
+    return change
+
+
+def _tiny_beside(x, q, kv):        # blocks of 1e-33, of 1 and of 1e-37 in turn
+    at = np.arange(x.shape[1]) // 32 % 3
+    x[:, :, q + kv:] *= np.array([1e-33, 1, 1e-37], np.float32)[at][None, :, None, None]
+
+
+@pytest.mark.parametrize("change", [_zero, _zero_late, _zero_early, _zero_head, _tiny(1e-33),
+                                    _tiny(3e-35), _tiny(1e-37), _tiny_beside],
+                         ids=["zero", "late", "early", "head", "1e-33", "3e-35", "1e-37", "beside"])
+@pytest.mark.parametrize("T,G", [r for r in ROWS if r[0] * r[1] < 80])
+@pytest.mark.parametrize("D", [64, 128])
+def test_few_rows_over_zero_and_tiny_values(g, D, T, G, change):
+    """Values that are zero, or so small that 2^15 over them passes fp32."""
+    lens = [0, 37, 96, 300]
+    s, d_q, q = _filled(g, lens, T, change, G=G, D=D)
+    _check(s, d_q, q, lens)
