@@ -466,10 +466,10 @@ __device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& 
     }
   };
   auto shares = [&](int s) {                 // by the first warp, lane i with group i's v_sc
-    float ref = v_sc <= kMaxFloat ? v_sc : 0.0f;
+    float ref = v_sc <= kMaxFloat ? fmaxf(v_sc, kMinRef) : kMinRef;
 #pragma unroll
     for (int o = 1; o < kGroups; o <<= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
-    if (r < kGroups) aux.share[s][r] = ref > 0.0f ? v_sc * (kPUp / ref) : v_sc;
+    if (r < kGroups) aux.share[s][r] = v_sc * (kPUp / ref);
     if (r == 0) aux.back[s] = ref * (1.0f / kPUp);
   };
   auto drained = [&](int slot, int m) {

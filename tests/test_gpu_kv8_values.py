@@ -132,13 +132,26 @@ def _tiny_beside(x, q, kv):        # blocks of 1e-33, of 1 and of 1e-37 in turn
     x[:, :, q + kv:] *= np.array([1e-33, 1, 1e-37], np.float32)[at][None, :, None, None]
 
 
-@pytest.mark.parametrize("change", [_zero, _zero_late, _zero_early, _zero_head, _tiny(1e-33),
-                                    _tiny(3e-35), _tiny(1e-37), _tiny_beside],
-                         ids=["zero", "late", "early", "head", "1e-33", "3e-35", "1e-37", "beside"])
+small = pytest.mark.parametrize(
+    "change", [_zero, _zero_late, _zero_early, _zero_head, _tiny(1e-33), _tiny(3e-35), _tiny(1e-37),
+               _tiny_beside],
+    ids=["zero", "late", "early", "head", "1e-33", "3e-35", "1e-37", "beside"])
+
+
+@small
 @pytest.mark.parametrize("T,G", [r for r in ROWS if r[0] * r[1] < 80])
 @pytest.mark.parametrize("D", [64, 128])
 def test_few_rows_over_zero_and_tiny_values(g, D, T, G, change):
     """Values that are zero, or so small that 2^15 over them passes fp32."""
+    lens = [0, 37, 96, 300]
+    s, d_q, q = _filled(g, lens, T, change, G=G, D=D)
+    _check(s, d_q, q, lens)
+
+
+@small
+@pytest.mark.parametrize("T,G", [r for r in ROWS if r[0] * r[1] >= 80])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_rows_over_zero_and_tiny_values(g, D, T, G, change):
     lens = [0, 37, 96, 300]
     s, d_q, q = _filled(g, lens, T, change, G=G, D=D)
     _check(s, d_q, q, lens)
