@@ -72,12 +72,15 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   lo = as_u32(__floats2half2_rn(d.x, d.y));
 }
 
-// 2^-e and 2^e for a largest magnitude with these bits (finite).
+// 2^-e and 2^e that take a largest magnitude with these bits (finite) to 2^14 or
+// above, below 2^15, and back.  fp16 hi + lo then hold what is 2^-39 of it or more
+// with the full 22 bits, and nothing to worse than 2^-39 of it (with the largest
+// at 1, values 1000 times smaller kept 15 bits).  Below 2^-112 it stays smaller.
 __device__ __forceinline__ void pow2_scale(uint32_t amax_bits, float& down, float& up) {
   int e = (int)(amax_bits >> 23);
-  e = e < 1 ? 1 : e > 253 ? 253 : e;
-  down = __uint_as_float((uint32_t)(254 - e) << 23);
-  up = __uint_as_float((uint32_t)e << 23);
+  e = e < 15 ? 15 : e > 253 ? 253 : e;
+  down = __uint_as_float((uint32_t)(268 - e) << 23);
+  up = __uint_as_float((uint32_t)(e - 14) << 23);
 }
 __device__ __forceinline__ uint32_t finite_abs(float x) {
   const uint32_t b = __float_as_uint(x) & 0x7fffffffu;

@@ -155,3 +155,23 @@ def test_many_rows_over_zero_and_tiny_values(g, D, T, G, change):
     lens = [0, 37, 96, 300]
     s, d_q, q = _filled(g, lens, T, change, G=G, D=D)
     _check(s, d_q, q, lens)
+
+
+def _wide(ratio):
+    """q with a channel `ratio` times the others, where the keys are zero (one
+    pair, which the rotation turns into itself)."""
+    def change(x, q, kv):
+        half = x.shape[-1] // 2
+        x[:, :, :q, [0, half]] *= np.float32(ratio)
+        x[:, :, q:q + kv, 0] = x[:, :, q:q + kv, half] = 0
+    return change
+
+
+@pytest.mark.parametrize("ratio", [300, 30000])
+@pytest.mark.parametrize("T,G", [(40, 4), (100, 1)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_rows_of_queries_with_a_wide_channel(g, D, T, G, ratio):
+    """The first rows see a key or two, so that a score's error shows as it is."""
+    lens = [0, 37, 300]
+    s, d_q, q = _filled(g, lens, T, _wide(ratio), G=G, D=D)
+    _check(s, d_q, q, lens)
