@@ -18,8 +18,8 @@
 // round towards zero, so a few tiles' products are added to the running
 // output in fp32.
 //
-// Rows of the tail are fp32: both operands are split into fp16 hi + lo,
-// scaled by powers of two, three products each.
+// Rows of the tail are fp32: both operands are split into fp16 hi + lo, each row
+// scaled by a power of two of its own, three products each.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -503,46 +503,47 @@ __device__ __forceinline__ void add_values(Running<D, NT>& run, const Frag<D> (&
         run.o[n][i][e] = fmaf(run.o[n][i][e], corr[n][e & 1], o[n][i][e]);
 }
 
-// Scores of one 16-key tile of the tail: fp32 rows, both operands split; c f as
-// for weigh().  The A operand's rows are q hi and q lo.  q: row g of each 8
-// (null: none).
+// Scores of one 16-key tile of the tail, in units of log 2: fp32 rows, both
+// operands split, each row and each key by its own power of two.  The A operand's
+// rows are q hi and q lo.  q: row g of each 8 (null: none).
 template <int D, int NT>
-__device__ __forceinline__ void tail_products(float (&c)[1][NT][4], float (&f)[1][NT],
-                                              const Keys<D>& kv, const float* const (&q)[NT],
-                                              float scale, int jb, int total, int g, int t) {
+__device__ __forceinline__ void tail_products(float (&c)[1][NT][4], const Keys<D>& kv,
+                                              const float* const (&q)[NT], float scale, int jb,
+                                              int total, int g, int t) {
   const int blk_mask = (1 << kv.shift) - 1;
   uint32_t kh[2][D / 16][2], kl[2][D / 16][2];   // keys key_at(g), + 8
-  float up_k, down;
-  {
-    float x[2][D / 64][16];
+  float up_k[4];                                 // of keys key_of(0 .. 3)
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    float x[D / 64][16], down, up;
     uint32_t mx = 0;
+    const int j = jb + key_at(g) + 8 * r;
+    const float* row = kv.kt + (int64_t)(j & blk_mask) * D + 16 * t;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int j = jb + key_at(g) + 8 * r;
-      const float* row = kv.kt + (int64_t)(j & blk_mask) * D + 16 * t;
+    for (int h = 0; h < D / 64; ++h)
 #pragma unroll
-      for (int h = 0; h < D / 64; ++h)
+      for (int i = 0; i < 4; ++i) {
+        const float4 v = j < total ? *(reinterpret_cast<const float4*>(row + 64 * h) + i)
+                                   : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[h][4 * i] = v.x;
+        x[h][4 * i + 1] = v.y;
+        x[h][4 * i + 2] = v.z;
+        x[h][4 * i + 3] = v.w;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float4 v = j < total ? *(reinterpret_cast<const float4*>(row + 64 * h) + i)
-                                     : make_float4(0.f, 0.f, 0.f, 0.f);
-          x[r][h][4 * i] = v.x;
-          x[r][h][4 * i + 1] = v.y;
-          x[r][h][4 * i + 2] = v.z;
-          x[r][h][4 * i + 3] = v.w;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mx = max(mx, finite_abs(x[r][h][4 * i + e]));
-        }
-    }
-    pow2_scale(__reduce_max_sync(0xffffffffu, mx), down, up_k);
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const int h = k / 4, i = 4 * (k % 4);
-        split2(x[r][h][i] * down, x[r][h][i + 1] * down, kh[r][k][0], kl[r][k][0]);
-        split2(x[r][h][i + 2] * down, x[r][h][i + 3] * down, kh[r][k][1], kl[r][k][1]);
+        for (int e = 0; e < 4; ++e) mx = max(mx, finite_abs(x[h][4 * i + e]));
       }
+    mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    pow2_scale(mx, down, up);
+    // column 2t of the products is key key_at(2t)
+    up_k[2 * r] = __shfl_sync(0xffffffffu, up, t * 8);
+    up_k[2 * r + 1] = __shfl_sync(0xffffffffu, up, t * 8 + 4);
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      const int h = k / 4, i = 4 * (k % 4);
+      split2(x[h][i] * down, x[h][i + 1] * down, kh[r][k][0], kl[r][k][0]);
+      split2(x[h][i + 2] * down, x[h][i + 3] * down, kh[r][k][1], kl[r][k][1]);
+    }
   }
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -563,11 +564,10 @@ __device__ __forceinline__ void tail_products(float (&c)[1][NT][4], float (&f)[1
         mma16816(s[r], a, kh[r][k][0], kh[r][k][1]);
       }
     }
+    up *= fabsf(scale) * kLog2e;
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) c[0][n][2 * r + e] = s[r][e] + s[r][e + 2];
-    f[0][n] = up * up_k * (fabsf(scale) * kLog2e);
+    for (int e = 0; e < 4; ++e)
+      c[0][n][e] = (s[e >> 1][e & 1] + s[e >> 1][(e & 1) + 2]) * up * up_k[e];
   }
 }
 
@@ -590,18 +590,19 @@ __device__ __forceinline__ void tail_tile(Running<D, NT>& run, const Keys<D>& kv
                                           const int (&last)[NT], int jb, int total, int g,
                                           int t) {
   const int blk_mask = (1 << kv.shift) - 1;
-  float c[1][NT][4], f[1][NT], corr[NT][2];
-  tail_products<D, NT>(c, f, kv, q, scale, jb, total, g, t);
+  float c[1][NT][4], one[1][NT], corr[NT][2];
+  tail_products<D, NT>(c, kv, q, scale, jb, total, g, t);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) one[0][n] = 1.0f;
   const uint32_t hidden = hidden_in<NT>(jb, last, t);
-  run.template weigh<1, true>(c, f, 0.0f, corr, hidden, t);
-  // V of keys key_of(0 .. 3)
-  float y[4][D / 8];
-  uint32_t mx = 0;
-  uint32_t bad[4];
+  run.template weigh<1, true>(c, one, 0.0f, corr, hidden, t);
+  // V of keys key_of(0 .. 3), each by its own power of two
+  float y[4][D / 8], up[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int j = jb + key_of(i, t);
     const float* row = kv.vt + (int64_t)(j & blk_mask) * D + D / 8 * g;
+    uint32_t mx = 0;
     bool odd = false;
 #pragma unroll
     for (int e = 0; e < D / 32; ++e) {
@@ -623,31 +624,50 @@ __device__ __forceinline__ void tail_tile(Running<D, NT>& run, const Keys<D>& kv
         mx = max(mx, __float_as_uint(u) & 0x7fffffffu);
       }
     }
-    bad[i] = __ballot_sync(0xffffffffu, odd);
+    // over the lanes that hold the key
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    float down;
+    pow2_scale(mx, down, up[i]);
+#pragma unroll
+    for (int e = 0; e < D / 8; ++e) y[i][e] *= down;
+    if (__ballot_sync(0xffffffffu, odd) >> t & 0x11111111u) up[i] = __int_as_float(0x7fc00000);
   }
-  float up_v, down;
-  pow2_scale(__reduce_max_sync(0xffffffffu, mx), down, up_v);
-  // The tile's sums are in units of up_v / 2^15, the running ones of ref / 2^15.
-  const float back = up_v * (1.0f / kPUp) * share_of<D, NT>(run, up_v, corr);
+  // The tile's sums of a row are in units of `most` / 2^15, the largest factor of
+  // the keys that it sees (others, later ones, do not matter to it), the running
+  // ones in units of ref / 2^15.
   uint32_t pf[NT][4];
+  float most[NT], all = 0.0f, back[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
+    most[n] = 0x1p-126f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      c[0][n][e] *= kPUp;
-      // some lane of those with this t holds a bad value of the key
-      if ((bad[e] >> t & 0x11111111u) && !(hidden >> (n * 4 + e) & 1u))
-        c[0][n][e] = __int_as_float(0x7fc00000);
-    }
+    for (int e = 0; e < 4; ++e)
+      if (!(hidden >> (n * 4 + e) & 1u)) most[n] = fmaxf(most[n], up[e]);
+    most[n] = fmaxf(most[n], __shfl_xor_sync(0xffffffffu, most[n], 1));
+    most[n] = fmaxf(most[n], __shfl_xor_sync(0xffffffffu, most[n], 2));
+    all = fmaxf(all, most[n]);
+    const float inv = __uint_as_float((254u << 23) - __float_as_uint(most[n]));   // exact
+#pragma unroll
+    for (int e = 0; e < 4; ++e)        // (a hidden key's factor may be NaN)
+      c[0][n][e] = hidden >> (n * 4 + e) & 1u ? 0.0f : c[0][n][e] * (up[e] * inv) * kPUp;
     p_frags(pf[n], c[0][n]);
   }
 #pragma unroll
+  for (int o = 4; o < 32; o <<= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
+  const float unit = share_of<D, NT>(run, all, corr) * (1.0f / kPUp);
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      back[n][e] = __shfl_sync(0xffffffffu, most[n], t * 8 + 4 * e) * unit;
+#pragma unroll
   for (int i = 0; i < D / 16; ++i) {
     uint32_t a[4], al[4];
-    split2(y[0][2 * i] * down, y[1][2 * i] * down, a[0], al[0]);
-    split2(y[0][2 * i + 1] * down, y[1][2 * i + 1] * down, a[1], al[1]);
-    split2(y[2][2 * i] * down, y[3][2 * i] * down, a[2], al[2]);
-    split2(y[2][2 * i + 1] * down, y[3][2 * i + 1] * down, a[3], al[3]);
+    split2(y[0][2 * i], y[1][2 * i], a[0], al[0]);
+    split2(y[0][2 * i + 1], y[1][2 * i + 1], a[1], al[1]);
+    split2(y[2][2 * i], y[3][2 * i], a[2], al[2]);
+    split2(y[2][2 * i + 1], y[3][2 * i + 1], a[3], al[3]);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float o[4] = {};
@@ -656,7 +676,7 @@ __device__ __forceinline__ void tail_tile(Running<D, NT>& run, const Keys<D>& kv
       mma16816(o, a, pf[n][0], pf[n][1]);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        run.o[n][i][e] = fmaf(run.o[n][i][e], corr[n][e & 1], back * o[e]);
+        run.o[n][i][e] = fmaf(run.o[n][i][e], corr[n][e & 1], back[n][e & 1] * o[e]);
     }
   }
 }
@@ -983,7 +1003,9 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
   for (int i = mine; closed + 16 * i < lim; i += cluster * W) {
     const float had = gathered(w_out, closed + 16 * i, len, g, t);
     float c[1][NT][4], fk[1][NT], w[4] = {};
-    tail_products<D, NT>(c, fk, kv, q_row, a.scale, closed + 16 * i, total, g, t);
+    tail_products<D, NT>(c, kv, q_row, a.scale, closed + 16 * i, total, g, t);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) fk[0][n] = 1.0f;
     add_weights<NT>(w, c, fk, 0.0f, z, hidden_in<NT>(closed + 16 * i, last, t));
     put_weights(w_out, w, had, closed + 16 * i, total, g, t);
   }
@@ -1064,7 +1086,8 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) kv8_weights_kernel(const
         } else {
           const int r = r0 + 8 * grp + g;
           const float* const row[1] = {r < rows ? a.q + row_at(r) * D : nullptr};
-          tail_products<D, 1>(c, fk, kv, row, a.scale, jb(k), total, g, t);
+          tail_products<D, 1>(c, kv, row, a.scale, jb(k), total, g, t);
+          fk[0][0] = 1.0f;
           add_weights<1>(w[k], c, fk, 0.0f, z, hidden_in<1>(jb(k), last, t));
         }
       }

@@ -71,7 +71,8 @@ def _bounds(q, K, V, tops, len0, scale):
     return out, lse, w
 
 
-def _check(s, d_q, q, len0, scale=None):
+def _check(s, d_q, q, len0, scale=None, skip=0):
+    """skip: this many of a sequence's last rows are not looked at (nor weights)."""
     B, T, G, D, Hq, S = s.B, s.T, s.G, s.D, s.Hq, s.S
     scale = D ** -0.5 if scale is None else scale
     out, lse = s.g.tensor(np.zeros((B * T, Hq, D), np.float32)), s.g.tensor(
@@ -82,11 +83,12 @@ def _check(s, d_q, q, len0, scale=None):
                       lse=lse, weights=w)
     o, z, wd = out.download().reshape(B, T, Hq, D), lse.download().reshape(B, T, Hq), w.download()
     for b in range(B):
-        n = s.new[b]
+        n = s.new[b] - skip
         for h in range(s.Hkv):
             hs = slice(h * G, (h + 1) * G)
             kc, K, V = s.np[b][h][0], *(c.values() for c in s.np[b][h])
             tops = 127 * kc.row_scales().astype(np.float64)
+            K, V, tops = (a[:len0[b] + n] for a in (K, V, tops))
             ro, rz, rw = N.attend(q[b, :n, hs], K, V, len0[b], scale)
             bo, bz, bw = _bounds(q[b, :n, hs], K, V, tops, len0[b], scale)
             for what, err, bound in (("out", np.abs(o[b, :n, hs] - ro), bo),
@@ -94,6 +96,8 @@ def _check(s, d_q, q, len0, scale=None):
                 worst = np.unravel_index(np.argmax(np.where(np.isnan(err), np.inf, err / bound)),
                                          err.shape)
                 assert np.all(err <= bound), (what, b, h, worst, err[worst], bound[worst])
+            if skip:
+                continue
             total = len(K)
             want = np.where(np.arange(total) < len0[b], w0[b, h, :total], 0) + rw
             err = np.abs(wd[b, h, :total] - want)
@@ -175,3 +179,31 @@ def test_many_rows_of_queries_with_a_wide_channel(g, D, T, G, ratio):
     lens = [0, 37, 300]
     s, d_q, q = _filled(g, lens, T, _wide(ratio), G=G, D=D)
     _check(s, d_q, q, lens)
+
+
+def _uneven(x, q, kv):             # neighbours of very different sizes
+    rng = np.random.default_rng(7)
+    x[:, :, q:q + kv] *= (10.0 ** rng.integers(-6, 1, x.shape[:2] + (kv, 1))).astype(np.float32)
+    x[:, :, q + kv:] *= (10.0 ** rng.integers(-9, 9, x.shape[:2] + (kv, 1))).astype(np.float32)
+
+
+def _giants(T, lens, first, factor):
+    """Heads `first` (k 0, v 1) of a sequence's last new token times `factor`."""
+    def change(x, q, kv):
+        for b, n in enumerate(lens):
+            x[b, n + T - 1:, q + first * kv:q + (first + 1) * kv] *= np.float32(factor)
+    return change
+
+
+FEW_OPEN = [(5, 8, 64), (5, 8, 128), (2, 8, 64), (8, 1, 64), (8, 1, 128), (9, 7, 64)]
+
+
+@pytest.mark.parametrize("T,G,D", FEW_OPEN)
+def test_few_rows_over_an_open_block_of_unlike_rows(g, T, G, D):
+    """What a later token holds does not reach the rows before it; rows next to
+    each other keep their own bits."""
+    lens = [0, 37, 96, 300, 20]
+    for change, skip in ((_uneven, 0), (_giants(T, lens, 1, 1e25), 0),
+                         (_giants(T, lens, 0, 1e18), 1)):
+        s, d_q, q = _filled(g, lens, T, change, G=G, D=D)
+        _check(s, d_q, q, lens, skip=skip)
