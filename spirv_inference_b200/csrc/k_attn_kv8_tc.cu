@@ -23,9 +23,9 @@
 // layout.  Turning bytes into fp16 leaves each four values in the order 0, 2,
 // 1, 3: q is stored in that order too, and the output comes out in it.
 //
-// A tile with rows of the tail (fp32) is two tiles: the hi parts, scaled by a
-// power of two for 16 keys, and the lo parts, whose products with the hi parts
-// of q and p are added.
+// A tile with rows of the tail (fp32) is two tiles: the hi parts, each row scaled
+// by a power of two, and the lo parts, whose products with the hi parts of q and p
+// are added.
 //
 // Four prompts of 777 to 1024 tokens onto 0 to 1000, 32 heads of 64 on 4 kv
 // heads: 140 us, 0.41 PFLOP/s of fp16 products, the weights another 102.  What
@@ -72,11 +72,15 @@ struct TcShape {
 };
 
 struct Aux {                   // of the slots
-  float k_scale[4][kGroups];   // of 16 keys
-  float v_raw[4][kGroups];
+  // A tile that every row sees in full: of 16 keys the factor of the scores and
+  // the share of the values in the tile's largest.
+  float k_scale[4][kGroups];
   float share[4][kGroups];
   float back[4];
-  alignas(16) uint8_t bad[4][kTile];   // the key's V has a NaN or an infinity (tail)
+  // The others: of each key the factors of scores and values (NaN: the key's V
+  // has a NaN or an infinity).
+  alignas(16) float k_key[4][kTile];
+  alignas(16) float v_key[4][kTile];
   uint64_t full[4], empty[4], q_full, s_ready[2], p_ready[2], done;
   uint32_t tmem;
   int abort_flag;
@@ -135,20 +139,6 @@ __device__ __forceinline__ void settled(float (&v)[N]) {
 #pragma unroll
   for (int e = 0; e < N; ++e) asm volatile("" : "+f"(v[e]));
 }
-// Barrier of so many threads; whether all of them came with `ok`.
-__device__ __forceinline__ bool vote(int id, int threads, bool ok) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.and.pred q, %2, %3, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"((uint32_t)ok), "r"(id), "r"(threads)
-      : "memory");
-  return r != 0;
-}
-
 // Of a warp that goes together, the lane that issues.
 __device__ __forceinline__ bool first_lane() { return (threadIdx.x & 31) == 0; }
 
@@ -186,6 +176,7 @@ __device__ __forceinline__ float4 finite4(float4 v, bool& odd) {
 template <int D>
 struct Unit {
   int h, b, r0, rows, len, total, closed, lim, first, tiles, G;
+  int all_see;           // the last slot that every row sees
   __device__ __forceinline__ Unit(const AttnArgs& a, int cluster) {
     G = a.Hq / a.c.kv_heads;
     // the last rows see the most keys: first, and those of all heads
@@ -200,6 +191,7 @@ struct Unit {
     total = min(len + n_new, a.c.max_seq);
     closed = total / a.c.block * a.c.block;
     lim = min(len + a.div_g(min(r0 + kRows, rows) - 1) + 1, a.c.max_seq);
+    all_see = min(len + a.div_g(r0), total - 1);
     // this CTA's tiles, `tiles` from `first` on
     const int all = (lim + kTile - 1) / kTile, rank = blockIdx.x % cluster;
     first = (int)((int64_t)all * rank / cluster);
@@ -367,59 +359,44 @@ __device__ __forceinline__ void issue_tiles(const Unit<D>& u, Aux& aux, const Is
 // ---- conversion of keys and values ------------------------------------------------
 // 16 rows of the tail, `n` of them there, as hi and lo parts of the operand's
 // rows r0 on, by a warp: a row's lanes next to each other, four loads at a time
-// (more cost the loop over closed tiles its registers), once for the largest
-// value and once more.  Returns what takes them back, a power of two.  V: a NaN
-// or an infinity becomes zero and marks its key.
+// (more cost the loop over closed tiles its registers).  Each row is scaled by a
+// power of two of its own, which goes to `factor`.  V: a NaN or an infinity
+// becomes zero and makes its key's factor NaN.
 template <int D, bool V>
-__device__ __forceinline__ float tail_group(uint8_t* hi_to, uint8_t* lo_to, int r0,
-                                            const float* rows, int n, uint8_t* bad, int lane) {
+__device__ __forceinline__ void tail_group(uint8_t* hi_to, uint8_t* lo_to, int r0,
+                                           const float* rows, int n, float* factor, int lane) {
   constexpr int L = D / 4, PER = 32 / L, N = 16 / PER;
   const int c = lane % L, r = lane / L;
-  auto load = [&](float4 (&v)[4], int from) {
+#pragma unroll 1
+  for (int from = 0; from < N; from += 4) {
+    float4 v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = (from + i) * PER + r;
       v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (row < n) v[i] = reinterpret_cast<const float4*>(rows)[row * L + c];
     }
-  };
-  uint32_t mx = 0;
-#pragma unroll 1
-  for (int from = 0; from < N; from += 4) {
-    float4 v[4];
-    load(v, from);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (V) {
-        const uint32_t all = __ballot_sync(
-            0xffffffffu, odd_bits(v[i].x) || odd_bits(v[i].y) || odd_bits(v[i].z) ||
-                             odd_bits(v[i].w));
-        if (c == 0)
-          bad[r0 + (from + i) * PER + r] = (L == 32 ? all : all >> (r * L) & 0xffffu) != 0;
-      }
-      mx = max(max(mx, finite_abs(v[i].x)),
-               max(finite_abs(v[i].y), max(finite_abs(v[i].z), finite_abs(v[i].w))));
-    }
-  }
-  float down, up;
-  pow2_scale(__reduce_max_sync(0xffffffffu, mx), down, up);
-#pragma unroll 1
-  for (int from = 0; from < N; from += 4) {
-    float4 v[4];
-    load(v, from);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      bool odd;
+      bool odd = false;
       if (V) v[i] = finite4(v[i], odd);
+      uint32_t mx = max(max(finite_abs(v[i].x), finite_abs(v[i].y)),
+                        max(finite_abs(v[i].z), finite_abs(v[i].w)));
+#pragma unroll
+      for (int o = 1; o < L; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const uint32_t who = __ballot_sync(0xffffffffu, odd);
+      float down, up;
+      pow2_scale(mx, down, up);
       uint2 hi, lo;
       split2(v[i].x * down, v[i].z * down, hi.x, lo.x);
       split2(v[i].y * down, v[i].w * down, hi.y, lo.y);
       const int to = r0 + (from + i) * PER + r;
       reinterpret_cast<uint2*>(piece<kTile>(hi_to, to, c >> 1))[c & 1] = hi;
       reinterpret_cast<uint2*>(piece<kTile>(lo_to, to, c >> 1))[c & 1] = lo;
+      if (c == 0)
+        factor[to] = (L == 32 ? who : who >> (r * L) & 0xffffu) ? __int_as_float(0x7fc00000) : up;
     }
   }
-  return up;
 }
 
 template <int D>
@@ -472,6 +449,18 @@ __device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& 
     if (r < kGroups) aux.share[s][r] = v_sc * (kPUp / ref);
     if (r == 0) aux.back[s] = ref * (1.0f / kPUp);
   };
+  // The factors of the tile's keys in closed blocks, each by its thread.
+  auto keys = [&](int s, int j0) {
+    const int key = j0 + r;
+    float k = 0.0f, v = 0.0f;
+    if (key < u.closed) {
+      const int64_t blk = ((bh * a.c.max_seq) >> shift) + (key >> shift);
+      k = __ldg(a.c.k_scale + blk);
+      v = __ldg(a.c.v_scale + blk);
+    }
+    aux.k_key[s][r] = k;
+    aux.v_key[s][r] = v <= kMaxFloat ? v : __int_as_float(0x7fc00000);
+  };
   auto drained = [&](int slot, int m) {
     return mb_wait(&aux.empty[slot], ((m >> 2) & 1) ^ 1, &aux.abort_flag, &g_at_status, kWaitNs,
                    64);
@@ -485,16 +474,15 @@ __device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& 
   int n = 0;                   // the tile's slot
   for (; n < whole; ++n) {
     const int s = n & 3;
-    if (!__all_sync(0xffffffffu, drained(s, n))) {
-      if (whole < u.tiles) vote(1, kTile, false);   // the other warp waits there
-      return;
-    }
+    if (!__all_sync(0xffffffffu, drained(s, n))) return;
     uint8_t* k_to = slots + s * S::kSlot;
     store(k_to, k_to + S::kHalf, kTile);
     if (r < 32) {
       if (r < kGroups) aux.k_scale[s][r] = k_sc;
       shares(s);
     }
+    const int j0 = (u.first + n) * kTile;
+    if (j0 + kTile - 1 > u.all_see) keys(s, j0);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mb_arrive(&aux.full[s]);
     if (n + 1 < whole) load(n + 1);
@@ -507,49 +495,32 @@ __device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& 
     load(tile);
     bool ok = drained(s, n);
     if (tail) ok = ok && drained(s2, n + 1);
-    ok = __all_sync(0xffffffffu, ok);
+    if (!__all_sync(0xffffffffu, ok)) return;
     uint8_t* k_to = slots + s * S::kSlot;
     uint8_t* v_to = k_to + S::kHalf;
     uint8_t* k_lo = slots + s2 * S::kSlot;
     uint8_t* v_lo = k_lo + S::kHalf;
-    if (ok) {
-      if (r < kGroups && (!tail || j0 + r * 16 < u.closed)) {
-        aux.k_scale[s][r] = k_sc;
-        aux.v_raw[s][r] = v_sc;
-      }
-      aux.bad[s][r] = 0;
-      store(k_to, v_to, u.closed - j0);
-      __syncwarp();
-      // Groups of 16 keys, two of the tile's four a warp: closed ones have no
-      // lo part; the others come from the tail if some row sees it.
+    keys(s, j0);
+    store(k_to, v_to, u.closed - j0);
+    __syncwarp();
+    // Groups of 16 keys, two of the tile's four a warp: closed ones have no
+    // lo part; the others come from the tail if some row sees it.
 #pragma unroll 1
-      for (int grp = r >> 5 << 1; grp < (r >> 5 << 1) + kGroups / 2; ++grp) {
-        const int key = j0 + grp * 16;
-        if (key < u.closed || !tail) {
-          if (tail || key >= u.closed)
-            for (int i = r & 31; i < D * 2; i += 32) {
-              const int row = grp * 16 + i / (D / 8), c = i % (D / 8);
-              *piece<kTile>(tail ? k_lo : k_to, row, c) = make_uint4(0, 0, 0, 0);
-              *piece<kTile>(tail ? v_lo : v_to, row, c) = make_uint4(0, 0, 0, 0);
-            }
-          continue;
-        }
-        const int64_t at = ((bh << shift) + (key & (a.c.block - 1))) * D;
-        const int rows = max(0, min(u.total - key, 16));
-        const float ku = tail_group<D, false>(k_to, k_lo, grp * 16, a.c.k_tail + at, rows, nullptr,
-                                              r & 31);
-        const float vu = tail_group<D, true>(v_to, v_lo, grp * 16, a.c.v_tail + at, rows,
-                                             aux.bad[s], r & 31);
-        if ((r & 31) == 0) {
-          aux.k_scale[s][grp] = ku;
-          aux.v_raw[s][grp] = vu;
-        }
+    for (int grp = r >> 5 << 1; grp < (r >> 5 << 1) + kGroups / 2; ++grp) {
+      const int key = j0 + grp * 16;
+      if (key < u.closed || !tail) {
+        if (tail || key >= u.closed)
+          for (int i = r & 31; i < D * 2; i += 32) {
+            const int row = grp * 16 + i / (D / 8), c = i % (D / 8);
+            *piece<kTile>(tail ? k_lo : k_to, row, c) = make_uint4(0, 0, 0, 0);
+            *piece<kTile>(tail ? v_lo : v_to, row, c) = make_uint4(0, 0, 0, 0);
+          }
+        continue;
       }
-    }
-    if (!vote(1, kTile, ok)) return;
-    if (r < 32) {
-      v_sc = r < kGroups ? aux.v_raw[s][r] : 0.0f;
-      shares(s);
+      const int64_t at = ((bh << shift) + (key & (a.c.block - 1))) * D;
+      const int rows = max(0, min(u.total - key, 16));
+      tail_group<D, false>(k_to, k_lo, grp * 16, a.c.k_tail + at, rows, aux.k_key[s], r & 31);
+      tail_group<D, true>(v_to, v_lo, grp * 16, a.c.v_tail + at, rows, aux.v_key[s], r & 31);
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mb_arrive(&aux.full[s]);
@@ -571,7 +542,6 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
   if (!wait(&aux.q_full, 0)) return false;
   const float qs = q_scale[x];
   const int last = min(u.len + a.div_g(min(u.r0 + x, u.rows - 1)), u.total - 1);
-  const int last_of_first = min(u.len + a.div_g(u.r0), u.total - 1);
   m = -INFINITY;
   l = 0.0f;
   // of the tile before, and of the one before that, whose output comes next
@@ -605,7 +575,7 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
     const uint32_t t_s = lanes + (tile & 1) * kTile;
     // The products before this tile's S are done, P V of two tiles back too.
     if (tile >= 2) take_output(tile - 2, corr2, back2);
-    const bool mask = j0 + kTile - 1 > last_of_first;
+    const bool mask = tail || j0 + kTile - 1 > u.all_see;
     const int seen = last - j0;         // the last column that the row sees
     float v[kTile];
 #pragma unroll
@@ -613,32 +583,34 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
       tmem_ld_32x32_async(t_s + c * 32, reinterpret_cast<uint32_t(&)[32]>(v[c * 32]));
     tmem_wait_ld();
     settled(v);
-    float f[kGroups], mt = -INFINITY;
+    float f[kGroups], mt = -INFINITY, most = kMinRef;
     if (mask) {
+      // Each key by its own factors; values beside the largest that the row sees
+      // (others, later ones, do not matter to it).
 #pragma unroll
-      for (int e = 0; e < kTile; ++e)
-        if (e > seen) v[e] = -INFINITY;
+      for (int e = 0; e < kTile; e += 4) {
+        const float4 kk = *reinterpret_cast<const float4*>(&aux.k_key[s][e]);
+        const float4 vk = *reinterpret_cast<const float4*>(&aux.v_key[s][e]);
+        const float ks[4] = {kk.x, kk.y, kk.z, kk.w}, vs[4] = {vk.x, vk.y, vk.z, vk.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[e + i] = e + i > seen ? -INFINITY : v[e + i] * qs * ks[i];
+          if (e + i <= seen) most = fmaxf(most, vs[i]);
+        }
+      }
     }
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
-      f[i] = aux.k_scale[s][i] * qs;
-      float most = v[i * 16];
+      f[i] = mask ? 1.0f : aux.k_scale[s][i] * qs;
+      float top = v[i * 16];
 #pragma unroll
-      for (int e = 1; e < 16; ++e) most = fmaxf(most, v[i * 16 + e]);
-      // (a factor of 0 or NaN would make NaN of -inf, which fmaxf passes over)
-      mt = fmaxf(mt, most * f[i]);
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, v[i * 16 + e]);
+      mt = fmaxf(mt, top * f[i]);
     }
     const float mn = fmaxf(m, mt), base = mn == -INFINITY ? 0.0f : mn;
     const float corr = ex2(m - base);
     m = mn;
-    bool any_bad = false;
-    if (tail) {
-#pragma unroll 1
-      for (int i = 0; i < kTile / 16; ++i) {
-        const uint4 w = reinterpret_cast<const uint4*>(aux.bad[s])[i];
-        any_bad |= (w.x | w.y | w.z | w.w) != 0;
-      }
-    }
+    const float by = kPUp / most;      // (of use where MASKED)
     float2 sum = make_float2(0.f, 0.f);
     auto weigh = [&](auto tag) {
       constexpr bool masked = decltype(tag)::value;
@@ -648,30 +620,25 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           const int k = c * 32 + e;
-          const float share = aux.share[s][k / 16];
           float2 w = fma2(make_float2(v[k], v[k + 1]), make_float2(f[k / 16], f[k / 16]),
                           make_float2(-base, -base));
           w = make_float2(ex2(w.x), ex2(w.y));
-          if (masked) {
-            if (k > seen) w.x = 0.0f;
-            if (k + 1 > seen) w.y = 0.0f;
-          }
           sum = add2(sum, w);
-          w = mul2(w, make_float2(share, share));
-          if (masked) {                // (a share may be NaN)
+          if (masked) {                // (a hidden key's factor may be NaN)
+            const float2 share = *reinterpret_cast<const float2*>(&aux.v_key[s][k]);
+            w = mul2(w, mul2(share, make_float2(by, by)));
             if (k > seen) w.x = 0.0f;
             if (k + 1 > seen) w.y = 0.0f;
-            if (any_bad) {
-              if (k <= seen && aux.bad[s][k]) w.x = __int_as_float(0x7fc00000);
-              if (k + 1 <= seen && aux.bad[s][k + 1]) w.y = __int_as_float(0x7fc00000);
-            }
+          } else {
+            const float share = aux.share[s][k / 16];
+            w = mul2(w, make_float2(share, share));
           }
           split2(w.x, w.y, p[e / 2], p[16 + e / 2]);
         }
         tmem_st_32x32(t_s + c * 32, p);
       }
     };
-    if (mask || any_bad)
+    if (mask)
       weigh(std::true_type());
     else
       weigh(std::false_type());
@@ -679,7 +646,7 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
     corr2 = corr1;
     back2 = back1;
     corr1 = corr;
-    back1 = aux.back[s];
+    back1 = mask ? most * (1.0f / kPUp) : aux.back[s];
     tmem_wait_st();
     tc_before();
     mb_arrive(&aux.p_ready[tile & 1]);

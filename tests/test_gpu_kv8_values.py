@@ -33,18 +33,22 @@ def _filled(g, lens, T, change, *, Hkv=2, G=8, D=64, S=512, blk=32, seed=0, new=
     return s, d_q, q
 
 
-def _bounds(q, K, V, tops, len0, scale):
+def _bounds(q, K, V, tops, vtops, len0, scale):
     """What the rows q [T][G][D] may be off by: out, lse, weights.  K, V [n][D],
-    tops [n]: the largest key value of a slot's closed block, or of an open slot.
+    tops, vtops [n]: the largest value of a slot's closed block, or of an open slot.
 
     A score: an element of q, or of an open key, has 22 bits (both of them, and
     the product of their last halves left out: 3 2^-22) or, with few rows, 2^-30 of
     the row's largest; D + 8 sums that may be cut, 2^-23 each of sum |q k|; a
     key of a block may carry 2^-30 of the row's largest times the block's.  An
     exponent: the score, the largest score and their difference rounded.  A
-    weight: that, exp2 and two halves of 11 bits (2^-20), and, held beside
-    the tile's largest, 2^-40 of a value.  Sums: 64 cut ones of a tile, and one
-    a tile."""
+    weight: that, exp2 and two halves of 11 bits (2^-20).  It is multiplied by
+    2^15 s / r, s its block's scale and r the largest that the row sees, and its
+    low half is a multiple of 2^-24: off by 2^-25, which times an int8 of at most
+    127 and r / 2^15 is 2^-40 of 127 r, the largest that a value of that block can
+    be (its own values may be smaller: they are only known to r / 2).  Sums: 64 cut
+    ones of a tile, and one a tile.  A row that sees a block closed around a key
+    1e18 times the others' has, by the block's term, scores to 1e9: no bound."""
     T, G, D = q.shape
     n = len(K)
     q, aK, aV = q.astype(np.float64), np.abs(K), np.abs(V)
@@ -60,13 +64,14 @@ def _bounds(q, K, V, tops, len0, scale):
         e = np.exp(s - top)
         p = e / e.sum(-1, keepdims=True)
         z = top[:, 0] + np.log(e.sum(-1))
-        d = np.expm1(d + (np.abs(s) + np.abs(top)) * 2.0 ** -22)
+        d = np.expm1(np.minimum(d + (np.abs(s) + np.abs(top)) * 2.0 ** -22, 1.0))
         all_d = (p * d).sum(-1, keepdims=True) + (m / 16 + 64) * 2.0 ** -24
-        assert all_d.max() < 0.1
-        rel = (d + all_d) / (1 - all_d) + 2.0 ** -20
+        with np.errstate(invalid="ignore"):
+            all_d = np.where(all_d < 0.1, all_d / (1 - all_d), np.inf)
+        rel = d * 1.12 + all_d + 2.0 ** -20        # (1 / 0.9 < 1.12)
         out[t] = (p * (rel + 64 * 2.0 ** -23 + (m / 16) * 2.0 ** -24)) @ v
-        out[t] += m * 2.0 ** -40 * v.max() + 2.0 ** -140
-        lse[t] = all_d[:, 0] / (1 - all_d[:, 0]) + 2.0 ** -21 * (1 + np.abs(z))
+        out[t] += m * 2.0 ** -40 * max(v.max(), vtops[:m].max()) + 2.0 ** -140
+        lse[t] = all_d[:, 0] + 2.0 ** -21 * (1 + np.abs(z))
         w[:m] += (p * (rel + np.abs(z)[:, None] * 2.0 ** -22)).sum(0) + G * 2.0 ** -120
     return out, lse, w
 
@@ -82,15 +87,17 @@ def _check(s, d_q, q, len0, scale=None, skip=0):
     s.g.attention_kv8(d_q, s.cache, out, q_len=T, q_heads=Hq, scale=scale, new_lens=s.d_new,
                       lse=lse, weights=w)
     o, z, wd = out.download().reshape(B, T, Hq, D), lse.download().reshape(B, T, Hq), w.download()
+    looked_at = of_all = 0
     for b in range(B):
         n = s.new[b] - skip
         for h in range(s.Hkv):
             hs = slice(h * G, (h + 1) * G)
-            kc, K, V = s.np[b][h][0], *(c.values() for c in s.np[b][h])
-            tops = 127 * kc.row_scales().astype(np.float64)
-            K, V, tops = (a[:len0[b] + n] for a in (K, V, tops))
+            K, V = (c.values()[:len0[b] + n] for c in s.np[b][h])
+            tops = [127 * c.row_scales().astype(np.float64)[:len0[b] + n] for c in s.np[b][h]]
             ro, rz, rw = N.attend(q[b, :n, hs], K, V, len0[b], scale)
-            bo, bz, bw = _bounds(q[b, :n, hs], K, V, tops, len0[b], scale)
+            bo, bz, bw = _bounds(q[b, :n, hs], K, V, *tops, len0[b], scale)
+            looked_at += np.isfinite(bz).sum()
+            of_all += bz.size
             for what, err, bound in (("out", np.abs(o[b, :n, hs] - ro), bo),
                                      ("lse", np.abs(z[b, :n, hs] - rz), bz)):
                 worst = np.unravel_index(np.argmax(np.where(np.isnan(err), np.inf, err / bound)),
@@ -103,6 +110,7 @@ def _check(s, d_q, q, len0, scale=None, skip=0):
             err = np.abs(wd[b, h, :total] - want)
             bw = bw + want * 2.0 ** -22 + n * G * 2.0 ** -24 * rw
             assert np.all(err <= bw), ("weights", b, h, np.argmax(err / bw))
+    assert looked_at > 0.8 * of_all
     return o, z, wd
 
 
@@ -187,11 +195,11 @@ def _uneven(x, q, kv):             # neighbours of very different sizes
     x[:, :, q + kv:] *= (10.0 ** rng.integers(-9, 9, x.shape[:2] + (kv, 1))).astype(np.float32)
 
 
-def _giants(T, lens, first, factor):
-    """Heads `first` (k 0, v 1) of a sequence's last new token times `factor`."""
+def _giants(T, lens, first, factor, at=-1):
+    """Heads `first` (k 0, v 1) of a sequence's new tokens from `at` on times `factor`."""
     def change(x, q, kv):
         for b, n in enumerate(lens):
-            x[b, n + T - 1:, q + first * kv:q + (first + 1) * kv] *= np.float32(factor)
+            x[b, n + at % T:, q + first * kv:q + (first + 1) * kv] *= np.float32(factor)
     return change
 
 
@@ -206,4 +214,15 @@ def test_few_rows_over_an_open_block_of_unlike_rows(g, T, G, D):
     for change, skip in ((_uneven, 0), (_giants(T, lens, 1, 1e25), 0),
                          (_giants(T, lens, 0, 1e18), 1)):
         s, d_q, q = _filled(g, lens, T, change, G=G, D=D)
+        _check(s, d_q, q, lens, skip=skip)
+
+
+@pytest.mark.parametrize("T,G,D,blk", [(16, 8, 64, 32), (16, 8, 128, 32), (40, 2, 64, 64),
+                                       (33, 8, 64, 16), (100, 1, 128, 16), (150, 4, 64, 128)])
+def test_many_rows_over_an_open_block_of_unlike_rows(g, T, G, D, blk):
+    """The same; and later blocks that have closed, next to those that a row sees."""
+    lens = [0, 37, 96, 300, 20]
+    for change, skip in ((_uneven, 0), (_giants(T, lens, 1, 1e25), 0),
+                         (_giants(T, lens, 1, 1e25, T // 2), 0), (_giants(T, lens, 0, 1e18), 1)):
+        s, d_q, q = _filled(g, lens, T, change, G=G, D=D, blk=blk)
         _check(s, d_q, q, lens, skip=skip)
