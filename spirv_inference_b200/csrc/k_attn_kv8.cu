@@ -7,9 +7,11 @@
 //
 // Tensor cores in fp32 accuracy, with the int8 operand as it is.
 //
-// Scores: a row of q, scaled to whole numbers of 23 bits, is three digits of 8
-// bits, and the products of each digit with the int8 keys are exact in int32
-// (mma m16n8k32); the scale of the keys' block multiplies their sum.
+// Scores: a row of q, scaled by a power of two to whole numbers below 2^30, is
+// four digits of 8 bits, and the products of each digit with the int8 keys are
+// exact in int32 (mma m16n8k32); the scale of the keys' block multiplies their
+// sum.  An element of q keeps its 24 bits down to 2^-6 of the row's largest, and
+// below that 2^-30 of it.
 //
 // Outputs: an int8 value is exact in fp16, p as fp16 hi + lo has 22 bits, and
 // each product is taken twice with fp32 sums.  p is multiplied by its block's
@@ -68,8 +70,8 @@ __device__ __forceinline__ void cluster_wait() {
 // its own running maxima and sums.
 //
 // Scores, S = Q K^T: the 16 rows of the A operand are the first and the second
-// digits of 8 rows of q (and in another product the third ones), the 8 columns
-// are keys.  Within a dot product the order of d is free, so lane (g, t) takes
+// digits of 8 rows of q, in another product the third and the fourth, the 8
+// columns are keys.  Within a dot product the order of d is free, so lane (g, t) takes
 // 16 contiguous bytes of a key, and they are its B operand as they come from
 // memory.  Lane (g, t) then holds row g and two keys of eight, which is also
 // how O^T = V^T P^T wants P as its B operand.  There the lane's V bytes of four
@@ -272,68 +274,70 @@ __device__ __forceinline__ uint32_t read_q(float (&x)[D / 64][16], bool& odd, co
 // factor that takes a product of row g to a score in units of log 2 (NaN for a
 // row with a NaN or an infinity).
 template <int D>
-__device__ __forceinline__ void load_q(uint32_t (&qd)[D / 32][3][2], float& qs, const float* row,
+__device__ __forceinline__ void load_q(uint32_t (&qd)[D / 32][4][2], float& qs, const float* row,
                                        float scale, int t) {
-  constexpr float kWhole = 8300000.0f;   // below 127 * (65536 + 256 + 1)
   float x[D / 64][16];
   bool odd;
-  const float amax = __uint_as_float(read_q<D>(x, odd, row, t));
-  float inv = amax > 1e-30f ? copysignf(kWhole / amax, scale) : 0.0f;
-  qs = amax * (1.0f / kWhole) * (fabsf(scale) * kLog2e);
+  int exp = (int)(read_q<D>(x, odd, row, t) >> 23);
+  exp = exp < 30 ? 30 : exp;             // (a row below 2^-97 stays smaller)
+  // the largest to 2^29 or above, below 2^30, and back
+  float down = __uint_as_float((uint32_t)(283 - exp) << 23);
+  if (scale < 0.0f) down = -down;
+  qs = __uint_as_float((uint32_t)(exp - 29) << 23) * (fabsf(scale) * kLog2e);
   if (odd) qs = __int_as_float(0x7fc00000);
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {     // four values: k-step i / 2, register i % 2
     uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      // digits in [-128, 127]: the bytes of v + 0x808080, less 128 each (of a
+      // digits in [-128, 127]: the bytes of v + 0x80808080, less 128 each (of a
       // NaN or an infinity, any)
-      w[e] = ((uint32_t)__float2int_rn(x[i / 4][4 * (i % 4) + e] * inv) + 0x808080u) ^ 0x808080u;
+      w[e] = ((uint32_t)__float2int_rn(x[i / 4][4 * (i % 4) + e] * down) + 0x80808080u) ^
+             0x80808080u;
     const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[2], w[3], 0x5140);
-    const uint32_t c = __byte_perm(w[0], w[1], 0x0062), d = __byte_perm(w[2], w[3], 0x0062);
-    qd[i / 2][0][i % 2] = __byte_perm(c, d, 0x5410);
-    qd[i / 2][1][i % 2] = __byte_perm(a, b, 0x7632);
-    qd[i / 2][2][i % 2] = __byte_perm(a, b, 0x5410);
+    const uint32_t c = __byte_perm(w[0], w[1], 0x7362), d = __byte_perm(w[2], w[3], 0x7362);
+    qd[i / 2][0][i % 2] = __byte_perm(c, d, 0x7632);
+    qd[i / 2][1][i % 2] = __byte_perm(c, d, 0x5410);
+    qd[i / 2][2][i % 2] = __byte_perm(a, b, 0x7632);
+    qd[i / 2][3][i % 2] = __byte_perm(a, b, 0x5410);
   }
 }
 
 // Q K^T of 8 NT rows and one int8 tile, before any scale, plus kBias: row g,
 // keys key_of(0 .. 3).
-constexpr float kBias = 12582912.0f;   // 1.5 2^23, of scores of about 2^30
+constexpr float kBias = 12582912.0f;   // 1.5 2^23, of scores of about 2^36
 template <int D, int NT>
 __device__ __forceinline__ void products(float (&c)[NT][4], const Frag<D>& f,
-                                         const uint32_t (&qd)[NT][D / 32][3][2]) {
+                                         const uint32_t (&qd)[NT][D / 32][4][2]) {
   constexpr int kOne = 0x4b400000;     // as a float, kBias; plus a sum, kBias + the sum
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
-    int hi[NT][4], lo[4];
+  for (int b = 0; b < 2; ++b)
 #pragma unroll
-    for (int s = 0; s < D / 32; ++s) {
-      const uint32_t* k = reinterpret_cast<const uint32_t*>(&f.k[b][s / 2]) + 2 * (s % 2);
+    for (int n = 0; n < NT; ++n) {
+      int hi[4], lo[4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-        if (s == 0)
-          mma16832(hi[n], qd[n][s][0][0], qd[n][s][1][0], qd[n][s][0][1], qd[n][s][1][1], k[0],
-                   k[1], 0, 0, 0, 0);
-        else
-          mma16832(hi[n], qd[n][s][0][0], qd[n][s][1][0], qd[n][s][0][1], qd[n][s][1][1], k[0],
-                   k[1], hi[n][0], hi[n][1], hi[n][2], hi[n][3]);
-      // third digits: of 8 rows and none, or of 16 rows
-      const uint32_t o0 = NT == 2 ? qd[NT - 1][s][2][0] : 0u;
-      const uint32_t o1 = NT == 2 ? qd[NT - 1][s][2][1] : 0u;
-      if (s == 0)
-        mma16832(lo, qd[0][s][2][0], o0, qd[0][s][2][1], o1, k[0], k[1], kOne, kOne, kOne, kOne);
-      else
-        mma16832(lo, qd[0][s][2][0], o0, qd[0][s][2][1], o1, k[0], k[1], lo[0], lo[1], lo[2],
-                 lo[3]);
+      for (int s = 0; s < D / 32; ++s) {
+        const uint32_t* k = reinterpret_cast<const uint32_t*>(&f.k[b][s / 2]) + 2 * (s % 2);
+        const uint32_t(&q)[4][2] = qd[n][s];
+        if (s == 0) {
+          mma16832(hi, q[0][0], q[1][0], q[0][1], q[1][1], k[0], k[1], 0, 0, 0, 0);
+          mma16832(lo, q[2][0], q[3][0], q[2][1], q[3][1], k[0], k[1], kOne, kOne, kOne, kOne);
+        } else {
+          mma16832(hi, q[0][0], q[1][0], q[0][1], q[1][1], k[0], k[1], hi[0], hi[1], hi[2], hi[3]);
+          mma16832(lo, q[2][0], q[3][0], q[2][1], q[3][1], k[0], k[1], lo[0], lo[1], lo[2], lo[3]);
+        }
+      }
+      // the last two digits with one bias of two, then all (hi: below 2^29)
+      const float2 third = add2(make_float2(__int_as_float(lo[0]), __int_as_float(lo[1])),
+                                make_float2(-kBias, -kBias));
+      const float2 low = fma2(third, make_float2(256.0f, 256.0f),
+                              make_float2(__int_as_float(lo[2]), __int_as_float(lo[3])));
+      const float2 sum = fma2(
+          make_float2((float)(hi[0] * 256 + hi[2]), (float)(hi[1] * 256 + hi[3])),
+          make_float2(65536.0f, 65536.0f), low);
+      c[n][2 * b] = sum.x;
+      c[n][2 * b + 1] = sum.y;
     }
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)      // at most 2^29 in the inner sum
-        c[n][2 * b + e] = fmaf((float)(hi[n][e] * 256 + hi[n][e + 2]), 256.0f,
-                               __int_as_float(lo[2 * n + e]));
-  }
 }
 
 // The running softmax of one warp: lane (g, t) holds maximum and sum of row g
@@ -768,7 +772,7 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
     const int tk = a.div_g(r);
     return ((int64_t)b * a.T + tk) * a.Hq + h * G + (r - tk * G);
   };
-  uint32_t qd[NT][D / 32][3][2];
+  uint32_t qd[NT][D / 32][4][2];
   float qs[NT];
   const float* q_row[NT];
 #pragma unroll
@@ -1016,7 +1020,7 @@ __global__ void __launch_bounds__(kFewMaxWarps * 32, FewShape<D, NT>::kBlocks)
 // turns 64 rows of q at a time into digits in shared memory, eight a warp.
 template <int D>
 __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) kv8_weights_kernel(const AttnArgs a) {
-  __shared__ uint32_t q_s[8][D / 32][3][2][32];
+  __shared__ uint32_t q_s[8][D / 32][4][2][32];
   __shared__ float qs_s[8][8], z_s[8][8];
   __shared__ int last_s[8][8];
   const int S = a.c.max_seq, G = a.Hq / a.c.kv_heads;
@@ -1049,13 +1053,13 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) kv8_weights_kernel(const
     {
       const int r = r0 + 8 * warp + g;
       const float* row = r < rows ? a.q + row_at(r) * D : nullptr;
-      uint32_t qd[D / 32][3][2];
+      uint32_t qd[D / 32][4][2];
       float qs;
       load_q<D>(qd, qs, row, a.scale, t);
 #pragma unroll
       for (int s = 0; s < D / 32; ++s)
 #pragma unroll
-        for (int d = 0; d < 3; ++d)
+        for (int d = 0; d < 4; ++d)
 #pragma unroll
           for (int i = 0; i < 2; ++i) q_s[warp][s][d][i][lane] = qd[s][d][i];
       if (t == 0) {
@@ -1066,11 +1070,11 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) kv8_weights_kernel(const
     }
     __syncthreads();
     for (int grp = 0; grp < 8 && r0 + 8 * grp < rows; ++grp) {
-      uint32_t qd[1][D / 32][3][2];
+      uint32_t qd[1][D / 32][4][2];
 #pragma unroll
       for (int s = 0; s < D / 32; ++s)
 #pragma unroll
-        for (int d = 0; d < 3; ++d)
+        for (int d = 0; d < 4; ++d)
 #pragma unroll
           for (int i = 0; i < 2; ++i) qd[0][s][d][i] = q_s[grp][s][d][i][lane];
       const float qs = qs_s[grp][g], z[1] = {z_s[grp][g]};

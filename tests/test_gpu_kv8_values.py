@@ -203,6 +203,29 @@ def _giants(T, lens, first, factor, at=-1):
     return change
 
 
+@pytest.mark.parametrize("ratio", [300, 30000])
+@pytest.mark.parametrize("T,G", [(40, 1), (70, 1), (3, 8), (1, 8)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_few_rows_of_queries_with_a_wide_channel(g, D, T, G, ratio):
+    """Lengths of 0 and 40 or more: the first rows see a key or two of a closed
+    block."""
+    lens = [0, 37, 300]
+    s, d_q, q = _filled(g, lens, T, _wide(ratio), G=G, D=D)
+    _check(s, d_q, q, lens)
+
+
+@pytest.mark.parametrize("T", [3, 40])
+def test_rows_of_queries_of_any_size(g, T):
+    """Each row with scores of size 1: queries of 1e-30 to 1e30 as they come, by
+    a scale that suits them."""
+    lens = [0, 37]
+    for power in (-30, -12, 0, 12, 24):
+        def change(x, q, kv, f=np.float32(10.0) ** power):
+            x[:, :, :q] *= f
+        s, d_q, q = _filled(g, lens, T, change, G=2)
+        _check(s, d_q, q, lens, scale=float(np.float32(0.1) / np.float32(10.0) ** power))
+
+
 FEW_OPEN = [(5, 8, 64), (5, 8, 128), (2, 8, 64), (8, 1, 64), (8, 1, 128), (9, 7, 64)]
 
 
