@@ -515,12 +515,10 @@ __device__ __forceinline__ void tail_products(float (&c)[1][NT][4], const Keys<D
                                               const float* const (&q)[NT], float scale, int jb,
                                               int total, int g, int t) {
   const int blk_mask = (1 << kv.shift) - 1;
-  uint32_t kh[2][D / 16][2], kl[2][D / 16][2];   // keys key_at(g), + 8
-  float up_k[4];                                 // of keys key_of(0 .. 3)
+  // All loads first: they do not move over the shuffles.
+  float x[2][D / 64][16];                        // keys key_at(g), + 8
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    float x[D / 64][16], down, up;
-    uint32_t mx = 0;
     const int j = jb + key_at(g) + 8 * r;
     const float* row = kv.kt + (int64_t)(j & blk_mask) * D + 16 * t;
 #pragma unroll
@@ -529,49 +527,60 @@ __device__ __forceinline__ void tail_products(float (&c)[1][NT][4], const Keys<D
       for (int i = 0; i < 4; ++i) {
         const float4 v = j < total ? *(reinterpret_cast<const float4*>(row + 64 * h) + i)
                                    : make_float4(0.f, 0.f, 0.f, 0.f);
-        x[h][4 * i] = v.x;
-        x[h][4 * i + 1] = v.y;
-        x[h][4 * i + 2] = v.z;
-        x[h][4 * i + 3] = v.w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx = max(mx, finite_abs(x[h][4 * i + e]));
+        x[r][h][4 * i] = v.x;
+        x[r][h][4 * i + 1] = v.y;
+        x[r][h][4 * i + 2] = v.z;
+        x[r][h][4 * i + 3] = v.w;
       }
-    mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    pow2_scale(mx, down, up);
-    // column 2t of the products is key key_at(2t)
-    up_k[2 * r] = __shfl_sync(0xffffffffu, up, t * 8);
-    up_k[2 * r + 1] = __shfl_sync(0xffffffffu, up, t * 8 + 4);
+  }
+  uint32_t a[NT][D / 16][4];
+  float up[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float y[D / 64][16], down;
+    bool odd;
+    pow2_scale(read_q<D>(y, odd, q[n], t), down, up[n]);
+    up[n] *= fabsf(scale) * kLog2e;
+    if (scale < 0.0f) down = -down;
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
       const int h = k / 4, i = 4 * (k % 4);
-      split2(x[h][i] * down, x[h][i + 1] * down, kh[r][k][0], kl[r][k][0]);
-      split2(x[h][i + 2] * down, x[h][i + 3] * down, kh[r][k][1], kl[r][k][1]);
+      split2(y[h][i] * down, y[h][i + 1] * down, a[n][k][0], a[n][k][1]);
+      split2(y[h][i + 2] * down, y[h][i + 3] * down, a[n][k][2], a[n][k][3]);
     }
   }
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    float x[D / 64][16], up, dn;
-    bool odd;
-    pow2_scale(read_q<D>(x, odd, q[n], t), dn, up);
-    if (scale < 0.0f) dn = -dn;
-    float s[2][4] = {};
+  for (int r = 0; r < 2; ++r) {
+    float down, up_k;
+    uint32_t mx = 0;
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = max(mx, finite_abs(x[r][h][i]));
+    mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    pow2_scale(mx, down, up_k);
+    float s[NT][4] = {};
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
       const int h = k / 4, i = 4 * (k % 4);
-      uint32_t a[4];
-      split2(x[h][i] * dn, x[h][i + 1] * dn, a[0], a[1]);
-      split2(x[h][i + 2] * dn, x[h][i + 3] * dn, a[2], a[3]);
+      uint32_t hi[2], lo[2];
+      split2(x[r][h][i] * down, x[r][h][i + 1] * down, hi[0], lo[0]);
+      split2(x[r][h][i + 2] * down, x[r][h][i + 3] * down, hi[1], lo[1]);
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        mma16816(s[r], a, kl[r][k][0], kl[r][k][1]);
-        mma16816(s[r], a, kh[r][k][0], kh[r][k][1]);
+      for (int n = 0; n < NT; ++n) {
+        mma16816(s[n], a[n][k], lo[0], lo[1]);
+        mma16816(s[n], a[n][k], hi[0], hi[1]);
       }
     }
-    up *= fabsf(scale) * kLog2e;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      c[0][n][e] = (s[e >> 1][e & 1] + s[e >> 1][(e & 1) + 2]) * up * up_k[e];
+    for (int e = 0; e < 2; ++e) {
+      // column 2t + e is key key_at(2t + e)
+      const float by = __shfl_sync(0xffffffffu, up_k, t * 8 + 4 * e);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        c[0][n][2 * r + e] = (s[n][e] + s[n][e + 2]) * up[n] * by;
+    }
   }
 }
 
@@ -600,42 +609,41 @@ __device__ __forceinline__ void tail_tile(Running<D, NT>& run, const Keys<D>& kv
   for (int n = 0; n < NT; ++n) one[0][n] = 1.0f;
   const uint32_t hidden = hidden_in<NT>(jb, last, t);
   run.template weigh<1, true>(c, one, 0.0f, corr, hidden, t);
-  // V of keys key_of(0 .. 3), each by its own power of two
-  float y[4][D / 8], up[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  // V of keys key_of(0 .. 3), each by its own power of two; rows of 128 are read
+  // once more for the products, piece by piece (all at once took the loop over
+  // whole groups registers).
+  auto piece = [&](int i, int e) {       // NaNs and infinities as they are
     const int j = jb + key_of(i, t);
-    const float* row = kv.vt + (int64_t)(j & blk_mask) * D + D / 8 * g;
-    uint32_t mx = 0;
-    bool odd = false;
+    return j < total ? *(reinterpret_cast<const float4*>(
+                             kv.vt + (int64_t)(j & blk_mask) * D + D / 8 * g) +
+                         e)
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  float up[4], down[4];
+  float4 y[4][D / 32];
+  uint32_t mx[4] = {}, any[4] = {};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)            // (loads do not move over shuffles)
 #pragma unroll
     for (int e = 0; e < D / 32; ++e) {
-      const float4 v = j < total ? *(reinterpret_cast<const float4*>(row) + e)
-                                 : make_float4(0.f, 0.f, 0.f, 0.f);
-      y[i][4 * e] = v.x;
-      y[i][4 * e + 1] = v.y;
-      y[i][4 * e + 2] = v.z;
-      y[i][4 * e + 3] = v.w;
-#pragma unroll
-      for (int z = 0; z < 4; ++z) {
-        // A NaN or infinity would reach rows that do not see this key: it
-        // goes into the key's weight instead, where the mask stops it.
-        float& u = y[i][4 * e + z];
-        if ((__float_as_uint(u) & 0x7f800000u) == 0x7f800000u) {
-          odd = true;
-          u = 0.0f;
-        }
-        mx = max(mx, __float_as_uint(u) & 0x7fffffffu);
-      }
+      const float4 v = y[i][e] = piece(i, e);
+      mx[i] = max(max(mx[i], finite_abs(v.x)),
+                  max(finite_abs(v.y), max(finite_abs(v.z), finite_abs(v.w))));
+      any[i] = max(max(any[i], __float_as_uint(v.x) & 0x7fffffffu),
+                   max(__float_as_uint(v.y) & 0x7fffffffu,
+                       max(__float_as_uint(v.z) & 0x7fffffffu,
+                           __float_as_uint(v.w) & 0x7fffffffu)));
     }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
     // over the lanes that hold the key
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    float down;
-    pow2_scale(mx, down, up[i]);
-#pragma unroll
-    for (int e = 0; e < D / 8; ++e) y[i][e] *= down;
-    if (__ballot_sync(0xffffffffu, odd) >> t & 0x11111111u) up[i] = __int_as_float(0x7fc00000);
+    for (int o = 4; o < 32; o <<= 1) mx[i] = max(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
+    pow2_scale(mx[i], down[i], up[i]);
+    // A NaN or infinity would reach rows that do not see this key: it goes into
+    // the key's weight instead, where the mask stops it.
+    if (__ballot_sync(0xffffffffu, any[i] >= 0x7f800000u) >> t & 0x11111111u)
+      up[i] = __int_as_float(0x7fc00000);
   }
   // The tile's sums of a row are in units of `most` / 2^15, the largest factor of
   // the keys that it sees (others, later ones, do not matter to it), the running
@@ -666,21 +674,37 @@ __device__ __forceinline__ void tail_tile(Running<D, NT>& run, const Keys<D>& kv
     for (int e = 0; e < 2; ++e)
       back[n][e] = __shfl_sync(0xffffffffu, most[n], t * 8 + 4 * e) * unit;
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
-    uint32_t a[4], al[4];
-    split2(y[0][2 * i], y[1][2 * i], a[0], al[0]);
-    split2(y[0][2 * i + 1], y[1][2 * i + 1], a[1], al[1]);
-    split2(y[2][2 * i], y[3][2 * i], a[2], al[2]);
-    split2(y[2][2 * i + 1], y[3][2 * i + 1], a[3], al[3]);
+  for (int e = 0; e < D / 32; ++e) {
+    float x[4][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float o[4] = {};
-      mma16816(o, al, pf[n][0], pf[n][1]);
-      mma16816(o, a, pf[n][2], pf[n][3]);
-      mma16816(o, a, pf[n][0], pf[n][1]);
+    for (int i = 0; i < 4; ++i) {
+      const float4 v = D == 64 ? y[i][e] : piece(i, e);
+      x[i][0] = v.x;
+      x[i][1] = v.y;
+      x[i][2] = v.z;
+      x[i][3] = v.w;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        run.o[n][i][e] = fmaf(run.o[n][i][e], corr[n][e & 1], back[n][e & 1] * o[e]);
+      for (int z = 0; z < 4; ++z)
+        x[i][z] = (__float_as_uint(x[i][z]) & 0x7f800000u) == 0x7f800000u ? 0.0f
+                                                                          : x[i][z] * down[i];
+    }
+#pragma unroll
+    for (int z = 0; z < 4; z += 2) {     // d = 4 e + z and + 1 of the lane's
+      uint32_t a[4], al[4];
+      split2(x[0][z], x[1][z], a[0], al[0]);
+      split2(x[0][z + 1], x[1][z + 1], a[1], al[1]);
+      split2(x[2][z], x[3][z], a[2], al[2]);
+      split2(x[2][z + 1], x[3][z + 1], a[3], al[3]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float o[4] = {};
+        mma16816(o, al, pf[n][0], pf[n][1]);
+        mma16816(o, a, pf[n][2], pf[n][3]);
+        mma16816(o, a, pf[n][0], pf[n][1]);
+        float(&to)[4] = run.o[n][2 * e + z / 2];
+#pragma unroll
+        for (int f = 0; f < 4; ++f) to[f] = fmaf(to[f], corr[n][f & 1], back[n][f & 1] * o[f]);
+      }
     }
   }
 }

@@ -72,13 +72,12 @@ struct TcShape {
 };
 
 struct Aux {                   // of the slots
-  // A tile that every row sees in full: of 16 keys the factor of the scores and
-  // the share of the values in the tile's largest.
-  float k_scale[4][kGroups];
+  // Closed blocks: of 16 keys the scales (NaN: V has a NaN or an infinity), and
+  // the share of V's in the tile's largest.
+  float k_scale[4][kGroups], v_scale[4][kGroups];
   float share[4][kGroups];
   float back[4];
-  // The others: of each key the factors of scores and values (NaN: the key's V
-  // has a NaN or an infinity).
+  // A tile with rows of the tail: the same of each key.
   alignas(16) float k_key[4][kTile];
   alignas(16) float v_key[4][kTile];
   uint64_t full[4], empty[4], q_full, s_ready[2], p_ready[2], done;
@@ -203,6 +202,10 @@ struct Unit {
   }
   __device__ __forceinline__ bool has_tail(int tile) const {
     return closed < lim && (first + tile + 1) * kTile > closed;
+  }
+  // how many tiles have no rows of the tail; the others come behind them
+  __device__ __forceinline__ int plain() const {
+    return closed < lim ? max(0, min(tiles, closed / kTile - first)) : tiles;
   }
 };
 
@@ -449,17 +452,9 @@ __device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& 
     if (r < kGroups) aux.share[s][r] = v_sc * (kPUp / ref);
     if (r == 0) aux.back[s] = ref * (1.0f / kPUp);
   };
-  // The factors of the tile's keys in closed blocks, each by its thread.
-  auto keys = [&](int s, int j0) {
-    const int key = j0 + r;
-    float k = 0.0f, v = 0.0f;
-    if (key < u.closed) {
-      const int64_t blk = ((bh * a.c.max_seq) >> shift) + (key >> shift);
-      k = __ldg(a.c.k_scale + blk);
-      v = __ldg(a.c.v_scale + blk);
-    }
-    aux.k_key[s][r] = k;
-    aux.v_key[s][r] = v <= kMaxFloat ? v : __int_as_float(0x7fc00000);
+  auto put_scales = [&](int s) {             // by lane i of the first warp, group i's
+    aux.k_scale[s][r] = k_sc;
+    aux.v_scale[s][r] = v_sc <= kMaxFloat ? v_sc : __int_as_float(0x7fc00000);
   };
   auto drained = [&](int slot, int m) {
     return mb_wait(&aux.empty[slot], ((m >> 2) & 1) ^ 1, &aux.abort_flag, &g_at_status, kWaitNs,
@@ -478,11 +473,9 @@ __device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& 
     uint8_t* k_to = slots + s * S::kSlot;
     store(k_to, k_to + S::kHalf, kTile);
     if (r < 32) {
-      if (r < kGroups) aux.k_scale[s][r] = k_sc;
+      if (r < kGroups) put_scales(s);
       shares(s);
     }
-    const int j0 = (u.first + n) * kTile;
-    if (j0 + kTile - 1 > u.all_see) keys(s, j0);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     mb_arrive(&aux.full[s]);
     if (n + 1 < whole) load(n + 1);
@@ -500,7 +493,17 @@ __device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& 
     uint8_t* v_to = k_to + S::kHalf;
     uint8_t* k_lo = slots + s2 * S::kSlot;
     uint8_t* v_lo = k_lo + S::kHalf;
-    keys(s, j0);
+    if (tail) {                // the keys of closed blocks
+      const int key = j0 + r;
+      if (key < u.closed) {
+        const int64_t blk = ((bh * a.c.max_seq) >> shift) + (key >> shift);
+        const float v = __ldg(a.c.v_scale + blk);
+        aux.k_key[s][r] = __ldg(a.c.k_scale + blk);
+        aux.v_key[s][r] = v <= kMaxFloat ? v : __int_as_float(0x7fc00000);
+      }
+    } else if (r < kGroups) {  // (no row sees a key behind the closed ones)
+      put_scales(s);
+    }
     store(k_to, v_to, u.closed - j0);
     __syncwarp();
     // Groups of 16 keys, two of the tile's four a warp: closed ones have no
@@ -563,19 +566,34 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
       }
     }
   };
-  int n = 0;
-  for (int tile = 0; tile < u.tiles; ++tile) {
-    const int s = n & 3, j0 = (u.first + tile) * kTile;
-    const bool tail = u.has_tail(tile);
-    // (the slot for its scales)
-    if (!wait(&aux.full[s], (n >> 2) & 1)) return false;
+  // A tile's S and the slot of its scales, `n`, are there, and O of two tiles back,
+  // which is taken.
+  auto begin = [&](int tile, int n) {
+    if (!wait(&aux.full[n & 3], (n >> 2) & 1)) return false;
     if (!wait(&aux.s_ready[tile & 1], (tile >> 1) & 1)) return false;
-    n += tail ? 2 : 1;
     tc_after();
-    const uint32_t t_s = lanes + (tile & 1) * kTile;
     // The products before this tile's S are done, P V of two tiles back too.
     if (tile >= 2) take_output(tile - 2, corr2, back2);
-    const bool mask = tail || j0 + kTile - 1 > u.all_see;
+    return true;
+  };
+  // A tile's P is there: its part of the sum, what it does to the outputs before
+  // it, and what takes its output to its size.
+  auto end = [&](int tile, float2 sum, float corr, float back) {
+    l = fmaf(l, corr, sum.x + sum.y);
+    corr2 = corr1;
+    back2 = back1;
+    corr1 = corr;
+    back1 = back;
+    tmem_wait_st();
+    tc_before();
+    mb_arrive(&aux.p_ready[tile & 1]);
+  };
+  const int plain = u.plain();
+  for (int tile = 0; tile < plain; ++tile) {
+    const int s = tile & 3, j0 = (u.first + tile) * kTile;
+    if (!begin(tile, tile)) return false;
+    const uint32_t t_s = lanes + (tile & 1) * kTile;
+    const bool mask = j0 + kTile - 1 > u.all_see;
     const int seen = last - j0;         // the last column that the row sees
     float v[kTile];
 #pragma unroll
@@ -583,36 +601,26 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
       tmem_ld_32x32_async(t_s + c * 32, reinterpret_cast<uint32_t(&)[32]>(v[c * 32]));
     tmem_wait_ld();
     settled(v);
-    float f[kGroups], mt = -INFINITY, most = kMinRef;
+    float f[kGroups], mt = -INFINITY;
     if (mask) {
-      // Each key by its own factors; values beside the largest that the row sees
-      // (others, later ones, do not matter to it).
 #pragma unroll
-      for (int e = 0; e < kTile; e += 4) {
-        const float4 kk = *reinterpret_cast<const float4*>(&aux.k_key[s][e]);
-        const float4 vk = *reinterpret_cast<const float4*>(&aux.v_key[s][e]);
-        const float ks[4] = {kk.x, kk.y, kk.z, kk.w}, vs[4] = {vk.x, vk.y, vk.z, vk.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[e + i] = e + i > seen ? -INFINITY : v[e + i] * qs * ks[i];
-          if (e + i <= seen) most = fmaxf(most, vs[i]);
-        }
-      }
+      for (int e = 0; e < kTile; ++e)
+        if (e > seen) v[e] = -INFINITY;
     }
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
-      f[i] = mask ? 1.0f : aux.k_scale[s][i] * qs;
+      f[i] = aux.k_scale[s][i] * qs;
       float top = v[i * 16];
 #pragma unroll
       for (int e = 1; e < 16; ++e) top = fmaxf(top, v[i * 16 + e]);
+      // (a factor of 0 or NaN would make NaN of -inf, which fmaxf passes over)
       mt = fmaxf(mt, top * f[i]);
     }
     const float mn = fmaxf(m, mt), base = mn == -INFINITY ? 0.0f : mn;
     const float corr = ex2(m - base);
     m = mn;
-    const float by = kPUp / most;      // (of use where MASKED)
     float2 sum = make_float2(0.f, 0.f);
-    auto weigh = [&](auto tag) {
+    auto weigh = [&](auto tag, float by) {
       constexpr bool masked = decltype(tag)::value;
 #pragma unroll
       for (int c = 0; c < kTile / 32; ++c) {
@@ -620,36 +628,89 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           const int k = c * 32 + e;
+          const float share = masked ? aux.v_scale[s][k / 16] * by : aux.share[s][k / 16];
           float2 w = fma2(make_float2(v[k], v[k + 1]), make_float2(f[k / 16], f[k / 16]),
                           make_float2(-base, -base));
           w = make_float2(ex2(w.x), ex2(w.y));
-          sum = add2(sum, w);
-          if (masked) {                // (a hidden key's factor may be NaN)
-            const float2 share = *reinterpret_cast<const float2*>(&aux.v_key[s][k]);
-            w = mul2(w, mul2(share, make_float2(by, by)));
+          if (masked) {
             if (k > seen) w.x = 0.0f;
             if (k + 1 > seen) w.y = 0.0f;
-          } else {
-            const float share = aux.share[s][k / 16];
-            w = mul2(w, make_float2(share, share));
+          }
+          sum = add2(sum, w);
+          w = mul2(w, make_float2(share, share));
+          if (masked) {                // (a share may be NaN)
+            if (k > seen) w.x = 0.0f;
+            if (k + 1 > seen) w.y = 0.0f;
           }
           split2(w.x, w.y, p[e / 2], p[16 + e / 2]);
         }
         tmem_st_32x32(t_s + c * 32, p);
       }
     };
-    if (mask)
-      weigh(std::true_type());
-    else
-      weigh(std::false_type());
-    l = fmaf(l, corr, sum.x + sum.y);
-    corr2 = corr1;
-    back2 = back1;
-    corr1 = corr;
-    back1 = mask ? most * (1.0f / kPUp) : aux.back[s];
-    tmem_wait_st();
-    tc_before();
-    mb_arrive(&aux.p_ready[tile & 1]);
+    float back;
+    if (mask) {
+      // Values are taken beside the largest that the row sees: others, later ones,
+      // do not matter to it.
+      float most = kMinRef;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i)
+        if (i * 16 <= seen) most = fmaxf(most, aux.v_scale[s][i]);
+      weigh(std::true_type(), kPUp / most);
+      back = most * (1.0f / kPUp);
+    } else {
+      weigh(std::false_type(), 0.0f);
+      back = aux.back[s];
+    }
+    end(tile, sum, corr, back);
+  }
+  // Tiles with rows of the tail, by each key's own factors: apart, and in halves
+  // with S read twice, since their code and their registers in the other loop's way
+  // took 128 to 143 us over four prompts of 1024.
+#pragma unroll 1
+  for (int tile = plain; tile < u.tiles; ++tile) {
+    const int n = 2 * tile - plain, s = n & 3, seen = last - (u.first + tile) * kTile;
+    if (!begin(tile, n)) return false;
+    const uint32_t t_s = lanes + (tile & 1) * kTile;
+    float mt = -INFINITY, most = kMinRef;
+    // a half's scores, in units of log 2
+    auto scores = [&](int c, float (&v)[32]) {
+      tmem_ld_32x32(t_s + c * 32, v);
+      settled(v);
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        v[e] = c * 32 + e > seen ? -INFINITY : v[e] * (aux.k_key[s][c * 32 + e] * qs);
+    };
+#pragma unroll 1
+    for (int c = 0; c < kTile / 32; ++c) {
+      float v[32];
+      scores(c, v);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        mt = fmaxf(mt, v[e]);
+        if (c * 32 + e <= seen) most = fmaxf(most, aux.v_key[s][c * 32 + e]);
+      }
+    }
+    const float mn = fmaxf(m, mt), base = mn == -INFINITY ? 0.0f : mn;
+    const float corr = ex2(m - base), by = kPUp / most;
+    m = mn;
+    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll 1
+    for (int c = 0; c < kTile / 32; ++c) {
+      float v[32];
+      uint32_t p[32];
+      scores(c, v);
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) {
+        const int k = c * 32 + e;
+        float2 w = make_float2(ex2(v[e] - base), ex2(v[e + 1] - base));
+        sum = add2(sum, w);
+        w.x = k > seen ? 0.0f : w.x * (aux.v_key[s][k] * by);   // (a factor may be NaN)
+        w.y = k + 1 > seen ? 0.0f : w.y * (aux.v_key[s][k + 1] * by);
+        split2(w.x, w.y, p[e / 2], p[16 + e / 2]);
+      }
+      tmem_st_32x32(t_s + c * 32, p);
+    }
+    end(tile, sum, corr, most * (1.0f / kPUp));
   }
   if (!wait(&aux.done, 0)) return false;
   tc_after();
