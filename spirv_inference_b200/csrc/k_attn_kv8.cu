@@ -1151,9 +1151,10 @@ int launch_few(cudaStream_t s, const AttnArgs& a) {
   const size_t smem = FewShape<D, NT>::smem(W);
   auto kern = attention_kv8_few_kernel<D, NT>;
   int rc;
-  if (smem > 48 * 1024 &&
-      (rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                            (int)smem),
+  // (the most that any call asks for: the attribute is the function's, and another
+  // thread's smaller one must not come between this one and the launch)
+  if ((rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            (int)FewShape<D, NT>::smem(kFewMaxWarps)),
                        "attention_kv8: smem attribute")))
     return rc;
   if ((int64_t)groups * a.c.kv_heads * kMaxCluster > INT32_MAX || a.c.batch > 65535)
