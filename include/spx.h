@@ -601,8 +601,8 @@ int spx_op_rope_kv8_append(spx_graph* g, const float* qkv, int64_t ld_qkv, const
  * [max_seq], to which each slot's attention weight, summed over the new tokens
  * and the heads of the group, is added; the new tokens' slots start from 0.
  * A NaN or an infinity in a row of q, or in a K or V row that it sees, makes
- * all of the row's output NaN, and the weights it adds; one that it does not
- * see does nothing.  At most 2^31 - 1 rows of q in all, 65535 sequences times
+ * all of the row's output NaN; in q or K, also its lse and the weights that it
+ * adds (V takes no part in those); one that it does not see does nothing.  At most 2^31 - 1 rows of q in all, 65535 sequences times
  * kv heads, and (q_len times heads of a group) times heads of a group below
  * 2^32. */
 int spx_op_attention_kv8(spx_graph* g, const float* q, const spx_kv8_cache* cache,

@@ -249,3 +249,28 @@ def test_many_rows_over_an_open_block_of_unlike_rows(g, T, G, D, blk):
                          (_giants(T, lens, 1, 1e25, T // 2), 0), (_giants(T, lens, 0, 1e18), 1)):
         s, d_q, q = _filled(g, lens, T, change, G=G, D=D, blk=blk)
         _check(s, d_q, q, lens, skip=skip)
+
+
+@pytest.mark.parametrize("T", [1, 3, 24])
+@pytest.mark.parametrize("closed", [False, True])
+def test_where_a_nan_goes(g, T, closed):
+    """In q or K: to output, lse and weights of the rows that see it; in V: to
+    their outputs alone."""
+    for part in ("q", "k", "v"):
+        n0 = 96 - T if closed else 100
+
+        def change(x, q, kv):
+            first = {"q": 0, "k": q, "v": q + kv}[part]
+            x[0, n0 + T - 1, first, 5] = np.nan
+        s, d_q, q = _filled(g, [n0], T, change, Hkv=1, G=8)
+        out, lse, w = g.alloc((T, 8, 64)), g.alloc((T, 8)), g.tensor(np.zeros((1, 1, 512), np.float32))
+        g.attention_kv8(d_q, s.cache, out, q_len=T, q_heads=8, scale=0.125, lse=lse, weights=w)
+        o, z, w = np.isnan(out.download()), np.isnan(lse.download()), np.isnan(w.download()[0, 0])
+        # rotation spreads one element over a pair; a closed block is all NaN
+        late = (np.arange(n0, n0 + T) >= 64) if closed and part != "q" else np.arange(T) == T - 1
+        want = np.repeat(late[:, None], 8, 1)
+        if part == "q":
+            want[T - 1, 1:] = False
+        assert np.array_equal(o.all(-1), want) and np.array_equal(o.any(-1), want), part
+        assert np.array_equal(z, want & (part != "v")), part
+        assert w[:n0 + T].all() == (part != "v") and w.any() == (part != "v"), part
