@@ -565,7 +565,8 @@ int spx_op_argmax_merge(spx_graph* g, const float* packed, int32_t parts, int32_
  * Slots 0 .. lens[b] - 1 of sequence b hold its tokens in order; every call
  * that takes new tokens reads lens as it was before them, and sequence b
  * brings new_lens[b] of the q_len rows that it has in q and qkv (NULL: all of
- * them; rows behind are not read, and what belongs to them is left as it was).
+ * them; rows behind have no part in anything, and what belongs to them is left as
+ * it was; attention may load theirs of q, so q has to hold q_len rows).
  * Tokens behind slot max_seq - 1 are dropped.  lens and new_lens live on the
  * device, so a step can be captured once and replayed; values outside
  * [0, max_seq] and [0, q_len] are taken as the nearest one inside.

@@ -90,6 +90,9 @@ def _check(s, d_q, q, len0, scale=None, skip=0):
     looked_at = of_all = 0
     for b in range(B):
         n = s.new[b] - skip
+        if n == 0:
+            assert np.array_equal(wd[b], w0[b])
+            continue
         for h in range(s.Hkv):
             hs = slice(h * G, (h + 1) * G)
             K, V = (c.values()[:len0[b] + n] for c in s.np[b][h])
@@ -274,3 +277,19 @@ def test_where_a_nan_goes(g, T, closed):
         assert np.array_equal(o.all(-1), want) and np.array_equal(o.any(-1), want), part
         assert np.array_equal(z, want & (part != "v")), part
         assert w[:n0 + T].all() == (part != "v") and w.any() == (part != "v"), part
+
+
+@pytest.mark.parametrize("T,G", [(5, 1), (8, 2), (9, 8), (24, 8)])
+def test_rows_behind_the_new_tokens_have_no_part(g, T, G):
+    lens, new = [0, 37, 96], [T - 3, 0, 1]
+    s, d_q, q = _filled(g, lens, T, lambda x, a, b: None, G=G, new=new)
+    got = []
+    for junk in (0.0, np.nan, np.inf, 3e38):
+        x = q.copy()
+        for b, n in enumerate(new):
+            x[b, n:] = junk
+        d_q.upload(x.reshape(d_q.shape))
+        got.append(_check(s, d_q, q, lens))
+        s.rng = np.random.default_rng(1)
+    for other in got[2:]:
+        assert all(np.array_equal(a, b) for a, b in zip(got[1], other))
