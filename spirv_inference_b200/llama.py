@@ -308,6 +308,7 @@ class LlamaDecoder:
         self._host_pos = 0     # slots in use, the same for every sequence
         self._step = 0
         self._score = {}       # buffers of score(), made when it is first called
+        self._scored = False   # the cache is score()'s, tokens() and the rest are not
 
     # -- helpers -----------------------------------------------------------
     def _torch_buf(self, t) -> DeviceTensor:
@@ -481,6 +482,7 @@ class LlamaDecoder:
             self.g.zero(self.pos)
         self._host_pos = 0
         self._step = 0
+        self._scored = False
         self._forward(self.prompt_ids, self.P)
         self._after_step()
 
@@ -488,6 +490,9 @@ class LlamaDecoder:
         """One cached decode step.  With `capture` the step (kernels and, at
         world > 1, its NCCL collectives) is recorded once as a CUDA graph and
         replayed; if recording fails the step runs eagerly from then on."""
+        if self._scored:       # goes on from score()'s text
+            self._copy(self._first_rows(), self._score["own"])
+            self._scored = False
         self._make_room(1)
         if self.capture and not self._captured:
             try:
@@ -506,6 +511,17 @@ class LlamaDecoder:
         else:
             self._forward(self.ids, 1)
         self._after_step()
+
+    def _first_rows(self) -> list:
+        """What a prefill writes of the answer: the first tokens and their log
+        probabilities."""
+        lp = self.lp.values() if self.n_top is not None else ()
+        return [t.view((self.B,) + t.shape[1:] if i else (self.B,))
+                for i, t in enumerate([self.hist, *lp])]
+
+    def _copy(self, to: list, frm: list) -> None:
+        for a, b in zip(to, frm):
+            self.g.copy_d2d(a, b.ptr, a.nbytes)
 
     def _after_step(self) -> None:
         if self.n_top is not None and self._step < self.n_new:
@@ -542,19 +558,27 @@ class LlamaDecoder:
     def score(self, prompt: np.ndarray, top_k: int = 0) -> dict:
         """Of the tokens 1 .. P - 1 of a prompt [B, P], given those before
         them: logprobs, entropy and rank [B, P - 1], and with top_k top_ids and
-        top_logprobs [B, P - 1, top_k].  Leaves the cache as a prefill does."""
+        top_logprobs [B, P - 1, top_k].  Leaves the cache as a prefill does, for
+        decode_step() to go on from; until then tokens() and token_logprobs()
+        stay the last answer's."""
         if self.world > 1:
             raise ValueError("score() runs on one rank")
         if not 0 <= top_k <= min(64, self.cfg.vocab):
             raise ValueError("top_k: 0..64 alternatives")
         g, B, P, H, V = self.g, self.B, self.P, self.cfg.hidden, self.cfg.vocab
-        self.upload_prompt(prompt)
-        self.prefill()
         M = B * P
         rows = min(M, 256)     # logits of so many positions at a time
-        buf = self._score
+        buf, first = self._score, self._first_rows()
         if not buf:
-            buf.update(logits=g.alloc((rows, V)), ids=g.alloc((M,), np.int32))
+            buf.update(logits=g.alloc((rows, V)), ids=g.alloc((M,), np.int32),
+                       answer=[g.alloc(t.shape, t.dtype) for t in first],
+                       own=[g.alloc(t.shape, t.dtype) for t in first])
+        self.upload_prompt(prompt)
+        self._copy(buf["answer"], first)
+        self.prefill()
+        self._copy(buf["own"], first)
+        self._copy(first, buf["answer"])
+        self._scored = True
         if top_k not in buf:
             buf[top_k] = self._logprob_buffers(M, top_k)
         logits, ids, lp = buf["logits"], buf["ids"], buf[top_k]
