@@ -17,6 +17,7 @@ struct AttnArgs {
   float* out;
   float* lse;
   float* weights;
+  int slot;         // of the graph's status word (many rows)
   // r / (heads of a group), exact while r times those is below 2^32
   __device__ __forceinline__ int div_g(int r) const {
     return g_mul ? (int)__umulhi((uint32_t)r, g_mul) : r;

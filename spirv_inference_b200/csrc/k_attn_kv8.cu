@@ -1204,7 +1204,7 @@ int launch_few(cudaStream_t s, const AttnArgs& a) {
 
 int launch_attention_kv8(cudaStream_t s, int64_t* cnt, const float* q, const spx_kv8_cache* c,
                          const int32_t* new_lens, int T, int Hq, float scale, float* out,
-                         float* lse, float* weights) {
+                         float* lse, float* weights, int* slot) {
   int rc = kv8_check(c, "attention_kv8");
   if (rc) return rc;
   if (T <= 0 || Hq <= 0 || Hq % c->kv_heads)
@@ -1223,7 +1223,8 @@ int launch_attention_kv8(cudaStream_t s, int64_t* cnt, const float* q, const spx
   const int64_t rows = (int64_t)T * G;
   if (rows * G > UINT32_MAX) return fail(SPX_ERR_UNSUPPORTED, "attention_kv8: too many rows");
   const uint32_t g_mul = G > 1 ? (uint32_t)(((1ull << 32) + G - 1) / G) : 0u;
-  const AttnArgs a{q, *c, new_lens, T, Hq, g_mul, scale, out, lse, weights};
+  if (rows >= kTcRows && *slot < 0) *slot = at_slot_get();
+  const AttnArgs a{q, *c, new_lens, T, Hq, g_mul, scale, out, lse, weights, *slot};
   const bool wide = rows > 8;
   // A group of rows that is alone adds its weights itself.
   const bool apart = rows > (c->head_dim == 64 ? 16 : 8);

@@ -35,6 +35,7 @@
 #include <cooperative_groups.h>
 #include <cuda.h>
 
+#include <mutex>
 #include <type_traits>
 
 #include "attn_kv8.cuh"
@@ -42,9 +43,13 @@
 
 namespace spx {
 
-__device__ int g_at_status = 0;
+// Of each graph that runs these kernels, a word that a wait which gave up sets.
+constexpr int kAtSlots = 1024;
+__device__ int g_at_status[kAtSlots];
 
 namespace {
+
+__device__ __forceinline__ int* status_of(const AttnArgs& a) { return g_at_status + a.slot; }
 
 using namespace sm100;
 namespace cg = cooperative_groups;
@@ -287,19 +292,21 @@ struct Issue {
       mma_f16_ta(to, p + (i >> 1) * 32 + PART + (i & 1) * 8,
                  from + i * (2048 >> 4), kO, MORE || i ? 1u : 0u);
   }
-  static __device__ __forceinline__ bool wait(Aux& aux, uint64_t* bar, int parity) {
-    const bool ok = mb_wait(bar, parity, &aux.abort_flag, &g_at_status, kWaitNs, 32);
+  static __device__ __forceinline__ bool wait(const AttnArgs& a, Aux& aux, uint64_t* bar,
+                                              int parity) {
+    const bool ok = mb_wait(bar, parity, &aux.abort_flag, status_of(a), kWaitNs, 32);
     if (!__all_sync(0xffffffffu, ok)) return false;
     tc_after();
     return true;
   }
   // S of a tile whose rows are in slot n (and n + 1), once they are there.
-  __device__ __forceinline__ bool tile_scores(Aux& aux, int tile, int n, bool tail) const {
+  __device__ __forceinline__ bool tile_scores(const AttnArgs& a, Aux& aux, int tile, int n,
+                                              bool tail) const {
     const int s = n & 3, s2 = (n + 1) & 3, j = tile & 1;
     const uint64_t from = k + (uint64_t)s * (S::kSlot >> 4);
     const uint64_t from2 = k + (uint64_t)s2 * (S::kSlot >> 4);
     const uint32_t to = tmem + j * kTile;
-    if (!wait(aux, &aux.full[s], (n >> 2) & 1)) return false;
+    if (!wait(a, aux, &aux.full[s], (n >> 2) & 1)) return false;
     if (first_lane()) {
       scores<false>(q_lo, from, to);
       scores<true>(q_hi, from, to);
@@ -307,7 +314,7 @@ struct Issue {
     }
     __syncwarp();
     if (!tail) return true;
-    if (!wait(aux, &aux.full[s2], ((n + 1) >> 2) & 1)) return false;
+    if (!wait(a, aux, &aux.full[s2], ((n + 1) >> 2) & 1)) return false;
     if (first_lane()) {
       scores<true>(q_hi, from2, to);
       mma_commit(&aux.s_ready[j]);
@@ -316,12 +323,13 @@ struct Issue {
     return true;
   }
   // O of a tile, once P is there.
-  __device__ __forceinline__ bool tile_values(Aux& aux, int tile, int n, bool tail) const {
+  __device__ __forceinline__ bool tile_values(const AttnArgs& a, Aux& aux, int tile, int n,
+                                              bool tail) const {
     const int s = n & 3, s2 = (n + 1) & 3, j = tile & 1;
     const uint64_t from = v + (uint64_t)s * (S::kSlot >> 4);
     const uint64_t from2 = v + (uint64_t)s2 * (S::kSlot >> 4);
     const uint32_t p = tmem + j * kTile, to = tmem + 2 * kTile + j * D;
-    if (!wait(aux, &aux.p_ready[j], (tile >> 1) & 1)) return false;
+    if (!wait(a, aux, &aux.p_ready[j], (tile >> 1) & 1)) return false;
     if (first_lane()) {
       values<16, false>(p, from, to);
       values<0, true>(p, from, to);
@@ -336,15 +344,16 @@ struct Issue {
 
 // All products of the tiles, by one lane: a commit follows all issued before it.
 template <int D>
-__device__ __forceinline__ void issue_tiles(const Unit<D>& u, Aux& aux, const Issue<D>& issue) {
-  bool ok = Issue<D>::wait(aux, &aux.q_full, 0);
+__device__ __forceinline__ void issue_tiles(const AttnArgs& a, const Unit<D>& u, Aux& aux,
+                                            const Issue<D>& issue) {
+  bool ok = Issue<D>::wait(a, aux, &aux.q_full, 0);
   int n = 0, n1 = 0, n2 = 0;   // the slots of tiles j, j - 1, j - 2
   for (int j = 0; ok && j < u.tiles + 2; ++j) {
-    if (j >= 2) ok = issue.tile_values(aux, j - 2, n2, u.has_tail(j - 2));
+    if (j >= 2) ok = issue.tile_values(a, aux, j - 2, n2, u.has_tail(j - 2));
     n2 = n1;
     if (!ok || j >= u.tiles) continue;
     const bool tail = u.has_tail(j);
-    ok = issue.tile_scores(aux, j, n, tail);
+    ok = issue.tile_scores(a, aux, j, n, tail);
     n1 = n;
     n += tail ? 2 : 1;
   }
@@ -353,7 +362,7 @@ __device__ __forceinline__ void issue_tiles(const Unit<D>& u, Aux& aux, const Is
     if (!ok) {
       // The products in flight end before shared memory and TMEM are given up.
       volatile int never = 0;
-      mb_wait(&aux.done, 0, &never, &g_at_status, 200000000ull, 64);
+      mb_wait(&aux.done, 0, &never, status_of(a), 200000000ull, 64);
     }
   }
   __syncwarp();
@@ -457,7 +466,7 @@ __device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& 
     aux.v_scale[s][r] = v_sc <= kMaxFloat ? v_sc : __int_as_float(0x7fc00000);
   };
   auto drained = [&](int slot, int m) {
-    return mb_wait(&aux.empty[slot], ((m >> 2) & 1) ^ 1, &aux.abort_flag, &g_at_status, kWaitNs,
+    return mb_wait(&aux.empty[slot], ((m >> 2) & 1) ^ 1, &aux.abort_flag, status_of(a), kWaitNs,
                    64);
   };
   // (Apart from the others, whose code cost this loop its registers: 40 us of
@@ -539,7 +548,7 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
                                               float (&o)[D], float& m, float& l) {
   const uint32_t lanes = tmem + ((uint32_t)((x >> 5) * 32) << 16);
   auto wait = [&](uint64_t* b, int parity) {
-    const bool ok = mb_wait(b, parity, &aux.abort_flag, &g_at_status, kWaitNs, 32);
+    const bool ok = mb_wait(b, parity, &aux.abort_flag, status_of(a), kWaitNs, 32);
     return __all_sync(0xffffffffu, ok) != 0;   // a warp goes on or ends as one
   };
   if (!wait(&aux.q_full, 0)) return false;
@@ -842,7 +851,7 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
       convert_tiles<D>(a, u, slots, aux, x);
     } else if (warp == 6) {
       const Issue<D> issue(sa(q_hi), sa(q_lo), sa(slots), tmem);
-      issue_tiles<D>(u, aux, issue);
+      issue_tiles<D>(a, u, aux, issue);
     }
     if (SPLIT) {                              // (of join)
       __syncwarp();
@@ -936,7 +945,7 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
   if (cluster > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   const uint32_t tmem = aux.tmem;
   auto wait = [&](uint64_t* bar, int parity) {
-    return mb_wait(bar, parity, &aux.abort_flag, &g_at_status, kWaitNs, 32);
+    return mb_wait(bar, parity, &aux.abort_flag, status_of(a), kWaitNs, 32);
   };
   float w = 0.0f;
   if (warp >= 8) {
@@ -959,7 +968,7 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
       uint8_t* to = slots + s * S::kSlot;
       auto put = [&](int r, float f) { aux.row[s][r].x = f; };
       const bool drained = mb_wait(&aux.empty[s], ((i >> 1) & 1) ^ 1, &aux.abort_flag,
-                                   &g_at_status, kWaitNs, 128);
+                                   status_of(a), kWaitNs, 128);
       if (!__all_sync(0xffffffffu, drained)) break;
       q.convert(x, 0, a.scale, to, to + S::kSlot / 2, put);
       load(i, 1);
@@ -1086,7 +1095,7 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
       // The products in flight end before shared memory and TMEM are given up.
       volatile int never = 0;
       mma_commit(&aux.done[s]);
-      mb_wait(&aux.done[s], 0, &never, &g_at_status, 200000000ull, 64);
+      mb_wait(&aux.done[s], 0, &never, status_of(a), 200000000ull, 64);
     }
     if (s == 1) aux.odd_tiles[x] = w;
   }
@@ -1196,17 +1205,39 @@ int launch_attention_kv8_tc(cudaStream_t s, const AttnArgs& a) {
   return a.c.head_dim == 64 ? launch_tc<64>(s, a) : launch_tc<128>(s, a);
 }
 
-int at_take_status() {
-  int v = 0;
-  if (cudaMemcpyFromSymbol(&v, g_at_status, sizeof(int)) != cudaSuccess) {
+namespace {
+std::mutex g_slot_mu;
+bool g_slot_used[kAtSlots - 1];
+}  // namespace
+
+int at_slot_get() {
+  std::lock_guard<std::mutex> lock(g_slot_mu);
+  for (int i = 0; i < kAtSlots - 1; ++i)
+    if (!g_slot_used[i]) {
+      g_slot_used[i] = true;
+      return i;
+    }
+  return kAtSlots - 1;         // shared by all that come later
+}
+
+void at_slot_put(int slot) {
+  std::lock_guard<std::mutex> lock(g_slot_mu);
+  if (slot >= 0 && slot < kAtSlots - 1) g_slot_used[slot] = false;
+}
+
+int at_take_status(int slot) {
+  const int from = slot < 0 ? 0 : slot, n = slot < 0 ? kAtSlots : 1;
+  int v[kAtSlots] = {}, any = 0;
+  if (cudaMemcpyFromSymbol(v, g_at_status, n * sizeof(int), from * sizeof(int)) != cudaSuccess) {
     cudaGetLastError();
     return 0;
   }
-  if (v) {
-    int zero = 0;
-    cudaMemcpyToSymbol(g_at_status, &zero, sizeof(int));
+  for (int i = 0; i < n; ++i) {
+    any |= v[i];
+    v[i] = 0;
   }
-  return v;
+  if (any) cudaMemcpyToSymbol(g_at_status, v, n * sizeof(int), from * sizeof(int));
+  return any;
 }
 
 }  // namespace spx

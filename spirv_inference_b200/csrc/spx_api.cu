@@ -591,9 +591,6 @@ static int device_status(const char* what) {
   if (tc_take_status())
     return fail(SPX_ERR_CUDA, "%s: a tensor-core pipeline wait timed out; tiles were abandoned",
                 what);
-  if (at_take_status())
-    return fail(SPX_ERR_CUDA, "%s: an attention pipeline wait timed out; rows were abandoned",
-                what);
   if (ar_take_status())
     return fail(SPX_ERR_CUDA,
                 "%s: an all-reduce waited %lld us for a peer rank and gave up; reset the "
@@ -602,7 +599,18 @@ static int device_status(const char* what) {
   return SPX_OK;
 }
 
-int spx_device_status(void) { return device_status("device status"); }
+// (Apart: other graphs' calls need not read it, nor take it from the one it is for.)
+static int attention_status(int slot, const char* what) {
+  if (at_take_status(slot))
+    return fail(SPX_ERR_CUDA, "%s: an attention pipeline wait timed out; rows were abandoned",
+                what);
+  return SPX_OK;
+}
+
+int spx_device_status(void) {
+  int rc = device_status("device status");
+  return rc ? rc : attention_status(-1, "device status");
+}
 
 int spx_kernel_count(void) { return kNumKernels; }
 const char* spx_kernel_name(int i) { return i >= 0 && i < kNumKernels ? kKernels[i].name : nullptr; }
@@ -723,6 +731,10 @@ int spx_graph_destroy(spx_graph* g) {
   if (g->cuda_exec) cudaGraphExecDestroy(g->cuda_exec);
   if (g->cuda_graph) cudaGraphDestroy(g->cuda_graph);
   if (g->own_stream) cudaStreamDestroy(g->stream);
+  if (g->at_slot >= 0) {
+    at_take_status(g->at_slot);
+    at_slot_put(g->at_slot);
+  }
   delete g;
   return SPX_OK;
 }
@@ -745,7 +757,8 @@ int spx_graph_sync(spx_graph* g) {
   SPX_G(g);
   int rc = check_cuda(cudaStreamSynchronize(g->stream), "graph execution");
   if (rc) return rc;
-  return device_status("graph execution");
+  if ((rc = device_status("graph execution")) || g->at_slot < 0) return rc;
+  return attention_status(g->at_slot, "graph execution");
 }
 
 int spx_graph_capture_begin(spx_graph* g) {
@@ -1083,7 +1096,7 @@ int spx_op_attention_kv8(spx_graph* g, const float* q, const spx_kv8_cache* cach
   SPX_G(g);
   if (!q || !cache || !out) return fail(SPX_ERR_INVALID_ARGUMENT, "attention_kv8: null");
   return launch_attention_kv8(g->stream, &g->launches, q, cache, new_lens, q_len, q_heads, scale,
-                              out, lse, weights);
+                              out, lse, weights, &g->at_slot);
 }
 
 int spx_op_kv8_read(spx_graph* g, const spx_kv8_cache* cache, const int32_t* new_lens,

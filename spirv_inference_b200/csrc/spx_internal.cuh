@@ -21,6 +21,7 @@ struct spx_graph {
   int64_t launches = 0;          // kernels launched (or replayed)
   int64_t captured_launches = 0; // kernels inside the captured CUDA graph
   int64_t capture_start = 0;
+  int at_slot = -1;              // status word of its attention, once it has run any
 };
 
 namespace spx {
@@ -232,7 +233,7 @@ int launch_rope_kv8_append(cudaStream_t s, int64_t* cnt, const float* qkv, int64
                            float* q_out, const spx_kv8_cache* c);
 int launch_attention_kv8(cudaStream_t s, int64_t* cnt, const float* q, const spx_kv8_cache* c,
                          const int32_t* new_lens, int T, int Hq, float scale, float* out,
-                         float* lse, float* weights);
+                         float* lse, float* weights, int* slot);
 int launch_kv8_read(cudaStream_t s, int64_t* cnt, const spx_kv8_cache* c, const int32_t* new_lens,
                     int q_len, const int32_t* starts, int count, float* k_out, float* v_out);
 int launch_kv8_evict(cudaStream_t s, int64_t* cnt, const spx_kv8_cache* src, const float* weights,
@@ -331,7 +332,10 @@ int launch_stem_tc(cudaStream_t s, int64_t* cnt, const float* x, const float* w_
 int launch_dw_project(cudaStream_t s, int64_t* cnt, const float* x, const float* wd,
                       const float* bd, const float* w_hi, const float* w_lo, const float* bp,
                       const float* res, float* y, const spx_dwproj_params* q, bool dry_run);
-int at_take_status();   // attention over the 8-bit cache
+// Attention over the 8-bit cache: status words, one a graph (-1: all of them).
+int at_slot_get();
+void at_slot_put(int slot);
+int at_take_status(int slot);
 int ar_take_status();
 
 // Process-wide dense-contraction path: 0 auto, 1 SIMT only, 2 tensor cores

@@ -41,3 +41,27 @@ def test_attention_of_few_rows_from_two_threads(gpu):
         t.join()
     assert not errors, errors
     assert outs == {64: True, 1024: True}
+
+
+def test_many_graphs_over_a_process(gpu):
+    """More graphs than there are status words for attention of many rows, some at
+    the same time: each syncs, and so does one that never ran it."""
+    with Graph(gpu) as other:
+        for _ in range(22):
+            graphs = [Graph(gpu) for _ in range(50)]
+            try:
+                outs = []
+                for g in graphs:
+                    c = g.kv8_cache(1, 1, 64, 64, block=32)
+                    for t in (c.k_tail, c.v_tail):
+                        t.upload(np.ones(t.shape, np.float32))
+                    q, out = g.tensor(np.ones((10, 8, 64), np.float32)), g.alloc((10, 8, 64))
+                    g.attention_kv8(q, c, out, q_len=10, q_heads=8, scale=1.0)
+                    outs.append(out)
+                for g, out in zip(graphs, outs):
+                    g.sync()
+                    assert np.all(out.download() == 1.0)
+                other.sync()
+            finally:
+                for g in graphs:
+                    g.close()
