@@ -32,8 +32,8 @@ the weight that each slot receives, and when the next step would not fit,
 every layer and head drops to its first `kv_sink`, last `kv_recent` and
 heaviest other slots, kv_keep in all; generation then goes on past max_seq.
 
-Answers: generate() gives tokens; with `logprobs` = k the decoder also keeps
-each token's log probability, rank, entropy and k alternatives
+Answers: generate() gives tokens; with `logprobs` = k (0: none; None: off) the
+decoder also keeps each token's log probability, rank, entropy and k alternatives
 (token_logprobs()), and score() gives the same for the tokens of a prompt.
 
 Weights (seeded, N(0, 0.02); norm gains 1 + N(0, 0.02)) are generated in the
@@ -226,6 +226,10 @@ class LlamaDecoder:
         elif prompt_len + n_new - 1 > cfg.max_seq:
             raise ValueError(f"prompt {prompt_len} + {n_new} new tokens exceed max_seq "
                              f"{cfg.max_seq}")
+        if logprobs is False:
+            logprobs = None
+        if logprobs is True:
+            raise ValueError("logprobs: a number of alternatives, or None")
         if logprobs is not None and (world > 1 or not 0 <= logprobs <= min(64, cfg.vocab)):
             raise ValueError("logprobs: 0..64 alternatives, on one rank")
         self.n_top = logprobs

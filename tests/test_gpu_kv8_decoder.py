@@ -40,3 +40,14 @@ def test_score_leaves_the_last_answer(gpu, kv_cache, logprobs):
         assert same(answer(), of_a)
     finally:
         dec.close()
+
+
+def test_logprobs_false_is_off(gpu):
+    cfg = llama.TINY_TEST
+    dec = llama.LlamaDecoder(cfg, llama.make_weights(cfg, 0), 1, 4, 2, device=gpu, logprobs=False)
+    try:
+        dec.generate(llama.make_prompt(cfg, 1, 4))
+        with pytest.raises(ValueError):
+            dec.token_logprobs()
+    finally:
+        dec.close()
