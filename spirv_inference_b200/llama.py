@@ -208,6 +208,8 @@ class LlamaDecoder:
         if kv_cache not in ("fp32", "int8"):
             raise ValueError(f"kv_cache {kv_cache!r}: fp32 or int8")
         self.kv8 = kv_cache == "int8"
+        if self.kv8 and cfg.head_dim not in (64, 128):
+            raise ValueError(f"kv_cache 'int8' with head_dim {cfg.head_dim}: 64 or 128")
         if self.kv8 and kv_block not in (16, 32, 64, 128):
             raise ValueError(f"kv_block {kv_block}: 16, 32, 64 or 128")
         # Slots of the int8 cache: whole blocks.
