@@ -587,7 +587,8 @@ typedef struct spx_kv8_cache {
 int spx_kv8_supported(const spx_kv8_cache* cache);
 /* RoPE as in spx_op_rope_kv_append on q and k of the new tokens, token t of
  * sequence b at position pos[b] + t (which an eviction leaves larger than its
- * slot); q written to q_out, k and v taken into the cache.  The tables have
+ * slot); q written to q_out, which shares no memory with qkv, k and v taken
+ * into the cache.  The tables have
  * table_rows rows; a position outside them gives NaN.  lens and pos are not
  * changed (spx_op_kv8_advance). */
 int spx_op_rope_kv8_append(spx_graph* g, const float* qkv, int64_t ld_qkv, const float* cos_table,

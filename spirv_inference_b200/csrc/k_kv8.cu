@@ -638,6 +638,10 @@ int launch_rope_kv8_append(cudaStream_t s, int64_t* cnt, const float* qkv, int64
     return fail(SPX_ERR_INVALID_ARGUMENT, "rope_kv8_append: bad shape");
   if (!al16(q_out))
     return fail(SPX_ERR_INVALID_ARGUMENT, "rope_kv8_append: q_out must be 16-byte aligned");
+  const uint64_t rows = (uint64_t)c->batch * T, row = (uint64_t)(Hq + 2 * c->kv_heads) * c->head_dim;
+  const uintptr_t in = (uintptr_t)qkv, out = (uintptr_t)q_out;   // one's rows, others still read
+  if (in < out + rows * Hq * c->head_dim * 4 && out < in + ((rows - 1) * ld_qkv + row) * 4)
+    return fail(SPX_ERR_INVALID_ARGUMENT, "rope_kv8_append: qkv and q_out share memory");
   AppendArgs a;
   a.qkv = qkv;
   a.ld = ld_qkv;
