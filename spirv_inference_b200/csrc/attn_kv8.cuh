@@ -27,6 +27,10 @@ struct AttnArgs {
 namespace {
 
 __device__ __forceinline__ int clamp_len(int v, int hi) { return v < 0 ? 0 : v > hi ? hi : v; }
+// len + n, at most hi, for 0 <= len <= hi and any n >= 0.
+__device__ __forceinline__ int add_len(int len, int n, int hi) {
+  return n > hi - len ? hi : len + n;
+}
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;

@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(256)
   u >>= 1;
   const int b = u / c.kv_heads, h = u - b * c.kv_heads;
   const int n = new_lens ? clamp_len(new_lens[b], q_len) : q_len;
-  const int len = min(clamp_len(c.lens[b], c.max_seq) + n, c.max_seq);
+  const int len = add_len(clamp_len(c.lens[b], c.max_seq), n, c.max_seq);
   const int closed = len / blk * blk;
   const int64_t start = starts ? starts[b] : 0;
   const KvView kv = view_of(c, b, h, is_v);
@@ -599,7 +599,7 @@ __global__ void kv8_advance_kernel(int32_t* lens, int32_t* pos, const int32_t* n
                                    int q_len, int limit) {
   for (int b = blockIdx.x * blockDim.x + threadIdx.x; b < batch; b += gridDim.x * blockDim.x) {
     const int n = new_lens ? clamp_len(new_lens[b], q_len) : q_len;
-    if (lens) lens[b] = min(clamp_len(lens[b], limit) + n, limit);
+    if (lens) lens[b] = add_len(clamp_len(lens[b], limit), n, limit);
     if (pos) pos[b] += n;
   }
 }

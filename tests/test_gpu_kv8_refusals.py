@@ -29,3 +29,23 @@ def test_new_tokens_and_rotated_queries_apart(g):
         g.rope_kv8_append(both.view((end,), qkv), 4 * 64, s.cos, s.sin, s.pos,
                           both.view((3, 2, 64), q), s.cache, q_len=3, q_heads=2)
     g.sync()
+
+
+def test_more_new_tokens_than_32_bits_add_up(g):
+    """lens + q_len past 2^31: as many as the cache has slots."""
+    most = 2 ** 31 - 1
+    s = Setup(g, 3, 1, 1, 64, 64, 32, lens=[64, 64, 64])
+    got = []
+    for q_len in (0, most):
+        k, v = g.alloc((3, 1, 64, 64)), g.alloc((3, 1, 64, 64))
+        g.kv8_read(s.cache, k, v, count=64, q_len=q_len)
+        got.append((k.download(), v.download()))
+    assert np.abs(got[0][0]).max() > 1
+    assert all(np.array_equal(a, b) for a, b in zip(*got))
+    s.cache.lens.upload(np.array([0, 3, 64], np.int32))
+    g.kv8_advance(s.cache, q_len=most)
+    assert s.cache.lens.download().tolist() == [64, 64, 64]
+    s.cache.lens.upload(np.array([0, 3, 64], np.int32))
+    g.kv8_advance(s.cache, q_len=most, new_lens=g.tensor(np.array([most, 2, most], np.int32),
+                                                         np.int32), limit=most)
+    assert s.cache.lens.download().tolist() == [most, 5, most]
