@@ -442,8 +442,9 @@ __global__ void __launch_bounds__(kLpWarps * 32, kLpPerSm)
       const int done = r, done_id = id;
       const float done_one = one;
       const bool done_has = has;
-      r += warps * gridDim.x;
-      const bool more = r < a.rows;
+      const int step = warps * gridDim.x;
+      const bool more = step < a.rows - r;   // (r + step may pass 2^31)
+      r += more ? step : 0;
       if (more) take_row();            // its copies start before this row's results
       emit(a, done, st, list, lane, 32, done_one, done_id, done_has);
       __syncwarp();
