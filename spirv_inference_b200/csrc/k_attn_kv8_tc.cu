@@ -137,12 +137,7 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
-// After a wait for loads: their values are used behind it, not before.
-template <int N>
-__device__ __forceinline__ void settled(float (&v)[N]) {
-#pragma unroll
-  for (int e = 0; e < N; ++e) asm volatile("" : "+f"(v[e]));
-}
+
 // Of a warp that goes together, the lane that issues.
 __device__ __forceinline__ bool first_lane() { return (threadIdx.x & 31) == 0; }
 
@@ -564,7 +559,6 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
     for (int c = 0; c < D / 32; ++c) {
       float v[32];
       tmem_ld_32x32(lanes + 2 * kTile + (tile & 1) * D + c * 32, v);
-      settled(v);
 #pragma unroll
       for (int e = 0; e < 32; e += 2) {
         const float2 r = fma2(make_float2(o[c * 32 + e], o[c * 32 + e + 1]),
@@ -684,7 +678,6 @@ __device__ __forceinline__ bool softmax_tiles(const AttnArgs& a, const Unit<D>& 
     // a half's scores, in units of log 2
     auto scores = [&](int c, float (&v)[32]) {
       tmem_ld_32x32(t_s + c * 32, v);
-      settled(v);
 #pragma unroll
       for (int e = 0; e < 32; ++e)
         v[e] = c * 32 + e > seen ? -INFINITY : v[e] * (aux.k_key[s][c * 32 + e] * qs);
@@ -1065,7 +1058,6 @@ __global__ void __launch_bounds__(kWeightThreads, TcShape<D>::kBlocks)
         for (int c = 0; c < kRows / 32; ++c) {
           float v[32];
           tmem_ld_32x32(tmem + s * kRows + lanes + c * 32, v);
-          settled(v);
           float2 part = make_float2(0.f, 0.f);
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {

@@ -386,7 +386,10 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
       : "r"(taddr));
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+  for (int i = 0; i < 32; ++i) {
+    asm volatile("" : "+r"(r[i]));     // used behind the wait, which names no register
+    v[i] = __uint_as_float(r[i]);
+  }
 }
 
 // v += the 32 columns at taddr (two 16-column loads, fewer live registers).
@@ -403,7 +406,10 @@ __device__ __forceinline__ void add_tmem32(uint32_t taddr, float (&v)[32]) {
         : "r"(taddr + (uint32_t)(h * 16)));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[16 * h + i] += __uint_as_float(r[i]);
+    for (int i = 0; i < 16; ++i) {
+      asm volatile("" : "+r"(r[i]));   // (as above)
+      v[16 * h + i] += __uint_as_float(r[i]);
+    }
   }
 }
 

@@ -153,6 +153,19 @@ __device__ __forceinline__ void tc_before() {
 __device__ __forceinline__ void tc_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
+// After a wait for TMEM loads: their values are used behind it.  (The wait names
+// no register, so that without this nothing keeps a use from being scheduled
+// before it.)
+template <int N>
+__device__ __forceinline__ void settled(uint32_t (&v)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) asm volatile("" : "+r"(v[e]));
+}
+template <int N>
+__device__ __forceinline__ void settled(float (&v)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) asm volatile("" : "+f"(v[e]));
+}
 // 32 TMEM lanes (this warp's quarter) x 32 consecutive columns from taddr.
 __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, float (&v)[32]) {
   uint32_t r[32];
@@ -168,11 +181,13 @@ __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, float (&v)[32]) {
         "=r"(r[31])
       : "r"(taddr));
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  settled(r);
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// The same load without waiting (several loads, then one tmem_wait_ld).
+// The same load without waiting (several loads, then one tmem_wait_ld and
+// settled() of all of them).
 __device__ __forceinline__ void tmem_ld_32x32_async(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
