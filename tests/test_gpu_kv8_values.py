@@ -293,3 +293,27 @@ def test_rows_behind_the_new_tokens_have_no_part(g, T, G):
         s.rng = np.random.default_rng(1)
     for other in got[2:]:
         assert all(np.array_equal(a, b) for a, b in zip(got[1], other))
+
+
+def _zero_keys(x, q, kv):
+    x[:, :, q] = 0                      # kv head 0: all keys; kv head 1: some
+    x[:, 5::3, q + 1:q + kv] = 0
+
+
+def _zero_queries(x, q, kv):
+    x[:, :, 0] = 0
+    x[:, -1, :q] = 0
+
+
+def _tiny_keys(x, q, kv):
+    x[:, :, q:q + kv] *= np.float32(1e-36)
+    x[:, ::7, q:q + kv] = 0
+
+
+@pytest.mark.parametrize("change", [_zero_keys, _zero_queries, _tiny_keys])
+@pytest.mark.parametrize("T,G,D", [(1, 8, 64), (2, 8, 64), (5, 8, 128), (16, 8, 64), (20, 8, 128)])
+def test_zero_and_tiny_keys_and_queries(g, T, G, D, change):
+    lens = [0, 37, 96, 300]
+    s, d_q, q = _filled(g, lens, T, change, G=G, D=D)
+    for scale in (None, -0.3, 0.0):
+        _check(s, d_q, q, lens, scale=scale)
