@@ -394,6 +394,13 @@ __device__ __forceinline__ void tail_group(uint8_t* hi_to, uint8_t* lo_to, int r
       const uint32_t who = __ballot_sync(0xffffffffu, odd);
       float down, up;
       pow2_scale(mx, down, up);
+      if (V) {
+        // To 2^10, between the 2^14 that would suit the values and the 2^7 of int8
+        // ones: a tile's keys share the unit of their weights, whose low halves
+        // are multiples of 2^-24, and both then lose 2^-36 of the largest at most.
+        down *= 0x1p-4f;
+        up *= 0x1p4f;
+      }
       uint2 hi, lo;
       split2(v[i].x * down, v[i].z * down, hi.x, lo.x);
       split2(v[i].y * down, v[i].w * down, hi.y, lo.y);
