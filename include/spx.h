@@ -597,16 +597,22 @@ int spx_op_rope_kv8_append(spx_graph* g, const float* qkv, int64_t ld_qkv, const
                            const spx_kv8_cache* cache);
 /* Causal grouped-query attention of the new tokens over the cache, after their
  * append: the token in slot i sees the slots up to i, out = softmax(scale q
- * k^T) v in fp32 accuracy.  q and out are [batch * q_len][q_heads][head_dim],
- * 16-byte aligned, and share no memory.  lse (may be NULL): [batch * q_len][q_heads], the log of
- * each softmax sum.  weights (may be NULL; needs lse): [batch][kv_heads]
- * [max_seq], to which each slot's attention weight, summed over the new tokens
- * and the heads of the group, is added; the new tokens' slots start from 0.
+ * k^T) v.  q and out are [batch * q_len][q_heads][head_dim], 16-byte aligned, and
+ * share no memory.  lse (may be NULL): [batch * q_len][q_heads], the log of each
+ * softmax sum.  weights (may be NULL; needs lse): [batch][kv_heads][max_seq], to
+ * which each slot's attention weight, summed over the new tokens and the heads
+ * of the group, is added; the new tokens' slots start from 0.
+ * Sums are in fp32.  Into the products go an element of q or of an open row of k
+ * or v to 2^-22 of itself or, if that is more, 2^-30 (v: 2^-36) of the largest of
+ * its row; a softmax weight to 2^-20 of itself or, times a value, 2^-36 of the
+ * largest that the row sees (of a closed block: that its scale can hold).  A score
+ * may carry 2^-36 of the largest q times the largest k of the key's block besides.
+ * What a row does not see has no part in its accuracy.
  * A NaN or an infinity in a row of q, or in a K or V row that it sees, makes
  * all of the row's output NaN; in q or K, also its lse and the weights that it
- * adds (V takes no part in those); one that it does not see does nothing.  At most 2^31 - 1 rows of q in all, 65535 sequences times
- * kv heads, and (q_len times heads of a group) times heads of a group below
- * 2^32. */
+ * adds (V takes no part in those); one that it does not see does nothing.  At
+ * most 2^31 - 1 rows of q in all, 65535 sequences times kv heads, and (q_len
+ * times heads of a group) times heads of a group below 2^32. */
 int spx_op_attention_kv8(spx_graph* g, const float* q, const spx_kv8_cache* cache,
                          const int32_t* new_lens, int32_t q_len, int32_t q_heads, float scale,
                          float* out, float* lse, float* weights);

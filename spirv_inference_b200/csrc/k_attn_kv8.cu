@@ -86,8 +86,9 @@ __device__ __forceinline__ void cluster_wait() {
 //
 // What bounds it: the cache's bytes, 2 D + 8 / block a key and head, and close
 // behind the instructions, about 150 for 16 keys of D = 64 and 8 rows (48 of
-// them turn V into fp16).  So tiles that every row sees in full take a path
-// without masks, and the others, one by one, another.
+// them turn V into fp16); with sequences of unlike lengths, the longest one.  So
+// tiles that every row sees in full take a path without masks, and the others, one
+// by one, another.
 // Which key of eight stands in column n: the order in which lanes' reads of K
 // (keys_at(g), 16 bytes at t) and of V (keys_at(2t), keys_at(2t + 1), 8 bytes
 // at g) meet no bank of shared memory twice.
@@ -1127,11 +1128,24 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) kv8_weights_kernel(const
 }
 
 // From so many rows of a sequence and kv head on, tcgen05.  In us, this file's
-// kernels against those, with weights, caches of 300 to 1500 tokens, 4 kv heads:
-//                  4 sequences of 64    32 of 64    4 of 128     32 of 128
-//    64 rows             37, 34          63, 74      49, 47      118, 130
-//    96 rows             46, 34          90, 74      62, 48      167, 134
-//   128 rows             56, 35         112, 76      77, 49      208, 137
+// kernels against those, with weights, 4 kv heads:
+//                                        64 rows     80 rows     128 rows
+//   64 values a head, tokens in the cache
+//     32 to 64, 1 sequence                18, 24      21, 25       29, 26
+//     32 to 64, 32                        33, 26      42, 27       61, 27
+//     300 to 1500, 4                      36, 34      41, 35       54, 35
+//     300 to 1500, 32                     60, 74      74, 75      107, 75
+//     16 thousand, 1                      47, 71      52, 72       76, 72
+//     16 thousand, 32                    497, 635    702, 646     952, 653
+//     100 thousand, 1                    185, 324    200, 328     293, 331
+//   128 values a head
+//     300 to 1500, 4                      49, 47      55, 48       77, 49
+//     300 to 1500, 32                    117, 131    146, 133     210, 140
+//     16 thousand, 1                      75, 109     86, 110     103, 112
+//     16 thousand, 32                    978, 1331  1245, 1355   1798, 1399
+// The two cross between 64 and 128 rows in all of these; one long sequence of 80 to
+// 127 rows is where the rule costs most (its tcgen05 row tile is one, on 8 CTAs a
+// kv head).
 constexpr int kTcRows = 80;
 
 template <int D, int NT>
@@ -1141,9 +1155,9 @@ int launch_few(cudaStream_t s, const AttnArgs& a) {
   const int64_t units = (int64_t)groups * a.c.kv_heads * a.c.batch;
   // Spread a sequence's keys over a CTA's warps, then over CTAs, while that does
   // not make more warps than are resident at a time (16 an SM) and a warp still
-  // has a group of tiles.  64 sequences of 1500 to 4096, 4 kv heads: 8 warps
-  // 44 us, 4 warps 57, 2 CTAs 47.  One of 131 thousand tokens: 1, 2, 4, 8 CTAs
-  // 619, 314, 161, 85.  One of 37: 4 warps 4.5, 8 warps 5.0, 2 CTAs 5.7.
+  // has a group of tiles.  64 sequences of 611 to 4095, 4 kv heads, with weights: 8
+  // warps 45 us, 4 warps 53, 2 CTAs of 8 warps 48.  One of 131 thousand tokens: 1,
+  // 2, 4, 8 CTAs 632, 321, 166, 88.  One of 45: 4 warps 4.9, 8 warps 5.2, 2 CTAs 6.1.
   const int steps = (int)ceil_div(a.c.max_seq, 16 * FewShape<D, NT>::KT);
   int W = 4, C = 1;
   while (W < kFewMaxWarps && units * W * 2 <= 16 * kNumSms && W * 2 <= steps) W *= 2;
@@ -1175,7 +1189,7 @@ int launch_few(cudaStream_t s, const AttnArgs& a) {
     // Few sequences: larger clusters, of as many CTAs as the GPU has room for
     // at a time (a cluster's SMs are neighbours: 8 clusters of 16 may not fit).
     // At one sequence of 131 thousand tokens, 8 kv heads of 128, 8 CTAs a head
-    // take 85 us, 10 take 71.
+    // take 88 us, 10 take 74.
     if ((rc = check_cuda(
              cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
              "attention_kv8: cluster attribute")))

@@ -28,10 +28,11 @@
 // are added.
 //
 // Four prompts of 777 to 1024 tokens onto 0 to 1000, 32 heads of 64 on 4 kv
-// heads: 140 us, 0.41 PFLOP/s of fp16 products, the weights another 102.  What
-// bounds it: the softmax warps' instructions, about 9 a score; two CTAs an SM (D
-// = 64) are two such warps a scheduler, which wait for each other's issue slots
-// and for the tensor memory.
+// heads: 128 us, 0.45 PFLOP/s of fp16 products, the weights another 104.  What
+// bounds it: no unit (issue slots 45 % of the active cycles, exponentials 25,
+// tensor pipe 24), but a chain in too few warps.  Two CTAs an SM (D = 64) are two
+// softmax warps a scheduler, and each of them, for every 64 keys, waits for O, then
+// for S, and takes the maximum, the exponentials, the split and the store in turn.
 #include <cooperative_groups.h>
 #include <cuda.h>
 
@@ -471,8 +472,8 @@ __device__ __forceinline__ void convert_tiles(const AttnArgs& a, const Unit<D>& 
     return mb_wait(&aux.empty[slot], ((m >> 2) & 1) ^ 1, &aux.abort_flag, status_of(a), kWaitNs,
                    64);
   };
-  // (Apart from the others, whose code cost this loop its registers: 40 us of
-  // 172 over four prompts.)
+  // (Apart from the others, whose code cost this loop its registers: 32 us when
+  // four prompts took 172.)
   // Tiles of closed blocks only, each one's bytes on their way while the one
   // before drains.
   const int whole = max(0, min(u.tiles, u.closed / kTile - u.first));
@@ -774,7 +775,7 @@ __device__ __forceinline__ void join(const AttnArgs& a, const Unit<D>& u, uint8_
 }
 
 // SPLIT: the keys are dealt to a cluster.  (Apart: the join costs the others
-// registers, 168 against 180 us over four prompts of 1024.)
+// registers; when four prompts of 1024 took 168 us, they took 180 with it.)
 template <int D, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
     attention_kv8_tc_kernel(const AttnArgs a, int ctas) {
@@ -877,9 +878,10 @@ __global__ void __launch_bounds__(kThreads, TcShape<D>::kBlocks)
 // TMEM, issue its products themselves and add exp(score - lse) over its rows, a
 // key a thread: while one waits for its products, the other adds.  The row
 // tiles are dealt to a cluster's CTAs, whose sums are added in order.  About 3
-// instructions a score, and 4 a value of q.  Four prompts as above: 102 us (one
-// group adding and two converting: 106; clusters of 2 and 8 in place of 4, when
-// this took 137: 141 and 162).
+// instructions a score, and 4 a value of q, which is turned into operands again for
+// every 128 keys.  Four prompts as above: 104 us (one group adding and two
+// converting: 4 % more; clusters of 2 and 8 in place of 4, when this took 137: 141
+// and 162).
 constexpr int kWeightCluster = 4, kKeys = 128, kWeightThreads = 384;
 
 struct WeightAux {
